@@ -39,7 +39,11 @@ typedef enum pl_status {
   PL_ERR_SPAN_NOT_FULL = 7,      /* "non-last page spans must be full pages"        */
   PL_ERR_CUDA = 8,               /* a CUDA runtime call failed (see pl_last_cuda_error) */
   PL_ERR_TIMEOUT = 9,            /* device: a bounded wait ran out (kernel returned) */
-  PL_ERR_NO_DEVICE = 10
+  PL_ERR_NO_DEVICE = 10,
+  PL_ERR_POOL_EXHAUSTED = 11,    /* device: fewer free pages than the call needs      */
+  PL_ERR_ROW_CAPACITY = 12,      /* device: a row would outgrow its page list         */
+  PL_ERR_PAGE_SHARED = 13,       /* device: a row's partial last page has other owners */
+  PL_ERR_REFCOUNT = 14           /* device: a page given back more often than held    */
 } pl_status;
 
 /* ---------------------------------------------------------------- library */
@@ -849,6 +853,230 @@ int32_t pl_embed(const int64_t *token_ids, const void *table, int64_t vocab,
 int32_t pl_argmax(const void *logits, int64_t stride, int32_t vocab,
                   int32_t num_tokens, int64_t *out_ids, void *workspace,
                   int64_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------ drafted-token trees */
+
+/*
+ * Attention of a tree of drafted tokens over the paged cache (the
+ * verification step of speculative decoding).  No reference counterpart:
+ * the reference decodes one token per row and step.
+ *   q          bf16 [total_q, num_qo_heads, head_dim]: request b owns the rows
+ *              qo_indptr[b] .. qo_indptr[b+1), its n_b drafted tokens; their
+ *              K/V are the last n_b of the request's cached positions
+ *   kv_cache, kv_indptr, kv_indices, kv_last_page_len  as pl_paged_prefill;
+ *              total_pages = entries of kv_indices
+ *   tree_mask  int32 bit words [total_q][mask_words], row stride mask_stride:
+ *              bit j%32 of word j/32 set = the row's token sees drafted token
+ *              j of its request (bits from n_b on are ignored); every token
+ *              sees all positions in front of the drafted ones.  A row that
+ *              sees nothing yields O = 0 and LSE = -inf; inf or NaN in the
+ *              K/V of drafted tokens that a row does not see stays out of it
+ *   out        bf16 (strides as q's), out_lse fp32 [total_q, num_qo_heads]
+ *              natural log, nullable
+ *   workspace  16-byte aligned, pl_tree_workspace_bytes; needs no
+ *              initialisation and keeps nothing between calls
+ * Supported: head_dim 64 or 128, page_size 16 / 32 / 64 / 128, any group up
+ * to 128.  A request with n_b > its cached tokens or > 32 * mask_words, or
+ * with a table outside kv_indices, writes PL_ERR_INVALID_ARGUMENT to
+ * *status_dev.
+ */
+int64_t pl_tree_workspace_bytes(int32_t batch, int32_t total_q,
+                                int32_t num_qo_heads, int32_t num_kv_heads,
+                                int32_t head_dim);
+int32_t pl_paged_tree_attention(const void *q, int64_t q_stride_t,
+                                int64_t q_stride_h, const void *kv_cache,
+                                int64_t num_pages, const int32_t *qo_indptr,
+                                const int32_t *kv_indptr,
+                                const int32_t *kv_indices,
+                                const int32_t *kv_last_page_len,
+                                int64_t total_pages, const int32_t *tree_mask,
+                                int64_t mask_stride, int32_t mask_words,
+                                int32_t batch, int32_t total_q,
+                                int32_t num_qo_heads, int32_t num_kv_heads,
+                                int32_t head_dim, int32_t page_size,
+                                float sm_scale, void *out,
+                                int64_t out_stride_t, int64_t out_stride_h,
+                                float *out_lse, void *workspace,
+                                int64_t workspace_bytes, int32_t *status_dev,
+                                void *stream);
+
+/*
+ * Ancestor-or-self bits of drafted tokens from their parents (index in the
+ * request, -1: the context; a parent comes before its children): mask as
+ * pl_paged_tree_attention reads it (all mask_words words of every row are
+ * written), depth[total_q] (ancestors of the token; nullable) and
+ * positions[total_q] = base_positions[b] + depth (RoPE positions; nullable,
+ * base_positions nullable: 0).  At most 1024 tokens a request; a parent that
+ * does not come first, or a request that does not fit, writes
+ * PL_ERR_INVALID_ARGUMENT to *status_dev.  No reference counterpart.
+ */
+int32_t pl_tree_mask(const int32_t *parents, const int32_t *qo_indptr,
+                     const int32_t *base_positions, int32_t batch,
+                     int32_t total_q, int32_t mask_words, int32_t *mask,
+                     int64_t mask_stride, int32_t *depth, int32_t *positions,
+                     int32_t *status_dev, void *stream);
+
+/*
+ * Greedy acceptance.  Drafted token i is taken when it and all its ancestors
+ * are what the model chose after their parents (tokens[i] ==
+ * targets[parent]; a token on the context is taken); the deepest taken token
+ * (lowest index among equals) ends the kept path.
+ *   keep        int32 [batch][max_keep], row stride keep_stride: base_positions[b]
+ *               + index of the path's tokens in order, then -1
+ *   keep_count  int32 [batch]; next_token int64 [batch]: the model's choice
+ *               after the path (-1 for a request without tokens)
+ * A path longer than max_keep writes PL_ERR_INVALID_ARGUMENT and keeps
+ * nothing.  No reference counterpart.
+ */
+int32_t pl_tree_accept(const int32_t *parents, const int64_t *tokens,
+                       const int64_t *targets, const int32_t *qo_indptr,
+                       const int32_t *base_positions, int32_t batch,
+                       int32_t total_q, int32_t max_keep, int32_t *keep,
+                       int64_t keep_stride, int32_t *keep_count,
+                       int64_t *next_token, int32_t *status_dev, void *stream);
+
+/* ---------------------------------------------------------- pages of a cache */
+
+/*
+ * Page bookkeeping on the device, and the copies that follow from it.  The
+ * reference reserves slots on the host (model/kvcache/paged_kvcache_manager.py
+ * :195-213, reserve_chunk), one chunk of a row at a time).
+ *   refcount       int32 [num_pages]: rows that hold the page; 0 = free
+ *   row_pages      int32 [num_rows][row_capacity], row_num_pages and
+ *   last_page_len  int32 [num_rows]: as pl_page_table_advance
+ * A call that needs N pages takes the N lowest free ids, in row order.  One
+ * that cannot be served writes its reason to *status_dev
+ * (PL_ERR_INVALID_ARGUMENT, _POOL_EXHAUSTED, _ROW_CAPACITY, _PAGE_SHARED,
+ * _PAGE_OUT_OF_RANGE) and changes nothing.  A page id outside the pool that
+ * is met while pages are shared or given back, or a page given back more
+ * often than held (PL_ERR_REFCOUNT), is skipped and reported.  num_rows <=
+ * 4096, page_size <= 128, num_pages * page_size < 2^31.
+ *
+ * pl_page_release: the listed rows give their pages back and become empty
+ * (row_pages stays as it is).
+ *
+ * pl_page_reserve: row r grows by tok_indptr[r+1] - tok_indptr[r] tokens
+ * (tok_indptr[0] = 0, tok_indptr[num_rows] = total_tokens), whose slots go to
+ * slot_page / slot_offset [total_tokens] and, when given, whose positions in
+ * the row go to positions_out.  out_indptr [num_rows+1] / out_indices
+ * [max_indices] (nullable) receive the new page table.  A row's partial last
+ * page has to be its own (PL_ERR_PAGE_SHARED).
+ *
+ * pl_page_fork: row dst_rows[i] (empty, listed once) becomes a copy of
+ * src_rows[i]: full pages are shared, a partial last page is copied (its
+ * used tokens, every layer) to a page of its own.
+ *   pool           num_layers x [num_pages][2][page_size][token], layers
+ *                  layer_stride_bytes apart, K before V; token_bytes = bytes
+ *                  of one token's K in one layer (a multiple of 16; any type)
+ *
+ * pl_cache_compact: row r keeps its tokens [0, keep_from[r]) and the
+ * positions keep[r][0 .. keep_count[r]), ascending and from keep_from[r] on,
+ * and is as long as what it keeps.  Whole pages in front of the first token
+ * that moves stay; the kept tokens behind them go to new pages (every
+ * layer), the old ones are given back, so rows that share them keep their
+ * contents.  A row where nothing moves is cut in place, unless its new
+ * partial last page is shared.  A position outside the row writes
+ * PL_ERR_INVALID_ARGUMENT and leaves that slot unwritten.
+ *   keep           int32 [num_rows][max_keep], row stride keep_stride
+ *   workspace      16-byte aligned, no initialisation
+ */
+int32_t pl_page_release(int32_t *refcount, int64_t num_pages,
+                        int32_t *row_pages, int32_t *row_num_pages,
+                        int32_t *last_page_len, int32_t num_rows,
+                        int32_t row_capacity, const int32_t *rows,
+                        int32_t num_released, int32_t *status_dev,
+                        void *stream);
+int32_t pl_page_reserve(int32_t *refcount, int64_t num_pages,
+                        int32_t *row_pages, int32_t *row_num_pages,
+                        int32_t *last_page_len, int32_t num_rows,
+                        int32_t row_capacity, int32_t page_size,
+                        const int32_t *tok_indptr, int32_t total_tokens,
+                        int32_t *slot_page, int32_t *slot_offset,
+                        int32_t *positions_out, int32_t *out_indptr,
+                        int32_t *out_indices, int64_t max_indices,
+                        int32_t *status_dev, void *stream);
+int64_t pl_page_fork_workspace_bytes(int32_t num_forks);
+int32_t pl_page_fork(void *pool, int64_t layer_stride_bytes,
+                     int32_t num_layers, int64_t token_bytes,
+                     int32_t *refcount, int64_t num_pages, int32_t *row_pages,
+                     int32_t *row_num_pages, int32_t *last_page_len,
+                     int32_t num_rows, int32_t row_capacity, int32_t page_size,
+                     const int32_t *src_rows, const int32_t *dst_rows,
+                     int32_t num_forks, void *workspace,
+                     int64_t workspace_bytes, int32_t *status_dev,
+                     void *stream);
+int64_t pl_cache_compact_workspace_bytes(int32_t num_rows,
+                                         int32_t row_capacity);
+int32_t pl_cache_compact(void *pool, int64_t layer_stride_bytes,
+                         int32_t num_layers, int64_t token_bytes,
+                         int32_t *refcount, int64_t num_pages,
+                         int32_t *row_pages, int32_t *row_num_pages,
+                         int32_t *last_page_len, int32_t num_rows,
+                         int32_t row_capacity, int32_t page_size,
+                         const int32_t *keep_from, const int32_t *keep,
+                         int64_t keep_stride, const int32_t *keep_count,
+                         int32_t max_keep, void *workspace,
+                         int64_t workspace_bytes, int32_t *status_dev,
+                         void *stream);
+
+/* -------------------------------------------------------- sparse attention */
+
+/*
+ * int8 bounds of the keys of pages page_ids[0 .. n), the first page_len[i]
+ * tokens of each (nullable: all): with a = max |k| and s = a / 127 (fp32:
+ * a * fl(1/127)) over a page's tokens and channels of one kv head,
+ * bounds[page][head][0][d] = floor(min_t k / s) and [1][d] = ceil(max_t k /
+ * s), within +-127, and bound_scale[page][head] = s.  A page with an inf or
+ * NaN key gets bounds 0 and scale +inf.  bounds int8 [num_pages][num_kv_heads]
+ * [2][head_dim] (16-byte aligned), bound_scale fp32 [num_pages][num_kv_heads];
+ * only the listed pages are written.  head_dim 64 or 128.  No reference
+ * counterpart.
+ */
+int32_t pl_page_bounds(const void *kv_cache, int64_t num_pages,
+                       int32_t num_kv_heads, int32_t head_dim,
+                       int32_t page_size, const int32_t *page_ids,
+                       const int32_t *page_len, int32_t n, int8_t *bounds,
+                       float *bound_scale, int32_t *status_dev, void *stream);
+
+/*
+ * Paged decode, one query token per row, over the pages that a score of the
+ * bounds selects for each (row, kv head).  A row with at most num_select
+ * pages attends to all of them.  Otherwise the first sink_pages and the last
+ * recent_pages (>= 1; their bounds are not read, so the page that is being
+ * filled needs none) are taken, and the others by falling score
+ *   fl32(max_h sum_d max(qi_hd lo_d, qi_hd hi_d)) * s
+ * over the group's query heads h (qi = rint(q / sq) within +-127, sq =
+ * max |q| of the group * fl(1/127)), lower index first among equals, up to
+ * num_select pages.
+ *   q, kv_cache, indptr, indices, last_page_len, out, out_lse  as
+ *            pl_paged_decode; total_pages = entries of indices; max_pages:
+ *            no row has more (a longer one writes PL_ERR_INVALID_ARGUMENT
+ *            and counts as empty)
+ *   selected int32 [batch][num_kv_heads][num_select]: the taken pages of the
+ *            row (index in its page list), ascending, then -1
+ *   workspace 16-byte aligned, pl_sparse_workspace_bytes, no initialisation
+ *            (unused, nullable, when max_pages <= num_select)
+ * Supported: head_dim 64 or 128, page_size 16 or 32, group <= 16.  No
+ * reference counterpart.
+ */
+int64_t pl_sparse_workspace_bytes(int32_t batch, int32_t num_kv_heads,
+                                  int32_t max_pages);
+int32_t pl_paged_sparse_decode(const void *q, int64_t q_stride_b,
+                               int64_t q_stride_h, const void *kv_cache,
+                               int64_t num_pages, const int32_t *indptr,
+                               const int32_t *indices,
+                               const int32_t *last_page_len,
+                               int64_t total_pages, int32_t max_pages,
+                               const int8_t *bounds, const float *bound_scale,
+                               int32_t batch, int32_t num_qo_heads,
+                               int32_t num_kv_heads, int32_t head_dim,
+                               int32_t page_size, float sm_scale,
+                               int32_t num_select, int32_t sink_pages,
+                               int32_t recent_pages, void *out,
+                               int64_t o_stride_b, int64_t o_stride_h,
+                               float *out_lse, int32_t *selected,
+                               void *workspace, int64_t workspace_bytes,
+                               int32_t *status_dev, void *stream);
 
 #ifdef __cplusplus
 }

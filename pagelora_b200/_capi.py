@@ -27,6 +27,10 @@ PL_ERR_SPAN_NOT_FULL = 7
 PL_ERR_CUDA = 8
 PL_ERR_TIMEOUT = 9
 PL_ERR_NO_DEVICE = 10
+PL_ERR_POOL_EXHAUSTED = 11
+PL_ERR_ROW_CAPACITY = 12
+PL_ERR_PAGE_SHARED = 13
+PL_ERR_REFCOUNT = 14
 
 PL_PROLOGUE_NONE = 0
 PL_PROLOGUE_RMSNORM = 1
@@ -164,6 +168,35 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "pl_embed": (_I32, [_P, _P, _I64, _I32, _I32, _P, _P, _P]),
     "pl_argmax": (_I32, [_P, _I64, _I32, _I32, _P, _P, _I64, _P]),
+    "pl_tree_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32]),
+    "pl_paged_tree_attention": (
+        _I32,
+        [_P, _I64, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F, _P,
+         _I64, _I64, _P, _P, _I64, _P, _P],
+    ),
+    "pl_tree_mask": (_I32, [_P, _P, _P, _I32, _I32, _I32, _P, _I64, _P, _P, _P, _P]),
+    "pl_tree_accept": (_I32, [_P, _P, _P, _P, _P, _I32, _I32, _I32, _P, _I64, _P, _P, _P, _P]),
+    "pl_page_release": (_I32, [_P, _I64, _P, _P, _P, _I32, _I32, _P, _I32, _P, _P]),
+    "pl_page_reserve": (
+        _I32, [_P, _I64, _P, _P, _P, _I32, _I32, _I32, _P, _I32, _P, _P, _P, _P, _P, _I64, _P, _P],
+    ),
+    "pl_page_fork_workspace_bytes": (_I64, [_I32]),
+    "pl_page_fork": (
+        _I32,
+        [_P, _I64, _I32, _I64, _P, _I64, _P, _P, _P, _I32, _I32, _I32, _P, _P, _I32, _P, _I64, _P, _P],
+    ),
+    "pl_cache_compact_workspace_bytes": (_I64, [_I32, _I32]),
+    "pl_cache_compact": (
+        _I32,
+        [_P, _I64, _I32, _I64, _P, _I64, _P, _P, _P, _I32, _I32, _I32, _P, _P, _I64, _P, _I32, _P, _I64, _P, _P],
+    ),
+    "pl_page_bounds": (_I32, [_P, _I64, _I32, _I32, _I32, _P, _P, _I32, _P, _P, _P, _P]),
+    "pl_sparse_workspace_bytes": (_I64, [_I32, _I32, _I32]),
+    "pl_paged_sparse_decode": (
+        _I32,
+        [_P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _F, _I32, _I32,
+         _I32, _P, _I64, _I64, _P, _P, _P, _I64, _P, _P],
+    ),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

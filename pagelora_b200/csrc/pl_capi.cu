@@ -91,6 +91,10 @@ extern "C" const char* pl_status_string(int32_t status) {
     case PL_ERR_CUDA: return "CUDA runtime error";
     case PL_ERR_TIMEOUT: return "device wait timed out";
     case PL_ERR_NO_DEVICE: return "no CUDA device";
+    case PL_ERR_POOL_EXHAUSTED: return "page pool exhausted";
+    case PL_ERR_ROW_CAPACITY: return "row page list full";
+    case PL_ERR_PAGE_SHARED: return "last page shared with another row";
+    case PL_ERR_REFCOUNT: return "page released more often than held";
     default: return "unknown status";
   }
 }

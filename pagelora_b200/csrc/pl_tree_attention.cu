@@ -1,0 +1,951 @@
+// Attention for a tree of drafted tokens over the paged KV cache, with the
+// tree's ancestor mask and the greedy acceptance of a path.
+//
+// Request b has n_b query tokens (its drafted tree); their K/V are the last
+// n_b of its kv_len_b cached positions.  Token i sees the whole context
+// (positions below kv_len_b - n_b) and the drafted tokens whose bit is set
+// in its mask row:
+//   o_i = sum_t p_t v_t / l,  p_t = 2^(s_t - m),  s_t = q_i.k_t * sm_scale * log2(e)
+// over the seen positions t; lse_i = ln 2 * (m + log2 l).  A row that sees
+// nothing gives o = 0 and lse = -inf.
+//
+// A work item is (request, kv head, row tile): 128 * NT tensor-core rows,
+// row R = token * group + head of the group, so all rows that read one K/V
+// tile (128 positions) sit in one CTA.  The items' tiles form one line
+// (request, kv head, row tile, position) that is cut into equal pieces, one
+// per CTA (one CTA per SM), so ragged contexts fill the device; a CTA takes
+// the one or few item segments of its piece in turn.  A segment that covers
+// its item writes the output; the others leave (O, m, l) in the workspace
+// and tree_merge_kernel joins them.  Within a segment:
+//   warp 0     TMA producer: K_0, V_0, K_1, V_1, ... through a ring of tiles;
+//   warp 1     one lane issues tcgen05.mma: S = Q.K^T into TMEM, O += P.V;
+//   warps 2..  softmax, one thread per row: scores from TMEM, mask, online
+//              softmax (log2 domain), P (bf16) as the swizzled A operand.
+// P is rounded to bf16 as the tensor core's operand; l sums the unrounded
+// fp32 values.  Waits are bounded: on expiry the kernel records
+// PL_ERR_TIMEOUT, drains its copies and returns.
+#include "pl_common.cuh"
+
+namespace pl {
+
+constexpr int kTreeM = 128;              // rows of one tile
+constexpr int kTreeN = 128;              // positions of one K/V tile
+constexpr float kTreeSlack = 8.0f;       // log2 growth of a row's maximum that is tolerated before O is rescaled
+constexpr int kTreeMaxTokens = 1024;     // drafted tokens of one request (tree_mask / tree_accept)
+
+struct TreeArgs {
+  const bf16* q;
+  const bf16* kv;  // the pool the tensor map covers (read for inf / NaN elements of V only)
+  int64_t q_stride_t, q_stride_h;
+  const int32_t* qo_indptr;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_last;
+  const uint32_t* mask;  // [total_q][words]
+  int64_t mask_stride;
+  int64_t num_pages, total_pages;
+  int32_t words, batch, total_q, num_qo_heads, num_kv_heads, group, page_size, min_share, ctas;
+  float scale_log2;
+  bf16* out;
+  int64_t out_stride_t, out_stride_h;
+  float* lse;      // optional [total_q, Hq], natural log
+  float* part_o;   // [2 * ctas][128 * NT][D]
+  float* part_ml;  // [2 * ctas][2][128 * NT]
+  int32_t* status;
+};
+
+template <int D, int NT>
+struct TreeCfg {
+  static constexpr int kThreads = 64 + 128 * NT;
+  static constexpr int kRows = kTreeM * NT;
+  static constexpr int kChunks = D / 64;
+  static constexpr int kChunkBytes = kTreeM * 128;
+  static constexpr int kQBytes = kChunks * kChunkBytes;
+  static constexpr int kKVBytes = kChunks * kChunkBytes;
+  static constexpr int kPBytes = 2 * kChunkBytes;
+  static constexpr int kSlots = NT == 1 ? 5 : 3;
+  static constexpr int kQOff = 0;
+  static constexpr int kPOff = kQOff + NT * kQBytes;
+  static constexpr int kSlotOff = kPOff + NT * kPBytes;
+  static constexpr int kBarOff = kSlotOff + kSlots * kKVBytes;
+  static constexpr int kNumBars = 2 * kSlots + 8 + 1;  // full empty | s[2] p[2] o[2] q[2] | fin
+  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+  static constexpr int kSmemBytes = 1024 + kMiscOff + 96;
+  static constexpr int kTmemCols = 512;  // S_x at 128 x, O_x at 256 + 128 x
+  static_assert(kSmemBytes <= 232448, "tree tiles exceed the shared-memory limit");
+};
+
+__device__ __forceinline__ uint32_t tr_swz(int r, int u) { return r * 128 + ((u ^ (r & 7)) << 4); }
+__device__ __forceinline__ float tr_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Sizes of one request: query tokens, cached tokens, row tiles, K/V tiles.
+struct TreeReq {
+  int q0, n, kv_begin, n_pages, kv_len, rts, ntiles;
+  __device__ __forceinline__ void load(const TreeArgs& a, int b, int rows) {
+    q0 = a.qo_indptr[b];
+    const int q1 = a.qo_indptr[b + 1];
+    const bool ok = q0 >= 0 && q1 >= q0 && q1 <= a.total_q;
+    n = ok ? q1 - q0 : 0;
+    // a table that leaves [0, total_pages) counts as empty (and is reported)
+    kv_begin = a.kv_indptr[b];
+    const int kv_end = a.kv_indptr[b + 1];
+    n_pages = kv_begin >= 0 && kv_end >= kv_begin && kv_end <= a.total_pages ? kv_end - kv_begin : 0;
+    int last = a.kv_last[b];
+    last = last < 0 ? 0 : (last > a.page_size ? a.page_size : last);
+    kv_len = n_pages > 0 ? (n_pages - 1) * a.page_size + last : 0;
+    rts = (int)(((int64_t)n * a.group + rows - 1) / rows);
+    ntiles = max(1, (kv_len + kTreeN - 1) / kTreeN);  // an empty context still writes its zero rows
+  }
+  __device__ __forceinline__ int64_t work(int hkv) const { return (int64_t)rts * hkv * ntiles; }
+};
+
+// Total tiles over all requests, and the tiles in front of request `upto`
+// (one warp; every lane gets the results).
+__device__ __forceinline__ void tree_prefix(const TreeArgs& a, int rows, int upto, int64_t& total, int64_t& before) {
+  const int lane = threadIdx.x & 31;
+  int64_t t = 0, p = 0;
+  for (int b = lane; b < a.batch; b += 32) {
+    TreeReq r;
+    r.load(a, b, rows);
+    const int64_t w = r.work(a.num_kv_heads);
+    t += w;
+    if (b < upto) p += w;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    t += __shfl_xor_sync(0xffffffffu, t, o);
+    p += __shfl_xor_sync(0xffffffffu, p, o);
+  }
+  total = t;
+  before = p;
+}
+
+__device__ __forceinline__ int64_t tree_share(int64_t total, int ctas, int min_share) {
+  const int64_t s = (total + ctas - 1) / ctas;
+  return s < min_share ? min_share : s;
+}
+
+// The request that holds tile w of the line (batch: past the end) and its
+// first tile.  A cut that falls inside an item of at most min_share tiles
+// moves to the item's start, so short items are never split (and never
+// merged).  One warp.
+struct TreeAt {
+  int b;
+  int64_t base, w;
+};
+__device__ __forceinline__ TreeAt tree_locate(const TreeArgs& a, int rows, int64_t w) {
+  const int lane = threadIdx.x & 31;
+  TreeAt at{a.batch, 0, w};
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    TreeReq r;
+    int64_t n = 0;
+    r.ntiles = 1;
+    if (b0 + lane < a.batch) {
+      r.load(a, b0 + lane, rows);
+      n = r.work(a.num_kv_heads);
+    }
+    int64_t inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, n > 0 && w < at.base + inc);
+    if (hit != 0) {
+      const int l = __ffs(hit) - 1;
+      at.b = b0 + l;
+      at.base += __shfl_sync(0xffffffffu, inc - n, l);
+      const int nt = __shfl_sync(0xffffffffu, r.ntiles, l);
+      if (nt <= a.min_share) at.w = w - (w - at.base) % nt;
+      return at;
+    }
+    at.base += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return at;
+}
+
+// Walks the item segments of the tile range [w, w_end).
+struct TreeIter {
+  TreeReq r;
+  int b, kvh, rt, j0, j1;
+  int64_t w, w_end, base;  // base: first tile of request b
+  __device__ __forceinline__ void init(const TreeArgs& a, int rows, int b_, int64_t base_, int64_t w_, int64_t e) {
+    b = b_;
+    base = base_;
+    w = w_;
+    w_end = e;
+    if (w < w_end) r.load(a, b, rows);
+  }
+  __device__ __forceinline__ bool next(const TreeArgs& a, int rows) {
+    if (w >= w_end) return false;
+    while (w - base >= r.work(a.num_kv_heads)) {
+      base += r.work(a.num_kv_heads);
+      ++b;
+      r.load(a, b, rows);
+    }
+    const int64_t off = w - base;
+    const int64_t item = off / r.ntiles;
+    j0 = (int)(off - item * r.ntiles);
+    rt = (int)(item % r.rts);
+    kvh = (int)(item / r.rts);
+    const int64_t left = w_end - w;
+    j1 = (int)(left < r.ntiles - j0 ? j0 + left : r.ntiles);
+    w += j1 - j0;
+    return true;
+  }
+};
+
+// Bits of a mask row from bit `off` on (off >= 0), zero past the row's words.
+__device__ __forceinline__ uint32_t tree_bits(const uint32_t* row, int words, int off) {
+  const int i = off >> 5, s = off & 31;
+  const uint32_t lo = i < words ? row[i] : 0u;
+  const uint32_t hi = i + 1 < words ? row[i + 1] : 0u;
+  return __funnelshift_r(lo, hi, s);
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
+    paged_tree_kernel(const __grid_constant__ CUtensorMap kv_map, const TreeArgs a) {
+  using C = TreeCfg<D, NT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + C::kSlots;
+  uint64_t* sready = bars + 2 * C::kSlots;  // [2] S_x in TMEM
+  uint64_t* pready = sready + 2;            // [2] P_x staged (128 arrivals)
+  uint64_t* odone = sready + 4;             // [2] O_x += P_x.V finished
+  uint64_t* qready = sready + 6;            // [2] Q_x staged (128 arrivals)
+  uint64_t* fin = sready + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
+  volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, issued, consumed
+  int64_t* range = reinterpret_cast<int64_t*>(smem + C::kMiscOff + 32);                    // base, w0, w1
+  int32_t* range_b = reinterpret_cast<int32_t*>(smem + C::kMiscOff + 56);
+  uint32_t* any_bad = reinterpret_cast<uint32_t*>(smem + C::kMiscOff + 64);  // a drafted V held inf or NaN
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&sready[x], 1);
+      mbar_init(&pready[x], 128);
+      mbar_init(&odone[x], 1);
+      mbar_init(&qready[x], 128);
+    }
+    mbar_init(fin, 1);
+    flags[0] = flags[1] = flags[2] = 0;
+    any_bad[0] = 0;
+    fence_barrier_init();
+  }
+  if (threadIdx.x == 32) prefetch_tensormap(&kv_map);
+  __syncthreads();
+  pdl_launch_dependents();
+  pdl_wait();
+
+  if (warp == 0) {
+    int64_t total, dummy;
+    tree_prefix(a, C::kRows, 0, total, dummy);
+    const int64_t share = tree_share(total, a.ctas, a.min_share);
+    const int64_t w0 = min(total, (int64_t)blockIdx.x * share), w1 = min(total, w0 + share);
+    const TreeAt at0 = tree_locate(a, C::kRows, w0), at1 = tree_locate(a, C::kRows, w1);
+    if (lane == 0) {
+      range[0] = at0.base;
+      range[1] = at0.w;
+      range[2] = at1.w;
+      range_b[0] = at0.b;
+    }
+    // arguments that no launch can check on the host
+    if (blockIdx.x == 0)
+      for (int b = lane; b < a.batch; b += 32) {
+        TreeReq r;
+        r.load(a, b, C::kRows);
+        if (r.n != a.qo_indptr[b + 1] - r.q0 || r.n_pages != a.kv_indptr[b + 1] - r.kv_begin ||
+            r.n > 32 * a.words || r.n > r.kv_len)
+          set_status(a.status, PL_ERR_INVALID_ARGUMENT);
+      }
+  }
+  __syncthreads();
+  if (range[1] >= range[2]) return;  // nothing allocated yet
+
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  TreeIter it;
+  it.init(a, C::kRows, range_b[0], range[0], range[1], range[2]);
+  const int PS = a.page_size;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    const int ppt = kTreeN / PS;
+    const int boxes = ppt * C::kChunks;  // <= 16
+    const int p = lane / C::kChunks, hh = lane % C::kChunks;
+    int i = 0;
+    bool go = true;
+    while (go && it.next(a, C::kRows)) {
+      for (int j = it.j0; go && j < it.j1; ++j)
+        for (int kv = 0; kv < 2; ++kv, ++i) {
+          const int s = i % C::kSlots;
+          bool ok = true;
+          if (i >= C::kSlots) ok = mbar_wait(&empty[s], ((i / C::kSlots) - 1) & 1);
+          if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) {
+            if (lane == 0 && !__all_sync(0xffffffffu, ok)) set_status(a.status, PL_ERR_TIMEOUT);
+            flags[0] = 1;
+            go = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&full[s], C::kKVBytes);
+          __syncwarp();
+          if (lane < boxes) {
+            const int page_idx = j * ppt + p;
+            int32_t coord = (int32_t)(2 * a.num_pages);  // out of range: the copy writes zeros
+            if (page_idx < it.r.n_pages) {
+              const int32_t pid = a.kv_indices[it.r.kv_begin + page_idx];
+              if (pid >= 0 && (int64_t)pid < a.num_pages)
+                coord = 2 * pid + kv;
+              else
+                set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
+            }
+            uint8_t* dst = smem + C::kSlotOff + s * C::kKVBytes + hh * C::kChunkBytes + p * PS * 128;
+            tma_load_4d(dst, &kv_map, hh * 64, it.kvh, 0, coord, &full[s]);
+          }
+        }
+    }
+    if (lane == 0) flags[1] = i;
+  } else if (warp == 1) {
+    // ---------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = umma_idesc_bf16(kTreeM, kTreeN);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(kTreeM, D) | (1u << 16);  // B (V) MN-major
+      int consumed = 0;
+      auto wait_item = [&](int item) -> bool {
+        const bool r = mbar_wait(&full[item % C::kSlots], (item / C::kSlots) & 1) && !flags[0];
+        if (r && item + 1 > consumed) consumed = item + 1;
+        if (r) tc_fence_after();
+        return r;
+      };
+      auto issue_s = [&](int x, int t) {
+        const uint32_t qb = smem_u32(smem + C::kQOff + x * C::kQBytes);
+        const uint32_t kb = smem_u32(smem + C::kSlotOff + ((2 * t) % C::kSlots) * C::kKVBytes);
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16(tmem + (uint32_t)(x * kTreeN), umma_desc_k_sw128(qb + c * C::kChunkBytes + 32 * k),
+                      umma_desc_k_sw128(kb + c * C::kChunkBytes + 32 * k), idesc_s, (c | k) ? 1u : 0u);
+        umma_commit(&sready[x]);
+      };
+      auto issue_pv = [&](int x, int t, bool first) {
+        const uint32_t pb = smem_u32(smem + C::kPOff + x * C::kPBytes);
+        const uint32_t vb = smem_u32(smem + C::kSlotOff + ((2 * t + 1) % C::kSlots) * C::kKVBytes);
+#pragma unroll
+        for (int kk = 0; kk < kTreeN / 16; ++kk)
+          umma_bf16(tmem + (uint32_t)(256 + x * 128), umma_desc_k_sw128(pb + (kk >> 2) * C::kChunkBytes + 32 * (kk & 3)),
+                    umma_desc_mn_sw128(vb + kk * 16 * 128, C::kChunkBytes, 1024), idesc_o,
+                    (!first || kk > 0) ? 1u : 0u);
+        umma_commit(&odone[x]);
+      };
+      bool ok = true;
+      int t = 0;  // tiles of this CTA so far
+      for (int seg = 0; ok && it.next(a, C::kRows); ++seg) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x) ok = ok && mbar_wait(&qready[x], seg & 1);
+        ok = ok && wait_item(2 * t);
+        if (!ok) break;
+#pragma unroll
+        for (int x = 0; x < NT; ++x) issue_s(x, t);
+        umma_commit(&empty[(2 * t) % C::kSlots]);
+        for (int j = it.j0; ok && j < it.j1; ++j, ++t) {
+          const bool more = j + 1 < it.j1;
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            ok = ok && mbar_wait(&pready[x], t & 1) && !flags[0];
+            if (ok && x == 0) ok = wait_item(2 * t + 1);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(x, t, j == it.j0);
+            if (x == NT - 1) umma_commit(&empty[(2 * t + 1) % C::kSlots]);
+            if (more) {
+              if (x == 0) ok = wait_item(2 * t + 2);
+              if (!ok) break;
+              issue_s(x, t + 1);
+              if (x == NT - 1) umma_commit(&empty[(2 * t + 2) % C::kSlots]);
+            }
+          }
+        }
+      }
+      if (!ok) {
+        set_status(a.status, PL_ERR_TIMEOUT);
+        flags[0] = 1;
+      }
+      flags[2] = consumed;
+      umma_commit(fin);
+      if (!mbar_wait(fin, 0)) set_status(a.status, PL_ERR_TIMEOUT);
+    }
+  } else {
+    // -------------------------------------------------- softmax / epilogue
+    const int x = (warp - 2) / 4;
+    const int quad = warp & 3;
+    const int m = 32 * quad + lane;  // row of the tile == TMEM lane
+    const uint32_t row_tmem = tmem + ((uint32_t)(32 * quad) << 16);
+    const uint32_t s_tmem = row_tmem + (uint32_t)(x * kTreeN);
+    const uint32_t o_tmem = row_tmem + (uint32_t)(256 + x * 128);
+    const float sl2 = a.scale_log2;
+    bool ok = true;
+    int t = 0;
+    for (int seg = 0; ok && it.next(a, C::kRows); ++seg) {
+      const int row = it.rt * C::kRows + x * kTreeM + m;  // row of the request
+      const int tok = row / a.group;
+      const int head = it.kvh * a.group + row % a.group;
+      const bool row_ok = tok < it.r.n;
+      const int kv_len = it.r.kv_len, ctx = kv_len - it.r.n;  // drafted token j sits at position ctx + j
+      {
+        const bf16* src = a.q + (int64_t)(it.r.q0 + tok) * a.q_stride_t + (int64_t)head * a.q_stride_h;
+        uint8_t* qs = smem + C::kQOff + x * C::kQBytes;
+#pragma unroll
+        for (int u = 0; u < D / 8; ++u) {
+          const uint4 v = row_ok ? __ldg(reinterpret_cast<const uint4*>(src) + u) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(qs + (u >> 3) * C::kChunkBytes + tr_swz(m, u & 7)) = v;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&qready[x]);
+      }
+      const uint32_t* mrow = a.mask + (int64_t)(it.r.q0 + (row_ok ? tok : 0)) * a.mask_stride;
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int j = it.j0; j < it.j1; ++j, ++t) {
+        ok = mbar_wait(&sready[x], t & 1);
+        if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int kv0 = j * kTreeN;
+        const bool masked = kv0 + kTreeN > ctx;  // uniform over the CTA: the tile reaches the drafted tokens
+        uint32_t vm[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int rel = kv0 + 32 * c - ctx;  // drafted index of the column group's first position
+            uint32_t w = 0;
+            if (row_ok) {
+              if (rel >= 0)
+                w = tree_bits(mrow, a.words, rel);
+              else if (rel > -32)
+                w = (0xffffffffu >> (32 + rel)) | (tree_bits(mrow, a.words, 0) << (-rel));
+              else
+                w = 0xffffffffu;
+            }
+            const int live = kv_len - (kv0 + 32 * c);
+            vm[c] = live >= 32 ? w : (live <= 0 ? 0u : w & (0xffffffffu >> (32 - live)));
+          }
+        }
+        if (j > it.j0) ok = mbar_wait(&odone[x], (t - 1) & 1);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint8_t* pt = smem + C::kPOff + x * C::kPBytes;
+        // row maximum of the seen scores
+        float mx[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx[k] = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < kTreeN / 64; ++h) {
+          float v[64];
+          tmem_ld64(s_tmem + 64 * h, v);
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            const bool see = !masked || ((vm[2 * h + i / 32] >> (i & 31)) & 1u);
+            mx[i & 7] = fmaxf(mx[i & 7], see ? v[i] : -INFINITY);
+          }
+        }
+        float tmax =
+            fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+        tmax *= sl2;
+        const float m_new = fmaxf(m_run, tmax);
+        const bool rescale = m_run != -INFINITY && m_new > m_run + kTreeSlack;
+        const float m_use = (m_run == -INFINITY || rescale) ? m_new : m_run;
+        if (__any_sync(0xffffffffu, rescale)) {
+          const float alpha = rescale ? tr_exp2(m_run - m_use) : 1.f;
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            float v[16];
+            tmem_ld16(o_tmem + 16 * c, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] *= alpha;
+            tmem_st16_wait(o_tmem + 16 * c, v);
+          }
+          l_run *= alpha;
+        }
+        m_run = m_use;
+        const float nb = m_use == -INFINITY ? 0.f : -m_use;
+        float sm[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sm[k] = 0.f;
+#pragma unroll
+        for (int h = 0; h < kTreeN / 64; ++h) {
+          float v[64];
+          tmem_ld64(s_tmem + 64 * h, v);
+          uint32_t pk[32];
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) {
+            float p0 = tr_exp2(fmaf(v[i], sl2, nb));
+            float p1 = tr_exp2(fmaf(v[i + 1], sl2, nb));
+            if (masked) {
+              p0 = ((vm[2 * h + i / 32] >> (i & 31)) & 1u) ? p0 : 0.f;
+              p1 = ((vm[2 * h + i / 32] >> ((i + 1) & 31)) & 1u) ? p1 : 0.f;
+            }
+            sm[(i >> 1) & 7] += p0 + p1;
+            pk[i / 2] = pack_bf16x2(p0, p1);
+          }
+          uint8_t* chunk = pt + h * C::kChunkBytes;
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            *reinterpret_cast<uint4*>(chunk + tr_swz(m, u)) =
+                make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
+        }
+        l_run += ((sm[0] + sm[1]) + (sm[2] + sm[3])) + ((sm[4] + sm[5]) + (sm[6] + sm[7]));
+        // V rows past the last token hold whatever the pool had there, and a
+        // drafted token's V may hold inf or NaN that a row which masks the
+        // token must not meet (0 * NaN is NaN): tile 0's threads clear the
+        // former, and replace the latter's inf / NaN elements by zero and
+        // note their tokens, for the rows that do see them (epilogue).
+        if (masked && x == 0) {
+          const int item = 2 * t + 1;
+          if (mbar_wait(&full[item % C::kSlots], (item / C::kSlots) & 1)) {
+            uint8_t* vt = smem + C::kSlotOff + (item % C::kSlots) * C::kKVBytes;
+            const int r0 = max(ctx - kv0, 0), r_live = min(kTreeN, kv_len - kv0), units = C::kChunks * 8;
+            for (int idx = m; idx < (kTreeN - r0) * units; idx += 128) {
+              const int r = r0 + idx / units, hh = (idx / 8) % C::kChunks, u = idx % 8;
+              uint4* at = reinterpret_cast<uint4*>(vt + hh * C::kChunkBytes + r * 128 + u * 16);
+              if (r >= r_live) {
+                *at = make_uint4(0, 0, 0, 0);
+              } else {
+                uint4 v = *at;
+                uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+                bool hit = false;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  if ((w[k] & 0x7f80u) == 0x7f80u) { w[k] &= 0xffff0000u; hit = true; }
+                  if ((w[k] & 0x7f800000u) == 0x7f800000u) { w[k] &= 0x0000ffffu; hit = true; }
+                }
+                if (hit) {
+                  *at = v;
+                  atomicOr(any_bad, 1u);
+                }
+              }
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(&pready[x]);
+      }
+      if (!ok) {
+        set_status(a.status, PL_ERR_TIMEOUT);
+        flags[0] = 1;
+        break;
+      }
+      // ---- epilogue of the segment
+      ok = __all_sync(0xffffffffu, mbar_wait(&odone[x], (t - 1) & 1));
+      if (!ok) {
+        set_status(a.status, PL_ERR_TIMEOUT);
+        flags[0] = 1;
+        break;
+      }
+      tc_fence_after();
+      const bool whole = it.j0 == 0 && it.j1 == it.r.ntiles;
+      // any_bad is final: every P of the segment was waited for by its P.V
+      const bool check_bad = *reinterpret_cast<volatile uint32_t*>(any_bad) != 0 && it.j1 * kTreeN > ctx;
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+      const int slot = 2 * (int)blockIdx.x + (it.j0 > 0 ? 0 : 1);
+      bf16* dst = a.out + (int64_t)(it.r.q0 + tok) * a.out_stride_t + (int64_t)head * a.out_stride_h;
+      float* pdst = a.part_o + ((int64_t)slot * C::kRows + x * kTreeM + m) * D;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        float v[32];
+        tmem_ld32(o_tmem + 32 * c, v);
+        if (check_bad && row_ok) {
+          // the inf / NaN elements of the seen drafted tokens of this segment
+          const int64_t tstride = (int64_t)a.num_kv_heads * D;
+          for (int jj = max(0, max(-ctx, it.j0 * kTreeN - ctx)); jj < it.r.n && ctx + jj < it.j1 * kTreeN; ++jj) {
+            if (!(tree_bits(mrow, a.words, jj) & 1u)) continue;
+            const int pos = ctx + jj;
+            const int32_t pid = a.kv_indices[it.r.kv_begin + pos / PS];
+            if (pid < 0 || (int64_t)pid >= a.num_pages) continue;
+            const bf16* vrow =
+                a.kv + (((int64_t)pid * 2 + 1) * PS + pos % PS) * tstride + (int64_t)it.kvh * D + 32 * c;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float e = bf2f(vrow[i]);
+              if (!isfinite(e)) v[i] += e;
+            }
+          }
+        }
+        if (row_ok) {
+          if (whole) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) pk[i / 2] = pack_bf16x2(v[i] * inv, v[i + 1] * inv);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              reinterpret_cast<uint4*>(dst + 32 * c)[u] =
+                  make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              reinterpret_cast<float4*>(pdst + 32 * c)[u] = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+          }
+        }
+      }
+      if (row_ok) {
+        if (whole) {
+          if (a.lse != nullptr)
+            a.lse[(int64_t)(it.r.q0 + tok) * a.num_qo_heads + head] =
+                l_run == 0.f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
+        } else {
+          float* ml = a.part_ml + (int64_t)slot * 2 * C::kRows + x * kTreeM + m;
+          ml[0] = m_run;
+          ml[C::kRows] = l_run;
+        }
+      }
+      tc_fence_before();  // O was read: the next segment's first P.V (issued after its P arrives) may overwrite it
+    }
+  }
+
+  // ------------------------------------------------------------ teardown
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int issued = flags[1], consumed = flags[2];
+    for (int i = consumed; i < issued; ++i) (void)mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// Joins the partial states of the items that several CTAs shared: one warp
+// per (query token, head), the states weighted by 2^(m - max m).
+template <int D>
+__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int rows) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int tok_g = blockIdx.x;
+  // the request of this token
+  int req = a.batch;
+  for (int b0 = 0; b0 < a.batch && req == a.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const bool in = b < a.batch && a.qo_indptr[b] <= tok_g && tok_g < a.qo_indptr[b + 1];
+    const uint32_t hit = __ballot_sync(0xffffffffu, in);
+    if (hit != 0) req = b0 + __ffs(hit) - 1;
+  }
+  if (req == a.batch) return;
+  TreeReq r;
+  r.load(a, req, rows);
+  if (r.ntiles <= a.min_share || r.n == 0) return;  // never split
+  int64_t total, base;
+  tree_prefix(a, rows, req, total, base);
+  const int64_t share = tree_share(total, a.ctas, a.min_share);
+  for (int head = threadIdx.x / 32; head < a.num_qo_heads; head += blockDim.x / 32) {
+    const int row = (tok_g - r.q0) * a.group + head % a.group;
+    const int64_t w = base + ((int64_t)(head / a.group) * r.rts + row / rows) * r.ntiles;
+    const int m = row % rows;
+    const int64_t ca = w / share, cb = (w + r.ntiles - 1) / share;
+    if (ca == cb) continue;
+    auto slot = [&](int64_t c) { return 2 * c + (c == ca ? 1 : 0); };
+    float M = -INFINITY;
+    for (int64_t c = ca + lane; c <= cb; c += 32) {
+      const float v = a.part_ml[slot(c) * 2 * rows + m];
+      M = fmaxf(M, v);
+    }
+    M = warp_max(M);
+    constexpr int E = D / 32;
+    float acc[E], L = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int64_t c = ca; c <= cb; ++c) {
+      const float* ml = a.part_ml + slot(c) * 2 * rows + m;
+      const float mc = ml[0], lc = ml[rows];
+      const float wt = mc == -INFINITY ? 0.f : exp2f(mc - M);
+      const float* o = a.part_o + (slot(c) * rows + m) * D + lane * E;
+      float v[E];
+      if constexpr (E == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(o);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+      } else {
+        const float2 f = *reinterpret_cast<const float2*>(o);
+        v[0] = f.x; v[1] = f.y;
+      }
+      if (mc != -INFINITY) {  // a state that saw nothing holds no values
+        L += wt * lc;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += wt * v[e];
+      }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    bf16* dst = a.out + (int64_t)tok_g * a.out_stride_t + (int64_t)head * a.out_stride_h + lane * E;
+    if constexpr (E == 4) {
+      *reinterpret_cast<uint2*>(dst) =
+          make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+    } else {
+      *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    }
+    if (a.lse != nullptr && lane == 0)
+      a.lse[(int64_t)tok_g * a.num_qo_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+  }
+}
+
+// --------------------------------------------------------------- the tree
+// Ancestor-or-self bits of every drafted token: thread (token, word) walks
+// the parent chain in shared memory and keeps the bits of its word.
+__global__ void __launch_bounds__(256)
+    tree_mask_kernel(const int32_t* __restrict__ parents, const int32_t* __restrict__ qo_indptr,
+                     const int32_t* __restrict__ base_pos, int total_q, int words, uint32_t* __restrict__ mask,
+                     int64_t mask_stride, int32_t* __restrict__ depth, int32_t* __restrict__ positions,
+                     int32_t* status) {
+  __shared__ int16_t par[kTreeMaxTokens];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.x;
+  const int q0 = qo_indptr[b], q1 = qo_indptr[b + 1];
+  const int n = q1 - q0;
+  if (q0 < 0 || n < 0 || q1 > total_q || n > kTreeMaxTokens || n > 32 * words) {
+    if (threadIdx.x == 0) set_status(status, PL_ERR_INVALID_ARGUMENT);
+    return;
+  }
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    int p = parents[q0 + i];
+    if (p < -1 || p >= i) {  // not in topological order: the token stands alone
+      set_status(status, PL_ERR_INVALID_ARGUMENT);
+      p = -1;
+    }
+    par[i] = (int16_t)p;
+  }
+  __syncthreads();
+  for (int idx = blockIdx.y * blockDim.x + threadIdx.x; idx < n * words; idx += gridDim.y * blockDim.x) {
+    const int i = idx / words, w = idx % words;
+    uint32_t bits = 0;
+    int d = -1;
+    for (int j = i; j >= 0; j = par[j], ++d)
+      if ((j >> 5) == w) bits |= 1u << (j & 31);
+    mask[(int64_t)(q0 + i) * mask_stride + w] = bits;
+    if (w == 0) {
+      if (depth != nullptr) depth[q0 + i] = d;
+      if (positions != nullptr) positions[q0 + i] = (base_pos != nullptr ? base_pos[b] : 0) + d;
+    }
+  }
+}
+
+// Greedy acceptance: a drafted token is taken when it and all its ancestors
+// are what the model chose after their parents; the deepest taken token
+// (lowest index among equals) ends the kept path.
+__global__ void __launch_bounds__(128)
+    tree_accept_kernel(const int32_t* __restrict__ parents, const int64_t* __restrict__ tokens,
+                       const int64_t* __restrict__ targets, const int32_t* __restrict__ qo_indptr,
+                       const int32_t* __restrict__ base_pos, int total_q, int max_keep, int32_t* __restrict__ keep,
+                       int64_t keep_stride, int32_t* __restrict__ keep_count, int64_t* __restrict__ next_token,
+                       int32_t* status) {
+  __shared__ int16_t par[kTreeMaxTokens];
+  __shared__ uint8_t good[kTreeMaxTokens];
+  __shared__ int best_s;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.x;
+  const int q0 = qo_indptr[b], q1 = qo_indptr[b + 1];
+  const int n = q1 - q0;
+  if (q0 < 0 || n < 0 || q1 > total_q || n > kTreeMaxTokens) {
+    if (threadIdx.x == 0) {
+      set_status(status, PL_ERR_INVALID_ARGUMENT);
+      keep_count[b] = 0;
+      next_token[b] = -1;
+    }
+    return;
+  }
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    int p = parents[q0 + i];
+    bool ok = true;
+    if (p < -1 || p >= i) {  // not in topological order: never taken
+      set_status(status, PL_ERR_INVALID_ARGUMENT);
+      p = -1;
+      ok = false;
+    }
+    par[i] = (int16_t)p;
+    good[i] = ok && (p < 0 || tokens[q0 + i] == targets[q0 + p]);
+  }
+  if (threadIdx.x == 0) best_s = 0;
+  __syncthreads();
+  // key: depth + 1 of a taken token, then the lower index
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    int d = 0, j = i;
+    while (j >= 0 && good[j]) {
+      ++d;
+      j = par[j];
+    }
+    if (j < 0) atomicMax(&best_s, d * kTreeMaxTokens + (kTreeMaxTokens - 1 - i));
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int key = best_s;
+    int count = key / kTreeMaxTokens;
+    const int best = kTreeMaxTokens - 1 - key % kTreeMaxTokens;
+    if (count > max_keep) {
+      set_status(status, PL_ERR_INVALID_ARGUMENT);
+      count = 0;
+    }
+    next_token[b] = count > 0 ? targets[q0 + best] : -1;
+    keep_count[b] = count;
+    int j = best;
+    for (int i = count - 1; i >= 0; --i, j = par[j]) keep[(int64_t)b * keep_stride + i] = base_pos[b] + j;
+    best_s = count;
+  }
+  __syncthreads();
+  for (int i = best_s + threadIdx.x; i < max_keep; i += blockDim.x) keep[(int64_t)b * keep_stride + i] = -1;
+}
+
+}  // namespace pl
+
+// =================================================================== host
+namespace {
+
+// Two row tiles per CTA when the requests average more rows than one holds.
+bool tree_two_tiles(int total_q, int batch, int group) {
+  return (int64_t)total_q * group > (int64_t)batch * pl::kTreeM;
+}
+
+constexpr int kTreeMinShare = 2;
+
+template <int D, int NT>
+int32_t launch_tree(const CUtensorMap& map, const pl::TreeArgs& a, bool merge, void* stream) {
+  using C = pl::TreeCfg<D, NT>;
+  auto kern = pl::paged_tree_kernel<D, NT>;
+  int32_t st = pl_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
+  if (st != PL_OK) return st;
+  st = pl_host::launch_pdl(kern, dim3(a.ctas), dim3(C::kThreads), C::kSmemBytes, stream, map, a);
+  if (st != PL_OK || !merge) return st;
+  return pl_host::launch_pdl(pl::tree_merge_kernel<D>, dim3(a.total_q), dim3(256), 0, stream, a, (int)C::kRows);
+}
+
+}  // namespace
+
+extern "C" int64_t pl_tree_workspace_bytes(int32_t batch, int32_t total_q, int32_t num_qo_heads, int32_t num_kv_heads,
+                                           int32_t head_dim) {
+  if (batch <= 0 || total_q <= 0 || num_kv_heads <= 0 || num_qo_heads <= 0 || num_qo_heads % num_kv_heads != 0 ||
+      head_dim <= 0)
+    return 0;
+  const int sms = pl_host::sm_count();
+  const int64_t rows = pl::kTreeM * (tree_two_tiles(total_q, batch, num_qo_heads / num_kv_heads) ? 2 : 1);
+  return 2 * (int64_t)(sms > 0 ? sms : 148) * rows * (head_dim + 2) * 4;
+}
+
+extern "C" int32_t pl_paged_tree_attention(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv_cache, int64_t num_pages,
+    const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* kv_last_page_len,
+    int64_t total_pages, const int32_t* tree_mask, int64_t mask_stride, int32_t mask_words, int32_t batch,
+    int32_t total_q, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float sm_scale,
+    void* out, int64_t out_stride_t, int64_t out_stride_h, float* out_lse, void* workspace, int64_t workspace_bytes,
+    int32_t* status_dev, void* stream) {
+  if (q == nullptr || kv_cache == nullptr || qo_indptr == nullptr || kv_indptr == nullptr || kv_indices == nullptr ||
+      kv_last_page_len == nullptr || tree_mask == nullptr || out == nullptr || batch < 0 || total_q < 0 ||
+      num_pages <= 0 || num_pages > 0x3FFFFFFF || total_pages < 0 || mask_words <= 0 || mask_stride < mask_words ||
+      num_kv_heads <= 0 || num_qo_heads <= 0 || num_qo_heads % num_kv_heads != 0 || !(sm_scale > 0.f))
+    return PL_ERR_INVALID_ARGUMENT;
+  const int group = num_qo_heads / num_kv_heads;
+  if (group > pl::kTreeM || (head_dim != 64 && head_dim != 128) ||
+      (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) || num_kv_heads > 65535)
+    return PL_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(kv_cache) & 15) != 0 || (reinterpret_cast<uintptr_t>(q) & 15) != 0 ||
+      (reinterpret_cast<uintptr_t>(out) & 15) != 0 || (q_stride_t % 8) != 0 || (q_stride_h % 8) != 0 ||
+      (out_stride_t % 8) != 0 || (out_stride_h % 8) != 0)
+    return PL_ERR_INVALID_ARGUMENT;
+  if (batch == 0 || total_q == 0) return PL_OK;
+  // no request has more than total_pages pages: below kTreeMinShare tiles nothing is split
+  const bool merge = total_pages * page_size > (int64_t)kTreeMinShare * pl::kTreeN;
+  if (merge && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
+                workspace_bytes < pl_tree_workspace_bytes(batch, total_q, num_qo_heads, num_kv_heads, head_dim)))
+    return PL_ERR_WORKSPACE_TOO_SMALL;
+
+  CUtensorMap map;
+  int32_t st = pl_host::kv_tensor_map(kv_cache, num_pages, num_kv_heads, head_dim, page_size, &map);
+  if (st != PL_OK) return st;
+  const int sms = pl_host::sm_count();
+  if (sms <= 0) return PL_ERR_NO_DEVICE;
+
+  const bool two = tree_two_tiles(total_q, batch, group);
+  pl::TreeArgs a;
+  a.q = static_cast<const pl::bf16*>(q);
+  a.kv = static_cast<const pl::bf16*>(kv_cache);
+  a.q_stride_t = q_stride_t;
+  a.q_stride_h = q_stride_h;
+  a.qo_indptr = qo_indptr;
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.kv_last = kv_last_page_len;
+  a.mask = reinterpret_cast<const uint32_t*>(tree_mask);
+  a.mask_stride = mask_stride;
+  a.num_pages = num_pages;
+  a.total_pages = total_pages;
+  a.words = mask_words;
+  a.batch = batch;
+  a.total_q = total_q;
+  a.num_qo_heads = num_qo_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.group = group;
+  a.page_size = page_size;
+  a.min_share = kTreeMinShare;
+  a.ctas = sms;
+  a.scale_log2 = sm_scale * pl::kLog2e;
+  a.out = static_cast<pl::bf16*>(out);
+  a.out_stride_t = out_stride_t;
+  a.out_stride_h = out_stride_h;
+  a.lse = out_lse;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = workspace == nullptr ? nullptr : a.part_o + 2 * (int64_t)sms * pl::kTreeM * (two ? 2 : 1) * head_dim;
+  a.status = status_dev;
+  if (head_dim == 128) return two ? launch_tree<128, 2>(map, a, merge, stream) : launch_tree<128, 1>(map, a, merge, stream);
+  return two ? launch_tree<64, 2>(map, a, merge, stream) : launch_tree<64, 1>(map, a, merge, stream);
+}
+
+extern "C" int32_t pl_tree_mask(const int32_t* parents, const int32_t* qo_indptr, const int32_t* base_positions,
+                                int32_t batch, int32_t total_q, int32_t mask_words, int32_t* mask, int64_t mask_stride,
+                                int32_t* depth, int32_t* positions, int32_t* status_dev, void* stream) {
+  if (parents == nullptr || qo_indptr == nullptr || mask == nullptr || batch < 0 || total_q < 0 || mask_words <= 0 ||
+      mask_stride < mask_words)
+    return PL_ERR_INVALID_ARGUMENT;
+  if (batch == 0 || total_q == 0) return PL_OK;
+  const int64_t per = ((int64_t)total_q * mask_words + 255) / 256;
+  const int gy = (int)(per < 1 ? 1 : (per > 16 ? 16 : per));
+  return pl_host::launch_pdl(pl::tree_mask_kernel, dim3(batch, gy), dim3(256), 0, stream, parents, qo_indptr,
+                             base_positions, (int)total_q, (int)mask_words, reinterpret_cast<uint32_t*>(mask),
+                             mask_stride, depth, positions, status_dev);
+}
+
+extern "C" int32_t pl_tree_accept(const int32_t* parents, const int64_t* tokens, const int64_t* targets,
+                                  const int32_t* qo_indptr, const int32_t* base_positions, int32_t batch,
+                                  int32_t total_q, int32_t max_keep, int32_t* keep, int64_t keep_stride,
+                                  int32_t* keep_count, int64_t* next_token, int32_t* status_dev, void* stream) {
+  if (parents == nullptr || tokens == nullptr || targets == nullptr || qo_indptr == nullptr ||
+      base_positions == nullptr || keep == nullptr || keep_count == nullptr || next_token == nullptr || batch < 0 ||
+      total_q < 0 || max_keep <= 0 || keep_stride < max_keep)
+    return PL_ERR_INVALID_ARGUMENT;
+  if (batch == 0) return PL_OK;
+  return pl_host::launch_pdl(pl::tree_accept_kernel, dim3(batch), dim3(128), 0, stream, parents, tokens, targets,
+                             qo_indptr, base_positions, (int)total_q, (int)max_keep, keep, keep_stride, keep_count,
+                             next_token, status_dev);
+}

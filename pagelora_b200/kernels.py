@@ -792,3 +792,331 @@ def argmax(logits: torch.Tensor, out: torch.Tensor, workspace: torch.Tensor | No
     call("pl_argmax", ptr(logits), _row_stride(logits, "logits"), int(vocab), int(t), ptr(out), ptr(workspace),
          int(workspace.numel()), stream_handle())
     return out
+
+
+# ----------------------------------------------------- drafted-token trees
+def _need_pool(kv_cache: torch.Tensor) -> None:
+    _need(kv_cache, torch.bfloat16, "kv_cache")
+    if kv_cache.dim() != 5 or kv_cache.size(1) != 2 or not kv_cache.is_contiguous():
+        raise ValueError("kv_cache must be a contiguous [pages, 2, page_size, kv_heads, head_dim] tensor")
+
+
+def _need_vec(t: torch.Tensor, name: str, dtype: torch.dtype = torch.int32, size: int | None = None) -> None:
+    _need(t, dtype, name)
+    if not t.is_contiguous() or (size is not None and t.numel() < size):
+        raise ValueError(f"{name} must be contiguous" + ("" if size is None else f" with at least {size} entries"))
+
+
+def _workspace(workspace: torch.Tensor | None, need: int, device: torch.device) -> torch.Tensor:
+    return torch.empty(max(need, 16), dtype=torch.uint8, device=device) if workspace is None else workspace
+
+
+def tree_mask(parents: torch.Tensor, qo_indptr: torch.Tensor, words: int, *, base_positions: torch.Tensor | None = None,
+              mask: torch.Tensor | None = None, depth: torch.Tensor | None = None,
+              positions: torch.Tensor | None = None, status: torch.Tensor | None = None
+              ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Ancestor-or-self bits of drafted tokens (pl_tree_mask): ``parents``
+    int32 [total_q], index in the request, -1 for the context.  Returns
+    (mask int32 [total_q, words], depth int32 [total_q]); ``positions``
+    receives ``base_positions[request] + depth``."""
+
+    _need_cuda(parents, qo_indptr, base_positions, mask, depth, positions)
+    total = parents.numel()
+    batch = qo_indptr.numel() - 1
+    _need_vec(parents, "parents")
+    _need_vec(qo_indptr, "qo_indptr")
+    if words < 1:
+        raise ValueError("words must be at least 1")
+    if mask is None:
+        mask = torch.empty(total, words, dtype=torch.int32, device=parents.device)
+    if depth is None:
+        depth = torch.empty(total, dtype=torch.int32, device=parents.device)
+    _need(mask, torch.int32, "mask")
+    if mask.shape != (total, words) or (words > 1 and mask.stride(1) != 1):
+        raise ValueError("mask must be [total_q, words] with contiguous rows")
+    for name, t, n in (("depth", depth, total), ("positions", positions, total), ("base_positions", base_positions, batch)):
+        if t is not None:
+            _need_vec(t, name, size=n)
+    call("pl_tree_mask", ptr(parents), ptr(qo_indptr), ptr(base_positions), int(batch), int(total), int(words),
+         ptr(mask), max(mask.stride(0), words), ptr(depth), ptr(positions), ptr(status), stream_handle())
+    return mask, depth
+
+
+def tree_workspace_bytes(batch: int, total_q: int, num_qo_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """Workspace of :func:`paged_tree_attention` (no initialisation)."""
+
+    return int(_capi.load_library().pl_tree_workspace_bytes(int(batch), int(total_q), int(num_qo_heads),
+                                                            int(num_kv_heads), int(head_dim)))
+
+
+def paged_tree_attention(
+    q: torch.Tensor,
+    kv_cache: torch.Tensor,
+    qo_indptr: torch.Tensor,
+    kv_indptr: torch.Tensor,
+    kv_indices: torch.Tensor,
+    kv_last_page_len: torch.Tensor,
+    tree_mask: torch.Tensor,
+    *,
+    sm_scale: float | None = None,
+    out: torch.Tensor | None = None,
+    out_lse: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of drafted-token trees over the paged cache
+    (pl_paged_tree_attention): q [total_q, Hq, D] bf16, request b owns tokens
+    qo_indptr[b]:qo_indptr[b+1], whose K/V are the last of its cached
+    positions; ``tree_mask`` int32 [total_q, words] from :func:`tree_mask` or
+    any bits.  ``out`` bf16 like q, ``out_lse`` fp32 [total_q, Hq]."""
+
+    _need_cuda(q, kv_cache, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, tree_mask, out, out_lse, workspace)
+    _need(q, torch.bfloat16, "q")
+    _need_pool(kv_cache)
+    if q.dim() != 3 or q.stride(-1) != 1:
+        raise ValueError("q must be [tokens, qo_heads, head_dim] with unit last stride")
+    total_q, hq, d = q.shape
+    num_pages, _, page_size, hkv, d2 = kv_cache.shape
+    if d2 != d:
+        raise ValueError("q and kv_cache head_dim differ")
+    batch = qo_indptr.numel() - 1
+    _need_vec(qo_indptr, "qo_indptr")
+    _need_vec(kv_indptr, "kv_indptr", size=batch + 1)
+    _need_vec(kv_indices, "kv_indices")
+    _need_vec(kv_last_page_len, "kv_last_page_len", size=batch)
+    _need(tree_mask, torch.int32, "tree_mask")
+    if tree_mask.dim() != 2 or tree_mask.shape[0] != total_q or tree_mask.stride(1) != 1:
+        raise ValueError("tree_mask must be [total_q, words] with contiguous rows")
+    words = tree_mask.shape[1]
+    if out is None:
+        out = torch.empty_like(q)
+    _need(out, torch.bfloat16, "out")
+    if out.shape != q.shape or out.stride(-1) != 1:
+        raise ValueError("out must have q's shape and unit last stride")
+    if out_lse is not None:
+        _need_vec(out_lse, "out_lse", torch.float32, total_q * hq)
+    workspace = _workspace(workspace, tree_workspace_bytes(batch, total_q, hq, hkv, d), q.device)
+    scale = (1.0 / math.sqrt(d)) if sm_scale is None else float(sm_scale)
+    call("pl_paged_tree_attention", ptr(q), q.stride(0), q.stride(1), ptr(kv_cache), num_pages, ptr(qo_indptr),
+         ptr(kv_indptr), ptr(kv_indices), ptr(kv_last_page_len), kv_indices.numel(), ptr(tree_mask),
+         max(tree_mask.stride(0), words), words, batch, total_q, hq, hkv, d, page_size, scale, ptr(out), out.stride(0),
+         out.stride(1), ptr(out_lse), ptr(workspace), workspace.numel() * workspace.element_size(), ptr(status),
+         stream_handle())
+    return out
+
+
+def tree_accept(parents: torch.Tensor, tokens: torch.Tensor, targets: torch.Tensor, qo_indptr: torch.Tensor,
+                base_positions: torch.Tensor, *, keep: torch.Tensor, keep_count: torch.Tensor,
+                next_token: torch.Tensor, status: torch.Tensor | None = None) -> None:
+    """Longest path of drafted ``tokens`` (int64 [total_q]) that the model's
+    choices ``targets`` (int64 [total_q], the choice after each drafted token)
+    confirm (pl_tree_accept): ``keep`` int32 [batch, max_keep] receives
+    base_positions[b] + index of its tokens, ``keep_count`` int32 [batch] their
+    number, ``next_token`` int64 [batch] the choice after it."""
+
+    _need_cuda(parents, tokens, targets, qo_indptr, base_positions, keep, keep_count, next_token)
+    total, batch = parents.numel(), qo_indptr.numel() - 1
+    _need_vec(parents, "parents")
+    _need_vec(qo_indptr, "qo_indptr")
+    for name, t in (("tokens", tokens), ("targets", targets)):
+        _need_vec(t, name, torch.int64, total)
+    _need_vec(base_positions, "base_positions", size=batch)
+    _need_vec(keep_count, "keep_count", size=batch)
+    _need_vec(next_token, "next_token", torch.int64, batch)
+    _need(keep, torch.int32, "keep")
+    if keep.dim() != 2 or keep.shape[0] < batch or keep.stride(1) != 1:
+        raise ValueError("keep must be [batch, max_keep] with contiguous rows")
+    call("pl_tree_accept", ptr(parents), ptr(tokens), ptr(targets), ptr(qo_indptr), ptr(base_positions), batch, total,
+         keep.shape[1], ptr(keep), max(keep.stride(0), keep.shape[1]), ptr(keep_count), ptr(next_token), ptr(status),
+         stream_handle())
+
+
+# --------------------------------------------------------- pages of a cache
+def _pool_tables(refcount: torch.Tensor, row_pages: torch.Tensor, row_num_pages: torch.Tensor,
+                 last_page_len: torch.Tensor) -> tuple:
+    """Checked arguments (refcount .. row capacity) of the page operations."""
+
+    _need_cuda(refcount, row_pages, row_num_pages, last_page_len)
+    _need_vec(refcount, "refcount")
+    _need_vec(row_pages, "row_pages")
+    if row_pages.dim() != 2:
+        raise ValueError("row_pages must be [rows, capacity]")
+    rows, cap = row_pages.shape
+    _need_vec(row_num_pages, "row_num_pages", size=rows)
+    _need_vec(last_page_len, "last_page_len", size=rows)
+    return (ptr(refcount), refcount.numel(), ptr(row_pages), ptr(row_num_pages), ptr(last_page_len), rows, cap)
+
+
+def _pool_data(pool: torch.Tensor, refcount: torch.Tensor) -> tuple[tuple, int]:
+    """Checked (base, layer stride, layers, token bytes) of a pool
+    [layers, pages, 2, page_size, ...] (any dtype) and its page size."""
+
+    _need_cuda(pool)
+    if pool.dim() < 5 or pool.size(2) != 2 or pool.size(1) != refcount.numel():
+        raise ValueError("pool must be [layers, pages, 2, page_size, ...] with one refcount per page")
+    layer = pool[0]
+    if not layer.is_contiguous() or pool.stride(0) < layer.numel():
+        raise ValueError("every layer of the pool must be contiguous")
+    size = pool.element_size()
+    token = layer.numel() // (layer.size(0) * 2 * layer.size(2)) * size
+    return (ptr(pool), pool.stride(0) * size, pool.size(0), token), layer.size(2)
+
+
+def page_release(refcount: torch.Tensor, row_pages: torch.Tensor, row_num_pages: torch.Tensor,
+                 last_page_len: torch.Tensor, rows: torch.Tensor, status: torch.Tensor | None = None) -> None:
+    """The rows ``rows`` (int32) give their pages back and become empty (pl_page_release)."""
+
+    tables = _pool_tables(refcount, row_pages, row_num_pages, last_page_len)
+    _need_cuda(rows)
+    _need_vec(rows, "rows")
+    call("pl_page_release", *tables, ptr(rows), rows.numel(), ptr(status), stream_handle())
+
+
+def page_reserve(refcount: torch.Tensor, row_pages: torch.Tensor, row_num_pages: torch.Tensor,
+                 last_page_len: torch.Tensor, tok_indptr: torch.Tensor, page_size: int, *, slot_page: torch.Tensor,
+                 slot_offset: torch.Tensor, positions: torch.Tensor | None = None,
+                 out_indptr: torch.Tensor | None = None, out_indices: torch.Tensor | None = None,
+                 status: torch.Tensor | None = None) -> None:
+    """Row r grows by tok_indptr[r+1] - tok_indptr[r] tokens (pl_page_reserve):
+    their slots go to ``slot_page`` / ``slot_offset`` (one entry per token), the
+    new page table to ``out_indptr`` / ``out_indices`` when given."""
+
+    tables = _pool_tables(refcount, row_pages, row_num_pages, last_page_len)
+    _need_cuda(tok_indptr, slot_page, slot_offset, positions, out_indptr, out_indices)
+    rows, total = row_pages.shape[0], slot_page.numel()
+    _need_vec(tok_indptr, "tok_indptr", size=rows + 1)
+    _need_vec(slot_page, "slot_page")
+    _need_vec(slot_offset, "slot_offset", size=total)
+    for name, t, n in (("positions", positions, total), ("out_indptr", out_indptr, rows + 1),
+                       ("out_indices", out_indices, 0)):
+        if t is not None:
+            _need_vec(t, name, size=n)
+    call("pl_page_reserve", *tables, int(page_size), ptr(tok_indptr), total, ptr(slot_page), ptr(slot_offset),
+         ptr(positions), ptr(out_indptr), ptr(out_indices), 0 if out_indices is None else out_indices.numel(),
+         ptr(status), stream_handle())
+
+
+def page_fork(pool: torch.Tensor, refcount: torch.Tensor, row_pages: torch.Tensor, row_num_pages: torch.Tensor,
+              last_page_len: torch.Tensor, src_rows: torch.Tensor, dst_rows: torch.Tensor, *,
+              workspace: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
+    """Empty row dst_rows[i] becomes a copy of src_rows[i] (pl_page_fork): full
+    pages are shared, the partial last page is copied in every layer of
+    ``pool`` [layers, pages, 2, page_size, ...]."""
+
+    tables = _pool_tables(refcount, row_pages, row_num_pages, last_page_len)
+    data, page_size = _pool_data(pool, refcount)
+    _need_cuda(src_rows, dst_rows, workspace)
+    n = src_rows.numel()
+    _need_vec(src_rows, "src_rows")
+    _need_vec(dst_rows, "dst_rows", size=n)
+    if dst_rows.numel() != n:
+        raise ValueError("src_rows and dst_rows differ in length")
+    workspace = _workspace(workspace, int(_capi.load_library().pl_page_fork_workspace_bytes(n)), pool.device)
+    call("pl_page_fork", *data, *tables, page_size, ptr(src_rows), ptr(dst_rows), n, ptr(workspace),
+         workspace.numel() * workspace.element_size(), ptr(status), stream_handle())
+
+
+def cache_compact(pool: torch.Tensor, refcount: torch.Tensor, row_pages: torch.Tensor, row_num_pages: torch.Tensor,
+                  last_page_len: torch.Tensor, keep_from: torch.Tensor, keep: torch.Tensor, keep_count: torch.Tensor,
+                  *, workspace: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
+    """Row r keeps its first ``keep_from[r]`` tokens and the ascending
+    positions ``keep[r, :keep_count[r]]``, moved together in every layer of
+    ``pool`` [layers, pages, 2, page_size, ...] (pl_cache_compact)."""
+
+    tables = _pool_tables(refcount, row_pages, row_num_pages, last_page_len)
+    data, page_size = _pool_data(pool, refcount)
+    _need_cuda(keep_from, keep, keep_count, workspace)
+    rows, cap = row_pages.shape
+    _need_vec(keep_from, "keep_from", size=rows)
+    _need_vec(keep_count, "keep_count", size=rows)
+    _need(keep, torch.int32, "keep")
+    if keep.dim() != 2 or keep.shape[0] < rows or (keep.shape[1] > 1 and keep.stride(1) != 1):
+        raise ValueError("keep must be [rows, max_keep] with contiguous rows")
+    workspace = _workspace(workspace, int(_capi.load_library().pl_cache_compact_workspace_bytes(rows, cap)),
+                           pool.device)
+    call("pl_cache_compact", *data, *tables, page_size, ptr(keep_from), ptr(keep),
+         max(keep.stride(0), keep.shape[1]), ptr(keep_count), keep.shape[1], ptr(workspace),
+         workspace.numel() * workspace.element_size(), ptr(status), stream_handle())
+
+
+# -------------------------------------------------------- sparse attention
+def page_bounds(kv_cache: torch.Tensor, page_ids: torch.Tensor, bounds: torch.Tensor, bound_scale: torch.Tensor, *,
+                page_len: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
+    """int8 bounds [pages, Hkv, 2, D] and scale [pages, Hkv] of the keys of
+    pages ``page_ids`` (pl_page_bounds); ``page_len``: tokens in each (all)."""
+
+    _need_cuda(kv_cache, page_ids, bounds, bound_scale, page_len)
+    _need_pool(kv_cache)
+    num_pages, _, page_size, hkv, d = kv_cache.shape
+    n = page_ids.numel()
+    _need_vec(page_ids, "page_ids")
+    _need_vec(bounds, "bounds", torch.int8, num_pages * hkv * 2 * d)
+    _need_vec(bound_scale, "bound_scale", torch.float32, num_pages * hkv)
+    if page_len is not None:
+        _need_vec(page_len, "page_len", size=n)
+    call("pl_page_bounds", ptr(kv_cache), num_pages, hkv, d, page_size, ptr(page_ids), ptr(page_len), n, ptr(bounds),
+         ptr(bound_scale), ptr(status), stream_handle())
+
+
+def paged_sparse_decode(
+    q: torch.Tensor,
+    kv_cache: torch.Tensor,
+    indptr: torch.Tensor,
+    indices: torch.Tensor,
+    last_page_len: torch.Tensor,
+    bounds: torch.Tensor,
+    bound_scale: torch.Tensor,
+    *,
+    num_select: int,
+    sink_pages: int = 1,
+    recent_pages: int = 1,
+    max_pages: int | None = None,
+    sm_scale: float | None = None,
+    out: torch.Tensor | None = None,
+    out_lse: torch.Tensor | None = None,
+    selected: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Paged decode over the ``num_select`` pages per (row, kv head) that the
+    bounds' score selects (pl_paged_sparse_decode): the first ``sink_pages``,
+    the last ``recent_pages`` and the highest scores.  q [B, Hq, D] bf16;
+    ``max_pages``: pages of the longest row (default: all of ``indices``);
+    ``selected`` int32 [B, Hkv, num_select] receives the taken pages."""
+
+    _need_cuda(q, kv_cache, indptr, indices, last_page_len, bounds, bound_scale, out, out_lse, selected, workspace)
+    _need(q, torch.bfloat16, "q")
+    _need_pool(kv_cache)
+    if q.dim() != 3 or q.stride(-1) != 1:
+        raise ValueError("q must be [batch, qo_heads, head_dim] with unit last stride")
+    batch, hq, d = q.shape
+    num_pages, _, page_size, hkv, d2 = kv_cache.shape
+    if d2 != d:
+        raise ValueError("q and kv_cache head_dim differ")
+    _need_vec(indptr, "indptr", size=batch + 1)
+    _need_vec(indices, "indices")
+    _need_vec(last_page_len, "last_page_len", size=batch)
+    _need_vec(bounds, "bounds", torch.int8, num_pages * hkv * 2 * d)
+    _need_vec(bound_scale, "bound_scale", torch.float32, num_pages * hkv)
+    if out is None:
+        out = torch.empty_like(q)
+    _need(out, torch.bfloat16, "out")
+    if out.shape != q.shape or out.stride(-1) != 1:
+        raise ValueError("out must have q's shape and unit last stride")
+    if out_lse is not None:
+        _need_vec(out_lse, "out_lse", torch.float32, batch * hq)
+    if selected is None:
+        selected = torch.empty(batch, hkv, max(num_select, 1), dtype=torch.int32, device=q.device)
+    _need_vec(selected, "selected", size=batch * hkv * num_select)
+    if max_pages is None:
+        max_pages = indices.numel()
+    if max_pages > num_select and workspace is None:
+        workspace = _workspace(None, int(_capi.load_library().pl_sparse_workspace_bytes(batch, hkv, int(max_pages))),
+                               q.device)
+    scale = (1.0 / math.sqrt(d)) if sm_scale is None else float(sm_scale)
+    call("pl_paged_sparse_decode", ptr(q), q.stride(0), q.stride(1), ptr(kv_cache), num_pages, ptr(indptr),
+         ptr(indices), ptr(last_page_len), indices.numel(), int(max_pages), ptr(bounds), ptr(bound_scale), batch, hq,
+         hkv, d, page_size, scale, int(num_select), int(sink_pages), int(recent_pages), ptr(out), out.stride(0),
+         out.stride(1), ptr(out_lse), ptr(selected), ptr(workspace),
+         0 if workspace is None else workspace.numel() * workspace.element_size(), ptr(status), stream_handle())
+    return out
