@@ -19,8 +19,9 @@
 // and tree_merge_kernel joins them.  Within a segment:
 //   warp 0     TMA producer: K_0, V_0, K_1, V_1, ... through a ring of tiles;
 //   warp 1     one lane issues tcgen05.mma: S = Q.K^T into TMEM, O += P.V;
-//   warps 2..  softmax, one thread per row: scores from TMEM, mask, online
-//              softmax (log2 domain), P (bf16) as the swizzled A operand.
+//   warps 2..  softmax, two threads per row (half of the tile's positions
+//              each): scores from TMEM, mask, online softmax (log2 domain),
+//              P (bf16) into the scores' TMEM columns as the A operand.
 // P is rounded to bf16 as the tensor core's operand; l sums the unrounded
 // fp32 values.  Waits are bounded: on expiry the kernel records
 // PL_ERR_TIMEOUT, drains its copies and returns.
@@ -56,26 +57,28 @@ struct TreeArgs {
 
 template <int D, int NT>
 struct TreeCfg {
-  static constexpr int kThreads = 64 + 128 * NT;
+  static constexpr int kSoftmaxThreads = 256 * NT;  // two per row
+  static constexpr int kThreads = 64 + kSoftmaxThreads;
   static constexpr int kRows = kTreeM * NT;
   static constexpr int kChunks = D / 64;
   static constexpr int kChunkBytes = kTreeM * 128;
   static constexpr int kQBytes = kChunks * kChunkBytes;
   static constexpr int kKVBytes = kChunks * kChunkBytes;
-  static constexpr int kPBytes = 2 * kChunkBytes;
-  static constexpr int kSlots = NT == 1 ? 5 : 3;
+  static constexpr int kSlots = 7 - NT;  // fills the shared memory at D = 128
   static constexpr int kQOff = 0;
-  static constexpr int kPOff = kQOff + NT * kQBytes;
-  static constexpr int kSlotOff = kPOff + NT * kPBytes;
-  static constexpr int kBarOff = kSlotOff + kSlots * kKVBytes;
+  static constexpr int kSlotOff = kQOff + NT * kQBytes;
+  static constexpr int kPairOff = kSlotOff + kSlots * kKVBytes;  // [NT][128] words shared by a row's two threads
+  static constexpr int kBarOff = kPairOff + kRows * 4;
   static constexpr int kNumBars = 2 * kSlots + 8 + 1;  // full empty | s[2] p[2] o[2] q[2] | fin
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
-  static constexpr int kSmemBytes = 1024 + kMiscOff + 96;
-  static constexpr int kTmemCols = 512;  // S_x at 128 x, O_x at 256 + 128 x
+  static constexpr int kSmemBytes = 1024 + kMiscOff + 80;
+  static constexpr int kTmemCols = 512;  // S_x at 128 x (P_x in its place), O_x at 256 + 128 x
   static_assert(kSmemBytes <= 232448, "tree tiles exceed the shared-memory limit");
 };
 
+// Byte offset of 16-byte unit `u` of row `r` in a 128B-swizzled K-major chunk.
 __device__ __forceinline__ uint32_t tr_swz(int r, int u) { return r * 128 + ((u ^ (r & 7)) << 4); }
+// 2^x on the multi-function unit (PTX ex2.approx, flush-to-zero); x = -inf gives 0.
 __device__ __forceinline__ float tr_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -217,9 +220,9 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   uint64_t* full = bars;
   uint64_t* empty = bars + C::kSlots;
   uint64_t* sready = bars + 2 * C::kSlots;  // [2] S_x in TMEM
-  uint64_t* pready = sready + 2;            // [2] P_x staged (128 arrivals)
+  uint64_t* pready = sready + 2;            // [2] P_x in TMEM (256 arrivals)
   uint64_t* odone = sready + 4;             // [2] O_x += P_x.V finished
-  uint64_t* qready = sready + 6;            // [2] Q_x staged (128 arrivals)
+  uint64_t* qready = sready + 6;            // [2] Q_x staged (256 arrivals)
   uint64_t* fin = sready + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
   volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, issued, consumed
@@ -235,9 +238,9 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&sready[x], 1);
-      mbar_init(&pready[x], 128);
+      mbar_init(&pready[x], 256);
       mbar_init(&odone[x], 1);
-      mbar_init(&qready[x], 128);
+      mbar_init(&qready[x], 256);
     }
     mbar_init(fin, 1);
     flags[0] = flags[1] = flags[2] = 0;
@@ -347,13 +350,13 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         umma_commit(&sready[x]);
       };
       auto issue_pv = [&](int x, int t, bool first) {
-        const uint32_t pb = smem_u32(smem + C::kPOff + x * C::kPBytes);
         const uint32_t vb = smem_u32(smem + C::kSlotOff + ((2 * t + 1) % C::kSlots) * C::kKVBytes);
 #pragma unroll
         for (int kk = 0; kk < kTreeN / 16; ++kk)
-          umma_bf16(tmem + (uint32_t)(256 + x * 128), umma_desc_k_sw128(pb + (kk >> 2) * C::kChunkBytes + 32 * (kk & 3)),
-                    umma_desc_mn_sw128(vb + kk * 16 * 128, C::kChunkBytes, 1024), idesc_o,
-                    (!first || kk > 0) ? 1u : 0u);
+          // P of positions 0..63 starts at S_x's first column, of 64..127 at its 64th
+          umma_bf16_ts(tmem + (uint32_t)(256 + x * 128), tmem + (uint32_t)(x * kTreeN + (kk >> 2) * 64 + (kk & 3) * 8),
+                       umma_desc_mn_sw128(vb + kk * 16 * 128, C::kChunkBytes, 1024), idesc_o,
+                       (!first || kk > 0) ? 1u : 0u);
         umma_commit(&odone[x]);
       };
       bool ok = true;
@@ -395,12 +398,20 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
     }
   } else {
     // -------------------------------------------------- softmax / epilogue
-    const int x = (warp - 2) / 4;
+    // Warps 2.. : per row tile x two groups of four warps; group `half` has
+    // the positions 64 half .. 64 half + 63 of every K/V tile, so a row's two
+    // threads share its running maximum (through shared memory) and keep a
+    // sum each.
+    const int x = (warp - 2) / 8;
+    const int half = ((warp - 2) / 4) & 1;
     const int quad = warp & 3;
     const int m = 32 * quad + lane;  // row of the tile == TMEM lane
     const uint32_t row_tmem = tmem + ((uint32_t)(32 * quad) << 16);
-    const uint32_t s_tmem = row_tmem + (uint32_t)(x * kTreeN);
-    const uint32_t o_tmem = row_tmem + (uint32_t)(256 + x * 128);
+    const uint32_t s_tmem = row_tmem + (uint32_t)(x * kTreeN + 64 * half);
+    const uint32_t o_tmem = row_tmem + (uint32_t)(256 + x * 128 + half * (D / 2));
+    const uint32_t pair_bar = 1 + x * 4 + quad;
+    uint32_t* pair = reinterpret_cast<uint32_t*>(smem + C::kPairOff) + x * kTreeM + m;
+    bf16* pair_max = reinterpret_cast<bf16*>(pair);  // [half]
     const float sl2 = a.scale_log2;
     bool ok = true;
     int t = 0;
@@ -409,12 +420,14 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       const int tok = row / a.group;
       const int head = it.kvh * a.group + row % a.group;
       const bool row_ok = tok < it.r.n;
+      const bool warp_ok = __any_sync(0xffffffffu, row_ok);  // else: rows past the request's, nothing to compute
       const int kv_len = it.r.kv_len, ctx = kv_len - it.r.n;  // drafted token j sits at position ctx + j
       {
         const bf16* src = a.q + (int64_t)(it.r.q0 + tok) * a.q_stride_t + (int64_t)head * a.q_stride_h;
         uint8_t* qs = smem + C::kQOff + x * C::kQBytes;
 #pragma unroll
-        for (int u = 0; u < D / 8; ++u) {
+        for (int i = 0; i < D / 16; ++i) {
+          const int u = half * (D / 16) + i;
           const uint4 v = row_ok ? __ldg(reinterpret_cast<const uint4*>(src) + u) : make_uint4(0, 0, 0, 0);
           *reinterpret_cast<uint4*>(qs + (u >> 3) * C::kChunkBytes + tr_swz(m, u & 7)) = v;
         }
@@ -432,109 +445,99 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         tc_fence_after();
         const int kv0 = j * kTreeN;
         const bool masked = kv0 + kTreeN > ctx;  // uniform over the CTA: the tile reaches the drafted tokens
-        uint32_t vm[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int rel = kv0 + 32 * c - ctx;  // drafted index of the column group's first position
-            uint32_t w = 0;
-            if (row_ok) {
-              if (rel >= 0)
-                w = tree_bits(mrow, a.words, rel);
-              else if (rel > -32)
-                w = (0xffffffffu >> (32 + rel)) | (tree_bits(mrow, a.words, 0) << (-rel));
-              else
-                w = 0xffffffffu;
-            }
-            const int live = kv_len - (kv0 + 32 * c);
-            vm[c] = live >= 32 ? w : (live <= 0 ? 0u : w & (0xffffffffu >> (32 - live)));
-          }
-        }
+        // S_x(j) was issued after P_x.V of the tile before, but completes
+        // in order with it: O_x may be rescaled
         if (j > it.j0) ok = mbar_wait(&odone[x], (t - 1) & 1);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        uint8_t* pt = smem + C::kPOff + x * C::kPBytes;
-        // row maximum of the seen scores
-        float mx[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mx[k] = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < kTreeN / 64; ++h) {
+        if (warp_ok) {
           float v[64];
-          tmem_ld64(s_tmem + 64 * h, v);
+          tmem_ld64(s_tmem, v);
+          if (masked) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            const bool see = !masked || ((vm[2 * h + i / 32] >> (i & 31)) & 1u);
-            mx[i & 7] = fmaxf(mx[i & 7], see ? v[i] : -INFINITY);
-          }
-        }
-        float tmax =
-            fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-        tmax *= sl2;
-        const float m_new = fmaxf(m_run, tmax);
-        const bool rescale = m_run != -INFINITY && m_new > m_run + kTreeSlack;
-        const float m_use = (m_run == -INFINITY || rescale) ? m_new : m_run;
-        if (__any_sync(0xffffffffu, rescale)) {
-          const float alpha = rescale ? tr_exp2(m_run - m_use) : 1.f;
-#pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
-            float v[16];
-            tmem_ld16(o_tmem + 16 * c, v);
+            for (int c = 0; c < 2; ++c) {
+              const int pos = kv0 + 64 * half + 32 * c;
+              const int rel = pos - ctx;  // drafted index of the column group's first position
+              uint32_t w = 0;
+              if (row_ok) {
+                if (rel >= 0)
+                  w = tree_bits(mrow, a.words, rel);
+                else if (rel > -32)
+                  w = (0xffffffffu >> (32 + rel)) | (tree_bits(mrow, a.words, 0) << (-rel));
+                else
+                  w = 0xffffffffu;
+              }
+              const int live = kv_len - pos;
+              w = live >= 32 ? w : (live <= 0 ? 0u : w & (0xffffffffu >> (32 - live)));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] *= alpha;
-            tmem_st16_wait(o_tmem + 16 * c, v);
-          }
-          l_run *= alpha;
-        }
-        m_run = m_use;
-        const float nb = m_use == -INFINITY ? 0.f : -m_use;
-        float sm[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sm[k] = 0.f;
-#pragma unroll
-        for (int h = 0; h < kTreeN / 64; ++h) {
-          float v[64];
-          tmem_ld64(s_tmem + 64 * h, v);
-          uint32_t pk[32];
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) {
-            float p0 = tr_exp2(fmaf(v[i], sl2, nb));
-            float p1 = tr_exp2(fmaf(v[i + 1], sl2, nb));
-            if (masked) {
-              p0 = ((vm[2 * h + i / 32] >> (i & 31)) & 1u) ? p0 : 0.f;
-              p1 = ((vm[2 * h + i / 32] >> ((i + 1) & 31)) & 1u) ? p1 : 0.f;
+              for (int i = 0; i < 32; ++i) v[32 * c + i] = ((w >> i) & 1u) ? v[32 * c + i] : -INFINITY;
             }
-            sm[(i >> 1) & 7] += p0 + p1;
-            pk[i / 2] = pack_bf16x2(p0, p1);
           }
-          uint8_t* chunk = pt + h * C::kChunkBytes;
+          float mx[4];
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            *reinterpret_cast<uint4*>(chunk + tr_swz(m, u)) =
-                make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
+          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(v[k], v[k + 4]);
+#pragma unroll
+          for (int i = 8; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+          // both threads of the row take the larger of the two maxima, as
+          // rounded to bf16 (any common reference near the maximum serves)
+          const bf16 mine = f2bf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
+          pair_max[half] = mine;
+          named_barrier(pair_bar, 64);
+          const float tmax = fmaxf(bf2f(mine), bf2f(*const_cast<volatile bf16*>(&pair_max[half ^ 1])));
+          const float m_new = fmaxf(m_run, tmax);
+          const bool rescale = m_run != -INFINITY && m_new > m_run + kTreeSlack;
+          const float m_use = (m_run == -INFINITY || rescale) ? m_new : m_run;
+          if (__any_sync(0xffffffffu, rescale)) {
+            const float alpha = rescale ? tr_exp2(m_run - m_use) : 1.f;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float o[16];
+              tmem_ld16(o_tmem + 16 * c, o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] *= alpha;
+              tmem_st16_wait(o_tmem + 16 * c, o);
+            }
+            l_run *= alpha;
+          }
+          m_run = m_use;
+          const float nb = m_use == -INFINITY ? 0.f : -m_use;
+          float sm[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float p0 = tr_exp2(fmaf(v[32 * c + i], sl2, nb));
+              const float p1 = tr_exp2(fmaf(v[32 * c + i + 1], sl2, nb));
+              sm[(i >> 1) & 3] += p0 + p1;
+              pk[i / 2] = pack_bf16x2(p0, p1);
+            }
+            tmem_st16_u32(s_tmem + 16 * c, pk);
+          }
+          l_run += (sm[0] + sm[1]) + (sm[2] + sm[3]);
+          tmem_st_wait();
         }
-        l_run += ((sm[0] + sm[1]) + (sm[2] + sm[3])) + ((sm[4] + sm[5]) + (sm[6] + sm[7]));
         // V rows past the last token hold whatever the pool had there, and a
         // drafted token's V may hold inf or NaN that a row which masks the
         // token must not meet (0 * NaN is NaN): tile 0's threads clear the
         // former, and replace the latter's inf / NaN elements by zero and
-        // note their tokens, for the rows that do see them (epilogue).
+        // note that there were some, for the rows that do see them (epilogue).
         if (masked && x == 0) {
           const int item = 2 * t + 1;
           if (mbar_wait(&full[item % C::kSlots], (item / C::kSlots) & 1)) {
             uint8_t* vt = smem + C::kSlotOff + (item % C::kSlots) * C::kKVBytes;
             const int r0 = max(ctx - kv0, 0), r_live = min(kTreeN, kv_len - kv0), units = C::kChunks * 8;
-            for (int idx = m; idx < (kTreeN - r0) * units; idx += 128) {
+            for (int idx = half * 128 + m; idx < (kTreeN - r0) * units; idx += 256) {
               const int r = r0 + idx / units, hh = (idx / 8) % C::kChunks, u = idx % 8;
               uint4* at = reinterpret_cast<uint4*>(vt + hh * C::kChunkBytes + r * 128 + u * 16);
               if (r >= r_live) {
                 *at = make_uint4(0, 0, 0, 0);
               } else {
-                uint4 v = *at;
-                uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+                uint4 e = *at;
+                uint32_t* w = reinterpret_cast<uint32_t*>(&e);
                 bool hit = false;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -542,14 +545,14 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
                   if ((w[k] & 0x7f800000u) == 0x7f800000u) { w[k] &= 0x0000ffffu; hit = true; }
                 }
                 if (hit) {
-                  *at = v;
+                  *at = e;
                   atomicOr(any_bad, 1u);
                 }
               }
             }
+            fence_proxy_async_smem();
           }
         }
-        fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(&pready[x]);
       }
@@ -558,7 +561,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         flags[0] = 1;
         break;
       }
-      // ---- epilogue of the segment
+      // ---- epilogue of the segment: each thread of a row has half of its channels
       ok = __all_sync(0xffffffffu, mbar_wait(&odone[x], (t - 1) & 1));
       if (!ok) {
         set_status(a.status, PL_ERR_TIMEOUT);
@@ -566,15 +569,22 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         break;
       }
       tc_fence_after();
+      if (!warp_ok) continue;
+      float* pair_sum = reinterpret_cast<float*>(pair);
+      if (half == 1) *pair_sum = l_run;
+      named_barrier(pair_bar, 64);
+      if (half == 0) *pair_sum = l_run += *const_cast<volatile float*>(pair_sum);
+      named_barrier(pair_bar, 64);
+      l_run = *const_cast<volatile float*>(pair_sum);
       const bool whole = it.j0 == 0 && it.j1 == it.r.ntiles;
       // any_bad is final: every P of the segment was waited for by its P.V
-      const bool check_bad = *reinterpret_cast<volatile uint32_t*>(any_bad) != 0 && it.j1 * kTreeN > ctx;
+      const bool check_bad = *const_cast<volatile uint32_t*>(any_bad) != 0 && it.j1 * kTreeN > ctx;
       const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
       const int slot = 2 * (int)blockIdx.x + (it.j0 > 0 ? 0 : 1);
-      bf16* dst = a.out + (int64_t)(it.r.q0 + tok) * a.out_stride_t + (int64_t)head * a.out_stride_h;
-      float* pdst = a.part_o + ((int64_t)slot * C::kRows + x * kTreeM + m) * D;
+      bf16* dst = a.out + (int64_t)(it.r.q0 + tok) * a.out_stride_t + (int64_t)head * a.out_stride_h + half * (D / 2);
+      float* pdst = a.part_o + ((int64_t)slot * C::kRows + x * kTreeM + m) * D + half * (D / 2);
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = 0; c < D / 64; ++c) {
         float v[32];
         tmem_ld32(o_tmem + 32 * c, v);
         if (check_bad && row_ok) {
@@ -585,8 +595,8 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
             const int pos = ctx + jj;
             const int32_t pid = a.kv_indices[it.r.kv_begin + pos / PS];
             if (pid < 0 || (int64_t)pid >= a.num_pages) continue;
-            const bf16* vrow =
-                a.kv + (((int64_t)pid * 2 + 1) * PS + pos % PS) * tstride + (int64_t)it.kvh * D + 32 * c;
+            const bf16* vrow = a.kv + (((int64_t)pid * 2 + 1) * PS + pos % PS) * tstride + (int64_t)it.kvh * D +
+                               half * (D / 2) + 32 * c;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const float e = bf2f(vrow[i]);
@@ -610,7 +620,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           }
         }
       }
-      if (row_ok) {
+      if (row_ok && half == 0) {
         if (whole) {
           if (a.lse != nullptr)
             a.lse[(int64_t)(it.r.q0 + tok) * a.num_qo_heads + head] =
