@@ -87,6 +87,23 @@ __device__ __forceinline__ float2 unpack_bf16x2(uint32_t u) {
   return r;
 }
 
+// Two fp32 operations in one instruction (each rounded as the scalar one).
+__device__ __forceinline__ float2 fma_f32x2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
+        "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 add_f32x2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
 // ------------------------------------------------------------ shared memory
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -477,6 +494,17 @@ __device__ __forceinline__ float lora_dot(const bf16* brow, const float* drow, i
     for (int j = 0; j < rank; ++j) d = fmaf(bf2f(brow[j]), bfr(drow[j]), d);
   }
   return d;
+}
+
+// Registers per thread of the calling warpgroup (all four warps call it);
+// alloc waits until other warpgroups have given up as many.
+template <int kRegs>
+__device__ __forceinline__ void reg_alloc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void reg_dealloc() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
 // Named barrier among `count` threads (multiple of 32) of the CTA.

@@ -55,10 +55,22 @@ struct TreeArgs {
   int32_t* status;
 };
 
+// One segment of an item: K/V tiles [j0, j1).
+struct TreeSeg {
+  int q0, n, kv_begin, n_pages, kv_len, kvh, rt, j0, j1, whole;
+};
+
 template <int D, int NT>
 struct TreeCfg {
   static constexpr int kSoftmaxThreads = 256 * NT;  // two per row
-  static constexpr int kThreads = 64 + kSoftmaxThreads;
+  // Softmax warps first, then the producer and the MMA warp; two idle warps
+  // complete the last warpgroup where registers are dealt anew.
+  static constexpr int kProducerWarp = 8 * NT, kMmaWarp = 8 * NT + 1;
+  static constexpr int kThreads = NT == 2 ? 640 : 64 + kSoftmaxThreads;
+  // NT = 2: 20 warps are launched with 96 registers a thread (5 warps per
+  // scheduler); the softmax threads (4 warpgroups) take 104, the rest 64:
+  // 512 * 104 + 128 * 64 = 640 * 96.  The host refuses another launch count.
+  static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 104, kOtherRegs = 64;
   static constexpr int kRows = kTreeM * NT;
   static constexpr int kChunks = D / 64;
   static constexpr int kChunkBytes = kTreeM * 128;
@@ -70,8 +82,8 @@ struct TreeCfg {
   static constexpr int kPairOff = kSlotOff + kSlots * kKVBytes;  // [NT][128] words shared by a row's two threads
   static constexpr int kBarOff = kPairOff + kRows * 4;
   static constexpr int kNumBars = 2 * kSlots + 8 + 1;  // full empty | s[2] p[2] o[2] q[2] | fin
-  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
-  static constexpr int kSmemBytes = 1024 + kMiscOff + 80;
+  static constexpr int kMiscOff = kBarOff + kNumBars * 8;  // tmem slot, flags, range, any_bad, 2 segments
+  static constexpr int kSmemBytes = 1024 + kMiscOff + 64 + 2 * (int)sizeof(TreeSeg);
   static constexpr int kTmemCols = 512;  // S_x at 128 x (P_x in its place), O_x at 256 + 128 x
   static_assert(kSmemBytes <= 232448, "tree tiles exceed the shared-memory limit");
 };
@@ -103,18 +115,19 @@ struct TreeReq {
     rts = (int)(((int64_t)n * a.group + rows - 1) / rows);
     ntiles = max(1, (kv_len + kTreeN - 1) / kTreeN);  // an empty context still writes its zero rows
   }
-  __device__ __forceinline__ int64_t work(int hkv) const { return (int64_t)rts * hkv * ntiles; }
+  // tiles of the request (the host bounds the total of all requests)
+  __device__ __forceinline__ int work(int hkv) const { return rts * hkv * ntiles; }
 };
 
 // Total tiles over all requests, and the tiles in front of request `upto`
 // (one warp; every lane gets the results).
-__device__ __forceinline__ void tree_prefix(const TreeArgs& a, int rows, int upto, int64_t& total, int64_t& before) {
+__device__ __forceinline__ void tree_prefix(const TreeArgs& a, int rows, int upto, int& total, int& before) {
   const int lane = threadIdx.x & 31;
-  int64_t t = 0, p = 0;
+  int t = 0, p = 0;
   for (int b = lane; b < a.batch; b += 32) {
     TreeReq r;
     r.load(a, b, rows);
-    const int64_t w = r.work(a.num_kv_heads);
+    const int w = r.work(a.num_kv_heads);
     t += w;
     if (b < upto) p += w;
   }
@@ -127,8 +140,8 @@ __device__ __forceinline__ void tree_prefix(const TreeArgs& a, int rows, int upt
   before = p;
 }
 
-__device__ __forceinline__ int64_t tree_share(int64_t total, int ctas, int min_share) {
-  const int64_t s = (total + ctas - 1) / ctas;
+__device__ __forceinline__ int tree_share(int total, int ctas, int min_share) {
+  const int s = (total + ctas - 1) / ctas;
   return s < min_share ? min_share : s;
 }
 
@@ -137,24 +150,23 @@ __device__ __forceinline__ int64_t tree_share(int64_t total, int ctas, int min_s
 // moves to the item's start, so short items are never split (and never
 // merged).  One warp.
 struct TreeAt {
-  int b;
-  int64_t base, w;
+  int b, base, w;
 };
-__device__ __forceinline__ TreeAt tree_locate(const TreeArgs& a, int rows, int64_t w) {
+__device__ __forceinline__ TreeAt tree_locate(const TreeArgs& a, int rows, int w) {
   const int lane = threadIdx.x & 31;
   TreeAt at{a.batch, 0, w};
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     TreeReq r;
-    int64_t n = 0;
+    int n = 0;
     r.ntiles = 1;
     if (b0 + lane < a.batch) {
       r.load(a, b0 + lane, rows);
       n = r.work(a.num_kv_heads);
     }
-    int64_t inc = n;
+    int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
     const uint32_t hit = __ballot_sync(0xffffffffu, n > 0 && w < at.base + inc);
@@ -173,31 +185,29 @@ __device__ __forceinline__ TreeAt tree_locate(const TreeArgs& a, int rows, int64
 
 // Walks the item segments of the tile range [w, w_end).
 struct TreeIter {
-  TreeReq r;
-  int b, kvh, rt, j0, j1;
-  int64_t w, w_end, base;  // base: first tile of request b
-  __device__ __forceinline__ void init(const TreeArgs& a, int rows, int b_, int64_t base_, int64_t w_, int64_t e) {
-    b = b_;
-    base = base_;
-    w = w_;
-    w_end = e;
-    if (w < w_end) r.load(a, b, rows);
-  }
-  __device__ __forceinline__ bool next(const TreeArgs& a, int rows) {
+  int b, w, w_end, base;  // base: first tile of request b
+  __device__ __forceinline__ bool next(const TreeArgs& a, int rows, TreeSeg& s) {
     if (w >= w_end) return false;
+    TreeReq r;
+    r.load(a, b, rows);
     while (w - base >= r.work(a.num_kv_heads)) {
       base += r.work(a.num_kv_heads);
       ++b;
       r.load(a, b, rows);
     }
-    const int64_t off = w - base;
-    const int64_t item = off / r.ntiles;
-    j0 = (int)(off - item * r.ntiles);
-    rt = (int)(item % r.rts);
-    kvh = (int)(item / r.rts);
-    const int64_t left = w_end - w;
-    j1 = (int)(left < r.ntiles - j0 ? j0 + left : r.ntiles);
-    w += j1 - j0;
+    const int off = w - base;
+    const int item = off / r.ntiles;
+    s.q0 = r.q0;
+    s.n = r.n;
+    s.kv_begin = r.kv_begin;
+    s.n_pages = r.n_pages;
+    s.kv_len = r.kv_len;
+    s.j0 = off - item * r.ntiles;
+    s.j1 = min(s.j0 + (w_end - w), r.ntiles);
+    s.rt = item % r.rts;
+    s.kvh = item / r.rts;
+    s.whole = s.j0 == 0 && s.j1 == r.ntiles;
+    w += s.j1 - s.j0;
     return true;
   }
 };
@@ -210,6 +220,20 @@ __device__ __forceinline__ uint32_t tree_bits(const uint32_t* row, int words, in
   return __funnelshift_r(lo, hi, s);
 }
 
+// Wait of a whole warp: one lane polls (many pollers of one barrier slow all
+// shared-memory traffic).  false: the wait ran out or the CTA gave up.
+__device__ __forceinline__ bool tree_warp_wait(uint64_t* bar, uint32_t parity, volatile int32_t* flags) {
+  int ok = 0;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity) && flags[0] == 0;
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+// Arrival of a whole warp: its tensor-memory and shared-memory accesses are
+// ordered before the one lane's arrive.
+__device__ __forceinline__ void tree_warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 template <int D, int NT>
 __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
     paged_tree_kernel(const __grid_constant__ CUtensorMap kv_map, const TreeArgs a) {
@@ -219,16 +243,16 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
   uint64_t* full = bars;
   uint64_t* empty = bars + C::kSlots;
-  uint64_t* sready = bars + 2 * C::kSlots;  // [2] S_x in TMEM
-  uint64_t* pready = sready + 2;            // [2] P_x in TMEM (256 arrivals)
-  uint64_t* odone = sready + 4;             // [2] O_x += P_x.V finished
-  uint64_t* qready = sready + 6;            // [2] Q_x staged (256 arrivals)
+  uint64_t* sready = bars + 2 * C::kSlots;  // [2] S_x of a tile in TMEM, O_x of the tiles before it complete
+  uint64_t* pready = sready + 2;            // [2] P_x in TMEM (8 warps)
+  uint64_t* odone = sready + 4;             // [2] O_x of a segment complete
+  uint64_t* qready = sready + 6;            // [2] Q_x of a segment staged (8 warps)
   uint64_t* fin = sready + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
   volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, issued, consumed
-  int64_t* range = reinterpret_cast<int64_t*>(smem + C::kMiscOff + 32);                    // base, w0, w1
-  int32_t* range_b = reinterpret_cast<int32_t*>(smem + C::kMiscOff + 56);
-  uint32_t* any_bad = reinterpret_cast<uint32_t*>(smem + C::kMiscOff + 64);  // a drafted V held inf or NaN
+  volatile int32_t* range = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 32);  // b, w, w_end, base
+  uint32_t* any_bad = reinterpret_cast<uint32_t*>(smem + C::kMiscOff + 48);  // a drafted V held inf or NaN
+  TreeSeg* segs = reinterpret_cast<TreeSeg*>(smem + C::kMiscOff + 64);       // [2] the softmax warps' segment
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
@@ -238,9 +262,9 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&sready[x], 1);
-      mbar_init(&pready[x], 256);
+      mbar_init(&pready[x], 8);
       mbar_init(&odone[x], 1);
-      mbar_init(&qready[x], 256);
+      mbar_init(&qready[x], 8);
     }
     mbar_init(fin, 1);
     flags[0] = flags[1] = flags[2] = 0;
@@ -252,17 +276,17 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-  if (warp == 0) {
-    int64_t total, dummy;
+  if (warp == C::kProducerWarp) {
+    int total, dummy;
     tree_prefix(a, C::kRows, 0, total, dummy);
-    const int64_t share = tree_share(total, a.ctas, a.min_share);
-    const int64_t w0 = min(total, (int64_t)blockIdx.x * share), w1 = min(total, w0 + share);
+    const int share = tree_share(total, a.ctas, a.min_share);
+    const int w0 = (int)min((int64_t)total, (int64_t)blockIdx.x * share), w1 = min(total, w0 + share);
     const TreeAt at0 = tree_locate(a, C::kRows, w0), at1 = tree_locate(a, C::kRows, w1);
     if (lane == 0) {
-      range[0] = at0.base;
+      range[0] = at0.b;
       range[1] = at0.w;
       range[2] = at1.w;
-      range_b[0] = at0.b;
+      range[3] = at0.base;
     }
     // arguments that no launch can check on the host
     if (blockIdx.x == 0)
@@ -277,7 +301,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   __syncthreads();
   if (range[1] >= range[2]) return;  // nothing allocated yet
 
-  if (warp == 1) {
+  if (warp == C::kMmaWarp) {
     tmem_alloc(tmem_slot, C::kTmemCols);
     tmem_relinquish();
   }
@@ -285,25 +309,33 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  TreeIter it;
-  it.init(a, C::kRows, range_b[0], range[0], range[1], range[2]);
+  TreeIter it{range[0], range[1], range[2], range[3]};
   const int PS = a.page_size;
 
-  if (warp == 0) {
+  if (warp == C::kProducerWarp) {
+    if constexpr (NT == 2) reg_dealloc<C::kOtherRegs>();
     // ------------------------------------------------------------ producer
     const int ppt = kTreeN / PS;
     const int boxes = ppt * C::kChunks;  // <= 16
     const int p = lane / C::kChunks, hh = lane % C::kChunks;
     int i = 0;
     bool go = true;
-    while (go && it.next(a, C::kRows)) {
-      for (int j = it.j0; go && j < it.j1; ++j)
+    TreeSeg sg;
+    while (go && it.next(a, C::kRows, sg)) {
+      for (int j = sg.j0; go && j < sg.j1; ++j) {
+        // the tile's page (K and V alike); out of range: the copy writes zeros
+        int32_t coord = (int32_t)(2 * a.num_pages);
+        if (lane < boxes && j * ppt + p < sg.n_pages) {
+          const int32_t pid = a.kv_indices[sg.kv_begin + j * ppt + p];
+          if (pid >= 0 && (int64_t)pid < a.num_pages)
+            coord = 2 * pid;
+          else
+            set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
+        }
         for (int kv = 0; kv < 2; ++kv, ++i) {
           const int s = i % C::kSlots;
-          bool ok = true;
-          if (i >= C::kSlots) ok = mbar_wait(&empty[s], ((i / C::kSlots) - 1) & 1);
-          if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) {
-            if (lane == 0 && !__all_sync(0xffffffffu, ok)) set_status(a.status, PL_ERR_TIMEOUT);
+          if (i >= C::kSlots && !tree_warp_wait(&empty[s], ((i / C::kSlots) - 1) & 1, flags)) {
+            if (lane == 0) set_status(a.status, PL_ERR_TIMEOUT);
             flags[0] = 1;
             go = false;
             break;
@@ -311,22 +343,15 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           if (lane == 0) mbar_arrive_expect_tx(&full[s], C::kKVBytes);
           __syncwarp();
           if (lane < boxes) {
-            const int page_idx = j * ppt + p;
-            int32_t coord = (int32_t)(2 * a.num_pages);  // out of range: the copy writes zeros
-            if (page_idx < it.r.n_pages) {
-              const int32_t pid = a.kv_indices[it.r.kv_begin + page_idx];
-              if (pid >= 0 && (int64_t)pid < a.num_pages)
-                coord = 2 * pid + kv;
-              else
-                set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
-            }
             uint8_t* dst = smem + C::kSlotOff + s * C::kKVBytes + hh * C::kChunkBytes + p * PS * 128;
-            tma_load_4d(dst, &kv_map, hh * 64, it.kvh, 0, coord, &full[s]);
+            tma_load_4d(dst, &kv_map, hh * 64, sg.kvh, 0, coord + kv, &full[s]);
           }
         }
+      }
     }
     if (lane == 0) flags[1] = i;
-  } else if (warp == 1) {
+  } else if (warp == C::kMmaWarp) {
+    if constexpr (NT == 2) reg_dealloc<C::kOtherRegs>();
     // ---------------------------------------------------------- MMA issuer
     if (lane == 0) {
       constexpr uint32_t idesc_s = umma_idesc_bf16(kTreeM, kTreeN);
@@ -357,11 +382,11 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           umma_bf16_ts(tmem + (uint32_t)(256 + x * 128), tmem + (uint32_t)(x * kTreeN + (kk >> 2) * 64 + (kk & 3) * 8),
                        umma_desc_mn_sw128(vb + kk * 16 * 128, C::kChunkBytes, 1024), idesc_o,
                        (!first || kk > 0) ? 1u : 0u);
-        umma_commit(&odone[x]);
       };
       bool ok = true;
       int t = 0;  // tiles of this CTA so far
-      for (int seg = 0; ok && it.next(a, C::kRows); ++seg) {
+      TreeSeg sg;
+      for (int seg = 0; ok && it.next(a, C::kRows, sg); ++seg) {
 #pragma unroll
         for (int x = 0; x < NT; ++x) ok = ok && mbar_wait(&qready[x], seg & 1);
         ok = ok && wait_item(2 * t);
@@ -369,15 +394,16 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
 #pragma unroll
         for (int x = 0; x < NT; ++x) issue_s(x, t);
         umma_commit(&empty[(2 * t) % C::kSlots]);
-        for (int j = it.j0; ok && j < it.j1; ++j, ++t) {
-          const bool more = j + 1 < it.j1;
+        for (int j = sg.j0; ok && j < sg.j1; ++j, ++t) {
+          const bool more = j + 1 < sg.j1;
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
             ok = ok && mbar_wait(&pready[x], t & 1) && !flags[0];
             if (ok && x == 0) ok = wait_item(2 * t + 1);
             if (!ok) break;
             tc_fence_after();
-            issue_pv(x, t, j == it.j0);
+            issue_pv(x, t, j == sg.j0);
+            if (!more) umma_commit(&odone[x]);
             if (x == NT - 1) umma_commit(&empty[(2 * t + 1) % C::kSlots]);
             if (more) {
               if (x == 0) ok = wait_item(2 * t + 2);
@@ -396,14 +422,18 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       umma_commit(fin);
       if (!mbar_wait(fin, 0)) set_status(a.status, PL_ERR_TIMEOUT);
     }
+  } else if (warp > C::kMmaWarp) {
+    if constexpr (NT == 2) reg_dealloc<C::kOtherRegs>();
   } else {
+    if constexpr (NT == 2) reg_alloc<C::kSoftmaxRegs>();
     // -------------------------------------------------- softmax / epilogue
-    // Warps 2.. : per row tile x two groups of four warps; group `half` has
-    // the positions 64 half .. 64 half + 63 of every K/V tile, so a row's two
-    // threads share its running maximum (through shared memory) and keep a
-    // sum each.
-    const int x = (warp - 2) / 8;
-    const int half = ((warp - 2) / 4) & 1;
+    // Per row tile two groups of four warps; group `half` has the positions
+    // 64 half .. 64 half + 63 of every K/V tile, so a row's two threads share
+    // its running maximum (through shared memory) and keep a sum each.  A
+    // warp whose wait ran out does no further work but still meets its named
+    // barriers, so that no other warp is left in one.
+    const int x = warp / 8;
+    const int half = (warp / 4) & 1;
     const int quad = warp & 3;
     const int m = 32 * quad + lane;  // row of the tile == TMEM lane
     const uint32_t row_tmem = tmem + ((uint32_t)(32 * quad) << 16);
@@ -413,17 +443,25 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
     uint32_t* pair = reinterpret_cast<uint32_t*>(smem + C::kPairOff) + x * kTreeM + m;
     bf16* pair_max = reinterpret_cast<bf16*>(pair);  // [half]
     const float sl2 = a.scale_log2;
+    const bool writer = threadIdx.x == 0;
     bool ok = true;
     int t = 0;
-    for (int seg = 0; ok && it.next(a, C::kRows); ++seg) {
-      const int row = it.rt * C::kRows + x * kTreeM + m;  // row of the request
-      const int tok = row / a.group;
-      const int head = it.kvh * a.group + row % a.group;
-      const bool row_ok = tok < it.r.n;
-      const bool warp_ok = __any_sync(0xffffffffu, row_ok);  // else: rows past the request's, nothing to compute
-      const int kv_len = it.r.kv_len, ctx = kv_len - it.r.n;  // drafted token j sits at position ctx + j
-      {
-        const bf16* src = a.q + (int64_t)(it.r.q0 + tok) * a.q_stride_t + (int64_t)head * a.q_stride_h;
+    for (int seg = 0;; ++seg) {
+      TreeSeg* sp = &segs[seg & 1];
+      if (writer && !it.next(a, C::kRows, *sp)) sp->j0 = -1;
+      named_barrier(15, C::kSoftmaxThreads);
+      const volatile TreeSeg& sg = *sp;
+      const int j0 = sg.j0;
+      if (j0 < 0) break;
+      // this thread's row of the request, computed where it is needed
+      auto row_of = [&]() { return sg.rt * C::kRows + x * kTreeM + m; };
+      // else: rows past the request's, nothing to compute
+      const bool warp_ok = (sg.rt * C::kRows + x * kTreeM + 32 * quad) / a.group < sg.n;
+      if (ok) {
+        const int row = row_of(), tok = row / a.group;
+        const bool row_ok = tok < sg.n;
+        const int head = sg.kvh * a.group + row % a.group;
+        const bf16* src = a.q + (int64_t)(sg.q0 + tok) * a.q_stride_t + (int64_t)head * a.q_stride_h;
         uint8_t* qs = smem + C::kQOff + x * C::kQBytes;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
@@ -432,66 +470,66 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           *reinterpret_cast<uint4*>(qs + (u >> 3) * C::kChunkBytes + tr_swz(m, u & 7)) = v;
         }
         fence_proxy_async_smem();
-        mbar_arrive(&qready[x]);
+        tree_warp_arrive(&qready[x]);
       }
-      const uint32_t* mrow = a.mask + (int64_t)(it.r.q0 + (row_ok ? tok : 0)) * a.mask_stride;
       float m_run = -INFINITY, l_run = 0.f;
-      for (int j = it.j0; j < it.j1; ++j, ++t) {
-        ok = mbar_wait(&sready[x], t & 1);
-        if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) {
-          ok = false;
-          break;
+      const int j1 = sg.j1;
+      const int first_masked = (sg.kv_len - sg.n) / kTreeN;  // tiles from here on reach the drafted tokens
+      for (int j = j0; j < j1; ++j, ++t) {
+        // S_x(j) was issued after P_x.V of the tile before: O_x is complete too
+        ok = ok && tree_warp_wait(&sready[x], t & 1, flags);
+        if (!warp_ok) {
+          if (ok) tree_warp_arrive(&pready[x]);
+          continue;
         }
-        tc_fence_after();
-        const int kv0 = j * kTreeN;
-        const bool masked = kv0 + kTreeN > ctx;  // uniform over the CTA: the tile reaches the drafted tokens
-        // S_x(j) was issued after P_x.V of the tile before, but completes
-        // in order with it: O_x may be rescaled
-        if (j > it.j0) ok = mbar_wait(&odone[x], (t - 1) & 1);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (warp_ok) {
-          float v[64];
-          tmem_ld64(s_tmem, v);
-          if (masked) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int pos = kv0 + 64 * half + 32 * c;
-              const int rel = pos - ctx;  // drafted index of the column group's first position
-              uint32_t w = 0;
-              if (row_ok) {
-                if (rel >= 0)
-                  w = tree_bits(mrow, a.words, rel);
-                else if (rel > -32)
-                  w = (0xffffffffu >> (32 + rel)) | (tree_bits(mrow, a.words, 0) << (-rel));
-                else
-                  w = 0xffffffffu;
-              }
-              const int live = kv_len - pos;
-              w = live >= 32 ? w : (live <= 0 ? 0u : w & (0xffffffffu >> (32 - live)));
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[32 * c + i] = ((w >> i) & 1u) ? v[32 * c + i] : -INFINITY;
-            }
-          }
-          float mx[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(v[k], v[k + 4]);
-#pragma unroll
-          for (int i = 8; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
-          // both threads of the row take the larger of the two maxima, as
-          // rounded to bf16 (any common reference near the maximum serves)
-          const bf16 mine = f2bf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
-          pair_max[half] = mine;
+        if (!ok) {
           named_barrier(pair_bar, 64);
-          const float tmax = fmaxf(bf2f(mine), bf2f(*const_cast<volatile bf16*>(&pair_max[half ^ 1])));
+          continue;
+        }
+        tc_fence_after();
+        const bool masked = j >= first_masked;  // uniform over the CTA
+        float v[64];
+        tmem_ld64(s_tmem, v);
+        if (masked) {
+          const int kv_len = sg.kv_len, ctx = kv_len - sg.n;  // drafted token i sits at position ctx + i
+          const int tok = row_of() / a.group;
+          const bool row_ok = tok < sg.n;
+          const uint32_t* mrow = a.mask + (int64_t)(sg.q0 + (row_ok ? tok : 0)) * a.mask_stride;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int pos = j * kTreeN + 64 * half + 32 * c;
+            const int rel = pos - ctx;  // drafted index of the column group's first position
+            uint32_t w = 0;
+            if (row_ok) {
+              if (rel >= 0)
+                w = tree_bits(mrow, a.words, rel);
+              else if (rel > -32)
+                w = (0xffffffffu >> (32 + rel)) | (tree_bits(mrow, a.words, 0) << (-rel));
+              else
+                w = 0xffffffffu;
+            }
+            const int live = kv_len - pos;
+            w = live >= 32 ? w : (live <= 0 ? 0u : w & (0xffffffffu >> (32 - live)));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[32 * c + i] = ((w >> i) & 1u) ? v[32 * c + i] : -INFINITY;
+          }
+        }
+        float mx[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(v[k], v[k + 4]);
+#pragma unroll
+        for (int i = 8; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+        // both threads of the row take the larger of the two maxima, as
+        // rounded to bf16 (any common reference near the maximum serves)
+        const bf16 mine = f2bf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
+        pair_max[half] = mine;
+        named_barrier(pair_bar, 64);
+        const float tmax = fmaxf(bf2f(mine), bf2f(*const_cast<volatile bf16*>(&pair_max[half ^ 1])));
+        if (__any_sync(0xffffffffu, tmax > m_run + kTreeSlack || m_run == -INFINITY)) {
           const float m_new = fmaxf(m_run, tmax);
           const bool rescale = m_run != -INFINITY && m_new > m_run + kTreeSlack;
-          const float m_use = (m_run == -INFINITY || rescale) ? m_new : m_run;
+          const float alpha = rescale ? tr_exp2(m_run - m_new) : 1.f;
           if (__any_sync(0xffffffffu, rescale)) {
-            const float alpha = rescale ? tr_exp2(m_run - m_use) : 1.f;
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               float o[16];
@@ -502,35 +540,42 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
             }
             l_run *= alpha;
           }
-          m_run = m_use;
-          const float nb = m_use == -INFINITY ? 0.f : -m_use;
-          float sm[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float p0 = tr_exp2(fmaf(v[32 * c + i], sl2, nb));
-              const float p1 = tr_exp2(fmaf(v[32 * c + i + 1], sl2, nb));
-              sm[(i >> 1) & 3] += p0 + p1;
-              pk[i / 2] = pack_bf16x2(p0, p1);
-            }
-            tmem_st16_u32(s_tmem + 16 * c, pk);
-          }
-          l_run += (sm[0] + sm[1]) + (sm[2] + sm[3]);
-          tmem_st_wait();
+          if (rescale || m_run == -INFINITY) m_run = m_new;
         }
+        const float nb = m_run == -INFINITY ? 0.f : -m_run;
+        const float2 sl2_2 = make_float2(sl2, sl2), nb_2 = make_float2(nb, nb);
+        float2 sm[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sm[k] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float2 e = fma_f32x2(make_float2(v[32 * c + i], v[32 * c + i + 1]), sl2_2, nb_2);
+            e.x = tr_exp2(e.x);
+            e.y = tr_exp2(e.y);
+            sm[(i >> 1) & 3] = add_f32x2(sm[(i >> 1) & 3], e);
+            pk[i / 2] = pack_bf16x2(e.x, e.y);
+          }
+          tmem_st16_u32(s_tmem + 16 * c, pk);
+        }
+        sm[0] = add_f32x2(add_f32x2(sm[0], sm[1]), add_f32x2(sm[2], sm[3]));
+        l_run += sm[0].x + sm[0].y;
+        tmem_st_wait();
         // V rows past the last token hold whatever the pool had there, and a
         // drafted token's V may hold inf or NaN that a row which masks the
-        // token must not meet (0 * NaN is NaN): tile 0's threads clear the
-        // former, and replace the latter's inf / NaN elements by zero and
-        // note that there were some, for the rows that do see them (epilogue).
-        if (masked && x == 0) {
+        // token must not meet (0 * NaN is NaN): the former are cleared, the
+        // latter's inf / NaN elements replaced by zero and noted, for the
+        // rows that do see them (epilogue).  Row 0's warps of tile 0 always
+        // have rows, so they do it for the CTA.
+        if (masked && x == 0 && quad == 0) {
           const int item = 2 * t + 1;
-          if (mbar_wait(&full[item % C::kSlots], (item / C::kSlots) & 1)) {
+          if (tree_warp_wait(&full[item % C::kSlots], (item / C::kSlots) & 1, flags)) {
             uint8_t* vt = smem + C::kSlotOff + (item % C::kSlots) * C::kKVBytes;
-            const int r0 = max(ctx - kv0, 0), r_live = min(kTreeN, kv_len - kv0), units = C::kChunks * 8;
-            for (int idx = half * 128 + m; idx < (kTreeN - r0) * units; idx += 256) {
+            const int kv_len = sg.kv_len, ctx = kv_len - sg.n;
+            const int r0 = max(ctx - j * kTreeN, 0), r_live = min(kTreeN, kv_len - j * kTreeN), units = C::kChunks * 8;
+            for (int idx = half * 32 + lane; idx < (kTreeN - r0) * units; idx += 64) {
               const int r = r0 + idx / units, hh = (idx / 8) % C::kChunks, u = idx % 8;
               uint4* at = reinterpret_cast<uint4*>(vt + hh * C::kChunkBytes + r * 128 + u * 16);
               if (r >= r_live) {
@@ -554,34 +599,33 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           }
         }
         tc_fence_before();
-        mbar_arrive(&pready[x]);
-      }
-      if (!ok) {
-        set_status(a.status, PL_ERR_TIMEOUT);
-        flags[0] = 1;
-        break;
+        tree_warp_arrive(&pready[x]);
       }
       // ---- epilogue of the segment: each thread of a row has half of its channels
-      ok = __all_sync(0xffffffffu, mbar_wait(&odone[x], (t - 1) & 1));
+      if (ok) ok = tree_warp_wait(&odone[x], seg & 1, flags);
       if (!ok) {
-        set_status(a.status, PL_ERR_TIMEOUT);
+        if (lane == 0) set_status(a.status, PL_ERR_TIMEOUT);
         flags[0] = 1;
-        break;
       }
-      tc_fence_after();
       if (!warp_ok) continue;
+      tc_fence_after();
       float* pair_sum = reinterpret_cast<float*>(pair);
       if (half == 1) *pair_sum = l_run;
       named_barrier(pair_bar, 64);
       if (half == 0) *pair_sum = l_run += *const_cast<volatile float*>(pair_sum);
       named_barrier(pair_bar, 64);
+      if (!ok) continue;
       l_run = *const_cast<volatile float*>(pair_sum);
-      const bool whole = it.j0 == 0 && it.j1 == it.r.ntiles;
+      const int row = row_of(), tok = row / a.group;
+      const bool row_ok = tok < sg.n;
+      const int head = sg.kvh * a.group + row % a.group;
+      const int ctx = sg.kv_len - sg.n, n = sg.n;
+      const bool whole = sg.whole != 0;
       // any_bad is final: every P of the segment was waited for by its P.V
-      const bool check_bad = *const_cast<volatile uint32_t*>(any_bad) != 0 && it.j1 * kTreeN > ctx;
+      const bool check_bad = *const_cast<volatile uint32_t*>(any_bad) != 0 && j1 * kTreeN > ctx;
       const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-      const int slot = 2 * (int)blockIdx.x + (it.j0 > 0 ? 0 : 1);
-      bf16* dst = a.out + (int64_t)(it.r.q0 + tok) * a.out_stride_t + (int64_t)head * a.out_stride_h + half * (D / 2);
+      const int slot = 2 * (int)blockIdx.x + (j0 > 0 ? 0 : 1);
+      bf16* dst = a.out + (int64_t)(sg.q0 + tok) * a.out_stride_t + (int64_t)head * a.out_stride_h + half * (D / 2);
       float* pdst = a.part_o + ((int64_t)slot * C::kRows + x * kTreeM + m) * D + half * (D / 2);
 #pragma unroll 1
       for (int c = 0; c < D / 64; ++c) {
@@ -589,13 +633,14 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         tmem_ld32(o_tmem + 32 * c, v);
         if (check_bad && row_ok) {
           // the inf / NaN elements of the seen drafted tokens of this segment
+          const uint32_t* mrow = a.mask + (int64_t)(sg.q0 + tok) * a.mask_stride;
           const int64_t tstride = (int64_t)a.num_kv_heads * D;
-          for (int jj = max(0, max(-ctx, it.j0 * kTreeN - ctx)); jj < it.r.n && ctx + jj < it.j1 * kTreeN; ++jj) {
+          for (int jj = max(0, max(-ctx, j0 * kTreeN - ctx)); jj < n && ctx + jj < j1 * kTreeN; ++jj) {
             if (!(tree_bits(mrow, a.words, jj) & 1u)) continue;
             const int pos = ctx + jj;
-            const int32_t pid = a.kv_indices[it.r.kv_begin + pos / PS];
+            const int32_t pid = a.kv_indices[sg.kv_begin + pos / PS];
             if (pid < 0 || (int64_t)pid >= a.num_pages) continue;
-            const bf16* vrow = a.kv + (((int64_t)pid * 2 + 1) * PS + pos % PS) * tstride + (int64_t)it.kvh * D +
+            const bf16* vrow = a.kv + (((int64_t)pid * 2 + 1) * PS + pos % PS) * tstride + (int64_t)sg.kvh * D +
                                half * (D / 2) + 32 * c;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
@@ -623,7 +668,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       if (row_ok && half == 0) {
         if (whole) {
           if (a.lse != nullptr)
-            a.lse[(int64_t)(it.r.q0 + tok) * a.num_qo_heads + head] =
+            a.lse[(int64_t)(sg.q0 + tok) * a.num_qo_heads + head] =
                 l_run == 0.f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
         } else {
           float* ml = a.part_ml + (int64_t)slot * 2 * C::kRows + x * kTreeM + m;
@@ -643,7 +688,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == C::kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
   }
@@ -669,12 +714,12 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int r
   TreeReq r;
   r.load(a, req, rows);
   if (r.ntiles <= a.min_share || r.n == 0) return;  // never split
-  int64_t total, base;
+  int total, base;
   tree_prefix(a, rows, req, total, base);
-  const int64_t share = tree_share(total, a.ctas, a.min_share);
+  const int share = tree_share(total, a.ctas, a.min_share);
   for (int head = threadIdx.x / 32; head < a.num_qo_heads; head += blockDim.x / 32) {
     const int row = (tok_g - r.q0) * a.group + head % a.group;
-    const int64_t w = base + ((int64_t)(head / a.group) * r.rts + row / rows) * r.ntiles;
+    const int w = base + ((head / a.group) * r.rts + row / rows) * r.ntiles;
     const int m = row % rows;
     const int64_t ca = w / share, cb = (w + r.ntiles - 1) / share;
     if (ca == cb) continue;
@@ -847,6 +892,13 @@ int32_t launch_tree(const CUtensorMap& map, const pl::TreeArgs& a, bool merge, v
   auto kern = pl::paged_tree_kernel<D, NT>;
   int32_t st = pl_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (st != PL_OK) return st;
+  if (NT == 2) {  // the register split only adds up for this launch count
+    static const int regs = [&] {
+      cudaFuncAttributes f;
+      return cudaFuncGetAttributes(&f, kern) == cudaSuccess ? f.numRegs : -1;
+    }();
+    if (regs != C::kLaunchRegs) return PL_ERR_UNSUPPORTED;
+  }
   st = pl_host::launch_pdl(kern, dim3(a.ctas), dim3(C::kThreads), C::kSmemBytes, stream, map, a);
   if (st != PL_OK || !merge) return st;
   return pl_host::launch_pdl(pl::tree_merge_kernel<D>, dim3(a.total_q), dim3(256), 0, stream, a, (int)C::kRows);
@@ -898,6 +950,9 @@ extern "C" int32_t pl_paged_tree_attention(
   if (sms <= 0) return PL_ERR_NO_DEVICE;
 
   const bool two = tree_two_tiles(total_q, batch, group);
+  // the line of tiles is indexed in 32 bits; an upper bound of its length
+  const int64_t most_rts = (int64_t)total_q * group / pl::kTreeM + batch;
+  if (most_rts * num_kv_heads > 0x7FFFFFFFll / (total_pages * page_size / pl::kTreeN + 1)) return PL_ERR_UNSUPPORTED;
   pl::TreeArgs a;
   a.q = static_cast<const pl::bf16*>(q);
   a.kv = static_cast<const pl::bf16*>(kv_cache);
