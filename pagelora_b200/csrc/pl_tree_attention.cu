@@ -84,7 +84,12 @@ struct TreeCfg {
   static constexpr int kNumBars = 2 * kSlots + 8 + 1;  // full empty | s[2] p[2] o[2] q[2] | fin
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;  // tmem slot, flags, range, any_bad, 2 segments
   static constexpr int kSmemBytes = 1024 + kMiscOff + 64 + 2 * (int)sizeof(TreeSeg);
-  static constexpr int kTmemCols = 512;  // S_x at 128 x (P_x in its place), O_x at 256 + 128 x
+  // Scores take 128 columns at 128 * buf (P in their place), O_x at 256 +
+  // 128 x.  One row tile: its scores alternate between two buffers, so that
+  // the next tile's are computed during this one's softmax.
+  static constexpr int kTmemCols = 512;
+  __host__ __device__ static constexpr int buf(int x, int t) { return NT == 1 ? (t & 1) : x; }
+  __host__ __device__ static constexpr int phase(int t) { return NT == 1 ? (t >> 1) & 1 : t & 1; }
   static_assert(kSmemBytes <= 232448, "tree tiles exceed the shared-memory limit");
 };
 
@@ -243,13 +248,13 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
   uint64_t* full = bars;
   uint64_t* empty = bars + C::kSlots;
-  uint64_t* sready = bars + 2 * C::kSlots;  // [2] S_x of a tile in TMEM, O_x of the tiles before it complete
-  uint64_t* pready = sready + 2;            // [2] P_x in TMEM (8 warps)
-  uint64_t* odone = sready + 4;             // [2] O_x of a segment complete
+  uint64_t* sready = bars + 2 * C::kSlots;  // [2] scores of a tile in buffer [i]
+  uint64_t* pready = sready + 2;            // [2] P in buffer [i] (8 warps)
+  uint64_t* odone = sready + 4;             // [2] P_x.V of a tile complete
   uint64_t* qready = sready + 6;            // [2] Q_x of a segment staged (8 warps)
   uint64_t* fin = sready + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
-  volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, issued, consumed
+  volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, issued
   volatile int32_t* range = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 32);  // b, w, w_end, base
   uint32_t* any_bad = reinterpret_cast<uint32_t*>(smem + C::kMiscOff + 48);  // a drafted V held inf or NaN
   TreeSeg* segs = reinterpret_cast<TreeSeg*>(smem + C::kMiscOff + 64);       // [2] the softmax warps' segment
@@ -267,7 +272,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       mbar_init(&qready[x], 8);
     }
     mbar_init(fin, 1);
-    flags[0] = flags[1] = flags[2] = 0;
+    flags[0] = flags[1] = 0;
     any_bad[0] = 0;
     fence_barrier_init();
   }
@@ -356,10 +361,8 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
     if (lane == 0) {
       constexpr uint32_t idesc_s = umma_idesc_bf16(kTreeM, kTreeN);
       constexpr uint32_t idesc_o = umma_idesc_bf16(kTreeM, D) | (1u << 16);  // B (V) MN-major
-      int consumed = 0;
       auto wait_item = [&](int item) -> bool {
         const bool r = mbar_wait(&full[item % C::kSlots], (item / C::kSlots) & 1) && !flags[0];
-        if (r && item + 1 > consumed) consumed = item + 1;
         if (r) tc_fence_after();
         return r;
       };
@@ -370,16 +373,17 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         for (int c = 0; c < C::kChunks; ++c)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_bf16(tmem + (uint32_t)(x * kTreeN), umma_desc_k_sw128(qb + c * C::kChunkBytes + 32 * k),
+            umma_bf16(tmem + (uint32_t)(C::buf(x, t) * kTreeN), umma_desc_k_sw128(qb + c * C::kChunkBytes + 32 * k),
                       umma_desc_k_sw128(kb + c * C::kChunkBytes + 32 * k), idesc_s, (c | k) ? 1u : 0u);
-        umma_commit(&sready[x]);
+        umma_commit(&sready[C::buf(x, t)]);
       };
       auto issue_pv = [&](int x, int t, bool first) {
         const uint32_t vb = smem_u32(smem + C::kSlotOff + ((2 * t + 1) % C::kSlots) * C::kKVBytes);
 #pragma unroll
         for (int kk = 0; kk < kTreeN / 16; ++kk)
           // P of positions 0..63 starts at S_x's first column, of 64..127 at its 64th
-          umma_bf16_ts(tmem + (uint32_t)(256 + x * 128), tmem + (uint32_t)(x * kTreeN + (kk >> 2) * 64 + (kk & 3) * 8),
+          umma_bf16_ts(tmem + (uint32_t)(256 + x * 128),
+                       tmem + (uint32_t)(C::buf(x, t) * kTreeN + (kk >> 2) * 64 + (kk & 3) * 8),
                        umma_desc_mn_sw128(vb + kk * 16 * 128, C::kChunkBytes, 1024), idesc_o,
                        (!first || kk > 0) ? 1u : 0u);
       };
@@ -396,16 +400,22 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         umma_commit(&empty[(2 * t) % C::kSlots]);
         for (int j = sg.j0; ok && j < sg.j1; ++j, ++t) {
           const bool more = j + 1 < sg.j1;
+          if (NT == 1 && more) {  // the next scores are computed during this tile's softmax
+            ok = wait_item(2 * t + 2);
+            if (!ok) break;
+            issue_s(0, t + 1);
+            umma_commit(&empty[(2 * t + 2) % C::kSlots]);
+          }
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
-            ok = ok && mbar_wait(&pready[x], t & 1) && !flags[0];
+            ok = ok && mbar_wait(&pready[C::buf(x, t)], C::phase(t)) && !flags[0];
             if (ok && x == 0) ok = wait_item(2 * t + 1);
             if (!ok) break;
             tc_fence_after();
             issue_pv(x, t, j == sg.j0);
-            if (!more) umma_commit(&odone[x]);
+            umma_commit(&odone[x]);
             if (x == NT - 1) umma_commit(&empty[(2 * t + 1) % C::kSlots]);
-            if (more) {
+            if (NT == 2 && more) {
               if (x == 0) ok = wait_item(2 * t + 2);
               if (!ok) break;
               issue_s(x, t + 1);
@@ -418,7 +428,6 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         set_status(a.status, PL_ERR_TIMEOUT);
         flags[0] = 1;
       }
-      flags[2] = consumed;
       umma_commit(fin);
       if (!mbar_wait(fin, 0)) set_status(a.status, PL_ERR_TIMEOUT);
     }
@@ -437,7 +446,6 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
     const int quad = warp & 3;
     const int m = 32 * quad + lane;  // row of the tile == TMEM lane
     const uint32_t row_tmem = tmem + ((uint32_t)(32 * quad) << 16);
-    const uint32_t s_tmem = row_tmem + (uint32_t)(x * kTreeN + 64 * half);
     const uint32_t o_tmem = row_tmem + (uint32_t)(256 + x * 128 + half * (D / 2));
     const uint32_t pair_bar = 1 + x * 4 + quad;
     uint32_t* pair = reinterpret_cast<uint32_t*>(smem + C::kPairOff) + x * kTreeM + m;
@@ -476,10 +484,11 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       const int j1 = sg.j1;
       const int first_masked = (sg.kv_len - sg.n) / kTreeN;  // tiles from here on reach the drafted tokens
       for (int j = j0; j < j1; ++j, ++t) {
-        // S_x(j) was issued after P_x.V of the tile before: O_x is complete too
-        ok = ok && tree_warp_wait(&sready[x], t & 1, flags);
+        const int sb = C::buf(x, t);
+        const uint32_t s_tmem = row_tmem + (uint32_t)(sb * kTreeN + 64 * half);
+        ok = ok && tree_warp_wait(&sready[sb], C::phase(t), flags);
         if (!warp_ok) {
-          if (ok) tree_warp_arrive(&pready[x]);
+          if (ok) tree_warp_arrive(&pready[sb]);
           continue;
         }
         if (!ok) {
@@ -530,6 +539,11 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           const bool rescale = m_run != -INFINITY && m_new > m_run + kTreeSlack;
           const float alpha = rescale ? tr_exp2(m_run - m_new) : 1.f;
           if (__any_sync(0xffffffffu, rescale)) {
+            // O_x of the tiles before has to be complete.  Two row tiles: it
+            // is, S was issued after it.  One: S was issued after the P.V of
+            // the tile before the last, so phase t - 1 is the one to wait for.
+            if (NT == 1 && !tree_warp_wait(&odone[x], (t - 1) & 1, flags)) ok = false;
+            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               float o[16];
@@ -567,15 +581,15 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         // drafted token's V may hold inf or NaN that a row which masks the
         // token must not meet (0 * NaN is NaN): the former are cleared, the
         // latter's inf / NaN elements replaced by zero and noted, for the
-        // rows that do see them (epilogue).  Row 0's warps of tile 0 always
-        // have rows, so they do it for the CTA.
-        if (masked && x == 0 && quad == 0) {
+        // rows that do see them (epilogue).  All warps of tile 0 with rows do it.
+        if (masked && x == 0) {
           const int item = 2 * t + 1;
           if (tree_warp_wait(&full[item % C::kSlots], (item / C::kSlots) & 1, flags)) {
             uint8_t* vt = smem + C::kSlotOff + (item % C::kSlots) * C::kKVBytes;
             const int kv_len = sg.kv_len, ctx = kv_len - sg.n;
             const int r0 = max(ctx - j * kTreeN, 0), r_live = min(kTreeN, kv_len - j * kTreeN), units = C::kChunks * 8;
-            for (int idx = half * 32 + lane; idx < (kTreeN - r0) * units; idx += 64) {
+            const int quads = min(4, ((sg.n * a.group - sg.rt * C::kRows) + 31) / 32);
+            for (int idx = half * 32 * quads + m; idx < (kTreeN - r0) * units; idx += 64 * quads) {
               const int r = r0 + idx / units, hh = (idx / 8) % C::kChunks, u = idx % 8;
               uint4* at = reinterpret_cast<uint4*>(vt + hh * C::kChunkBytes + r * 128 + u * 16);
               if (r >= r_live) {
@@ -599,10 +613,13 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           }
         }
         tc_fence_before();
-        tree_warp_arrive(&pready[x]);
+        tree_warp_arrive(&pready[sb]);
       }
       // ---- epilogue of the segment: each thread of a row has half of its channels
-      if (ok) ok = tree_warp_wait(&odone[x], seg & 1, flags);
+      // (one row tile: the last scores only say that the P.V two tiles before
+      // is complete, so the phases are waited for one after the other)
+      if (NT == 1) ok = ok && tree_warp_wait(&odone[x], (t - 2) & 1, flags);
+      ok = ok && tree_warp_wait(&odone[x], (t - 1) & 1, flags);
       if (!ok) {
         if (lane == 0) set_status(a.status, PL_ERR_TIMEOUT);
         flags[0] = 1;
@@ -683,8 +700,10 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   // ------------------------------------------------------------ teardown
   __syncthreads();
   if (threadIdx.x == 0) {
-    const int issued = flags[1], consumed = flags[2];
-    for (int i = consumed; i < issued; ++i) (void)mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1);
+    // copies that were issued but not waited for (after a timeout) land before the exit
+    const int issued = flags[1];
+    for (int i = max(0, issued - C::kSlots); i < issued; ++i)
+      (void)mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1);
   }
   tc_fence_before();
   __syncthreads();
