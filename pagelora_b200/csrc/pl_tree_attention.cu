@@ -45,7 +45,7 @@ struct TreeArgs {
   const uint32_t* mask;  // [total_q][words]
   int64_t mask_stride;
   int64_t num_pages, total_pages;
-  int32_t words, batch, total_q, num_qo_heads, num_kv_heads, group, page_size, min_share, ctas;
+  int32_t words, batch, total_q, num_qo_heads, num_kv_heads, group, page_size, min_split, ctas;
   float scale_log2;
   bf16* out;
   int64_t out_stride_t, out_stride_h;
@@ -63,10 +63,11 @@ struct TreeSeg {
 template <int D, int NT>
 struct TreeCfg {
   static constexpr int kSoftmaxThreads = 256 * NT;  // two per row
-  // Softmax warps first, then the producer and the MMA warp; two idle warps
-  // complete the last warpgroup where registers are dealt anew.
-  static constexpr int kProducerWarp = 8 * NT, kMmaWarp = 8 * NT + 1;
-  static constexpr int kThreads = NT == 2 ? 640 : 64 + kSoftmaxThreads;
+  // Softmax warps first, then the K producer, the MMA and the V producer
+  // warp; an idle warp completes the last warpgroup where registers are
+  // dealt anew.
+  static constexpr int kProducerWarp = 8 * NT, kMmaWarp = 8 * NT + 1, kProducer2Warp = 8 * NT + 2;  // K, -, V
+  static constexpr int kThreads = NT == 2 ? 640 : 96 + kSoftmaxThreads;
   // NT = 2: 20 warps are launched with 96 registers a thread (5 warps per
   // scheduler); the softmax threads (4 warpgroups) take 104, the rest 64:
   // 512 * 104 + 128 * 64 = 640 * 96.  The host refuses another launch count.
@@ -124,43 +125,46 @@ struct TreeReq {
   __device__ __forceinline__ int work(int hkv) const { return rts * hkv * ntiles; }
 };
 
-// Total tiles over all requests, and the tiles in front of request `upto`
-// (one warp; every lane gets the results).
-__device__ __forceinline__ void tree_prefix(const TreeArgs& a, int rows, int upto, int& total, int& before) {
+// Inclusive prefix sum over a warp.
+__device__ __forceinline__ int tree_scan(int v) {
   const int lane = threadIdx.x & 31;
-  int t = 0, p = 0;
-  for (int b = lane; b < a.batch; b += 32) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Tiles of all requests (one warp).
+__device__ __forceinline__ int tree_total(const TreeArgs& a, int rows) {
+  int t = 0;
+  for (int b = threadIdx.x & 31; b < a.batch; b += 32) {
     TreeReq r;
     r.load(a, b, rows);
-    const int w = r.work(a.num_kv_heads);
-    t += w;
-    if (b < upto) p += w;
+    t += r.work(a.num_kv_heads);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    t += __shfl_xor_sync(0xffffffffu, t, o);
-    p += __shfl_xor_sync(0xffffffffu, p, o);
-  }
-  total = t;
-  before = p;
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  return t;
 }
 
-__device__ __forceinline__ int tree_share(int total, int ctas, int min_share) {
-  const int s = (total + ctas - 1) / ctas;
-  return s < min_share ? min_share : s;
-}
+// Tiles per CTA.
+__device__ __forceinline__ int tree_share(int total, int ctas) { return max(1, (total + ctas - 1) / ctas); }
 
-// The request that holds tile w of the line (batch: past the end) and its
-// first tile.  A cut that falls inside an item of at most min_share tiles
-// moves to the item's start, so short items are never split (and never
-// merged).  One warp.
+// The requests that hold tiles w0 and w1 of the line (batch: past the end)
+// and their first tiles.  A cut that falls inside an item of at most
+// min_split tiles moves to the item's start, so short items are never split
+// (and never merged).  One warp.
 struct TreeAt {
   int b, base, w;
 };
-__device__ __forceinline__ TreeAt tree_locate(const TreeArgs& a, int rows, int w) {
+__device__ __forceinline__ void tree_locate(const TreeArgs& a, int rows, TreeAt& at0, TreeAt& at1) {
   const int lane = threadIdx.x & 31;
-  TreeAt at{a.batch, 0, w};
-  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+  TreeAt* at[2] = {&at0, &at1};
+  int base = 0;
+  at0.b = at1.b = a.batch;
+  for (int b0 = 0; b0 < a.batch && at1.b == a.batch; b0 += 32) {
     TreeReq r;
     int n = 0;
     r.ntiles = 1;
@@ -168,24 +172,19 @@ __device__ __forceinline__ TreeAt tree_locate(const TreeArgs& a, int rows, int w
       r.load(a, b0 + lane, rows);
       n = r.work(a.num_kv_heads);
     }
-    int inc = n;
+    const int inc = base + tree_scan(n);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    const uint32_t hit = __ballot_sync(0xffffffffu, n > 0 && w < at.base + inc);
-    if (hit != 0) {
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t hit = __ballot_sync(0xffffffffu, n > 0 && at[i]->w < inc);
+      if (at[i]->b < a.batch || hit == 0) continue;
       const int l = __ffs(hit) - 1;
-      at.b = b0 + l;
-      at.base += __shfl_sync(0xffffffffu, inc - n, l);
+      at[i]->b = b0 + l;
+      at[i]->base = __shfl_sync(0xffffffffu, inc - n, l);
       const int nt = __shfl_sync(0xffffffffu, r.ntiles, l);
-      if (nt <= a.min_share) at.w = w - (w - at.base) % nt;
-      return at;
+      if (nt <= a.min_split) at[i]->w -= (at[i]->w - at[i]->base) % nt;
     }
-    at.base += __shfl_sync(0xffffffffu, inc, 31);
+    base = __shfl_sync(0xffffffffu, inc, 31);
   }
-  return at;
 }
 
 // Walks the item segments of the tile range [w, w_end).
@@ -254,7 +253,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   uint64_t* qready = sready + 6;            // [2] Q_x of a segment staged (8 warps)
   uint64_t* fin = sready + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
-  volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, issued
+  volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, K and V tiles issued
   volatile int32_t* range = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 32);  // b, w, w_end, base
   uint32_t* any_bad = reinterpret_cast<uint32_t*>(smem + C::kMiscOff + 48);  // a drafted V held inf or NaN
   TreeSeg* segs = reinterpret_cast<TreeSeg*>(smem + C::kMiscOff + 64);       // [2] the softmax warps' segment
@@ -272,89 +271,93 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       mbar_init(&qready[x], 8);
     }
     mbar_init(fin, 1);
-    flags[0] = flags[1] = 0;
+    flags[0] = flags[1] = flags[2] = 0;
     any_bad[0] = 0;
     fence_barrier_init();
   }
-  if (threadIdx.x == 32) prefetch_tensormap(&kv_map);
-  __syncthreads();
-  pdl_launch_dependents();
-  pdl_wait();
-
   if (warp == C::kProducerWarp) {
-    int total, dummy;
-    tree_prefix(a, C::kRows, 0, total, dummy);
-    const int share = tree_share(total, a.ctas, a.min_share);
-    const int w0 = (int)min((int64_t)total, (int64_t)blockIdx.x * share), w1 = min(total, w0 + share);
-    const TreeAt at0 = tree_locate(a, C::kRows, w0), at1 = tree_locate(a, C::kRows, w1);
+    if (lane == 0) prefetch_tensormap(&kv_map);
+    pdl_wait();
+    const int total = tree_total(a, C::kRows), share = tree_share(total, a.ctas);
+    TreeAt at0, at1;
+    at0.w = (int)min((int64_t)total, (int64_t)blockIdx.x * share);
+    at1.w = min(total, at0.w + share);
+    tree_locate(a, C::kRows, at0, at1);
     if (lane == 0) {
       range[0] = at0.b;
       range[1] = at0.w;
       range[2] = at1.w;
       range[3] = at0.base;
     }
-    // arguments that no launch can check on the host
-    if (blockIdx.x == 0)
-      for (int b = lane; b < a.batch; b += 32) {
-        TreeReq r;
-        r.load(a, b, C::kRows);
-        if (r.n != a.qo_indptr[b + 1] - r.q0 || r.n_pages != a.kv_indptr[b + 1] - r.kv_begin ||
-            r.n > 32 * a.words || r.n > r.kv_len)
-          set_status(a.status, PL_ERR_INVALID_ARGUMENT);
-      }
-  }
-  __syncthreads();
-  if (range[1] >= range[2]) return;  // nothing allocated yet
-
-  if (warp == C::kMmaWarp) {
+  } else if (warp == C::kMmaWarp) {
     tmem_alloc(tmem_slot, C::kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // after this wait a dependent grid may read the same tables: it is not
+  // released before every CTA has seen them complete
+  pdl_wait();
+  pdl_launch_dependents();
+  if (blockIdx.x == 0 && warp == C::kProducerWarp)  // arguments that no launch can check on the host
+    for (int b = lane; b < a.batch; b += 32) {
+      TreeReq r;
+      r.load(a, b, C::kRows);
+      if (r.n != a.qo_indptr[b + 1] - r.q0 || r.n_pages != a.kv_indptr[b + 1] - r.kv_begin || r.n > 32 * a.words ||
+          r.n > r.kv_len)
+        set_status(a.status, PL_ERR_INVALID_ARGUMENT);
+    }
   const uint32_t tmem = *tmem_slot;
-  TreeIter it{range[0], range[1], range[2], range[3]};
+  TreeIter it{range[0], range[1], range[2], range[3]};  // may be empty: nothing is loaded then
   const int PS = a.page_size;
 
-  if (warp == C::kProducerWarp) {
+  if (warp == C::kProducerWarp || warp == C::kProducer2Warp) {
     if constexpr (NT == 2) reg_dealloc<C::kOtherRegs>();
-    // ------------------------------------------------------------ producer
+    // ------------------------------------------------------------ producers
+    // One warp brings the K tiles, one the V tiles (ring item 2 t + kv): a
+    // page's box costs ~65 cycles of issue, 32 boxes a tile at 16-token
+    // pages, which one warp alone could not issue as fast as they arrive.
+    const int kv = warp == C::kProducerWarp ? 0 : 1;
     const int ppt = kTreeN / PS;
     const int boxes = ppt * C::kChunks;  // <= 16
     const int p = lane / C::kChunks, hh = lane % C::kChunks;
-    int i = 0;
+    int t = 0;
     bool go = true;
     TreeSeg sg;
     while (go && it.next(a, C::kRows, sg)) {
-      for (int j = sg.j0; go && j < sg.j1; ++j) {
-        // the tile's page (K and V alike); out of range: the copy writes zeros
+      // this lane's page of tile j; out of range: the copy writes zeros
+      auto page = [&](int j) {
         int32_t coord = (int32_t)(2 * a.num_pages);
-        if (lane < boxes && j * ppt + p < sg.n_pages) {
+        if (lane < boxes && j < sg.j1 && j * ppt + p < sg.n_pages) {
           const int32_t pid = a.kv_indices[sg.kv_begin + j * ppt + p];
           if (pid >= 0 && (int64_t)pid < a.num_pages)
-            coord = 2 * pid;
+            coord = 2 * pid + kv;
           else
             set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
         }
-        for (int kv = 0; kv < 2; ++kv, ++i) {
-          const int s = i % C::kSlots;
-          if (i >= C::kSlots && !tree_warp_wait(&empty[s], ((i / C::kSlots) - 1) & 1, flags)) {
-            if (lane == 0) set_status(a.status, PL_ERR_TIMEOUT);
-            flags[0] = 1;
-            go = false;
-            break;
-          }
-          if (lane == 0) mbar_arrive_expect_tx(&full[s], C::kKVBytes);
-          __syncwarp();
-          if (lane < boxes) {
-            uint8_t* dst = smem + C::kSlotOff + s * C::kKVBytes + hh * C::kChunkBytes + p * PS * 128;
-            tma_load_4d(dst, &kv_map, hh * 64, sg.kvh, 0, coord + kv, &full[s]);
-          }
+        return coord;
+      };
+      int32_t coord = page(sg.j0);
+      for (int j = sg.j0; j < sg.j1; ++j, ++t) {
+        const int32_t next = page(j + 1);
+        const int i = 2 * t + kv, s = i % C::kSlots;
+        if (i >= C::kSlots && !tree_warp_wait(&empty[s], ((i / C::kSlots) - 1) & 1, flags)) {
+          if (lane == 0) set_status(a.status, PL_ERR_TIMEOUT);
+          flags[0] = 1;
+          go = false;
+          break;
         }
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], C::kKVBytes);
+        __syncwarp();
+        if (lane < boxes) {
+          uint8_t* dst = smem + C::kSlotOff + s * C::kKVBytes + hh * C::kChunkBytes + p * PS * 128;
+          tma_load_4d(dst, &kv_map, hh * 64, sg.kvh, 0, coord, &full[s]);
+        }
+        coord = next;
       }
     }
-    if (lane == 0) flags[1] = i;
+    if (lane == 0) flags[1 + kv] = t;
   } else if (warp == C::kMmaWarp) {
     if constexpr (NT == 2) reg_dealloc<C::kOtherRegs>();
     // ---------------------------------------------------------- MMA issuer
@@ -431,7 +434,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       umma_commit(fin);
       if (!mbar_wait(fin, 0)) set_status(a.status, PL_ERR_TIMEOUT);
     }
-  } else if (warp > C::kMmaWarp) {
+  } else if (warp > C::kProducer2Warp) {
     if constexpr (NT == 2) reg_dealloc<C::kOtherRegs>();
   } else {
     if constexpr (NT == 2) reg_alloc<C::kSoftmaxRegs>();
@@ -482,12 +485,51 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       }
       float m_run = -INFINITY, l_run = 0.f;
       const int j1 = sg.j1;
+      // V rows past the last token hold whatever the pool had there, and a
+      // drafted token's V may hold inf or NaN that a row which masks the
+      // token must not meet (0 * NaN is NaN): the former are cleared, the
+      // latter's inf / NaN elements replaced by zero and noted, for the rows
+      // that do see them (epilogue).  Tile 0's warps without rows do it, or
+      // all of them when each has rows.
+      const int quads = min(4, (sg.n * a.group - sg.rt * C::kRows + 31) / 32);
+      auto clean_v = [&](int j, int t) {
+        const int item = 2 * t + 1;
+        if (!tree_warp_wait(&full[item % C::kSlots], (item / C::kSlots) & 1, flags)) return;
+        uint8_t* vt = smem + C::kSlotOff + (item % C::kSlots) * C::kKVBytes;
+        const int kv_len = sg.kv_len, ctx = kv_len - sg.n;
+        const int r0 = max(ctx - j * kTreeN, 0), r_live = min(kTreeN, kv_len - j * kTreeN), units = C::kChunks * 8;
+        const int per = quads == 4 ? 4 : 4 - quads;  // warps of each half that do it
+        const int at0 = (half * per + (quads == 4 ? quad : quad - quads)) * 32 + lane;
+        for (int idx = at0; idx < (kTreeN - r0) * units; idx += 64 * per) {
+          const int r = r0 + idx / units, hh = (idx / 8) % C::kChunks, u = idx % 8;
+          uint4* at = reinterpret_cast<uint4*>(vt + hh * C::kChunkBytes + r * 128 + u * 16);
+          if (r >= r_live) {
+            *at = make_uint4(0, 0, 0, 0);
+          } else {
+            uint4 e = *at;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&e);
+            bool hit = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if ((w[k] & 0x7f80u) == 0x7f80u) { w[k] &= 0xffff0000u; hit = true; }
+              if ((w[k] & 0x7f800000u) == 0x7f800000u) { w[k] &= 0x0000ffffu; hit = true; }
+            }
+            if (hit) {
+              *at = e;
+              atomicOr(any_bad, 1u);
+            }
+          }
+        }
+        fence_proxy_async_smem();
+      };
       const int first_masked = (sg.kv_len - sg.n) / kTreeN;  // tiles from here on reach the drafted tokens
       for (int j = j0; j < j1; ++j, ++t) {
         const int sb = C::buf(x, t);
         const uint32_t s_tmem = row_tmem + (uint32_t)(sb * kTreeN + 64 * half);
         ok = ok && tree_warp_wait(&sready[sb], C::phase(t), flags);
+        const bool masked = j >= first_masked;  // uniform over the CTA
         if (!warp_ok) {
+          if (ok && masked && x == 0) clean_v(j, t);
           if (ok) tree_warp_arrive(&pready[sb]);
           continue;
         }
@@ -496,7 +538,6 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           continue;
         }
         tc_fence_after();
-        const bool masked = j >= first_masked;  // uniform over the CTA
         float v[64];
         tmem_ld64(s_tmem, v);
         if (masked) {
@@ -577,41 +618,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         sm[0] = add_f32x2(add_f32x2(sm[0], sm[1]), add_f32x2(sm[2], sm[3]));
         l_run += sm[0].x + sm[0].y;
         tmem_st_wait();
-        // V rows past the last token hold whatever the pool had there, and a
-        // drafted token's V may hold inf or NaN that a row which masks the
-        // token must not meet (0 * NaN is NaN): the former are cleared, the
-        // latter's inf / NaN elements replaced by zero and noted, for the
-        // rows that do see them (epilogue).  All warps of tile 0 with rows do it.
-        if (masked && x == 0) {
-          const int item = 2 * t + 1;
-          if (tree_warp_wait(&full[item % C::kSlots], (item / C::kSlots) & 1, flags)) {
-            uint8_t* vt = smem + C::kSlotOff + (item % C::kSlots) * C::kKVBytes;
-            const int kv_len = sg.kv_len, ctx = kv_len - sg.n;
-            const int r0 = max(ctx - j * kTreeN, 0), r_live = min(kTreeN, kv_len - j * kTreeN), units = C::kChunks * 8;
-            const int quads = min(4, ((sg.n * a.group - sg.rt * C::kRows) + 31) / 32);
-            for (int idx = half * 32 * quads + m; idx < (kTreeN - r0) * units; idx += 64 * quads) {
-              const int r = r0 + idx / units, hh = (idx / 8) % C::kChunks, u = idx % 8;
-              uint4* at = reinterpret_cast<uint4*>(vt + hh * C::kChunkBytes + r * 128 + u * 16);
-              if (r >= r_live) {
-                *at = make_uint4(0, 0, 0, 0);
-              } else {
-                uint4 e = *at;
-                uint32_t* w = reinterpret_cast<uint32_t*>(&e);
-                bool hit = false;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  if ((w[k] & 0x7f80u) == 0x7f80u) { w[k] &= 0xffff0000u; hit = true; }
-                  if ((w[k] & 0x7f800000u) == 0x7f800000u) { w[k] &= 0x0000ffffu; hit = true; }
-                }
-                if (hit) {
-                  *at = e;
-                  atomicOr(any_bad, 1u);
-                }
-              }
-            }
-            fence_proxy_async_smem();
-          }
-        }
+        if (masked && x == 0 && quads == 4) clean_v(j, t);
         tc_fence_before();
         tree_warp_arrive(&pready[sb]);
       }
@@ -701,9 +708,10 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   __syncthreads();
   if (threadIdx.x == 0) {
     // copies that were issued but not waited for (after a timeout) land before the exit
-    const int issued = flags[1];
-    for (int i = max(0, issued - C::kSlots); i < issued; ++i)
-      (void)mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1);
+    auto issued = [&](int i) { return (i >> 1) < flags[1 + (i & 1)]; };
+    const int most = 2 * max((int)flags[1], (int)flags[2]);
+    for (int i = max(0, most - 2 * C::kSlots); i < most; ++i)
+      if (issued(i) && !issued(i + C::kSlots)) (void)mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1);
   }
   tc_fence_before();
   __syncthreads();
@@ -714,51 +722,66 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
 }
 
 // Joins the partial states of the items that several CTAs shared: one warp
-// per (query token, head), the states weighted by 2^(m - max m).
+// per (query token, head), the states weighted by 2^(m - max m).  The tables
+// are read before the wait for the attention's grid (which lets this one
+// start only once they are complete).
+constexpr int kMergeThreads = 128;
 template <int D>
-__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int rows) {
-  pdl_launch_dependents();
-  pdl_wait();
+__global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArgs a, int rows) {
   const int lane = threadIdx.x & 31;
   const int tok_g = blockIdx.x;
-  // the request of this token
-  int req = a.batch;
-  for (int b0 = 0; b0 < a.batch && req == a.batch; b0 += 32) {
-    const int b = b0 + lane;
-    const bool in = b < a.batch && a.qo_indptr[b] <= tok_g && tok_g < a.qo_indptr[b + 1];
-    const uint32_t hit = __ballot_sync(0xffffffffu, in);
-    if (hit != 0) req = b0 + __ffs(hit) - 1;
-  }
-  if (req == a.batch) return;
-  TreeReq r;
-  r.load(a, req, rows);
-  if (r.ntiles <= a.min_share || r.n == 0) return;  // never split
-  int total, base;
-  tree_prefix(a, rows, req, total, base);
-  const int share = tree_share(total, a.ctas, a.min_share);
-  for (int head = threadIdx.x / 32; head < a.num_qo_heads; head += blockDim.x / 32) {
-    const int row = (tok_g - r.q0) * a.group + head % a.group;
-    const int w = base + ((head / a.group) * r.rts + row / rows) * r.ntiles;
-    const int m = row % rows;
-    const int64_t ca = w / share, cb = (w + r.ntiles - 1) / share;
-    if (ca == cb) continue;
-    auto slot = [&](int64_t c) { return 2 * c + (c == ca ? 1 : 0); };
-    float M = -INFINITY;
-    for (int64_t c = ca + lane; c <= cb; c += 32) {
-      const float v = a.part_ml[slot(c) * 2 * rows + m];
-      M = fmaxf(M, v);
+  // the request of this token, the tiles in front of it, and all tiles
+  int q0 = 0, rts = 0, nt = 0, base = 0, total = 0;
+  bool found = false;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    TreeReq r;
+    r.n = r.rts = r.ntiles = r.q0 = 0;
+    if (b0 + lane < a.batch) r.load(a, b0 + lane, rows);
+    const int w = r.work(a.num_kv_heads), inc = total + tree_scan(w);
+    const uint32_t hit = __ballot_sync(0xffffffffu, r.q0 <= tok_g && tok_g < r.q0 + r.n);
+    if (hit != 0 && !found) {
+      const int l = __ffs(hit) - 1;
+      found = true;
+      q0 = __shfl_sync(0xffffffffu, r.q0, l);
+      rts = __shfl_sync(0xffffffffu, r.rts, l);
+      nt = __shfl_sync(0xffffffffu, r.ntiles, l);
+      base = __shfl_sync(0xffffffffu, inc - w, l);
     }
-    M = warp_max(M);
-    constexpr int E = D / 32;
-    float acc[E], L = 0.f;
+    total = __shfl_sync(0xffffffffu, inc, 31);
+  }
+  const int share = tree_share(total, a.ctas);
+  const int head = blockIdx.y * (kMergeThreads / 32) + threadIdx.x / 32;
+  const int row = (tok_g - q0) * a.group + head % a.group;
+  const int w = base + ((head / a.group) * rts + row / rows) * nt;
+  const int m = row % rows;
+  const int ca = w / share, cb = (w + nt - 1) / share;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (!found || nt <= a.min_split || head >= a.num_qo_heads || ca == cb) return;  // not split
+  auto slot = [&](int c) { return (int64_t)(2 * c + (c == ca ? 1 : 0)); };
+  constexpr int E = D / 32;
+  float acc[E], L = 0.f, M = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 4
-    for (int64_t c = ca; c <= cb; ++c) {
-      const float* ml = a.part_ml + slot(c) * 2 * rows + m;
-      const float mc = ml[0], lc = ml[rows];
-      const float wt = mc == -INFINITY ? 0.f : exp2f(mc - M);
-      const float* o = a.part_o + (slot(c) * rows + m) * D + lane * E;
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int c0 = ca; c0 <= cb; c0 += 32) {
+    // a lane per state: its maximum and sum; then all lanes add the states up
+    float mc = -INFINITY, lc = 0.f;
+    if (c0 + lane <= cb) {
+      const float* ml = a.part_ml + slot(c0 + lane) * 2 * rows + m;
+      mc = ml[0];
+      lc = ml[rows];
+    }
+    const float m_new = fmaxf(M, warp_max(mc));
+    const float old = M == -INFINITY ? 0.f : exp2f(M - m_new);
+    const float wt = mc == -INFINITY ? 0.f : exp2f(mc - m_new);
+    L = L * old + warp_sum(mc == -INFINITY ? 0.f : wt * lc);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= old;
+    M = m_new;
+    const int n = min(32, cb - c0 + 1);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float* o = a.part_o + (slot(c0 + i) * rows + m) * D + lane * E;
       float v[E];
       if constexpr (E == 4) {
         const float4 f = *reinterpret_cast<const float4*>(o);
@@ -767,23 +790,22 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int r
         const float2 f = *reinterpret_cast<const float2*>(o);
         v[0] = f.x; v[1] = f.y;
       }
-      if (mc != -INFINITY) {  // a state that saw nothing holds no values
-        L += wt * lc;
+      const float wi = __shfl_sync(0xffffffffu, wt, i);
+      const bool saw = __shfl_sync(0xffffffffu, mc, i) != -INFINITY;  // else the state holds no values
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += wt * v[e];
-      }
+      for (int e = 0; e < E; ++e) acc[e] += saw ? wi * v[e] : 0.f;
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    bf16* dst = a.out + (int64_t)tok_g * a.out_stride_t + (int64_t)head * a.out_stride_h + lane * E;
-    if constexpr (E == 4) {
-      *reinterpret_cast<uint2*>(dst) =
-          make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
-    } else {
-      *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-    }
-    if (a.lse != nullptr && lane == 0)
-      a.lse[(int64_t)tok_g * a.num_qo_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
   }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  bf16* dst = a.out + (int64_t)tok_g * a.out_stride_t + (int64_t)head * a.out_stride_h + lane * E;
+  if constexpr (E == 4) {
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+  } else {
+    *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  }
+  if (a.lse != nullptr && lane == 0)
+    a.lse[(int64_t)tok_g * a.num_qo_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
 // --------------------------------------------------------------- the tree
@@ -903,7 +925,7 @@ bool tree_two_tiles(int total_q, int batch, int group) {
   return (int64_t)total_q * group > (int64_t)batch * pl::kTreeM;
 }
 
-constexpr int kTreeMinShare = 2;
+constexpr int kTreeMinSplit = 2;
 
 template <int D, int NT>
 int32_t launch_tree(const CUtensorMap& map, const pl::TreeArgs& a, bool merge, void* stream) {
@@ -920,7 +942,9 @@ int32_t launch_tree(const CUtensorMap& map, const pl::TreeArgs& a, bool merge, v
   }
   st = pl_host::launch_pdl(kern, dim3(a.ctas), dim3(C::kThreads), C::kSmemBytes, stream, map, a);
   if (st != PL_OK || !merge) return st;
-  return pl_host::launch_pdl(pl::tree_merge_kernel<D>, dim3(a.total_q), dim3(256), 0, stream, a, (int)C::kRows);
+  constexpr int warps = pl::kMergeThreads / 32;
+  return pl_host::launch_pdl(pl::tree_merge_kernel<D>, dim3(a.total_q, (a.num_qo_heads + warps - 1) / warps),
+                             dim3(pl::kMergeThreads), 0, stream, a, (int)C::kRows);
 }
 
 }  // namespace
@@ -956,8 +980,8 @@ extern "C" int32_t pl_paged_tree_attention(
       (out_stride_t % 8) != 0 || (out_stride_h % 8) != 0)
     return PL_ERR_INVALID_ARGUMENT;
   if (batch == 0 || total_q == 0) return PL_OK;
-  // no request has more than total_pages pages: below kTreeMinShare tiles nothing is split
-  const bool merge = total_pages * page_size > (int64_t)kTreeMinShare * pl::kTreeN;
+  // no request has more than total_pages pages: below kTreeMinSplit tiles nothing is split
+  const bool merge = total_pages * page_size > (int64_t)kTreeMinSplit * pl::kTreeN;
   if (merge && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
                 workspace_bytes < pl_tree_workspace_bytes(batch, total_q, num_qo_heads, num_kv_heads, head_dim)))
     return PL_ERR_WORKSPACE_TOO_SMALL;
@@ -992,7 +1016,7 @@ extern "C" int32_t pl_paged_tree_attention(
   a.num_kv_heads = num_kv_heads;
   a.group = group;
   a.page_size = page_size;
-  a.min_share = kTreeMinShare;
+  a.min_split = kTreeMinSplit;
   a.ctas = sms;
   a.scale_log2 = sm_scale * pl::kLog2e;
   a.out = static_cast<pl::bf16*>(out);
