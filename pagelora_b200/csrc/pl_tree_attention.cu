@@ -224,11 +224,21 @@ __device__ __forceinline__ uint32_t tree_bits(const uint32_t* row, int words, in
   return __funnelshift_r(lo, hi, s);
 }
 
+// Wait for a phase of `bar`; false when it ran out or the CTA gave up (looked
+// at only while polling, so a wait that is met costs one poll).
+__device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, volatile int32_t* flags) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long c0 = clock64();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 0 && (flags[0] != 0 || clock64() - c0 > kWaitTimeoutCycles)) return false;
+  }
+}
 // Wait of a whole warp: one lane polls (many pollers of one barrier slow all
-// shared-memory traffic).  false: the wait ran out or the CTA gave up.
+// shared-memory traffic).
 __device__ __forceinline__ bool tree_warp_wait(uint64_t* bar, uint32_t parity, volatile int32_t* flags) {
   int ok = 0;
-  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity) && flags[0] == 0;
+  if ((threadIdx.x & 31) == 0) ok = tree_wait(bar, parity, flags);
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 // Arrival of a whole warp: its tensor-memory and shared-memory accesses are
@@ -249,7 +259,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   uint64_t* empty = bars + C::kSlots;
   uint64_t* sready = bars + 2 * C::kSlots;  // [2] scores of a tile in buffer [i]
   uint64_t* pready = sready + 2;            // [2] P in buffer [i] (8 warps)
-  uint64_t* odone = sready + 4;             // [2] P_x.V of a tile complete
+  uint64_t* odone = sready + 4;             // [2] P_x.V of a tile (two row tiles: of a segment) complete
   uint64_t* qready = sready + 6;            // [2] Q_x of a segment staged (8 warps)
   uint64_t* fin = sready + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
@@ -326,21 +336,13 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
     bool go = true;
     TreeSeg sg;
     while (go && it.next(a, C::kRows, sg)) {
-      // this lane's page of tile j; out of range: the copy writes zeros
+      // This lane's page of tile j (-1: past the row's pages), read two tiles ahead.
       auto page = [&](int j) {
-        int32_t coord = (int32_t)(2 * a.num_pages);
-        if (lane < boxes && j < sg.j1 && j * ppt + p < sg.n_pages) {
-          const int32_t pid = a.kv_indices[sg.kv_begin + j * ppt + p];
-          if (pid >= 0 && (int64_t)pid < a.num_pages)
-            coord = 2 * pid + kv;
-          else
-            set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
-        }
-        return coord;
+        return lane < boxes && j < sg.j1 && j * ppt + p < sg.n_pages ? a.kv_indices[sg.kv_begin + j * ppt + p] : -1;
       };
-      int32_t coord = page(sg.j0);
+      int32_t pid = page(sg.j0), pid1 = page(sg.j0 + 1);
       for (int j = sg.j0; j < sg.j1; ++j, ++t) {
-        const int32_t next = page(j + 1);
+        const int32_t pid2 = page(j + 2);
         const int i = 2 * t + kv, s = i % C::kSlots;
         if (i >= C::kSlots && !tree_warp_wait(&empty[s], ((i / C::kSlots) - 1) & 1, flags)) {
           if (lane == 0) set_status(a.status, PL_ERR_TIMEOUT);
@@ -351,10 +353,14 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         if (lane == 0) mbar_arrive_expect_tx(&full[s], C::kKVBytes);
         __syncwarp();
         if (lane < boxes) {
+          const bool in = pid >= 0 && (int64_t)pid < a.num_pages;
+          if (!in && j * ppt + p < sg.n_pages) set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
           uint8_t* dst = smem + C::kSlotOff + s * C::kKVBytes + hh * C::kChunkBytes + p * PS * 128;
-          tma_load_4d(dst, &kv_map, hh * 64, sg.kvh, 0, coord, &full[s]);
+          // out of range: the copy writes zeros
+          tma_load_4d(dst, &kv_map, hh * 64, sg.kvh, 0, in ? 2 * pid + kv : (int32_t)(2 * a.num_pages), &full[s]);
         }
-        coord = next;
+        pid = pid1;
+        pid1 = pid2;
       }
     }
     if (lane == 0) flags[1 + kv] = t;
@@ -365,9 +371,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       constexpr uint32_t idesc_s = umma_idesc_bf16(kTreeM, kTreeN);
       constexpr uint32_t idesc_o = umma_idesc_bf16(kTreeM, D) | (1u << 16);  // B (V) MN-major
       auto wait_item = [&](int item) -> bool {
-        const bool r = mbar_wait(&full[item % C::kSlots], (item / C::kSlots) & 1) && !flags[0];
-        if (r) tc_fence_after();
-        return r;
+        return tree_wait(&full[item % C::kSlots], (item / C::kSlots) & 1, flags);
       };
       auto issue_s = [&](int x, int t) {
         const uint32_t qb = smem_u32(smem + C::kQOff + x * C::kQBytes);
@@ -395,35 +399,37 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       TreeSeg sg;
       for (int seg = 0; ok && it.next(a, C::kRows, sg); ++seg) {
 #pragma unroll
-        for (int x = 0; x < NT; ++x) ok = ok && mbar_wait(&qready[x], seg & 1);
+        for (int x = 0; x < NT; ++x) ok = ok && tree_wait(&qready[x], seg & 1, flags);
         ok = ok && wait_item(2 * t);
         if (!ok) break;
+        tc_fence_after();
 #pragma unroll
         for (int x = 0; x < NT; ++x) issue_s(x, t);
         umma_commit(&empty[(2 * t) % C::kSlots]);
         for (int j = sg.j0; ok && j < sg.j1; ++j, ++t) {
           const bool more = j + 1 < sg.j1;
+          // K of the next tile and V of this one are waited for in front of
+          // P, whose arrival starts the products
+          if (more) ok = wait_item(2 * t + 2);
+          if (!ok) break;
           if (NT == 1 && more) {  // the next scores are computed during this tile's softmax
-            ok = wait_item(2 * t + 2);
-            if (!ok) break;
+            tc_fence_after();
             issue_s(0, t + 1);
             umma_commit(&empty[(2 * t + 2) % C::kSlots]);
           }
+          ok = wait_item(2 * t + 1);
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
-            ok = ok && mbar_wait(&pready[C::buf(x, t)], C::phase(t)) && !flags[0];
-            if (ok && x == 0) ok = wait_item(2 * t + 1);
+            ok = ok && tree_wait(&pready[C::buf(x, t)], C::phase(t), flags);
             if (!ok) break;
             tc_fence_after();
             issue_pv(x, t, j == sg.j0);
-            umma_commit(&odone[x]);
-            if (x == NT - 1) umma_commit(&empty[(2 * t + 1) % C::kSlots]);
             if (NT == 2 && more) {
-              if (x == 0) ok = wait_item(2 * t + 2);
-              if (!ok) break;
               issue_s(x, t + 1);
               if (x == NT - 1) umma_commit(&empty[(2 * t + 2) % C::kSlots]);
             }
+            if (NT == 1 || !more) umma_commit(&odone[x]);
+            if (x == NT - 1) umma_commit(&empty[(2 * t + 1) % C::kSlots]);
           }
         }
       }
@@ -626,7 +632,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       // (one row tile: the last scores only say that the P.V two tiles before
       // is complete, so the phases are waited for one after the other)
       if (NT == 1) ok = ok && tree_warp_wait(&odone[x], (t - 2) & 1, flags);
-      ok = ok && tree_warp_wait(&odone[x], (t - 1) & 1, flags);
+      ok = ok && tree_warp_wait(&odone[x], (NT == 1 ? t - 1 : seg) & 1, flags);
       if (!ok) {
         if (lane == 0) set_status(a.status, PL_ERR_TIMEOUT);
         flags[0] = 1;
