@@ -104,7 +104,6 @@ constexpr int kSparseThreads = 256;
 constexpr int kSparseWarps = kSparseThreads / 32;
 constexpr int kSparseUnit = 16;          // tokens a warp takes at a time
 constexpr int kSparseMaxCluster = 8;
-constexpr int kSparseKeys = 8192;        // keys held in shared memory; longer rows read them from L2 in every pass
 constexpr int kSparseBins = 2048;        // 11 bits of the key per pass
 
 struct SparseArgs {
@@ -160,57 +159,77 @@ __device__ __forceinline__ void mma_s8_16832(int* d, const uint32_t* a, uint32_t
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Keys of the pages of (row b, kv head): a matrix product of the group's
-// quantised queries (rows; per head min(qi, 0) against lo and max(qi, 0)
-// against hi, 2 D bytes) with the bounds of 8 pages a warp and step.  The
-// product's order along 2 D is free, so a lane's operand is what it loads:
-// 16 contiguous bytes of its page per 64.
+// Keys of the pages of row b.  A warp has one kv head and 8 pages a step: a
+// matrix product of the group's quantised queries (rows; per head min(qi, 0)
+// against lo and max(qi, 0) against hi, 2 D bytes) with the pages' bounds.
+// The product's order along 2 D is free, so a lane's operand is what it
+// loads: 16 contiguous bytes of its page per 64.  The warps of a CTA take
+// neighbouring heads of the same pages, whose bounds lie side by side.
 template <int D>
-__global__ void __launch_bounds__(kSparseThreads) sparse_score_kernel(const SparseArgs a) {
+__global__ void __launch_bounds__(kSparseThreads, 3) sparse_score_kernel(const SparseArgs a) {
   constexpr int kBytes = 2 * D;          // bounds of one page and head
   constexpr int kLd = kBytes / 64;       // 16-byte loads of a lane per page
-  __shared__ __align__(16) int8_t qs[16][kBytes + 16];
-  __shared__ float red[kSparseWarps];
+  __shared__ __align__(16) int8_t qs_all[kSparseWarps][16][kBytes + 16];
   pdl_wait();
   pdl_launch_dependents();
-  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int b = blockIdx.z;
   SparseRow r;
   r.load(a, b);
-  // pages that compete; forced ones have no key
-  const int p_end = r.pages - a.recent;
-  const int step = gridDim.x * kSparseWarps * 8;
-  if (r.pages <= a.select || a.sink + (int)blockIdx.x * kSparseWarps * 8 >= p_end) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  int p = a.sink + ((int)blockIdx.x * kSparseWarps + warp) * 8;
-  int pid = p + g < p_end ? a.indices[r.begin + p + g] : -1;
+  // heads side by side, and groups of 8 pages when there are fewer heads than warps
+  const int hw = min(kSparseWarps, a.num_kv_heads), pw = kSparseWarps / hw;
+  const int kvh = (int)blockIdx.y * kSparseWarps + warp % hw;
+  // pages that compete; forced ones have no key
+  const int p_end = r.pages - a.recent;
+  const int step = gridDim.x * pw * 8;
+  int p = a.sink + ((int)blockIdx.x * pw + warp / hw) * 8;
+  if (r.pages <= a.select || p >= p_end || warp >= hw * pw || kvh >= a.num_kv_heads) return;  // no block barrier below
 
-  // quantise the group's queries; a thread keeps its elements in registers
-  constexpr int kMost = 16 * D / kSparseThreads;
-  float v[kMost], m = 0.f;
+  auto page = [&](int at) { return at + g < p_end ? a.indices[r.begin + at + g] : -1; };
+  int pid = page(p);
+  // quantise the group's queries: 8 channels a lane and step
+  int8_t(*qs)[kBytes + 16] = qs_all[warp];
+  constexpr int kMost = 16 * D / 256;
+  uint4 qv[kMost];
+  float m = 0.f;
 #pragma unroll
   for (int k = 0; k < kMost; ++k) {
-    const int i = threadIdx.x + k * kSparseThreads;
-    v[k] = i < a.group * D
-               ? bf2f(a.q[(int64_t)b * a.q_stride_b + (int64_t)(kvh * a.group + i / D) * a.q_stride_h + i % D])
-               : 0.f;
-    m = fmaxf(m, fabsf(v[k]));
+    const int i = (k * 32 + lane) * 8;
+    qv[k] = i < a.group * D ? *reinterpret_cast<const uint4*>(a.q + (int64_t)b * a.q_stride_b +
+                                                              (int64_t)(kvh * a.group + i / D) * a.q_stride_h + i % D)
+                            : make_uint4(0, 0, 0, 0);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&qv[k]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack_bf16x2(w[e]);
+      m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+    }
   }
   m = warp_max(m);
-  if (lane == 0) red[warp] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kSparseWarps; ++w) m = fmaxf(m, red[w]);
-  const float sq = __fmul_rn(m, 1.0f / 127.0f);
+  const float sq = __fmul_rn(m, 1.0f / 127.0f), div = sq > 0.f ? sq : 1.f;
 #pragma unroll
   for (int k = 0; k < kMost; ++k) {
-    const int i = threadIdx.x + k * kSparseThreads;
-    const float x = rintf(__fdiv_rn(v[k], sq > 0.f ? sq : 1.f));
-    const int qi = isfinite(x) ? (int)fminf(fmaxf(x, -127.f), 127.f) : 0;
-    qs[i / D][i % D] = (int8_t)min(qi, 0);
-    qs[i / D][D + i % D] = (int8_t)max(qi, 0);
+    const int i = (k * 32 + lane) * 8;
+    if (k * 256 >= a.group * D) {  // no head's
+      *reinterpret_cast<uint2*>(&qs[i / D][i % D]) = make_uint2(0, 0);
+      *reinterpret_cast<uint2*>(&qs[i / D][D + i % D]) = make_uint2(0, 0);
+      continue;
+    }
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&qv[k]);
+    int8_t neg[8], pos[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 f = unpack_bf16x2(w[e / 2]);
+      const float x = rintf(__fdiv_rn(e % 2 ? f.y : f.x, div));
+      const int qi = isfinite(x) ? (int)fminf(fmaxf(x, -127.f), 127.f) : 0;
+      neg[e] = (int8_t)min(qi, 0);
+      pos[e] = (int8_t)max(qi, 0);
+    }
+    *reinterpret_cast<uint2*>(&qs[i / D][i % D]) = *reinterpret_cast<uint2*>(neg);
+    *reinterpret_cast<uint2*>(&qs[i / D][D + i % D]) = *reinterpret_cast<uint2*>(pos);
   }
-  __syncthreads();
+  __syncwarp();
   uint32_t qa[2 * kLd][4];
 #pragma unroll
   for (int j = 0; j < kLd; ++j)
@@ -225,21 +244,33 @@ __global__ void __launch_bounds__(kSparseThreads) sparse_score_kernel(const Spar
       qa[2 * j + h][3] = hi.y;
     }
   uint32_t* keys = a.keys + ((int64_t)b * a.num_kv_heads + kvh) * a.max_pages;
-  for (; p < p_end; p += step) {
-    const bool in = pid >= 0 && (int64_t)pid < a.num_pages;
-    if (!in && p + g < p_end && t == 0) set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
-    const int64_t slot = (int64_t)(in ? pid : 0) * a.num_kv_heads + kvh;
-    const uint4* src = reinterpret_cast<const uint4*>(a.bounds + slot * kBytes) + t;
+  // bounds are loaded a step ahead, page ids two
+  struct Step {
     uint4 w[kLd];
+    float sc;
+    bool in;
+  };
+  auto fetch = [&](Step& s, int at, int id) {
+    s.in = id >= 0 && (int64_t)id < a.num_pages;
+    if (!s.in && at + g < p_end && t == 0) set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
+    const int64_t slot = (int64_t)(s.in ? id : 0) * a.num_kv_heads + kvh;
+    const uint4* src = reinterpret_cast<const uint4*>(a.bounds + slot * kBytes) + t;
 #pragma unroll
-    for (int j = 0; j < kLd; ++j) w[j] = in ? __ldg(src + 4 * j) : make_uint4(0, 0, 0, 0);
-    const float sc = in ? __ldg(a.scale + slot) : 0.f;
-    pid = p + step + g < p_end ? a.indices[r.begin + p + step + g] : -1;
+    for (int j = 0; j < kLd; ++j) s.w[j] = s.in ? __ldg(src + 4 * j) : make_uint4(0, 0, 0, 0);
+    s.sc = s.in ? __ldg(a.scale + slot) : 0.f;
+  };
+  Step cur;
+  fetch(cur, p, pid);
+  pid = page(p + step);
+  for (; p < p_end; p += step) {
+    Step next;
+    if (p + step < p_end) fetch(next, p + step, pid);
+    pid = page(p + 2 * step);
     int c[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < kLd; ++j) {
-      mma_s8_16832(c, qa[2 * j], w[j].x, w[j].y);
-      mma_s8_16832(c, qa[2 * j + 1], w[j].z, w[j].w);
+      mma_s8_16832(c, qa[2 * j], cur.w[j].x, cur.w[j].y);
+      mma_s8_16832(c, qa[2 * j + 1], cur.w[j].z, cur.w[j].w);
     }
     // rows g and g + 8 of pages 2 t and 2 t + 1: the maximum over the heads
     int s0 = max(g < a.group ? c[0] : INT32_MIN, g + 8 < a.group ? c[2] : INT32_MIN);
@@ -254,8 +285,9 @@ __global__ void __launch_bounds__(kSparseThreads) sparse_score_kernel(const Spar
     const int e0 = __shfl_sync(0xffffffffu, s0, from), e1 = __shfl_sync(0xffffffffu, s1, from);
     if (t == 0 && p + g < p_end) {
       const int best = (g & 1) ? e1 : e0;
-      keys[p + g] = in ? order_key(isinf(sc) ? INFINITY : __fmul_rn((float)best, sc)) : 0u;
+      keys[p + g] = cur.in ? order_key(isinf(cur.sc) ? INFINITY : __fmul_rn((float)best, cur.sc)) : 0u;
     }
+    cur = next;
   }
 }
 
@@ -263,19 +295,20 @@ template <int D>
 struct SparseCfg {
   static constexpr int kRow = 2 * D;                           // bytes of one token's K (or V)
   static constexpr int kTile = kSparseUnit * kRow;             // K (or V) of one unit
-  static constexpr int kQRow = 2 * D + 16;                     // padded: conflict-free ldmatrix
   static constexpr int kOPad = D + 4;
-  static constexpr int kStages = kSparseWarps * 2 * kTile;     // a warp's unit: K, V
+  static constexpr int kRing = 3;                              // tiles (K, V, K, ...) of a warp in flight
+  static constexpr int kStages = kSparseWarps * kRing * kTile;
   static constexpr int kScratch = kSparseWarps * 16 * kOPad * 4;
-  static constexpr int kSelect = (kSparseKeys + kSparseBins) * 4;
-  // the selection, the units in flight and the join of the warps' states use
+  static constexpr int kSelect = kSparseBins * 4;
+  // the selection, the tiles in flight and the join of the warps' states use
   // the same bytes one after the other
   static constexpr int kArena = kStages > kScratch ? (kStages > kSelect ? kStages : kSelect)
                                                    : (kScratch > kSelect ? kScratch : kSelect);
-  static constexpr int kQOff = kArena;
-  static constexpr int kPartOff = kQOff + 16 * kQRow;          // [16][D] fp32: this CTA's state for the cluster
-  static constexpr int kMlOff = kPartOff + 16 * D * 4;         // [2][16] of the CTA, then [2][warps][16]
-  static constexpr int kListOff = kMlOff + (2 + 2 * kSparseWarps) * 16 * 4;
+  // what the cluster's CTAs send here: float4 chunks [i][CTA], and [CTA][2][16] m, l
+  static constexpr int kRecvOff = kArena;
+  static constexpr int kRecvMlOff = kRecvOff + (16 * D / 4 + kSparseMaxCluster) * 16;
+  static constexpr int kMlOff = kRecvMlOff + kSparseMaxCluster * 32 * 4;  // [2][warps][16]
+  static constexpr int kListOff = kMlOff + 2 * kSparseWarps * 16 * 4;
 };
 
 // Block-wide exclusive prefix sum of one value per thread; total to all.
@@ -303,32 +336,53 @@ __device__ __forceinline__ int sparse_scan(int v, int* warp_sums, int& total) {
 
 // The selected pages with rank [lo, hi) in index order, into list[0 ..
 // hi - lo); all of them to `all` when it is given.  keys[p] for the pages
-// [sink, n - recent); n > select.
-__device__ __forceinline__ void sparse_select(const SparseArgs& a, const uint32_t* keys, int n, uint8_t* arena, int lo,
+// [sink, n - recent); n > select.  Warp w has a contiguous range of the
+// competing pages, a lane every 32nd of it; kHold > 0: at most kHold keys a
+// thread, held in registers; 0: any number, read from L2 in every pass.
+template <int kHold>
+__device__ __forceinline__ void sparse_select(const SparseArgs& a, const uint32_t* keys, int n, int* hist, int lo,
                                               int hi, int32_t* list, int32_t* all) {
   __shared__ int warp_sums[kSparseWarps];
   __shared__ uint32_t mm[2 * kSparseWarps];
   __shared__ int found[3];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int first = a.sink, count = n - a.recent - a.sink, want = a.select - a.recent - a.sink;
-  uint32_t* held = reinterpret_cast<uint32_t*>(arena);
-  int* hist = reinterpret_cast<int*>(arena + kSparseKeys * 4);
-  const bool hold = count <= kSparseKeys;
-  uint32_t kmin = 0xffffffffu, kmax = 0;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < count; i += kSparseThreads) {
-    const uint32_t k = __ldcg(keys + first + i);
-    if (hold) held[i] = k;
-    kmin = min(kmin, k);
-    kmax = max(kmax, k);
+  keys += first;
+  const int per = (count + kSparseWarps * 32 - 1) / (kSparseWarps * 32);  // keys of a thread
+  const int base = warp * per * 32 + lane;
+  uint32_t held[kHold > 0 ? kHold : 1];
+  if constexpr (kHold > 0) {
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) held[j] = j < per && base + 32 * j < count ? __ldcg(keys + base + 32 * j) : 0u;
   }
-  auto key = [&](int i) { return hold ? held[i] : __ldcg(keys + first + i); };
+  // f(key, index) for the thread's keys, in order; every lane of a warp does every step
+  auto each = [&](auto f) {
+    if constexpr (kHold > 0) {
+#pragma unroll
+      for (int j = 0; j < kHold; ++j)
+        if (j < per) f(held[j], base + 32 * j);
+    } else {
+#pragma unroll 4
+      for (int j = 0; j < per; ++j) {
+        const int i = base + 32 * j;
+        f(i < count ? __ldcg(keys + i) : 0u, i);
+      }
+    }
+  };
+  uint32_t kmin = 0xffffffffu, kmax = 0;
+  each([&](uint32_t k, int i) {
+    if (i < count) {
+      kmin = min(kmin, k);
+      kmax = max(kmax, k);
+    }
+  });
   kmin = __reduce_min_sync(0xffffffffu, kmin);
   kmax = __reduce_max_sync(0xffffffffu, kmax);
   if (lane == 0) {
     mm[warp] = kmin;
     mm[kSparseWarps + warp] = kmax;
   }
+  for (int i = threadIdx.x; i < kSparseBins; i += kSparseThreads) hist[i] = 0;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kSparseWarps; ++w) {
@@ -339,16 +393,14 @@ __device__ __forceinline__ void sparse_select(const SparseArgs& a, const uint32_
   // taken are the keys whose bits from `shift` on are above `prefix`, and
   // `rest` of those where they equal it.
   int shift = kmin == kmax ? 0 : 32 - __clz(kmin ^ kmax);  // bits below are undecided
-  uint32_t prefix = shift < 32 ? kmax >> shift : 0u;       // common to all keys
+  auto upper = [](uint32_t k, int s) { return s == 32 ? 0u : k >> s; };
+  uint32_t prefix = upper(kmax, shift);  // common to all keys
   int rest = want;
   while (shift > 0 && rest > 0) {
     const int bits = min(11, shift), low = shift - bits;
-    for (int i = threadIdx.x; i < (1 << bits); i += kSparseThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < count; i += kSparseThreads) {
-      const uint32_t k = key(i);
-      if (shift == 32 || (k >> shift) == prefix) atomicAdd(&hist[(k >> low) & ((1u << bits) - 1)], 1);
-    }
+    each([&](uint32_t k, int i) {
+      if (i < count && upper(k, shift) == prefix) atomicAdd(&hist[(k >> low) & ((1u << bits) - 1)], 1);
+    });
     __syncthreads();
     // from the top: the bin in which the count passes `rest`; thread 0 has the highest bins
     constexpr int kPer = kSparseBins / kSparseThreads;
@@ -356,7 +408,11 @@ __device__ __forceinline__ void sparse_select(const SparseArgs& a, const uint32_
     const int top = (1 << bits) - 1 - threadIdx.x * kPer;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      h[j] = top - j >= 0 ? hist[top - j] : 0;
+      h[j] = 0;
+      if (top - j >= 0) {
+        h[j] = hist[top - j];
+        hist[top - j] = 0;  // for the next pass
+      }
       sum += h[j];
     }
     int total;
@@ -374,87 +430,110 @@ __device__ __forceinline__ void sparse_select(const SparseArgs& a, const uint32_
     prefix = shift == 32 ? (uint32_t)found[0] : (prefix << bits) | (uint32_t)found[0];
     rest = found[1];
     shift = low;
-    const bool exact = found[1] == found[2];
-    __syncthreads();
-    if (exact) break;  // all keys of the bin are taken
+    if (found[1] == found[2]) break;  // all keys of the bin are taken
   }
-  // Gather in index order: a warp has a contiguous range.
-  const int per = (count + kSparseWarps * 32 - 1) / (kSparseWarps * 32) * 32;
-  const int i0 = min(count, warp * per), i1 = min(count, i0 + per);
+  // gather in index order
   int n_gt = 0, n_eq = 0;
-  for (int i = i0 + lane; i < i1; i += 32) {
-    const uint32_t k = key(i);
-    const uint32_t top = shift == 32 ? 0u : k >> shift;
-    n_gt += top > prefix;
-    n_eq += top == prefix;
-  }
+  each([&](uint32_t k, int i) {
+    const uint32_t u = upper(k, shift);
+    n_gt += i < count && u > prefix;
+    n_eq += i < count && u == prefix;
+  });
   n_gt = __reduce_add_sync(0xffffffffu, n_gt);
   n_eq = __reduce_add_sync(0xffffffffu, n_eq);
+  __syncthreads();  // the extremes have been read
   if (lane == 0) {
     mm[warp] = n_gt;
     mm[kSparseWarps + warp] = n_eq;
   }
   __syncthreads();
   int gt = 0, eq = 0;
-  for (int w = 0; w < warp; ++w) {
-    gt += mm[w];
-    eq += mm[kSparseWarps + w];
+#pragma unroll
+  for (int w = 0; w < kSparseWarps; ++w) {
+    gt += w < warp ? mm[w] : 0;
+    eq += w < warp ? mm[kSparseWarps + w] : 0;
   }
   auto put = [&](int rank, int page) {
     if (rank >= lo && rank < hi) list[rank - lo] = page;
     if (all != nullptr) all[rank] = page;
   };
-  for (int i = i0; i < i1; i += 32) {
-    const uint32_t k = i + lane < i1 ? key(i + lane) : 0u;
-    const uint32_t top = shift == 32 ? 0u : k >> shift;
-    const bool is_gt = i + lane < i1 && top > prefix, is_eq = i + lane < i1 && top == prefix;
+  const uint32_t below = (1u << lane) - 1;
+  each([&](uint32_t k, int i) {
+    const uint32_t u = upper(k, shift);
+    const bool is_gt = i < count && u > prefix, is_eq = i < count && u == prefix;
     const uint32_t bg = __ballot_sync(0xffffffffu, is_gt), be = __ballot_sync(0xffffffffu, is_eq);
-    const uint32_t below = (1u << lane) - 1;
-    const int my_eq = eq + __popc(be & below);
-    if (is_gt || (is_eq && my_eq < rest))
-      put(first + gt + __popc(bg & below) + min(my_eq, rest), first + i + lane);
-    gt += __popc(bg);
-    eq += __popc(be);
-  }
+    if ((bg | be) != 0) {
+      const int my_eq = eq + __popc(be & below);
+      if (is_gt || (is_eq && my_eq < rest)) put(first + gt + __popc(bg & below) + min(my_eq, rest), first + i);
+      gt += __popc(bg);
+      eq += __popc(be);
+    }
+  });
   for (int i = threadIdx.x; i < a.sink; i += kSparseThreads) put(i, i);
   for (int i = threadIdx.x; i < a.recent; i += kSparseThreads) put(a.select - a.recent + i, n - a.recent + i);
   __syncthreads();
 }
 
-template <int D>
+// D(16x8) += A . B as mma_bf16_16816 with B given as two registers.
+__device__ __forceinline__ void mma_bf16_b(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  const uint32_t b[2] = {b0, b1};
+  mma_bf16_16816(d, a, b);
+}
+// Transpose of an 8x8 matrix of 16-bit elements held two to a lane.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// NH: tiles of 8 query heads (group <= 8 NH).  Tokens are the rows of the
+// score product (16 x 8 heads = K . q^T) and channels those of the output
+// (O^T = V^T . P), so a group of up to 8 heads wastes no rows; P goes from
+// one to the other by an 8x8 transpose in registers.
+template <int D, int NH>
 __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const SparseArgs a) {
   using C = SparseCfg<D>;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* part = reinterpret_cast<float*>(smem + C::kPartOff);
-  float* cml = reinterpret_cast<float*>(smem + C::kMlOff);  // [2][16]: the CTA's m, l
-  float* wml = cml + 32;                                    // [2][warps][16]
+  float* wml = reinterpret_cast<float*>(smem + C::kMlOff);  // [2][warps][16]
   int32_t* list = reinterpret_cast<int32_t*>(smem + C::kListOff);
   const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
   const int S = a.splits, PS = a.page_size, group = a.group;
   // q and the tables are read before the wait for the scores' grid, which
   // lets this one start only once they are complete (without that launch
   // this grid follows them directly and waits first)
   const bool scored = a.max_pages > a.select;
+  if (S > 1) cluster_arrive_relaxed();  // waited for before the first store into another CTA's memory
   if (!scored) pdl_wait();
   SparseRow r;
   r.load(a, b);
   const int taken = min(r.pages, a.select);
   const int lo = (int)((int64_t)taken * split / S), hi = (int)((int64_t)taken * (split + 1) / S);
-  constexpr int kUnits = D / 8;
-  for (int idx = threadIdx.x; idx < 16 * kUnits; idx += kSparseThreads) {
-    const int row = idx / kUnits, c = idx % kUnits;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < group)
-      v = *reinterpret_cast<const uint4*>(a.q + (int64_t)b * a.q_stride_b +
-                                          (int64_t)(kvh * group + row) * a.q_stride_h + c * 8);
-    *reinterpret_cast<uint4*>(smem + C::kQOff + row * C::kQRow + c * 16) = v;
+  // q as the B operand: head g of tile h, channels 16 kk + 2 t4 (+ 8)
+  uint32_t qb[NH][D / 16][2];
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+    const bool in = 8 * h + g < group;
+    const bf16* src = a.q + (int64_t)b * a.q_stride_b + (int64_t)(kvh * group + (in ? 8 * h + g : 0)) * a.q_stride_h;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        qb[h][kk][i] = in ? *reinterpret_cast<const uint32_t*>(src + 16 * kk + 8 * i + 2 * t4) : 0u;
   }
   if (scored) pdl_wait();
   pdl_launch_dependents();
   int32_t* all = split == 0 ? a.selected + ((int64_t)b * a.num_kv_heads + kvh) * a.select : nullptr;
   if (r.pages > a.select) {
-    sparse_select(a, a.keys + ((int64_t)b * a.num_kv_heads + kvh) * a.max_pages, r.pages, smem, lo, hi, list, all);
+    const uint32_t* keys = a.keys + ((int64_t)b * a.num_kv_heads + kvh) * a.max_pages;
+    int* hist = reinterpret_cast<int*>(smem);
+    if (r.pages <= 4 * kSparseThreads)
+      sparse_select<4>(a, keys, r.pages, hist, lo, hi, list, all);
+    else if (r.pages <= 32 * kSparseThreads)
+      sparse_select<32>(a, keys, r.pages, hist, lo, hi, list, all);
+    else
+      sparse_select<0>(a, keys, r.pages, hist, lo, hi, list, all);
   } else {
     for (int i = threadIdx.x; i < hi - lo; i += kSparseThreads) list[i] = lo + i;
     if (all != nullptr)
@@ -462,166 +541,179 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
     __syncthreads();
   }
 
-  // ---- a warp takes units of 16 tokens: K and V through its own buffer
-  const int upp = PS / kSparseUnit;  // units of a page
+  // ---- a warp takes units of 16 tokens: K, V, K, V, ... through its own ring
+  const int upp = PS / kSparseUnit;  // units of a page: 1 or 2
+  const int ushift = upp == 2 ? 1 : 0;
   const int units = (hi - lo) * upp;
-  uint8_t* kt = smem + warp * 2 * C::kTile;
-  uint8_t* vt = kt + C::kTile;
+  const uint32_t ring = smem_u32(smem) + warp * C::kRing * C::kTile;
   const int64_t token = (int64_t)a.num_kv_heads * D;
-  auto page_of = [&](int u) {  // page id of a unit of the list, -1: outside the pool
-    if (u >= units) return -1;
-    const int pg = a.indices[r.begin + list[u / upp]];
-    if (pg < 0 || (int64_t)pg >= a.num_pages) {
-      if (lane == 0) set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
-      return -1;
-    }
-    return pg;
-  };
-  auto live_of = [&](int u, int pg) {  // its tokens
-    if (u >= units || pg < 0) return 0;
-    const int len = list[u / upp] == r.pages - 1 ? r.last : PS;
-    return min(kSparseUnit, max(0, len - (u % upp) * kSparseUnit));
+  constexpr int kUnits = D / 8;               // 16-byte units of a row
+  constexpr int kRows = 32 / kUnits;          // rows that a warp's copy instruction covers
+  constexpr int kCopies = kSparseUnit / kRows;
+  const int row0 = lane / kUnits, col = lane % kUnits;
+  const bf16* kv_lane = a.kv + (int64_t)kvh * D + row0 * token + col * 8;
+  // page id of a unit (looked at when it is loaded), -1 past the last
+  auto page_of = [&](int u) { return u < units ? a.indices[r.begin + list[u >> ushift]] : -1; };
+  auto live_of = [&](int u) {  // its tokens
+    if (u >= units) return 0;
+    const int len = list[u >> ushift] == r.pages - 1 ? r.last : PS;
+    return min(kSparseUnit, max(0, len - (u & (upp - 1)) * kSparseUnit));
   };
   // 16-byte unit c of row t at t * kRow + ((c ^ (t & 7)) * 16); rows past `live` are zero-filled
-  auto load = [&](uint8_t* dst, int u, int pg, int live, int kv) {
-    const bf16* src = a.kv + (((int64_t)max(pg, 0) * 2 + kv) * PS + (u % upp) * kSparseUnit) * token + (int64_t)kvh * D;
+  auto load = [&](int slot, int u, int pg, int live, int kv) {
+    if (u < units) {
+      const bool in = pg >= 0 && (int64_t)pg < a.num_pages;
+      if (!in) {
+        if (lane == 0) set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
+        pg = 0;
+      }
+      const bf16* src = kv_lane + (((int64_t)pg * 2 + kv) * PS + (u & (upp - 1)) * kSparseUnit) * token;
+      const uint32_t dst = ring + slot * C::kTile + row0 * C::kRow;
 #pragma unroll
-    for (int i = 0; i < kSparseUnit * kUnits / 32; ++i) {
-      const int idx = i * 32 + lane, t = idx / kUnits, c = idx % kUnits;
-      const uint32_t to = smem_u32(dst + t * C::kRow + ((c ^ (t & 7)) << 4));
-      const int n = t < live ? 16 : 0;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src + (n ? t : 0) * token + c * 8), "r"(n)
-                   : "memory");
+      for (int i = 0; i < kCopies; ++i) {
+        const int t = i * kRows + row0;
+        const uint32_t to = dst + i * kRows * C::kRow + ((col ^ (t & 7)) << 4);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src + (int64_t)i * kRows * token),
+                     "r"(in && t < live ? 16 : 0)
+                     : "memory");
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  float o[D / 8][4];
+  float o[NH][D / 16][4];  // O^T: channels 16 j + g (+ 8), heads 8 h + 2 t4 (+ 1)
 #pragma unroll
-  for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  for (int h = 0; h < NH; ++h)
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) o[h][j][0] = o[h][j][1] = o[h][j][2] = o[h][j][3] = 0.f;
+  float m[NH][2], l[NH][2];
+#pragma unroll
+  for (int h = 0; h < NH; ++h) m[h][0] = m[h][1] = -INFINITY, l[h][0] = l[h][1] = 0.f;
   const float sl2 = a.scale_log2;
-  const int g = lane >> 2, t4 = lane & 3;
-  int pg = page_of(warp), live = live_of(warp, pg);
-  int pg_n = page_of(warp + kSparseWarps);
-  if (warp < units) {
-    load(kt, warp, pg, live, 0);
-    load(vt, warp, pg, live, 1);
-  }
+  // unit u, then the two after it; tiles 2 i (K) and 2 i + 1 (V) of the
+  // warp's i-th unit in slots (2 i + kv) % 3
+  int pg = page_of(warp), live = live_of(warp);
+  int pg1 = page_of(warp + kSparseWarps), live1 = live_of(warp + kSparseWarps);
+  load(0, warp, pg, live, 0);
+  load(1, warp, pg, live, 1);
+  load(2, warp + kSparseWarps, pg1, live1, 0);
+  int slot = 0;  // of this unit's K
   for (int u = warp; u < units; u += kSparseWarps) {
-    const int un = u + kSparseWarps;
-    const int live_n = live_of(un, pg_n);
-    asm volatile("cp.async.wait_group 1;" ::: "memory");  // K of this unit
+    const int un = u + kSparseWarps, unn = un + kSparseWarps;
+    const int pg2 = page_of(unn), live2 = live_of(unn);
+    const int vslot = slot == 2 ? 0 : slot + 1;
+    const uint32_t kt = ring + slot * C::kTile, vt = ring + vslot * C::kTile;
+    asm volatile("cp.async.wait_group 2;" ::: "memory");  // K of this unit
     __syncwarp();
-    float sc[2][4];
+    // ---- scores: tokens g, g + 8 x heads 2 t4, 2 t4 + 1
+    float sc[NH][4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+    for (int h = 0; h < NH; ++h) sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f;
+    {
+      const int tok = (lane & 7) + 8 * ((lane >> 3) & 1), c0 = lane >> 4;
+      const uint32_t at = kt + tok * C::kRow;
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      uint32_t qa[4], kb[4];
-      ldsm_x4(smem_u32(smem + C::kQOff + ((lane & 7) + 8 * ((lane >> 3) & 1)) * C::kQRow + (kk * 16 + 8 * (lane >> 4)) * 2),
-              qa[0], qa[1], qa[2], qa[3]);
-      const int mi = lane >> 3, tok = (mi >> 1) * 8 + (lane & 7), c = 2 * kk + (mi & 1);
-      ldsm_x4(smem_u32(kt + tok * C::kRow + ((c ^ (tok & 7)) << 4)), kb[0], kb[1], kb[2], kb[3]);
-      mma_bf16_16816(sc[0], qa, &kb[0]);
-      mma_bf16_16816(sc[1], qa, &kb[2]);
-    }
-    __syncwarp();
-    const int pg_nn = page_of(un + kSparseWarps);
-    if (un < units)
-      load(kt, un, pg_n, live_n, 0);
-    else
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    // ---- online softmax (rows g and g + 8), log2 domain
-    float mx0 = -INFINITY, mx1 = -INFINITY;
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t ka[4];
+        ldsm_x4(at + (((2 * kk + c0) ^ (tok & 7)) << 4), ka[0], ka[1], ka[2], ka[3]);
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const bool in = 8 * j + 2 * t4 + c < live;
-        sc[j][c] = in ? sc[j][c] * sl2 : -INFINITY;
-        sc[j][2 + c] = in ? sc[j][2 + c] * sl2 : -INFINITY;
-        mx0 = fmaxf(mx0, sc[j][c]);
-        mx1 = fmaxf(mx1, sc[j][2 + c]);
+        for (int h = 0; h < NH; ++h) mma_bf16_b(sc[h], ka, qb[h][kk][0], qb[h][kk][1]);
       }
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-    const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
-    const float a0 = m0 == -INFINITY ? 0.f : sp_exp2(m0 - mn0), a1 = m1 == -INFINITY ? 0.f : sp_exp2(m1 - mn1);
-    const float b0 = mn0 == -INFINITY ? 0.f : mn0, b1 = mn1 == -INFINITY ? 0.f : mn1;
-    m0 = mn0;
-    m1 = mn1;
-    float s0 = 0.f, s1 = 0.f;
+    }
+    __syncwarp();
+    load(slot, un, pg1, live1, 1);  // the next V into this K's place
+    // ---- online softmax (log2 domain), a column per head
+    uint32_t ph[NH][2], pr[NH][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int h = 0; h < NH; ++h) {
+      const bool in0 = g < live, in1 = g + 8 < live;
+      sc[h][0] = in0 ? sc[h][0] * sl2 : -INFINITY;
+      sc[h][1] = in0 ? sc[h][1] * sl2 : -INFINITY;
+      sc[h][2] = in1 ? sc[h][2] * sl2 : -INFINITY;
+      sc[h][3] = in1 ? sc[h][3] * sl2 : -INFINITY;
+      float al[2];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        sc[j][c] = sp_exp2(sc[j][c] - b0);
-        sc[j][2 + c] = sp_exp2(sc[j][2 + c] - b1);
-        s0 += sc[j][c];
-        s1 += sc[j][2 + c];
+      for (int i = 0; i < 2; ++i) {
+        float mx = fmaxf(sc[h][i], sc[h][2 + i]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        const float mn = fmaxf(m[h][i], mx);
+        al[i] = m[h][i] == mn ? 1.f : sp_exp2(m[h][i] - mn);  // m = -inf: 0 times a state of zeros
+        m[h][i] = mn;
+        const float base = mn == -INFINITY ? 0.f : mn;
+        sc[h][i] = sp_exp2(sc[h][i] - base);
+        sc[h][2 + i] = sp_exp2(sc[h][2 + i] - base);
+        l[h][i] = l[h][i] * al[i] + (sc[h][i] + sc[h][2 + i]);
       }
-    l0 = l0 * a0 + s0;
-    l1 = l1 * a1 + s1;
+      if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      o[j][0] *= a0;
-      o[j][1] *= a0;
-      o[j][2] *= a1;
-      o[j][3] *= a1;
-    }
-    // P as a bf16 pair (value and remainder): O keeps fp32's accuracy, for
-    // products that this memory-bound loop has to spare
-    uint32_t ph[4], pl_[4];
+        for (int j = 0; j < D / 16; ++j) {
+          o[h][j][0] *= al[0];
+          o[h][j][1] *= al[1];
+          o[h][j][2] *= al[0];
+          o[h][j][3] *= al[1];
+        }
+      }
+      // P as a bf16 pair (value and remainder): O keeps fp32's accuracy, for
+      // products that this memory-bound loop has to spare
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = sc[i >> 1][(i & 1) * 2], y = sc[i >> 1][(i & 1) * 2 + 1];
-      ph[i] = pack_bf16x2(x, y);
-      const float2 h = unpack_bf16x2(ph[i]);
-      pl_[i] = pack_bf16x2(x - h.x, y - h.y);
+      for (int i = 0; i < 2; ++i) {  // tokens g, g + 8
+        const uint32_t hi2 = pack_bf16x2(sc[h][2 * i], sc[h][2 * i + 1]);
+        const float2 f = unpack_bf16x2(hi2);
+        ph[h][i] = transpose_8x8(hi2);
+        pr[h][i] = transpose_8x8(pack_bf16x2(sc[h][2 * i] - f.x, sc[h][2 * i + 1] - f.y));
+      }
     }
-    asm volatile("cp.async.wait_group 1;" ::: "memory");  // V of this unit
+    asm volatile("cp.async.wait_group 2;" ::: "memory");  // V of this unit
     __syncwarp();
+    {
+      // A = V^T: rows = channels; lanes 8 i .. 8 i + 7 name the token rows of matrix i
+      const int tok = (lane & 7) + 8 * (lane >> 4), c0 = (lane >> 3) & 1;
+      const uint32_t at = vt + tok * C::kRow;
 #pragma unroll
-    for (int dc = 0; dc < D / 8; dc += 2) {
-      const int mi = lane >> 3, tok = (mi & 1) * 8 + (lane & 7), c = dc + (mi >> 1);
-      uint32_t vb[4];
-      ldsm_x4_trans(smem_u32(vt + tok * C::kRow + ((c ^ (tok & 7)) << 4)), vb[0], vb[1], vb[2], vb[3]);
-      mma_bf16_16816(o[dc], ph, &vb[0]);
-      mma_bf16_16816(o[dc + 1], ph, &vb[2]);
-      mma_bf16_16816(o[dc], pl_, &vb[0]);
-      mma_bf16_16816(o[dc + 1], pl_, &vb[2]);
+      for (int j = 0; j < D / 16; ++j) {
+        uint32_t va[4];
+        ldsm_x4_trans(at + (((2 * j + c0) ^ (tok & 7)) << 4), va[0], va[1], va[2], va[3]);
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          mma_bf16_b(o[h][j], va, ph[h][0], ph[h][1]);
+          mma_bf16_b(o[h][j], va, pr[h][0], pr[h][1]);
+        }
+      }
     }
     __syncwarp();
-    if (un < units)
-      load(vt, un, pg_n, live_n, 1);
-    else
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    live = live_n;
-    pg_n = pg_nn;
+    load(vslot, unn, pg2, live2, 0);  // the K after the next into this V's place
+    live = live1;
+    live1 = live2;
+    pg1 = pg2;
+    slot = slot == 0 ? 2 : slot - 1;  // K of the next unit: (slot + 2) % 3
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 
   // ---- the warps' states meet in shared memory
-  l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-  l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-  l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-  l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+#pragma unroll
+  for (int h = 0; h < NH; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) l[h][i] += __shfl_xor_sync(0xffffffffu, l[h][i], d);
   __syncthreads();  // every warp is done with its buffer
   float* ow = reinterpret_cast<float*>(smem) + warp * 16 * C::kOPad;
 #pragma unroll
-  for (int j = 0; j < D / 8; ++j) {
-    const int d = 8 * j + 2 * t4;
-    if (g < group) *reinterpret_cast<float2*>(ow + g * C::kOPad + d) = make_float2(o[j][0], o[j][1]);
-    if (g + 8 < group) *reinterpret_cast<float2*>(ow + (g + 8) * C::kOPad + d) = make_float2(o[j][2], o[j][3]);
-  }
-  if (t4 == 0) {
-    wml[warp * 16 + g] = m0;
-    wml[warp * 16 + g + 8] = m1;
-    wml[(kSparseWarps + warp) * 16 + g] = l0;
-    wml[(kSparseWarps + warp) * 16 + g + 8] = l1;
-  }
+  for (int h = 0; h < NH; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int head = 8 * h + 2 * t4 + i;
+      if (head < group)
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          ow[head * C::kOPad + 16 * j + g] = o[h][j][i];
+          ow[head * C::kOPad + 16 * j + 8 + g] = o[h][j][2 + i];
+        }
+      if (g == 0) {
+        wml[warp * 16 + head] = m[h][i];
+        wml[(kSparseWarps + warp) * 16 + head] = l[h][i];
+      }
+    }
   __syncthreads();
   auto write = [&](int row, int d, float4 acc, float L, float M) {
     const float inv = L == 0.f ? 0.f : 1.f / L;
@@ -632,6 +724,7 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
     if (d == 0 && a.out_lse != nullptr)
       a.out_lse[(int64_t)b * a.num_qo_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
   };
+  if (S > 1) cluster_wait();  // every CTA of the cluster runs
   for (int idx = threadIdx.x; idx < group * (D / 4); idx += kSparseThreads) {
     const int row = idx / (D / 4), d = 4 * (idx % (D / 4));
     float M = -INFINITY;
@@ -653,44 +746,42 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
     if (S == 1) {
       write(row, d, acc, L, M);
     } else {
-      *reinterpret_cast<float4*>(part + row * D + d) = acc;
+      // chunk idx is added up by CTA idx % S of the cluster
+      const uint32_t at = smem_u32(smem + C::kRecvOff) + ((idx / S) * S + split) * 16;
+      dsmem_st_f32x4(dsmem_map(at, idx % S), acc);
       if (d == 0) {
-        cml[row] = M;
-        cml[16 + row] = L;
+        const uint32_t ml = smem_u32(smem + C::kRecvMlOff) + (split * 32 + row) * 4;
+        for (int c = 0; c < S; ++c) {
+          dsmem_st_f32(dsmem_map(ml, c), M);
+          dsmem_st_f32(dsmem_map(ml + 64, c), L);
+        }
       }
     }
   }
   if (S == 1) return;
-  cluster_sync_all();
-  for (int idx = threadIdx.x * S + split; idx < group * (D / 4); idx += kSparseThreads * S) {
+  cluster_sync_all();  // every CTA's state has arrived; nothing is read remotely after it
+  const float4* recv = reinterpret_cast<const float4*>(smem + C::kRecvOff);
+  const float* recv_ml = reinterpret_cast<const float*>(smem + C::kRecvMlOff);
+  for (int i = threadIdx.x; i * S + split < group * (D / 4); i += kSparseThreads) {
+    const int idx = i * S + split;
     const int row = idx / (D / 4), d = 4 * (idx % (D / 4));
-    float mc[kSparseMaxCluster], lc[kSparseMaxCluster];
-    float4 v[kSparseMaxCluster];
     float M = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < kSparseMaxCluster; ++c) {
-      mc[c] = -INFINITY;
-      if (c >= S) continue;
-      mc[c] = dsmem_ld_f32(dsmem_map(smem_u32(cml + row), c));
-      lc[c] = dsmem_ld_f32(dsmem_map(smem_u32(cml + 16 + row), c));
-      v[c] = dsmem_ld_f32x4(dsmem_map(smem_u32(part + row * D + d), c));
-      M = fmaxf(M, mc[c]);
-    }
+    for (int c = 0; c < S; ++c) M = fmaxf(M, recv_ml[c * 32 + row]);
     float L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int c = 0; c < kSparseMaxCluster; ++c) {
-      if (mc[c] == -INFINITY) continue;  // a CTA without pages
-      const float f = exp2f(mc[c] - M);
-      L += f * lc[c];
-      acc.x += f * v[c].x;
-      acc.y += f * v[c].y;
-      acc.z += f * v[c].z;
-      acc.w += f * v[c].w;
+    for (int c = 0; c < S; ++c) {
+      const float mc = recv_ml[c * 32 + row];
+      if (mc == -INFINITY) continue;  // a CTA without pages
+      const float f = exp2f(mc - M);
+      const float4 v = recv[i * S + c];
+      L += f * recv_ml[c * 32 + 16 + row];
+      acc.x += f * v.x;
+      acc.y += f * v.y;
+      acc.z += f * v.z;
+      acc.w += f * v.w;
     }
     write(row, d, acc, L, M);
   }
-  cluster_sync_all();  // no CTA leaves while another reads its state
 }
 
 }  // namespace pl
@@ -698,9 +789,11 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
 // =================================================================== host
 namespace {
 
-template <int D>
-int32_t launch_attend(const pl::SparseArgs& a, int batch, void* stream) {
-  auto kern = pl::sparse_attend_kernel<D>;
+constexpr int kScoreCtasPerSm = 3;
+
+template <int D, int NH>
+int32_t launch_attend_nh(const pl::SparseArgs& a, int batch, void* stream) {
+  auto kern = pl::sparse_attend_kernel<D, NH>;
   const int list = 4 * ((a.select < a.max_pages ? a.select : a.max_pages) / a.splits + 2);
   const int smem = pl::SparseCfg<D>::kListOff + ((list + 15) & ~15);
   int32_t st = pl_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
@@ -708,6 +801,11 @@ int32_t launch_attend(const pl::SparseArgs& a, int batch, void* stream) {
   const dim3 grid(a.splits, a.num_kv_heads, batch);
   if (a.splits == 1) return pl_host::launch_pdl(kern, grid, dim3(pl::kSparseThreads), smem, stream, a);
   return pl_host::launch_pdl_cluster(kern, grid, dim3(pl::kSparseThreads), smem, stream, a.splits, a);
+}
+
+template <int D>
+int32_t launch_attend(const pl::SparseArgs& a, int batch, void* stream) {
+  return a.group <= 8 ? launch_attend_nh<D, 1>(a, batch, stream) : launch_attend_nh<D, 2>(a, batch, stream);
 }
 
 }  // namespace
@@ -794,13 +892,15 @@ extern "C" int32_t pl_paged_sparse_decode(
   const int64_t items = (int64_t)batch * num_kv_heads;
   int32_t st;
   if (max_pages > num_select) {
-    // a warp takes 8 pages a step; as many CTAs as fill the device a few
-    // times over, but no more than there are steps
-    const int64_t steps = (max_pages + 8 * pl::kSparseWarps - 1) / (8 * pl::kSparseWarps);
-    int64_t chunks = (8 * (int64_t)sms + items - 1) / items;
-    chunks = chunks < 1 ? 1 : (chunks > steps ? steps : chunks);
+    // a warp takes 8 pages a step; as many CTAs as the device holds at once,
+    // but no more than there are steps
+    const int hw = num_kv_heads < pl::kSparseWarps ? num_kv_heads : pl::kSparseWarps, pw = pl::kSparseWarps / hw;
+    const int head_groups = (num_kv_heads + pl::kSparseWarps - 1) / pl::kSparseWarps;
+    const int64_t steps = (max_pages + 8 * pw - 1) / (8 * pw);
+    int64_t chunks = kScoreCtasPerSm * (int64_t)sms / ((int64_t)batch * head_groups);
+    chunks = chunks > steps ? steps : (chunks < 1 ? 1 : chunks);
     auto score = head_dim == 128 ? pl::sparse_score_kernel<128> : pl::sparse_score_kernel<64>;
-    st = pl_host::launch_pdl(score, dim3((int)chunks, num_kv_heads, batch), dim3(pl::kSparseThreads), 0, stream, a);
+    st = pl_host::launch_pdl(score, dim3((int)chunks, head_groups, batch), dim3(pl::kSparseThreads), 0, stream, a);
     if (st != PL_OK) return st;
   }
   // CTAs per (row, kv head): two fit on an SM, and a warp should have a unit
