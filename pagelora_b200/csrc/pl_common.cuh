@@ -545,6 +545,8 @@ EncodeTiledFn encode_tiled_fn();
 // copy brings PS rows x 128 B (a 64-dim half of one page's K or V of one kv
 // head).  Defined with the decode kernel.
 int32_t kv_tensor_map(const void* cache, int64_t pages, int hkv, int d, int ps, CUtensorMap* out);
+// The same with copies of `rows` tokens (a divisor of PS).
+int32_t kv_tensor_map_rows(const void* cache, int64_t pages, int hkv, int d, int ps, int rows, CUtensorMap* out);
 
 // Opt a kernel into `bytes` of dynamic shared memory on the current device
 // (once per device and kernel).

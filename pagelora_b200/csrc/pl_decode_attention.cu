@@ -757,9 +757,9 @@ namespace {
 struct MapKey {
   const void* ptr;
   int64_t pages;
-  int32_t hkv, d, ps, dev;
+  int32_t hkv, d, ps, rows, dev;
   bool operator==(const MapKey& o) const {
-    return ptr == o.ptr && pages == o.pages && hkv == o.hkv && d == o.d && ps == o.ps && dev == o.dev;
+    return ptr == o.ptr && pages == o.pages && hkv == o.hkv && d == o.d && ps == o.ps && rows == o.rows && dev == o.dev;
   }
 };
 
@@ -776,11 +776,11 @@ MapCache g_maps;
 
 namespace pl_host {
 // Tensor map over one layer's pool viewed as [2*P][PS][Hkv][D] (innermost last):
-// dims (inner->outer) {D, Hkv, PS, 2P}, box {64, 1, PS, 1}, 128B swizzle.
-int32_t kv_tensor_map(const void* cache, int64_t pages, int hkv, int d, int ps, CUtensorMap* out) {
+// dims (inner->outer) {D, Hkv, PS, 2P}, box {64, 1, rows, 1}, 128B swizzle.
+int32_t kv_tensor_map_rows(const void* cache, int64_t pages, int hkv, int d, int ps, int rows, CUtensorMap* out) {
   int dev = 0;
   cudaGetDevice(&dev);
-  MapKey k{cache, pages, hkv, d, ps, dev};
+  MapKey k{cache, pages, hkv, d, ps, rows, dev};
   std::lock_guard<std::mutex> lock(g_maps.mu);
   for (int i = 0; i < g_maps.used; ++i)
     if (g_maps.key[i] == k) {
@@ -791,7 +791,7 @@ int32_t kv_tensor_map(const void* cache, int64_t pages, int hkv, int d, int ps, 
   if (enc == nullptr) return PL_ERR_CUDA;
   cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)hkv, (cuuint64_t)ps, (cuuint64_t)(2 * pages)};
   cuuint64_t strides[3] = {(cuuint64_t)d * 2, (cuuint64_t)hkv * d * 2, (cuuint64_t)ps * hkv * d * 2};
-  cuuint32_t box[4] = {64, 1, (cuuint32_t)ps, 1};
+  cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUtensorMap m;
   CUresult r = enc(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(cache), dims, strides, box, estr,
@@ -809,6 +809,10 @@ int32_t kv_tensor_map(const void* cache, int64_t pages, int hkv, int d, int ps, 
   g_maps.map[slot] = m;
   *out = m;
   return PL_OK;
+}
+
+int32_t kv_tensor_map(const void* cache, int64_t pages, int hkv, int d, int ps, CUtensorMap* out) {
+  return kv_tensor_map_rows(cache, pages, hkv, d, ps, ps, out);
 }
 }  // namespace pl_host
 

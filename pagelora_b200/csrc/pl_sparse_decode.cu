@@ -105,6 +105,7 @@ constexpr int kSparseWarps = kSparseThreads / 32;
 constexpr int kSparseUnit = 16;          // tokens a warp takes at a time
 constexpr int kSparseMaxCluster = 8;
 constexpr int kSparseBins = 2048;        // 11 bits of the key per pass
+constexpr float kSparseSlack = 8.0f;     // log2 growth of a maximum that is tolerated before the state is rescaled
 
 struct SparseArgs {
   const bf16* q;
@@ -293,8 +294,9 @@ __global__ void __launch_bounds__(kSparseThreads, 3) sparse_score_kernel(const S
 
 template <int D>
 struct SparseCfg {
-  static constexpr int kRow = 2 * D;                           // bytes of one token's K (or V)
-  static constexpr int kTile = kSparseUnit * kRow;             // K (or V) of one unit
+  static constexpr int kHalves = D / 64;                       // 64-channel boxes of a tile
+  static constexpr int kHalfBytes = kSparseUnit * 128;
+  static constexpr int kTile = kHalves * kHalfBytes;           // K (or V) of one unit: 128B-swizzled boxes
   static constexpr int kOPad = D + 4;
   static constexpr int kRing = 3;                              // tiles (K, V, K, ...) of a warp in flight
   static constexpr int kStages = kSparseWarps * kRing * kTile;
@@ -308,7 +310,8 @@ struct SparseCfg {
   static constexpr int kRecvOff = kArena;
   static constexpr int kRecvMlOff = kRecvOff + (16 * D / 4 + kSparseMaxCluster) * 16;
   static constexpr int kMlOff = kRecvMlOff + kSparseMaxCluster * 32 * 4;  // [2][warps][16]
-  static constexpr int kListOff = kMlOff + 2 * kSparseWarps * 16 * 4;
+  static constexpr int kBarOff = kMlOff + 2 * kSparseWarps * 16 * 4;      // [warps][kRing]
+  static constexpr int kListOff = kBarOff + kSparseWarps * kRing * 8;
 };
 
 // Block-wide exclusive prefix sum of one value per thread; total to all.
@@ -491,9 +494,12 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 // (O^T = V^T . P), so a group of up to 8 heads wastes no rows; P goes from
 // one to the other by an 8x8 transpose in registers.
 template <int D, int NH>
-__global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const SparseArgs a) {
+__global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const __grid_constant__ CUtensorMap kv_map,
+                                                                           const SparseArgs a) {
   using C = SparseCfg<D>;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
   float* wml = reinterpret_cast<float*>(smem + C::kMlOff);  // [2][warps][16]
   int32_t* list = reinterpret_cast<int32_t*>(smem + C::kListOff);
   const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
@@ -504,6 +510,11 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
   // lets this one start only once they are complete (without that launch
   // this grid follows them directly and waits first)
   const bool scored = a.max_pages > a.select;
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&kv_map);
+    for (int i = 0; i < kSparseWarps * C::kRing; ++i) mbar_init(&bars[i], 1);
+    fence_barrier_init();
+  }
   if (S > 1) cluster_arrive_relaxed();  // waited for before the first store into another CTA's memory
   if (!scored) pdl_wait();
   SparseRow r;
@@ -541,17 +552,16 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
     __syncthreads();
   }
 
+  // the selection's use of the ring's bytes, before the copies'
+  fence_proxy_async_smem();
+  __syncthreads();
+
   // ---- a warp takes units of 16 tokens: K, V, K, V, ... through its own ring
   const int upp = PS / kSparseUnit;  // units of a page: 1 or 2
   const int ushift = upp == 2 ? 1 : 0;
   const int units = (hi - lo) * upp;
-  const uint32_t ring = smem_u32(smem) + warp * C::kRing * C::kTile;
-  const int64_t token = (int64_t)a.num_kv_heads * D;
-  constexpr int kUnits = D / 8;               // 16-byte units of a row
-  constexpr int kRows = 32 / kUnits;          // rows that a warp's copy instruction covers
-  constexpr int kCopies = kSparseUnit / kRows;
-  const int row0 = lane / kUnits, col = lane % kUnits;
-  const bf16* kv_lane = a.kv + (int64_t)kvh * D + row0 * token + col * 8;
+  uint8_t* ring = smem + warp * C::kRing * C::kTile;
+  uint64_t* full = bars + warp * C::kRing;
   // page id of a unit (looked at when it is loaded), -1 past the last
   auto page_of = [&](int u) { return u < units ? a.indices[r.begin + list[u >> ushift]] : -1; };
   auto live_of = [&](int u) {  // its tokens
@@ -559,26 +569,20 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
     const int len = list[u >> ushift] == r.pages - 1 ? r.last : PS;
     return min(kSparseUnit, max(0, len - (u & (upp - 1)) * kSparseUnit));
   };
-  // 16-byte unit c of row t at t * kRow + ((c ^ (t & 7)) * 16); rows past `live` are zero-filled
-  auto load = [&](int slot, int u, int pg, int live, int kv) {
-    if (u < units) {
-      const bool in = pg >= 0 && (int64_t)pg < a.num_pages;
-      if (!in) {
-        if (lane == 0) set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
-        pg = 0;
-      }
-      const bf16* src = kv_lane + (((int64_t)pg * 2 + kv) * PS + (u & (upp - 1)) * kSparseUnit) * token;
-      const uint32_t dst = ring + slot * C::kTile + row0 * C::kRow;
+  // Tile into a slot: 16-byte unit c of token t at (c / 8) * kHalfBytes +
+  // t * 128 + (((c % 8) ^ (t % 8)) * 16).  One lane; the warp's reads of the
+  // slot are over.
+  auto load = [&](int slot, int u, int pg, int kv) {
+    if (u >= units || lane != 0) return;
+    const bool in = pg >= 0 && (int64_t)pg < a.num_pages;
+    if (!in) set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
+    mbar_arrive_expect_tx(&full[slot], C::kTile);
+    // out of range: the copy writes zeros
+    const int32_t at = in ? 2 * pg + kv : (int32_t)(2 * a.num_pages);
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        const int t = i * kRows + row0;
-        const uint32_t to = dst + i * kRows * C::kRow + ((col ^ (t & 7)) << 4);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src + (int64_t)i * kRows * token),
-                     "r"(in && t < live ? 16 : 0)
-                     : "memory");
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int h = 0; h < C::kHalves; ++h)
+      tma_load_4d(ring + slot * C::kTile + h * C::kHalfBytes, &kv_map, h * 64, kvh, (u & (upp - 1)) * kSparseUnit, at,
+                  &full[slot]);
   };
   float o[NH][D / 16][4];  // O^T: channels 16 j + g (+ 8), heads 8 h + 2 t4 (+ 1)
 #pragma unroll
@@ -589,38 +593,46 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
 #pragma unroll
   for (int h = 0; h < NH; ++h) m[h][0] = m[h][1] = -INFINITY, l[h][0] = l[h][1] = 0.f;
   const float sl2 = a.scale_log2;
-  // unit u, then the two after it; tiles 2 i (K) and 2 i + 1 (V) of the
-  // warp's i-th unit in slots (2 i + kv) % 3
-  int pg = page_of(warp), live = live_of(warp);
-  int pg1 = page_of(warp + kSparseWarps), live1 = live_of(warp + kSparseWarps);
-  load(0, warp, pg, live, 0);
-  load(1, warp, pg, live, 1);
-  load(2, warp + kSparseWarps, pg1, live1, 0);
-  int slot = 0;  // of this unit's K
-  for (int u = warp; u < units; u += kSparseWarps) {
+  // unit u, then the two after it; tile n = 2 i + kv of the warp's i-th unit
+  // in slot n % 3, phase (n / 3) & 1
+  int pg = page_of(warp);
+  int pg1 = page_of(warp + kSparseWarps);
+  load(0, warp, pg, 0);
+  load(1, warp, pg, 1);
+  load(2, warp + kSparseWarps, pg1, 0);
+  int n = 0;
+  bool ok = true;
+  for (int u = warp; u < units; u += kSparseWarps, n += 2) {
     const int un = u + kSparseWarps, unn = un + kSparseWarps;
-    const int pg2 = page_of(unn), live2 = live_of(unn);
-    const int vslot = slot == 2 ? 0 : slot + 1;
-    const uint32_t kt = ring + slot * C::kTile, vt = ring + vslot * C::kTile;
-    asm volatile("cp.async.wait_group 2;" ::: "memory");  // K of this unit
-    __syncwarp();
-    // ---- scores: tokens g, g + 8 x heads 2 t4, 2 t4 + 1
+    const int pg2 = page_of(unn), live = live_of(u);
+    const int kslot = n % C::kRing, vslot = (n + 1) % C::kRing;
+    const uint32_t kt = smem_u32(ring) + kslot * C::kTile, vt = smem_u32(ring) + vslot * C::kTile;
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[kslot], (n / C::kRing) & 1));  // K of this unit
+    if (!ok) break;
+    // ---- scores: tokens g, g + 8 x heads 2 t4, 2 t4 + 1; two chains of products
     float sc[NH][4];
-#pragma unroll
-    for (int h = 0; h < NH; ++h) sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f;
     {
+      float s1[NH][4];
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[h][i] = s1[h][i] = 0.f;
       const int tok = (lane & 7) + 8 * ((lane >> 3) & 1), c0 = lane >> 4;
-      const uint32_t at = kt + tok * C::kRow;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         uint32_t ka[4];
-        ldsm_x4(at + (((2 * kk + c0) ^ (tok & 7)) << 4), ka[0], ka[1], ka[2], ka[3]);
+        const int c = 2 * kk + c0;
+        ldsm_x4(kt + (kk / 4) * C::kHalfBytes + tok * 128 + (((c & 7) ^ (tok & 7)) << 4), ka[0], ka[1], ka[2], ka[3]);
 #pragma unroll
-        for (int h = 0; h < NH; ++h) mma_bf16_b(sc[h], ka, qb[h][kk][0], qb[h][kk][1]);
+        for (int h = 0; h < NH; ++h) mma_bf16_b(kk % 2 ? s1[h] : sc[h], ka, qb[h][kk][0], qb[h][kk][1]);
       }
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[h][i] += s1[h][i];
     }
     __syncwarp();
-    load(slot, un, pg1, live1, 1);  // the next V into this K's place
+    load(kslot, un, pg1, 1);  // the next V into this K's place
     // ---- online softmax (log2 domain), a column per head
     uint32_t ph[NH][2], pr[NH][2];
 #pragma unroll
@@ -630,21 +642,21 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
       sc[h][1] = in0 ? sc[h][1] * sl2 : -INFINITY;
       sc[h][2] = in1 ? sc[h][2] * sl2 : -INFINITY;
       sc[h][3] = in1 ? sc[h][3] * sl2 : -INFINITY;
-      float al[2];
+      // against the running maximum, unless a score exceeds it by 2^8 (or it
+      // is the first): then the maximum moves and the state is rescaled
+      if (__any_sync(0xffffffffu, fmaxf(sc[h][0], sc[h][2]) > m[h][0] + kSparseSlack ||
+                                      fmaxf(sc[h][1], sc[h][3]) > m[h][1] + kSparseSlack)) {
+        float al[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float mx = fmaxf(sc[h][i], sc[h][2 + i]);
+        for (int i = 0; i < 2; ++i) {
+          float mx = fmaxf(sc[h][i], sc[h][2 + i]);
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-        const float mn = fmaxf(m[h][i], mx);
-        al[i] = m[h][i] == mn ? 1.f : sp_exp2(m[h][i] - mn);  // m = -inf: 0 times a state of zeros
-        m[h][i] = mn;
-        const float base = mn == -INFINITY ? 0.f : mn;
-        sc[h][i] = sp_exp2(sc[h][i] - base);
-        sc[h][2 + i] = sp_exp2(sc[h][2 + i] - base);
-        l[h][i] = l[h][i] * al[i] + (sc[h][i] + sc[h][2 + i]);
-      }
-      if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+          for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const float mn = fmaxf(m[h][i], mx);
+          al[i] = m[h][i] == mn ? 1.f : sp_exp2(m[h][i] - mn);  // m = -inf: 0 times a state of zeros
+          m[h][i] = mn;
+          l[h][i] *= al[i];
+        }
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
           o[h][j][0] *= al[0];
@@ -652,6 +664,13 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
           o[h][j][2] *= al[0];
           o[h][j][3] *= al[1];
         }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float base = m[h][i] == -INFINITY ? 0.f : m[h][i];
+        sc[h][i] = sp_exp2(sc[h][i] - base);
+        sc[h][2 + i] = sp_exp2(sc[h][2 + i] - base);
+        l[h][i] += sc[h][i] + sc[h][2 + i];
       }
       // P as a bf16 pair (value and remainder): O keeps fp32's accuracy, for
       // products that this memory-bound loop has to spare
@@ -663,16 +682,30 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
         pr[h][i] = transpose_8x8(pack_bf16x2(sc[h][2 * i] - f.x, sc[h][2 * i + 1] - f.y));
       }
     }
-    asm volatile("cp.async.wait_group 2;" ::: "memory");  // V of this unit
-    __syncwarp();
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[vslot], ((n + 1) / C::kRing) & 1));  // V of this unit
+    if (!ok) {
+      n += 1;  // the next V is under way instead of this K
+      break;
+    }
+    if (live < kSparseUnit) {
+      // rows past the last token hold whatever the pool had there, and 0 * NaN is NaN
+      for (int idx = lane; idx < (kSparseUnit - live) * C::kHalves * 8; idx += 32) {
+        const int t = live + idx / (C::kHalves * 8), hh = (idx / 8) % C::kHalves, c = idx % 8;
+        *reinterpret_cast<uint4*>(ring + vslot * C::kTile + hh * C::kHalfBytes + t * 128 + c * 16) =
+            make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    }
     {
       // A = V^T: rows = channels; lanes 8 i .. 8 i + 7 name the token rows of matrix i
       const int tok = (lane & 7) + 8 * (lane >> 4), c0 = (lane >> 3) & 1;
-      const uint32_t at = vt + tok * C::kRow;
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) {
         uint32_t va[4];
-        ldsm_x4_trans(at + (((2 * j + c0) ^ (tok & 7)) << 4), va[0], va[1], va[2], va[3]);
+        const int c = 2 * j + c0;
+        ldsm_x4_trans(vt + (j / 4) * C::kHalfBytes + tok * 128 + (((c & 7) ^ (tok & 7)) << 4), va[0], va[1], va[2],
+                      va[3]);
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
           mma_bf16_b(o[h][j], va, ph[h][0], ph[h][1]);
@@ -681,13 +714,15 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
       }
     }
     __syncwarp();
-    load(vslot, unn, pg2, live2, 0);  // the K after the next into this V's place
-    live = live1;
-    live1 = live2;
+    load(vslot, unn, pg2, 0);  // the K after the next into this V's place
     pg1 = pg2;
-    slot = slot == 0 ? 2 : slot - 1;  // K of the next unit: (slot + 2) % 3
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (!ok) {
+    // give up: the copies under way (tiles n .. n + 2, as far as they exist) land first
+    if (lane == 0) set_status(a.status, PL_ERR_TIMEOUT);
+    const int tiles = 2 * ((units - warp + kSparseWarps - 1) / kSparseWarps);
+    for (int i = n; i < min(n + 3, tiles); ++i) (void)mbar_wait(&full[i % C::kRing], (i / C::kRing) & 1);
+  }
 
   // ---- the warps' states meet in shared memory
 #pragma unroll
@@ -792,20 +827,20 @@ namespace {
 constexpr int kScoreCtasPerSm = 3;
 
 template <int D, int NH>
-int32_t launch_attend_nh(const pl::SparseArgs& a, int batch, void* stream) {
+int32_t launch_attend_nh(const CUtensorMap& map, const pl::SparseArgs& a, int batch, void* stream) {
   auto kern = pl::sparse_attend_kernel<D, NH>;
   const int list = 4 * ((a.select < a.max_pages ? a.select : a.max_pages) / a.splits + 2);
-  const int smem = pl::SparseCfg<D>::kListOff + ((list + 15) & ~15);
+  const int smem = 1024 + pl::SparseCfg<D>::kListOff + ((list + 15) & ~15);
   int32_t st = pl_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
   if (st != PL_OK) return st;
   const dim3 grid(a.splits, a.num_kv_heads, batch);
-  if (a.splits == 1) return pl_host::launch_pdl(kern, grid, dim3(pl::kSparseThreads), smem, stream, a);
-  return pl_host::launch_pdl_cluster(kern, grid, dim3(pl::kSparseThreads), smem, stream, a.splits, a);
+  if (a.splits == 1) return pl_host::launch_pdl(kern, grid, dim3(pl::kSparseThreads), smem, stream, map, a);
+  return pl_host::launch_pdl_cluster(kern, grid, dim3(pl::kSparseThreads), smem, stream, a.splits, map, a);
 }
 
 template <int D>
-int32_t launch_attend(const pl::SparseArgs& a, int batch, void* stream) {
-  return a.group <= 8 ? launch_attend_nh<D, 1>(a, batch, stream) : launch_attend_nh<D, 2>(a, batch, stream);
+int32_t launch_attend(const CUtensorMap& map, const pl::SparseArgs& a, int batch, void* stream) {
+  return a.group <= 8 ? launch_attend_nh<D, 1>(map, a, batch, stream) : launch_attend_nh<D, 2>(map, a, batch, stream);
 }
 
 }  // namespace
@@ -842,8 +877,8 @@ extern "C" int32_t pl_paged_sparse_decode(
     int32_t* selected, void* workspace, int64_t workspace_bytes, int32_t* status_dev, void* stream) {
   if (q == nullptr || kv_cache == nullptr || indptr == nullptr || indices == nullptr || last_page_len == nullptr ||
       bounds == nullptr || bound_scale == nullptr || out == nullptr || selected == nullptr || batch < 0 ||
-      num_pages <= 0 || total_pages < 0 || max_pages < 0 || num_kv_heads <= 0 || num_qo_heads <= 0 ||
-      num_qo_heads % num_kv_heads != 0 || !(sm_scale > 0.f) || sink_pages < 0 || recent_pages < 1 || num_select < 1 ||
+      num_pages <= 0 || num_pages > 0x3FFFFFFF || total_pages < 0 || max_pages < 0 || num_kv_heads <= 0 ||
+      num_qo_heads <= 0 || num_qo_heads % num_kv_heads != 0 || !(sm_scale > 0.f) || sink_pages < 0 || recent_pages < 1 || num_select < 1 ||
       (int64_t)sink_pages + recent_pages > num_select)
     return PL_ERR_INVALID_ARGUMENT;
   const int group = num_qo_heads / num_kv_heads;
@@ -890,7 +925,9 @@ extern "C" int32_t pl_paged_sparse_decode(
   const int sms = pl_host::sm_count();
   if (sms <= 0) return PL_ERR_NO_DEVICE;
   const int64_t items = (int64_t)batch * num_kv_heads;
-  int32_t st;
+  CUtensorMap map;
+  int32_t st = pl_host::kv_tensor_map_rows(kv_cache, num_pages, num_kv_heads, head_dim, page_size, pl::kSparseUnit, &map);
+  if (st != PL_OK) return st;
   if (max_pages > num_select) {
     // a warp takes 8 pages a step; as many CTAs as the device holds at once,
     // but no more than there are steps
@@ -909,5 +946,5 @@ extern "C" int32_t pl_paged_sparse_decode(
   while (splits < pl::kSparseMaxCluster && items * splits * 2 <= 2 * sms && units >= (int64_t)splits * pl::kSparseWarps)
     splits *= 2;
   a.splits = splits;
-  return head_dim == 128 ? launch_attend<128>(a, batch, stream) : launch_attend<64>(a, batch, stream);
+  return head_dim == 128 ? launch_attend<128>(map, a, batch, stream) : launch_attend<64>(map, a, batch, stream);
 }
