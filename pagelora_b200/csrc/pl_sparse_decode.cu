@@ -118,14 +118,15 @@ struct SparseArgs {
   const int8_t* bounds;
   const float* scale;
   int32_t num_qo_heads, num_kv_heads, group, page_size, select, sink, recent;
-  int32_t max_pages;     // keys kept per (row, kv head)
+  int32_t max_pages;     // no row has more
+  int32_t key_stride;    // keys kept per (row, kv head), a multiple of 4
   int32_t splits;        // CTAs per (row, kv head) of the second launch
   float scale_log2;
   bf16* out;
   int64_t o_stride_b, o_stride_h;
   float* out_lse;
   int32_t* selected;     // [batch][hkv][select], ascending, -1 past the last
-  uint32_t* keys;        // workspace [batch][hkv][max_pages]
+  uint32_t* keys;        // workspace [batch][hkv][key_stride]: competing pages
   int32_t* status;
 };
 
@@ -160,17 +161,28 @@ __device__ __forceinline__ void mma_s8_16832(int* d, const uint32_t* a, uint32_t
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// 16 bytes of bounds: read once, so not kept in L1; L2 fetches the 256 bytes
+// around them at once.
+__device__ __forceinline__ uint4 ld_bounds(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
 // Keys of the pages of row b.  A warp has one kv head and 8 pages a step: a
 // matrix product of the group's quantised queries (rows; per head min(qi, 0)
 // against lo and max(qi, 0) against hi, 2 D bytes) with the pages' bounds.
 // The product's order along 2 D is free, so a lane's operand is what it
 // loads: 16 contiguous bytes of its page per 64.  The warps of a CTA take
 // neighbouring heads of the same pages, whose bounds lie side by side.
-template <int D>
+// NH = 1: at most 8 heads, the product's lower rows stay empty.
+template <int D, int NH>
 __global__ void __launch_bounds__(kSparseThreads, 3) sparse_score_kernel(const SparseArgs a) {
   constexpr int kBytes = 2 * D;          // bounds of one page and head
   constexpr int kLd = kBytes / 64;       // 16-byte loads of a lane per page
-  __shared__ __align__(16) int8_t qs_all[kSparseWarps][16][kBytes + 16];
+  __shared__ __align__(16) int8_t qs_all[kSparseWarps][8 * NH][kBytes + 16];
   pdl_wait();
   pdl_launch_dependents();
   const int b = blockIdx.z;
@@ -191,7 +203,7 @@ __global__ void __launch_bounds__(kSparseThreads, 3) sparse_score_kernel(const S
   int pid = page(p);
   // quantise the group's queries: 8 channels a lane and step
   int8_t(*qs)[kBytes + 16] = qs_all[warp];
-  constexpr int kMost = 16 * D / 256;
+  constexpr int kMost = 8 * NH * D / 256;
   uint4 qv[kMost];
   float m = 0.f;
 #pragma unroll
@@ -231,20 +243,23 @@ __global__ void __launch_bounds__(kSparseThreads, 3) sparse_score_kernel(const S
     *reinterpret_cast<uint2*>(&qs[i / D][D + i % D]) = *reinterpret_cast<uint2*>(pos);
   }
   __syncwarp();
-  uint32_t qa[2 * kLd][4];
+  uint32_t qa[2 * kLd][2 * NH];  // rows g (and g + 8) of the product, 8 bytes each
 #pragma unroll
   for (int j = 0; j < kLd; ++j)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = 64 * j + 16 * t + 8 * h;
-      const uint2 lo = *reinterpret_cast<const uint2*>(&qs[g][at]);
-      const uint2 hi = *reinterpret_cast<const uint2*>(&qs[g + 8][at]);
-      qa[2 * j + h][0] = lo.x;
-      qa[2 * j + h][1] = hi.x;
-      qa[2 * j + h][2] = lo.y;
-      qa[2 * j + h][3] = hi.y;
-    }
-  uint32_t* keys = a.keys + ((int64_t)b * a.num_kv_heads + kvh) * a.max_pages;
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < NH; ++i) {
+        const uint2 v = *reinterpret_cast<const uint2*>(&qs[g + 8 * i][64 * j + 16 * t + 8 * h]);
+        qa[2 * j + h][2 * i] = v.x;
+        qa[2 * j + h][2 * i + 1] = v.y;
+      }
+  auto product = [&](int* c, const uint32_t* q, uint32_t b0, uint32_t b1) {
+    const uint32_t full[4] = {q[0], NH == 2 ? q[2 * NH - 2] : 0u, q[1], NH == 2 ? q[2 * NH - 1] : 0u};
+    mma_s8_16832(c, full, b0, b1);
+  };
+  // keys of the competing pages, from the first on
+  uint32_t* keys = a.keys + ((int64_t)b * a.num_kv_heads + kvh) * a.key_stride - a.sink;
   // bounds are loaded a step ahead, page ids two
   struct Step {
     uint4 w[kLd];
@@ -257,7 +272,7 @@ __global__ void __launch_bounds__(kSparseThreads, 3) sparse_score_kernel(const S
     const int64_t slot = (int64_t)(s.in ? id : 0) * a.num_kv_heads + kvh;
     const uint4* src = reinterpret_cast<const uint4*>(a.bounds + slot * kBytes) + t;
 #pragma unroll
-    for (int j = 0; j < kLd; ++j) s.w[j] = s.in ? __ldg(src + 4 * j) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < kLd; ++j) s.w[j] = s.in ? ld_bounds(src + 4 * j) : make_uint4(0, 0, 0, 0);
     s.sc = s.in ? __ldg(a.scale + slot) : 0.f;
   };
   Step cur;
@@ -270,12 +285,12 @@ __global__ void __launch_bounds__(kSparseThreads, 3) sparse_score_kernel(const S
     int c[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < kLd; ++j) {
-      mma_s8_16832(c, qa[2 * j], cur.w[j].x, cur.w[j].y);
-      mma_s8_16832(c, qa[2 * j + 1], cur.w[j].z, cur.w[j].w);
+      product(c, qa[2 * j], cur.w[j].x, cur.w[j].y);
+      product(c, qa[2 * j + 1], cur.w[j].z, cur.w[j].w);
     }
     // rows g and g + 8 of pages 2 t and 2 t + 1: the maximum over the heads
-    int s0 = max(g < a.group ? c[0] : INT32_MIN, g + 8 < a.group ? c[2] : INT32_MIN);
-    int s1 = max(g < a.group ? c[1] : INT32_MIN, g + 8 < a.group ? c[3] : INT32_MIN);
+    int s0 = max(g < a.group ? c[0] : INT32_MIN, NH == 2 && g + 8 < a.group ? c[2] : INT32_MIN);
+    int s1 = max(g < a.group ? c[1] : INT32_MIN, NH == 2 && g + 8 < a.group ? c[3] : INT32_MIN);
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
       s0 = max(s0, __shfl_xor_sync(0xffffffffu, s0, o));
@@ -301,7 +316,7 @@ struct SparseCfg {
   static constexpr int kRing = 3;                              // tiles (K, V, K, ...) of a warp in flight
   static constexpr int kStages = kSparseWarps * kRing * kTile;
   static constexpr int kScratch = kSparseWarps * 16 * kOPad * 4;
-  static constexpr int kSelect = kSparseBins * 4;
+  static constexpr int kSelect = (kSparseBins + kSparseBins / 8) * 4;
   // the selection, the tiles in flight and the join of the warps' states use
   // the same bytes one after the other
   static constexpr int kArena = kStages > kScratch ? (kStages > kSelect ? kStages : kSelect)
@@ -337,12 +352,17 @@ __device__ __forceinline__ int sparse_scan(int v, int* warp_sums, int& total) {
   return before + inc - v;
 }
 
+// Histogram bin b lives at b + b / 8: a thread reads 8 bins in a row
+// without bank conflicts.
+__device__ __forceinline__ int sparse_bin(int b) { return b + (b >> 3); }
+
 // The selected pages with rank [lo, hi) in index order, into list[0 ..
-// hi - lo); all of them to `all` when it is given.  keys[p] for the pages
-// [sink, n - recent); n > select.  Warp w has a contiguous range of the
-// competing pages, a lane every 32nd of it; kHold > 0: at most kHold keys a
-// thread, held in registers; 0: any number, read from L2 in every pass.
-template <int kHold>
+// hi - lo); all of them to `all` when it is given.  keys: of the competing
+// pages [sink, n - recent), 16-byte aligned; n > select.  They are dealt in
+// quads of 4 neighbours, quad j of thread t at (j * threads + t) * 4.
+// kQuads > 0: held in registers (quads <= kQuads); 0: read from L2 in every
+// pass.
+template <int kQuads>
 __device__ __forceinline__ void sparse_select(const SparseArgs& a, const uint32_t* keys, int n, int* hist, int lo,
                                               int hi, int32_t* list, int32_t* all) {
   __shared__ int warp_sums[kSparseWarps];
@@ -350,34 +370,46 @@ __device__ __forceinline__ void sparse_select(const SparseArgs& a, const uint32_
   __shared__ int found[3];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int first = a.sink, count = n - a.recent - a.sink, want = a.select - a.recent - a.sink;
-  keys += first;
-  const int per = (count + kSparseWarps * 32 - 1) / (kSparseWarps * 32);  // keys of a thread
-  const int base = warp * per * 32 + lane;
-  uint32_t held[kHold > 0 ? kHold : 1];
-  if constexpr (kHold > 0) {
+  const int quads = (count + 4 * kSparseThreads - 1) / (4 * kSparseThreads);
+  auto at = [&](int j) { return (j * kSparseThreads + (int)threadIdx.x) * 4; };
+  auto quad = [&](int j) {
+    return at(j) < count ? *reinterpret_cast<const uint4*>(keys + at(j)) : make_uint4(0, 0, 0, 0);
+  };
+  uint4 held[kQuads > 0 ? kQuads : 1];
+  if constexpr (kQuads > 0) {
 #pragma unroll
-    for (int j = 0; j < kHold; ++j) held[j] = j < per && base + 32 * j < count ? __ldcg(keys + base + 32 * j) : 0u;
+    for (int j = 0; j < kQuads; ++j)
+      if (j < quads) held[j] = quad(j);
   }
-  // f(key, index) for the thread's keys, in order; every lane of a warp does every step
-  auto each = [&](auto f) {
-    if constexpr (kHold > 0) {
+  // f(key, index) for the keys of quad j
+  auto four = [&](int j, auto f) {
+    uint4 q;
+    if constexpr (kQuads > 0)
+      q = held[j];
+    else
+      q = quad(j);
+    const int i = at(j);
+    if (i < count) f(q.x, i);
+    if (i + 1 < count) f(q.y, i + 1);
+    if (i + 2 < count) f(q.z, i + 2);
+    if (i + 3 < count) f(q.w, i + 3);
+  };
+  // every(j) for the quads in use
+  auto quads_of = [&](auto every) {
+    if constexpr (kQuads > 0) {
 #pragma unroll
-      for (int j = 0; j < kHold; ++j)
-        if (j < per) f(held[j], base + 32 * j);
+      for (int j = 0; j < kQuads; ++j)
+        if (j < quads) every(j);
     } else {
-#pragma unroll 4
-      for (int j = 0; j < per; ++j) {
-        const int i = base + 32 * j;
-        f(i < count ? __ldcg(keys + i) : 0u, i);
-      }
+#pragma unroll 1
+      for (int j = 0; j < quads; ++j) every(j);
     }
   };
+  auto each = [&](auto f) { quads_of([&](int j) { four(j, f); }); };
   uint32_t kmin = 0xffffffffu, kmax = 0;
-  each([&](uint32_t k, int i) {
-    if (i < count) {
-      kmin = min(kmin, k);
-      kmax = max(kmax, k);
-    }
+  each([&](uint32_t k, int) {
+    kmin = min(kmin, k);
+    kmax = max(kmax, k);
   });
   kmin = __reduce_min_sync(0xffffffffu, kmin);
   kmax = __reduce_max_sync(0xffffffffu, kmax);
@@ -385,7 +417,7 @@ __device__ __forceinline__ void sparse_select(const SparseArgs& a, const uint32_
     mm[warp] = kmin;
     mm[kSparseWarps + warp] = kmax;
   }
-  for (int i = threadIdx.x; i < kSparseBins; i += kSparseThreads) hist[i] = 0;
+  for (int i = threadIdx.x; i < kSparseBins + kSparseBins / 8; i += kSparseThreads) hist[i] = 0;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kSparseWarps; ++w) {
@@ -396,13 +428,13 @@ __device__ __forceinline__ void sparse_select(const SparseArgs& a, const uint32_
   // taken are the keys whose bits from `shift` on are above `prefix`, and
   // `rest` of those where they equal it.
   int shift = kmin == kmax ? 0 : 32 - __clz(kmin ^ kmax);  // bits below are undecided
-  auto upper = [](uint32_t k, int s) { return s == 32 ? 0u : k >> s; };
+  auto upper = [](uint32_t k, int s) { return __funnelshift_rc(k, 0u, s); };  // k >> s, 0 for s = 32
   uint32_t prefix = upper(kmax, shift);  // common to all keys
   int rest = want;
   while (shift > 0 && rest > 0) {
     const int bits = min(11, shift), low = shift - bits;
-    each([&](uint32_t k, int i) {
-      if (i < count && upper(k, shift) == prefix) atomicAdd(&hist[(k >> low) & ((1u << bits) - 1)], 1);
+    each([&](uint32_t k, int) {
+      if (upper(k, shift) == prefix) atomicAdd(&hist[sparse_bin((k >> low) & ((1u << bits) - 1))], 1);
     });
     __syncthreads();
     // from the top: the bin in which the count passes `rest`; thread 0 has the highest bins
@@ -411,17 +443,14 @@ __device__ __forceinline__ void sparse_select(const SparseArgs& a, const uint32_
     const int top = (1 << bits) - 1 - threadIdx.x * kPer;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      h[j] = 0;
-      if (top - j >= 0) {
-        h[j] = hist[top - j];
-        hist[top - j] = 0;  // for the next pass
-      }
+      h[j] = top - j >= 0 ? hist[sparse_bin(top - j)] : 0;
       sum += h[j];
     }
     int total;
     int before = sparse_scan(sum, warp_sums, total);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
+      if (top - j >= 0) hist[sparse_bin(top - j)] = 0;  // for the next pass
       if (before < rest && before + h[j] >= rest) {
         found[0] = top - j;
         found[1] = rest - before;
@@ -435,43 +464,79 @@ __device__ __forceinline__ void sparse_select(const SparseArgs& a, const uint32_
     shift = low;
     if (found[1] == found[2]) break;  // all keys of the bin are taken
   }
-  // gather in index order
-  int n_gt = 0, n_eq = 0;
-  each([&](uint32_t k, int i) {
-    const uint32_t u = upper(k, shift);
-    n_gt += i < count && u > prefix;
-    n_eq += i < count && u == prefix;
-  });
-  n_gt = __reduce_add_sync(0xffffffffu, n_gt);
-  n_eq = __reduce_add_sync(0xffffffffu, n_eq);
-  __syncthreads();  // the extremes have been read
-  if (lane == 0) {
-    mm[warp] = n_gt;
-    mm[kSparseWarps + warp] = n_eq;
-  }
-  __syncthreads();
-  int gt = 0, eq = 0;
+  // gather in index order, row of quads after row; counts above and at the
+  // prefix in 16 bits each (a row has 4 * threads keys)
+  auto bits_of = [&](int j) {  // bit e: key e of the quad is above the prefix; bit 4 + e: at it
+    const int i = at(j);
+    uint32_t m = 0;
+    four(j, [&](uint32_t k, int at_k) {
+      const uint32_t u = upper(k, shift);
+      m |= (u > prefix ? 1u : u == prefix ? 0x10u : 0u) << (at_k - i);
+    });
+    return m;
+  };
+  auto count_of = [](uint32_t m) { return __popc(m & 0xfu) + (__popc(m & 0xf0u) << 16); };
+  uint32_t bits[kQuads > 0 ? kQuads : 1];
+  int own[kQuads > 0 ? kQuads : 1];  // this thread's count of the row, and the warp's up to it
+  int inc[kQuads > 0 ? kQuads : 1];
+  auto scan = [&](int v) {
 #pragma unroll
-  for (int w = 0; w < kSparseWarps; ++w) {
-    gt += w < warp ? mm[w] : 0;
-    eq += w < warp ? mm[kSparseWarps + w] : 0;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  };
   auto put = [&](int rank, int page) {
     if (rank >= lo && rank < hi) list[rank - lo] = page;
     if (all != nullptr) all[rank] = page;
   };
-  const uint32_t below = (1u << lane) - 1;
-  each([&](uint32_t k, int i) {
-    const uint32_t u = upper(k, shift);
-    const bool is_gt = i < count && u > prefix, is_eq = i < count && u == prefix;
-    const uint32_t bg = __ballot_sync(0xffffffffu, is_gt), be = __ballot_sync(0xffffffffu, is_eq);
-    if ((bg | be) != 0) {
-      const int my_eq = eq + __popc(be & below);
-      if (is_gt || (is_eq && my_eq < rest)) put(first + gt + __popc(bg & below) + min(my_eq, rest), first + i);
-      gt += __popc(bg);
-      eq += __popc(be);
+  auto place = [&](int j, uint32_t m, int gt, int eq) {  // gt, eq: in front of this thread's quad
+#pragma unroll 1
+    for (uint32_t left = (m | m >> 4) & 0xfu; left != 0; left &= left - 1) {
+      const int e = __ffs(left) - 1;
+      const bool above = (m >> e) & 1u;
+      if (above || eq < rest) put(first + gt + min(eq, rest), first + at(j) + e);
+      gt += above ? 1 : 0;
+      eq += above ? 0 : 1;
     }
-  });
+  };
+  if constexpr (kQuads > 0) {
+    __shared__ int rows[kQuads][kSparseWarps];
+    quads_of([&](int j) {
+      bits[j] = bits_of(j);
+      own[j] = count_of(bits[j]);
+      inc[j] = scan(own[j]);
+      if (lane == 31) rows[j][warp] = inc[j];
+    });
+    __syncthreads();
+    int gt = 0, eq = 0;  // of the rows before
+    quads_of([&](int j) {
+      int g = 0, e = 0, ga = 0, ea = 0;
+#pragma unroll
+      for (int w = 0; w < kSparseWarps; ++w) {
+        const int v = rows[j][w];
+        g += w < warp ? v & 0xffff : 0;
+        e += w < warp ? v >> 16 : 0;
+        ga += v & 0xffff;
+        ea += v >> 16;
+      }
+      const int before = inc[j] - own[j];
+      if (own[j] != 0) place(j, bits[j], gt + g + (before & 0xffff), eq + e + (before >> 16));
+      gt += ga;
+      eq += ea;
+    });
+  } else {
+    int gt = 0, eq = 0;
+    quads_of([&](int j) {
+      bits[0] = bits_of(j);
+      int total;
+      const int before = sparse_scan(count_of(bits[0]), warp_sums, total);
+      if (bits[0] != 0) place(j, bits[0], gt + (before & 0xffff), eq + (before >> 16));
+      gt += total & 0xffff;
+      eq += total >> 16;
+    });
+  }
   for (int i = threadIdx.x; i < a.sink; i += kSparseThreads) put(i, i);
   for (int i = threadIdx.x; i < a.recent; i += kSparseThreads) put(a.select - a.recent + i, n - a.recent + i);
   __syncthreads();
@@ -537,12 +602,12 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
   pdl_launch_dependents();
   int32_t* all = split == 0 ? a.selected + ((int64_t)b * a.num_kv_heads + kvh) * a.select : nullptr;
   if (r.pages > a.select) {
-    const uint32_t* keys = a.keys + ((int64_t)b * a.num_kv_heads + kvh) * a.max_pages;
+    const uint32_t* keys = a.keys + ((int64_t)b * a.num_kv_heads + kvh) * a.key_stride;
     int* hist = reinterpret_cast<int*>(smem);
     if (r.pages <= 4 * kSparseThreads)
-      sparse_select<4>(a, keys, r.pages, hist, lo, hi, list, all);
+      sparse_select<1>(a, keys, r.pages, hist, lo, hi, list, all);
     else if (r.pages <= 32 * kSparseThreads)
-      sparse_select<32>(a, keys, r.pages, hist, lo, hi, list, all);
+      sparse_select<8>(a, keys, r.pages, hist, lo, hi, list, all);
     else
       sparse_select<0>(a, keys, r.pages, hist, lo, hi, list, all);
   } else {
@@ -824,7 +889,7 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
 // =================================================================== host
 namespace {
 
-constexpr int kScoreCtasPerSm = 3;
+int32_t sparse_key_stride(int32_t max_pages) { return (int32_t)(((int64_t)max_pages + 3) & ~int64_t(3)); }
 
 template <int D, int NH>
 int32_t launch_attend_nh(const CUtensorMap& map, const pl::SparseArgs& a, int batch, void* stream) {
@@ -865,7 +930,7 @@ extern "C" int32_t pl_page_bounds(const void* kv_cache, int64_t num_pages, int32
 
 extern "C" int64_t pl_sparse_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t max_pages) {
   if (batch <= 0 || num_kv_heads <= 0 || max_pages <= 0) return 0;
-  return (int64_t)batch * num_kv_heads * max_pages * 4;
+  return (int64_t)batch * num_kv_heads * sparse_key_stride(max_pages) * 4;
 }
 
 extern "C" int32_t pl_paged_sparse_decode(
@@ -877,7 +942,7 @@ extern "C" int32_t pl_paged_sparse_decode(
     int32_t* selected, void* workspace, int64_t workspace_bytes, int32_t* status_dev, void* stream) {
   if (q == nullptr || kv_cache == nullptr || indptr == nullptr || indices == nullptr || last_page_len == nullptr ||
       bounds == nullptr || bound_scale == nullptr || out == nullptr || selected == nullptr || batch < 0 ||
-      num_pages <= 0 || num_pages > 0x3FFFFFFF || total_pages < 0 || max_pages < 0 || num_kv_heads <= 0 ||
+      num_pages <= 0 || num_pages > 0x3FFFFFFF || total_pages < 0 || max_pages < 0 || max_pages > 0x7FFFFFF0 || num_kv_heads <= 0 ||
       num_qo_heads <= 0 || num_qo_heads % num_kv_heads != 0 || !(sm_scale > 0.f) || sink_pages < 0 || recent_pages < 1 || num_select < 1 ||
       (int64_t)sink_pages + recent_pages > num_select)
     return PL_ERR_INVALID_ARGUMENT;
@@ -914,6 +979,7 @@ extern "C" int32_t pl_paged_sparse_decode(
   a.sink = sink_pages;
   a.recent = recent_pages;
   a.max_pages = max_pages;
+  a.key_stride = sparse_key_stride(max_pages);
   a.scale_log2 = sm_scale * pl::kLog2e;
   a.out = static_cast<pl::bf16*>(out);
   a.o_stride_b = o_stride_b;
@@ -934,9 +1000,10 @@ extern "C" int32_t pl_paged_sparse_decode(
     const int hw = num_kv_heads < pl::kSparseWarps ? num_kv_heads : pl::kSparseWarps, pw = pl::kSparseWarps / hw;
     const int head_groups = (num_kv_heads + pl::kSparseWarps - 1) / pl::kSparseWarps;
     const int64_t steps = (max_pages + 8 * pw - 1) / (8 * pw);
-    int64_t chunks = kScoreCtasPerSm * (int64_t)sms / ((int64_t)batch * head_groups);
+    int64_t chunks = 3 * (int64_t)sms / ((int64_t)batch * head_groups);
     chunks = chunks > steps ? steps : (chunks < 1 ? 1 : chunks);
-    auto score = head_dim == 128 ? pl::sparse_score_kernel<128> : pl::sparse_score_kernel<64>;
+    auto score = head_dim == 128 ? (group <= 8 ? pl::sparse_score_kernel<128, 1> : pl::sparse_score_kernel<128, 2>)
+                                 : (group <= 8 ? pl::sparse_score_kernel<64, 1> : pl::sparse_score_kernel<64, 2>);
     st = pl_host::launch_pdl(score, dim3((int)chunks, head_groups, batch), dim3(pl::kSparseThreads), 0, stream, a);
     if (st != PL_OK) return st;
   }
