@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(kBoundsThreads)
 // distributed shared memory.
 constexpr int kSparseThreads = 256;
 constexpr int kSparseWarps = kSparseThreads / 32;
+constexpr int kScorePages = 16;          // pages a warp scores at a time
 constexpr int kSparseUnit = 16;          // tokens a warp takes at a time
 constexpr int kSparseMaxCluster = 8;
 constexpr int kSparseBins = 2048;        // 11 bits of the key per pass
@@ -161,25 +162,15 @@ __device__ __forceinline__ void mma_s8_16832(int* d, const uint32_t* a, uint32_t
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 16 bytes of bounds: read once, so not kept in L1; L2 fetches the 256 bytes
-// around them at once.
-__device__ __forceinline__ uint4 ld_bounds(const uint4* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-
-// Keys of the pages of row b.  A warp has one kv head and 8 pages a step: a
-// matrix product of the group's quantised queries (rows; per head min(qi, 0)
-// against lo and max(qi, 0) against hi, 2 D bytes) with the pages' bounds.
-// The product's order along 2 D is free, so a lane's operand is what it
-// loads: 16 contiguous bytes of its page per 64.  The warps of a CTA take
-// neighbouring heads of the same pages, whose bounds lie side by side.
-// NH = 1: at most 8 heads, the product's lower rows stay empty.
+// Keys of the pages of row b.  A warp has one kv head and 16 pages a step: a
+// matrix product of the pages' bounds (rows) with the group's quantised
+// queries (columns; per head min(qi, 0) against lo and max(qi, 0) against hi,
+// 2 D bytes).  The product's order along 2 D is free, so a lane's operand is
+// what it loads: 16 contiguous bytes of two pages per 64.  The warps of a CTA
+// take neighbouring heads of the same pages, whose bounds lie side by side.
+// NH: tiles of 8 heads.
 template <int D, int NH>
-__global__ void __launch_bounds__(kSparseThreads, 3) sparse_score_kernel(const SparseArgs a) {
+__global__ void __launch_bounds__(kSparseThreads, 2) sparse_score_kernel(const SparseArgs a) {
   constexpr int kBytes = 2 * D;          // bounds of one page and head
   constexpr int kLd = kBytes / 64;       // 16-byte loads of a lane per page
   __shared__ __align__(16) int8_t qs_all[kSparseWarps][8 * NH][kBytes + 16];
@@ -190,16 +181,18 @@ __global__ void __launch_bounds__(kSparseThreads, 3) sparse_score_kernel(const S
   r.load(a, b);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  // heads side by side, and groups of 8 pages when there are fewer heads than warps
+  // heads side by side, and groups of 16 pages when there are fewer heads than warps
   const int hw = min(kSparseWarps, a.num_kv_heads), pw = kSparseWarps / hw;
   const int kvh = (int)blockIdx.y * kSparseWarps + warp % hw;
   // pages that compete; forced ones have no key
-  const int p_end = r.pages - a.recent;
-  const int step = gridDim.x * pw * 8;
-  int p = a.sink + ((int)blockIdx.x * pw + warp / hw) * 8;
-  if (r.pages <= a.select || p >= p_end || warp >= hw * pw || kvh >= a.num_kv_heads) return;  // no block barrier below
+  const int count = r.pages - a.recent - a.sink;
+  const int step = gridDim.x * pw * kScorePages;
+  int p = ((int)blockIdx.x * pw + warp / hw) * kScorePages;
+  if (r.pages <= a.select || p >= count || warp >= hw * pw || kvh >= a.num_kv_heads) return;  // no block barrier below
 
-  auto page = [&](int at) { return at + g < p_end ? a.indices[r.begin + at + g] : -1; };
+  const int32_t* ids = a.indices + r.begin + a.sink;
+  // lane pair (g, t): pages g (even t) and g + 8 (odd t) of a step
+  auto page = [&](int at) { return at + g + 8 * (t & 1) < count ? ids[at + g + 8 * (t & 1)] : -1; };
   int pid = page(p);
   // quantise the group's queries: 8 channels a lane and step
   int8_t(*qs)[kBytes + 16] = qs_all[warp];
@@ -243,67 +236,81 @@ __global__ void __launch_bounds__(kSparseThreads, 3) sparse_score_kernel(const S
     *reinterpret_cast<uint2*>(&qs[i / D][D + i % D]) = *reinterpret_cast<uint2*>(pos);
   }
   __syncwarp();
-  uint32_t qa[2 * kLd][2 * NH];  // rows g (and g + 8) of the product, 8 bytes each
+  uint2 qb[NH][2 * kLd];  // column g of tile h: the 8 bytes that meet a lane's
 #pragma unroll
-  for (int j = 0; j < kLd; ++j)
+  for (int h = 0; h < NH; ++h)
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < NH; ++i) {
-        const uint2 v = *reinterpret_cast<const uint2*>(&qs[g + 8 * i][64 * j + 16 * t + 8 * h]);
-        qa[2 * j + h][2 * i] = v.x;
-        qa[2 * j + h][2 * i + 1] = v.y;
-      }
-  auto product = [&](int* c, const uint32_t* q, uint32_t b0, uint32_t b1) {
-    const uint32_t full[4] = {q[0], NH == 2 ? q[2 * NH - 2] : 0u, q[1], NH == 2 ? q[2 * NH - 1] : 0u};
-    mma_s8_16832(c, full, b0, b1);
-  };
-  // keys of the competing pages, from the first on
-  uint32_t* keys = a.keys + ((int64_t)b * a.num_kv_heads + kvh) * a.key_stride - a.sink;
+    for (int j = 0; j < 2 * kLd; ++j)
+      qb[h][j] = *reinterpret_cast<const uint2*>(&qs[8 * h + g][64 * (j >> 1) + 16 * t + 8 * (j & 1)]);
+  uint32_t* keys = a.keys + ((int64_t)b * a.num_kv_heads + kvh) * a.key_stride;
+  const int8_t* bounds = a.bounds + (int64_t)kvh * kBytes + 16 * t;
+  const float* scale = a.scale + kvh;
   // bounds are loaded a step ahead, page ids two
   struct Step {
-    uint4 w[kLd];
-    float sc;
-    bool in;
+    uint4 w[2][kLd];
+    float sc;  // of this lane's page, NaN: outside the pool
   };
   auto fetch = [&](Step& s, int at, int id) {
-    s.in = id >= 0 && (int64_t)id < a.num_pages;
-    if (!s.in && at + g < p_end && t == 0) set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
-    const int64_t slot = (int64_t)(s.in ? id : 0) * a.num_kv_heads + kvh;
-    const uint4* src = reinterpret_cast<const uint4*>(a.bounds + slot * kBytes) + t;
+    const bool in = id >= 0 && (int64_t)id < a.num_pages;
+    if (!in && at + g + 8 * (t & 1) < count && t < 2) set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
+    const int mine = in ? id : 0;
 #pragma unroll
-    for (int j = 0; j < kLd; ++j) s.w[j] = s.in ? ld_bounds(src + 4 * j) : make_uint4(0, 0, 0, 0);
-    s.sc = s.in ? __ldg(a.scale + slot) : 0.f;
+    for (int i = 0; i < 2; ++i) {
+      const int pg = __shfl_sync(0xffffffffu, mine, (lane & ~3) + i);
+      const uint4* src = reinterpret_cast<const uint4*>(bounds + (int64_t)pg * a.num_kv_heads * kBytes);
+#pragma unroll
+      for (int j = 0; j < kLd; ++j) s.w[i][j] = __ldg(src + 4 * j);
+    }
+    s.sc = in ? __ldg(scale + (int64_t)mine * a.num_kv_heads) : __int_as_float(0x7fffffff);
   };
-  Step cur;
-  fetch(cur, p, pid);
+  auto score = [&](const Step& s, int at) {
+    int c[NH][4];
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      c[h][0] = c[h][1] = c[h][2] = c[h][3] = 0;
+#pragma unroll
+      for (int j = 0; j < kLd; ++j) {
+        const uint32_t lo[4] = {s.w[0][j].x, s.w[1][j].x, s.w[0][j].y, s.w[1][j].y};
+        const uint32_t hi[4] = {s.w[0][j].z, s.w[1][j].z, s.w[0][j].w, s.w[1][j].w};
+        mma_s8_16832(c[h], lo, qb[h][2 * j].x, qb[h][2 * j].y);
+        mma_s8_16832(c[h], hi, qb[h][2 * j + 1].x, qb[h][2 * j + 1].y);
+      }
+    }
+    // the maximum over the heads: columns 2 t, 2 t + 1 of pages g and g + 8
+    int s0 = INT32_MIN, s1 = INT32_MIN;
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (8 * h + 2 * t + i < a.group) {
+          s0 = max(s0, c[h][i]);
+          s1 = max(s1, c[h][2 + i]);
+        }
+    s0 = max(s0, __shfl_xor_sync(0xffffffffu, s0, 1));
+    s1 = max(s1, __shfl_xor_sync(0xffffffffu, s1, 1));
+    s0 = max(s0, __shfl_xor_sync(0xffffffffu, s0, 2));
+    s1 = max(s1, __shfl_xor_sync(0xffffffffu, s1, 2));
+    const int i = at + g + 8 * (t & 1);
+    if (t < 2 && i < count) {
+      const float best = (float)((t & 1) ? s1 : s0);
+      const bool in = __float_as_int(s.sc) != 0x7fffffff;
+      keys[i] = in ? order_key(isinf(s.sc) ? INFINITY : __fmul_rn(best, s.sc)) : 0u;
+    }
+  };
+  Step s0, s1;
+  fetch(s0, p, pid);
   pid = page(p + step);
-  for (; p < p_end; p += step) {
-    Step next;
-    if (p + step < p_end) fetch(next, p + step, pid);
+  while (true) {
+    if (p + step < count) fetch(s1, p + step, pid);
     pid = page(p + 2 * step);
-    int c[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < kLd; ++j) {
-      product(c, qa[2 * j], cur.w[j].x, cur.w[j].y);
-      product(c, qa[2 * j + 1], cur.w[j].z, cur.w[j].w);
-    }
-    // rows g and g + 8 of pages 2 t and 2 t + 1: the maximum over the heads
-    int s0 = max(g < a.group ? c[0] : INT32_MIN, NH == 2 && g + 8 < a.group ? c[2] : INT32_MIN);
-    int s1 = max(g < a.group ? c[1] : INT32_MIN, NH == 2 && g + 8 < a.group ? c[3] : INT32_MIN);
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      s0 = max(s0, __shfl_xor_sync(0xffffffffu, s0, o));
-      s1 = max(s1, __shfl_xor_sync(0xffffffffu, s1, o));
-    }
-    // lane 4 g holds page g's scale; its score sits with t = g / 2
-    const int from = g >> 1;
-    const int e0 = __shfl_sync(0xffffffffu, s0, from), e1 = __shfl_sync(0xffffffffu, s1, from);
-    if (t == 0 && p + g < p_end) {
-      const int best = (g & 1) ? e1 : e0;
-      keys[p + g] = cur.in ? order_key(isinf(cur.sc) ? INFINITY : __fmul_rn((float)best, cur.sc)) : 0u;
-    }
-    cur = next;
+    score(s0, p);
+    p += step;
+    if (p >= count) break;
+    if (p + step < count) fetch(s0, p + step, pid);
+    pid = page(p + 2 * step);
+    score(s1, p);
+    p += step;
+    if (p >= count) break;
   }
 }
 
@@ -995,12 +1002,11 @@ extern "C" int32_t pl_paged_sparse_decode(
   int32_t st = pl_host::kv_tensor_map_rows(kv_cache, num_pages, num_kv_heads, head_dim, page_size, pl::kSparseUnit, &map);
   if (st != PL_OK) return st;
   if (max_pages > num_select) {
-    // a warp takes 8 pages a step; as many CTAs as the device holds at once,
-    // but no more than there are steps
+    // as many CTAs as the device holds at once, but no more than there are steps
     const int hw = num_kv_heads < pl::kSparseWarps ? num_kv_heads : pl::kSparseWarps, pw = pl::kSparseWarps / hw;
     const int head_groups = (num_kv_heads + pl::kSparseWarps - 1) / pl::kSparseWarps;
-    const int64_t steps = (max_pages + 8 * pw - 1) / (8 * pw);
-    int64_t chunks = 3 * (int64_t)sms / ((int64_t)batch * head_groups);
+    const int64_t steps = ((int64_t)max_pages + pl::kScorePages * pw - 1) / (pl::kScorePages * pw);
+    int64_t chunks = 2 * (int64_t)sms / ((int64_t)batch * head_groups);
     chunks = chunks > steps ? steps : (chunks < 1 ? 1 : chunks);
     auto score = head_dim == 128 ? (group <= 8 ? pl::sparse_score_kernel<128, 1> : pl::sparse_score_kernel<128, 2>)
                                  : (group <= 8 ? pl::sparse_score_kernel<64, 1> : pl::sparse_score_kernel<64, 2>);
