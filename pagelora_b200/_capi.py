@@ -264,23 +264,37 @@ def check(fn: str, status: int) -> None:
 def call(fn: str, *args) -> None:
     """Call ``fn`` from the library and raise on a non-zero status."""
 
-    lib = load_library()
-    check(fn, getattr(lib, fn)(*args))
+    status = getattr(_lib or load_library(), fn)(*args)
+    if status:
+        check(fn, status)
 
 
 def ptr(tensor) -> int | None:
     """Raw device pointer of a tensor (None for None)."""
 
-    if tensor is None:
-        return None
-    return int(tensor.data_ptr())
+    return None if tensor is None else tensor.data_ptr()
 
 
 def stream_handle(stream=None) -> int:
     """cudaStream_t of a torch stream (the current stream by default)."""
 
+    if stream is not None:
+        return int(stream.cuda_stream)
+    return _current_stream()
+
+
+def _current_stream() -> int:
+    """Handle of the current stream of the current device.  torch's raw lookup
+    where it has one: building a Stream object takes longer than a small
+    kernel."""
+
+    global _current_stream
     import torch
 
-    if stream is None:
-        stream = torch.cuda.current_stream()
-    return int(stream.cuda_stream)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is None:
+        _current_stream = lambda: int(torch.cuda.current_stream().cuda_stream)  # noqa: E731
+    else:
+        device = torch.cuda.current_device
+        _current_stream = lambda: raw(device())  # noqa: E731
+    return _current_stream()

@@ -896,6 +896,8 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
 // =================================================================== host
 namespace {
 
+constexpr int kScoreSteps = 4;  // steps of a warp when rows differ in length
+
 int32_t sparse_key_stride(int32_t max_pages) { return (int32_t)(((int64_t)max_pages + 3) & ~int64_t(3)); }
 
 template <int D, int NH>
@@ -1007,6 +1009,10 @@ extern "C" int32_t pl_paged_sparse_decode(
     const int head_groups = (num_kv_heads + pl::kSparseWarps - 1) / pl::kSparseWarps;
     const int64_t steps = ((int64_t)max_pages + pl::kScorePages * pw - 1) / (pl::kScorePages * pw);
     int64_t chunks = 2 * (int64_t)sms / ((int64_t)batch * head_groups);
+    // Rows of unequal length: short pieces, so that the device stays full
+    // while the longest is read.
+    if (8 * total_pages < 7 * (int64_t)batch * max_pages && chunks < (steps + kScoreSteps - 1) / kScoreSteps)
+      chunks = (steps + kScoreSteps - 1) / kScoreSteps;
     chunks = chunks > steps ? steps : (chunks < 1 ? 1 : chunks);
     auto score = head_dim == 128 ? (group <= 8 ? pl::sparse_score_kernel<128, 1> : pl::sparse_score_kernel<128, 2>)
                                  : (group <= 8 ? pl::sparse_score_kernel<64, 1> : pl::sparse_score_kernel<64, 2>);

@@ -19,7 +19,7 @@ from pagelora_b200._capi import DecodePlan, call, ptr, stream_handle
 
 def _need_cuda(*tensors: torch.Tensor | None) -> None:
     for t in tensors:
-        if t is not None and t.device.type != "cuda":
+        if t is not None and not t.is_cuda:
             raise RuntimeError("pagelora_b200 kernels run on CUDA tensors only (no CPU path)")
 
 
@@ -802,7 +802,8 @@ def _need_pool(kv_cache: torch.Tensor) -> None:
 
 
 def _need_vec(t: torch.Tensor, name: str, dtype: torch.dtype = torch.int32, size: int | None = None) -> None:
-    _need(t, dtype, name)
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if not t.is_contiguous() or (size is not None and t.numel() < size):
         raise ValueError(f"{name} must be contiguous" + ("" if size is None else f" with at least {size} entries"))
 
