@@ -7,21 +7,25 @@
 // is no free list: a call that needs N pages takes the N lowest free ids, in
 // row order, so its result is a function of the state alone.
 //
-// The bookkeeping of one call runs in one thread-block cluster (the pool's
-// counts are read once, spread over its CTAs, and ranked by a two-level
-// prefix sum through distributed shared memory).  It checks everything that
-// can be refused before it changes anything; a refused call leaves the state
-// as it was and says why in the status word.  Moving the data is a second
-// launch over the jobs that the first one listed.
+// The bookkeeping of one call runs in one CTA, or, for a large pool, in one
+// thread-block cluster (the pool's counts are read once, spread over the
+// warps, and ranked by a prefix sum, across CTAs through distributed shared
+// memory).  It checks everything that can be refused before it changes
+// anything; a refused call leaves the state as it was and says why in the
+// status word.  Moving the data is a second launch over the jobs that the
+// first one listed.
 #include "pl_common.cuh"
 
 namespace pl {
 
 constexpr int kPoolThreads = 1024;
 constexpr int kPoolWarps = kPoolThreads / 32;
-constexpr int kPoolCtas = 8;        // one cluster
+constexpr int kPoolCtas = 8;        // of a cluster
 constexpr int kPoolMaxRows = 4096;  // rows of a table (as pl_page_table_build)
 constexpr int kPerThread = kPoolMaxRows / kPoolThreads;
+// Pools up to this size take one CTA: 32 warps read 16384 counts in four
+// steps, less than what starting and syncing a cluster takes.
+constexpr int kPoolOneCta = 16384;
 
 struct PoolState {
   int32_t* refcount;
@@ -43,9 +47,7 @@ struct PageJob {
 struct PoolSmem {
   int32_t first[kPoolMaxRows + 1];  // exclusive prefix of the pages wanted
   int32_t warp_sum[kPoolWarps];
-  int32_t total;
-  int32_t cta_free[2];
-  int32_t flag;
+  int32_t cta_free;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -54,37 +56,49 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 
-// Exclusive prefix over kPoolMaxRows values, kPerThread consecutive ones per
-// thread, into s.first[0 .. kPoolMaxRows]; every CTA does the same.
-__device__ __forceinline__ void pool_prefix(PoolSmem& s, const int* v) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int sum = 0;
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) sum += v[i];
-  int inc = sum;
+__device__ __forceinline__ int pool_warp_scan(int v) {  // inclusive
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += u;
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
   }
+  return v;
+}
+
+// Entries of a thread: `per` consecutive ones, per * kPoolThreads >= n.
+__device__ __forceinline__ int pool_per(int n) { return (n + kPoolThreads - 1) / kPoolThreads; }
+
+// Exclusive prefix over the entries (v[i] of entry threadIdx.x * per + i) into
+// s.first[0 .. n], and the total in s.first[kPoolMaxRows]; every CTA does the same.
+__device__ __forceinline__ void pool_prefix(PoolSmem& s, const int* v, int n) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = pool_per(n);
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) sum += i < per ? v[i] : 0;
+  const int inc = pool_warp_scan(sum);
   __syncthreads();
   if (lane == 31) s.warp_sum[warp] = inc;
   __syncthreads();
-  int before = 0;
-  for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
-  int at = before + inc - sum;
+  const int warps = pool_warp_scan(s.warp_sum[lane]);
+  int at = (warp > 0 ? __shfl_sync(0xffffffffu, warps, max(warp - 1, 0)) : 0) + inc - sum;
+  const int total = __shfl_sync(0xffffffffu, warps, 31);
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    s.first[threadIdx.x * kPerThread + i] = at;
-    at += v[i];
+    const int e = (int)threadIdx.x * per + i;
+    if (i < per && e <= n) s.first[e] = at;
+    at += i < per ? v[i] : 0;
   }
-  if (threadIdx.x == kPoolThreads - 1) s.first[kPoolMaxRows] = at;
+  if (threadIdx.x == 0) {
+    s.first[n] = total;
+    s.first[kPoolMaxRows] = total;
+  }
   __syncthreads();
 }
 
 // The entry that owns rank k: first[e] <= k < first[e + 1].
-__device__ __forceinline__ int pool_owner(const PoolSmem& s, int k) {
-  int lo = 0, hi = kPoolMaxRows;
+__device__ __forceinline__ int pool_owner(const PoolSmem& s, int k, int n) {
+  int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (s.first[mid] <= k) lo = mid; else hi = mid;
@@ -97,52 +111,73 @@ __device__ __forceinline__ int pool_owner(const PoolSmem& s, int k) {
 __device__ __forceinline__ bool pool_any(bool bad) { return __syncthreads_or(bad) != 0; }
 
 // Ranks the free pages and calls take(rank, page) for the `need` lowest.
-// false: fewer than `need` are free, nothing was called.  Every CTA of the
-// cluster calls it; the counts are read before any CTA goes on past the
-// cluster barrier in here, and taken pages' counts are set by `take`.
-template <typename Take>
+// false: fewer than `need` are free, nothing was called.  Every CTA calls
+// it; the counts are read before any CTA goes on past the barrier in here,
+// and taken pages' counts are set by `take`.
+template <int CTAS, typename Take>
 __device__ __forceinline__ bool pool_take(PoolSmem& s, const int32_t* refcount, int num_pages, int need, Take take) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t rank = cluster_rank();
+  const int rank = CTAS > 1 ? (int)cluster_rank() : 0;
+  auto sync = [] {
+    if constexpr (CTAS > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+  };
+  if (need == 0) {  // the same for every CTA; what follows may change counts
+    sync();
+    return true;
+  }
   // contiguous range of every warp, in steps of 128 pages
   const int steps = (num_pages + 127) / 128;
-  const int per = (steps + kPoolCtas * kPoolWarps - 1) / (kPoolCtas * kPoolWarps);
-  const int p0 = ((int)rank * kPoolWarps + warp) * per * 128;
-  const int p1 = min(num_pages, p0 + per * 128);
-  int count = 0;
-  for (int p = p0; p < p1; p += 128) {
-    int c[4];
+  const int per = (steps + CTAS * kPoolWarps - 1) / (CTAS * kPoolWarps);
+  const int p0 = (int)min((int64_t)num_pages, ((int64_t)rank * kPoolWarps + warp) * per * 128);
+  const int p1 = (int)min((int64_t)num_pages, (int64_t)p0 + per * 128);
+  auto load = [&](int p, int* c) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[i] = p + 32 * i + lane < p1 ? __ldcg(refcount + p + 32 * i + lane) : 1;
+  };
+  int count = 0;
+  int head[4] = {1, 1, 1, 1};  // the first step's counts, for the second pass
+#pragma unroll 4
+  for (int p = p0; p < p1; p += 128) {
+    int c[4];
+    load(p, c);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) count += __popc(__ballot_sync(0xffffffffu, c[i] == 0));
+    for (int i = 0; i < 4; ++i) {
+      if (p == p0) head[i] = c[i];
+      count += __popc(__ballot_sync(0xffffffffu, c[i] == 0));
+    }
   }
   __syncthreads();
   if (lane == 0) s.warp_sum[warp] = count;
   __syncthreads();
-  int before = 0, total = 0;
-  for (int w = 0; w < kPoolWarps; ++w) {
-    const int v = s.warp_sum[w];
-    before += w < warp ? v : 0;
-    total += v;
-  }
-  if (threadIdx.x == 0) s.cta_free[0] = total;
-  cluster_sync_all();
-  int all = 0;
-  for (int c = 0; c < kPoolCtas; ++c) {
-    uint32_t at = dsmem_map(smem_u32(&s.cta_free[0]), c);
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    before += c < (int)rank ? v : 0;
-    all += v;
+  const int warps = pool_warp_scan(s.warp_sum[lane]);
+  int before = warp > 0 ? __shfl_sync(0xffffffffu, warps, max(warp - 1, 0)) : 0;
+  int all = __shfl_sync(0xffffffffu, warps, 31);
+  if constexpr (CTAS > 1) {
+    if (threadIdx.x == 0) s.cta_free = all;
+    cluster_sync_all();
+    int v = 0;
+    if (lane < CTAS) {
+      const uint32_t at = dsmem_map(smem_u32(&s.cta_free), lane);
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    }
+    const int ctas = pool_warp_scan(v);
+    before += rank > 0 ? __shfl_sync(0xffffffffu, ctas, max(rank - 1, 0)) : 0;
+    all = __shfl_sync(0xffffffffu, ctas, 31);
   }
   const bool enough = all >= need;
   if (enough) {
     int k = before;
     for (int p = p0; p < p1 && k < need; p += 128) {
       int c[4];
+      if (p == p0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = p + 32 * i + lane < p1 ? __ldcg(refcount + p + 32 * i + lane) : 1;
+        for (int i = 0; i < 4; ++i) c[i] = head[i];
+      } else {
+        load(p, c);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t b = __ballot_sync(0xffffffffu, c[i] == 0);
@@ -152,7 +187,7 @@ __device__ __forceinline__ bool pool_take(PoolSmem& s, const int32_t* refcount, 
       }
     }
   }
-  cluster_sync_all();  // the remote reads are done, and every taken page is seen by the cluster
+  sync();  // the remote reads are done, and every taken page is seen by all
   return enough;
 }
 
@@ -194,7 +229,8 @@ __device__ __forceinline__ void pool_drop(const PoolState& p, int pg) {
 }
 
 // ---------------------------------------------------------------- reserve
-__global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads)
+template <int CTAS>
+__global__ void __launch_bounds__(kPoolThreads, 1)
     page_reserve_kernel(const PoolState p, const int32_t* __restrict__ tok_indptr, int total,
                         int32_t* __restrict__ slot_page, int32_t* __restrict__ slot_off,
                         int32_t* __restrict__ positions, int32_t* __restrict__ out_indptr,
@@ -203,16 +239,17 @@ __global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads
   __shared__ int32_t csr[kPoolMaxRows + 1];
   pdl_launch_dependents();
   pdl_wait();
-  const int rank = (int)cluster_rank();
+  const int rank = CTAS > 1 ? (int)cluster_rank() : 0;
   const int PS = p.page_size;
+  const int per = pool_per(p.rows);
   int want[kPerThread], grown[kPerThread];
   bool bad = threadIdx.x == 0 && (tok_indptr[0] != 0 || tok_indptr[p.rows] != total);
   int why = PL_ERR_INVALID_ARGUMENT;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    const int r = threadIdx.x * kPerThread + i;
+    const int r = threadIdx.x * per + i;
     want[i] = grown[i] = 0;
-    if (r >= p.rows) continue;
+    if (i >= per || r >= p.rows) continue;
     const int n = tok_indptr[r + 1] - tok_indptr[r];
     const int num = p.row_num[r], last = p.last_len[r];
     if (n < 0 || num < 0 || num > p.cap || (num > 0 && (last <= 0 || last > PS))) {
@@ -247,17 +284,17 @@ __global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads
   if (bad) set_status(p.status, why);
   bool refused = pool_any(bad);
   // page table offsets (out_indptr), then the pages wanted
-  pool_prefix(s, grown);
-  for (int i = threadIdx.x; i <= kPoolMaxRows; i += kPoolThreads) csr[i] = s.first[i];
+  pool_prefix(s, grown, p.rows);
+  for (int i = threadIdx.x; i <= p.rows; i += kPoolThreads) csr[i] = s.first[i];
   __syncthreads();
-  if (out_indices != nullptr && csr[kPoolMaxRows] > max_indices) {
+  if (out_indices != nullptr && csr[p.rows] > max_indices) {
     if (threadIdx.x == 0) set_status(p.status, PL_ERR_WORKSPACE_TOO_SMALL);
     refused = true;
   }
-  pool_prefix(s, want);
+  pool_prefix(s, want, p.rows);
   const int need = refused ? 0 : s.first[kPoolMaxRows];
-  const bool enough = pool_take(s, p.refcount, p.num_pages, need, [&](int k, int page) {
-    const int r = pool_owner(s, k);
+  const bool enough = pool_take<CTAS>(s, p.refcount, p.num_pages, need, [&](int k, int page) {
+    const int r = pool_owner(s, k, p.rows);
     p.row_pages[(int64_t)r * p.cap + p.row_num[r] + (k - s.first[r])] = page;
     p.refcount[page] = 1;
   });
@@ -265,7 +302,7 @@ __global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads
   if (refused || !enough) return;
   // slots of the new tokens and the page table, rows dealt over the warps
   const int lane = threadIdx.x & 31;
-  for (int r = rank * kPoolWarps + (threadIdx.x >> 5); r < p.rows; r += kPoolCtas * kPoolWarps) {
+  for (int r = rank * kPoolWarps + (threadIdx.x >> 5); r < p.rows; r += CTAS * kPoolWarps) {
     const int num = p.row_num[r], last = p.last_len[r];
     const int t0 = tok_indptr[r], n = tok_indptr[r + 1] - t0;
     const int g = csr[r + 1] - csr[r];
@@ -292,24 +329,26 @@ __global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads
 }
 
 // ------------------------------------------------------------------- fork
-__global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads)
+template <int CTAS>
+__global__ void __launch_bounds__(kPoolThreads, 1)
     page_fork_kernel(const PoolState p, const int32_t* __restrict__ src_rows, const int32_t* __restrict__ dst_rows,
                      int n, int32_t* __restrict__ job_count, PageJob* __restrict__ jobs) {
   __shared__ PoolSmem s;
   __shared__ uint32_t taken[kPoolMaxRows / 32];
   pdl_launch_dependents();
   pdl_wait();
-  const int rank = (int)cluster_rank();
+  const int rank = CTAS > 1 ? (int)cluster_rank() : 0;
   const int PS = p.page_size;
   if (threadIdx.x < kPoolMaxRows / 32) taken[threadIdx.x] = 0;
   __syncthreads();
+  const int per = pool_per(n);
   int want[kPerThread];
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    const int f = threadIdx.x * kPerThread + i;
+    const int f = threadIdx.x * per + i;
     want[i] = 0;
-    if (f >= n) continue;
+    if (i >= per || f >= n) continue;
     const int src = src_rows[f], dst = dst_rows[f];
     if (src < 0 || src >= p.rows || dst < 0 || dst >= p.rows || src == dst || p.row_num[dst] != 0) {
       bad = true;
@@ -326,16 +365,16 @@ __global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {  // a row that another fork fills is no source
-    const int f = threadIdx.x * kPerThread + i;
-    if (f < n && src_rows[f] >= 0 && src_rows[f] < p.rows && ((taken[src_rows[f] >> 5] >> (src_rows[f] & 31)) & 1u))
+    const int f = threadIdx.x * per + i;
+    if (i < per && f < n && src_rows[f] >= 0 && src_rows[f] < p.rows && ((taken[src_rows[f] >> 5] >> (src_rows[f] & 31)) & 1u))
       bad = true;
   }
   if (bad) set_status(p.status, PL_ERR_INVALID_ARGUMENT);
   const bool refused = pool_any(bad);
-  pool_prefix(s, want);
+  pool_prefix(s, want, n);
   const int need = refused ? 0 : s.first[kPoolMaxRows];
-  const bool enough = pool_take(s, p.refcount, p.num_pages, need, [&](int k, int page) {
-    const int f = pool_owner(s, k);
+  const bool enough = pool_take<CTAS>(s, p.refcount, p.num_pages, need, [&](int k, int page) {
+    const int f = pool_owner(s, k, n);
     const int src = src_rows[f], num = p.row_num[src];
     const int old = p.row_pages[(int64_t)src * p.cap + num - 1];
     const bool ok = old >= 0 && old < p.num_pages;
@@ -349,7 +388,7 @@ __global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads
   if (rank == 0 && threadIdx.x == 0) *job_count = done ? need : 0;
   if (!done) return;
   const int lane = threadIdx.x & 31;
-  for (int f = rank * kPoolWarps + (threadIdx.x >> 5); f < n; f += kPoolCtas * kPoolWarps) {
+  for (int f = rank * kPoolWarps + (threadIdx.x >> 5); f < n; f += CTAS * kPoolWarps) {
     const int src = src_rows[f], dst = dst_rows[f];
     const int num = p.row_num[src], last = p.last_len[src];
     const int shared = num - (num > 0 && last < PS ? 1 : 0);
@@ -389,12 +428,23 @@ __device__ __forceinline__ bool compact_row(const PoolState& p, int r, const int
   if (num < 0 || num > p.cap || (num > 0 && (last <= 0 || last > PS))) return false;
   const int64_t old = num > 0 ? (int64_t)(num - 1) * PS + last : 0;
   if (kf < 0 || k < 0 || k > max_keep || (int64_t)kf + k > old) return false;
-  // keep ascends, so keep[i] == kf + i holds up to some i: bisect
+  // keep ascends, so keep[i] == kf + i holds up to some i: search with 8
+  // probes a step (their loads overlap)
   const int32_t* kr = keep + (int64_t)r * keep_stride;
   int lo = 0, hi = k;
   while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (kr[mid] == kf + mid) lo = mid + 1; else hi = mid;
+    const int gap = (hi - lo + 8) / 9;
+    int v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int at = lo + (j + 1) * gap - 1;
+      v[j] = at < hi ? kr[at] - at : INT32_MAX;
+    }
+    int held = 0;  // leading probes that keep their place
+#pragma unroll
+    for (int j = 0; j < 8; ++j) held += held == j && v[j] == kf;
+    if (held < 8) hi = min(hi, lo + (held + 1) * gap - 1);
+    lo += held * gap;
   }
   const int stays = kf + lo;
   c.len = kf + k;
@@ -414,7 +464,8 @@ __device__ __forceinline__ bool compact_row(const PoolState& p, int r, const int
   return true;
 }
 
-__global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads)
+template <int CTAS>
+__global__ void __launch_bounds__(kPoolThreads, 1)
     page_compact_kernel(const PoolState p, const int32_t* __restrict__ keep_from, const int32_t* __restrict__ keep,
                         int64_t keep_stride, const int32_t* __restrict__ keep_count, int max_keep,
                         int32_t* __restrict__ job_count, int32_t* __restrict__ old_pages, int2* __restrict__ src_range,
@@ -423,16 +474,17 @@ __global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads
   __shared__ uint32_t full_s[kPoolMaxRows];  // pages that stay; top bit: one old page more is kept (a cut)
   pdl_launch_dependents();
   pdl_wait();
-  const int rank = (int)cluster_rank();
+  const int rank = CTAS > 1 ? (int)cluster_rank() : 0;
   const int PS = p.page_size;
+  const int per = pool_per(p.rows);
   int want[kPerThread];
   bool bad = false;
   int why = PL_OK;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    const int r = threadIdx.x * kPerThread + i;
+    const int r = threadIdx.x * per + i;
     want[i] = 0;
-    if (r >= p.rows) continue;
+    if (i >= per || r >= p.rows) continue;
     CompactRow c;
     int w;
     if (!compact_row(p, r, keep_from, keep, keep_stride, keep_count, max_keep, c, w)) {
@@ -444,10 +496,10 @@ __global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads
   }
   if (bad) set_status(p.status, why);
   const bool refused = pool_any(bad);
-  pool_prefix(s, want);
+  pool_prefix(s, want, p.rows);
   const int need = refused ? 0 : s.first[kPoolMaxRows];
-  const bool enough = pool_take(s, p.refcount, p.num_pages, need, [&](int k, int page) {
-    const int r = pool_owner(s, k), index = (int)(full_s[r] & 0x7fffffffu) + (k - s.first[r]);
+  const bool enough = pool_take<CTAS>(s, p.refcount, p.num_pages, need, [&](int k, int page) {
+    const int r = pool_owner(s, k, p.rows), index = (int)(full_s[r] & 0x7fffffffu) + (k - s.first[r]);
     const int len = keep_from[r] + keep_count[r];
     jobs[k] = PageJob{page, r, index, min(PS, len - index * PS)};
     p.refcount[page] = 1;
@@ -458,7 +510,7 @@ __global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads
   if (!done) return;
   // the old pages: noted for the copy, given back
   const int lane = threadIdx.x & 31;
-  for (int r = rank * kPoolWarps + (threadIdx.x >> 5); r < p.rows; r += kPoolCtas * kPoolWarps) {
+  for (int r = rank * kPoolWarps + (threadIdx.x >> 5); r < p.rows; r += CTAS * kPoolWarps) {
     const int num = p.row_num[r], len = keep_from[r] + keep_count[r];
     const int moved = s.first[r + 1] - s.first[r];
     const int full = (int)(full_s[r] & 0x7fffffffu), held = full + (int)(full_s[r] >> 31);
@@ -484,7 +536,8 @@ __global__ void __cluster_dims__(kPoolCtas, 1, 1) __launch_bounds__(kPoolThreads
 // ------------------------------------------------------------------- copy
 // Fills the listed pages in every layer.  One CTA takes (job, slice of the
 // 2 * layers K and V halves); the source slot of each of the page's tokens
-// is looked up once, then all threads copy 16-byte units.
+// is looked up once, a thread's places (16-byte units of the page) are
+// worked out once, and then it has kCopyDepth loads in flight per half.
 struct CopyArgs {
   char* pool;
   int64_t layer_stride;  // bytes
@@ -502,19 +555,24 @@ struct CopyArgs {
 };
 
 constexpr int kCopyThreads = 256;
-constexpr int kCopySlice = 4;  // K / V halves per CTA and step
+constexpr int kCopyDepth = 8;
+constexpr int kCopyCtasPerSm = 3;
 
-__global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const CopyArgs a) {
+__global__ void __launch_bounds__(kCopyThreads, kCopyCtasPerSm) page_copy_kernel(const CopyArgs a) {
   __shared__ int32_t src_slot[128];
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   const int jobs = *a.job_count;
-  const int PS = a.page_size;
-  const int slices = (2 * a.layers + kCopySlice - 1) / kCopySlice;
-  const int64_t half = (int64_t)PS * a.token_units * 16;
+  if (jobs == 0) return;
+  const int PS = a.page_size, halves = 2 * a.layers;
+  // halves of a slice: few jobs are spread over all CTAs, many are read in longer runs
+  const int64_t share = (int64_t)jobs * halves / (2 * gridDim.x);
+  const int slice = (int)max((int64_t)1, min((int64_t)8, share));
+  const int slices = (halves + slice - 1) / slice;
+  const int64_t half = (int64_t)PS * a.token_units;  // 16-byte units
   for (int64_t u = blockIdx.x; u < (int64_t)jobs * slices; u += gridDim.x) {
     const PageJob job = a.jobs[u / slices];
-    const int h0 = (int)(u % slices) * kCopySlice, h1 = min(2 * a.layers, h0 + kCopySlice);
+    const int h0 = (int)(u % slices) * slice, h1 = min(halves, h0 + slice);
     __syncthreads();
     for (int t = threadIdx.x; t < job.tokens; t += kCopyThreads) {
       int slot = -1;
@@ -533,18 +591,27 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const CopyArgs 
       src_slot[t] = slot;
     }
     __syncthreads();
-    const int per_half = job.tokens * a.token_units;
-    for (int idx = threadIdx.x; idx < (h1 - h0) * per_half; idx += kCopyThreads) {
-      const int h = h0 + idx / per_half, rem = idx % per_half;
-      const int t = rem / a.token_units, c = rem % a.token_units;
-      const int slot = src_slot[t];
-      if (slot < 0) continue;
-      char* layer = a.pool + (int64_t)(h >> 1) * a.layer_stride;
-      const uint4* from = reinterpret_cast<const uint4*>(
-          layer + ((int64_t)(slot / PS) * 2 + (h & 1)) * half + (int64_t)(slot % PS) * a.token_units * 16);
-      uint4* to = reinterpret_cast<uint4*>(layer + ((int64_t)job.page * 2 + (h & 1)) * half +
-                                           (int64_t)t * a.token_units * 16);
-      to[c] = from[c];
+    const int units = job.tokens * a.token_units;
+    for (int at = threadIdx.x; at < units; at += kCopyThreads * kCopyDepth) {
+      int64_t from[kCopyDepth];  // unit in a layer's half-0 plane, -1: none
+      int64_t to = (int64_t)job.page * 2 * half + at;
+#pragma unroll
+      for (int i = 0; i < kCopyDepth; ++i) {
+        const int x = at + i * kCopyThreads, t = x / a.token_units, c = x - t * a.token_units;
+        const int slot = x < units ? src_slot[t] : -1;
+        const int pg = slot / PS;
+        from[i] = slot < 0 ? -1 : (int64_t)pg * 2 * half + (int64_t)(slot - pg * PS) * a.token_units + c;
+      }
+      for (int h = h0; h < h1; ++h) {
+        uint4* plane = reinterpret_cast<uint4*>(a.pool + (int64_t)(h >> 1) * a.layer_stride) + (h & 1) * half;
+        uint4 v[kCopyDepth];
+#pragma unroll
+        for (int i = 0; i < kCopyDepth; ++i)
+          if (from[i] >= 0) v[i] = __ldcs(plane + from[i]);
+#pragma unroll
+        for (int i = 0; i < kCopyDepth; ++i)
+          if (from[i] >= 0) __stcs(plane + to + i * kCopyThreads, v[i]);
+      }
     }
   }
 }
@@ -592,10 +659,18 @@ int32_t copy_args(void* pool, int64_t layer_stride_bytes, int32_t layers, int64_
 int32_t launch_copy(const pl::CopyArgs& a, int64_t max_jobs, void* stream) {
   const int sms = pl_host::sm_count();
   if (sms <= 0) return PL_ERR_NO_DEVICE;
-  const int64_t units = max_jobs * ((2 * a.layers + pl::kCopySlice - 1) / pl::kCopySlice);
-  const int64_t most = (int64_t)sms * 8;
+  const int64_t units = max_jobs * 2 * a.layers, most = (int64_t)sms * pl::kCopyCtasPerSm;
   return pl_host::launch_pdl(pl::page_copy_kernel, dim3((int)(units < most ? units : most)), dim3(pl::kCopyThreads), 0,
                              stream, a);
+}
+
+// A bookkeeping kernel on one CTA or, for a large pool, one cluster.
+template <typename K1, typename K8, typename... Args>
+int32_t launch_pool(K1 one, K8 cluster, const pl::PoolState& p, void* stream, Args... args) {
+  if (p.num_pages <= pl::kPoolOneCta)
+    return pl_host::launch_pdl(one, dim3(1), dim3(pl::kPoolThreads), 0, stream, p, args...);
+  return pl_host::launch_pdl_cluster(cluster, dim3(pl::kPoolCtas), dim3(pl::kPoolThreads), 0, stream, pl::kPoolCtas, p,
+                                     args...);
 }
 
 }  // namespace
@@ -626,9 +701,8 @@ extern "C" int32_t pl_page_reserve(int32_t *refcount, int64_t num_pages, int32_t
       (total_tokens > 0 && (slot_page == nullptr || slot_offset == nullptr)))
     return PL_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return PL_OK;
-  return pl_host::launch_pdl(pl::page_reserve_kernel, dim3(pl::kPoolCtas), dim3(pl::kPoolThreads), 0, stream, p,
-                             tok_indptr, (int)total_tokens, slot_page, slot_offset, positions_out, out_indptr,
-                             out_indices, max_indices);
+  return launch_pool(pl::page_reserve_kernel<1>, pl::page_reserve_kernel<pl::kPoolCtas>, p, stream, tok_indptr,
+                     (int)total_tokens, slot_page, slot_offset, positions_out, out_indptr, out_indices, max_indices);
 }
 
 extern "C" int64_t pl_page_fork_workspace_bytes(int32_t num_forks) {
@@ -655,8 +729,8 @@ extern "C" int32_t pl_page_fork(void *pool, int64_t layer_stride_bytes, int32_t 
     return PL_ERR_WORKSPACE_TOO_SMALL;
   int32_t* count = static_cast<int32_t*>(workspace);
   pl::PageJob* jobs = reinterpret_cast<pl::PageJob*>(count + 4);
-  st = pl_host::launch_pdl(pl::page_fork_kernel, dim3(pl::kPoolCtas), dim3(pl::kPoolThreads), 0, stream, p, src_rows,
-                           dst_rows, (int)num_forks, count, jobs);
+  st = launch_pool(pl::page_fork_kernel<1>, pl::page_fork_kernel<pl::kPoolCtas>, p, stream, src_rows, dst_rows,
+                   (int)num_forks, count, jobs);
   if (st != PL_OK) return st;
   c.job_count = count;
   c.jobs = jobs;
@@ -694,9 +768,8 @@ extern "C" int32_t pl_cache_compact(void *pool, int64_t layer_stride_bytes, int3
   int32_t* old_pages = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(src_range) + align16(8 * (int64_t)num_rows));
   const int64_t n = (int64_t)num_rows * row_capacity;
   pl::PageJob* jobs = reinterpret_cast<pl::PageJob*>(reinterpret_cast<char*>(old_pages) + align16(4 * n));
-  st = pl_host::launch_pdl(pl::page_compact_kernel, dim3(pl::kPoolCtas), dim3(pl::kPoolThreads), 0, stream, p,
-                           keep_from, keep, keep_stride, keep_count, (int)max_keep, count, old_pages,
-                           src_range, jobs);
+  st = launch_pool(pl::page_compact_kernel<1>, pl::page_compact_kernel<pl::kPoolCtas>, p, stream, keep_from, keep,
+                   keep_stride, keep_count, (int)max_keep, count, old_pages, src_range, jobs);
   if (st != PL_OK) return st;
   c.job_count = count;
   c.jobs = jobs;

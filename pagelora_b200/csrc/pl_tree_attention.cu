@@ -931,7 +931,7 @@ bool tree_two_tiles(int total_q, int batch, int group) {
   return (int64_t)total_q * group > (int64_t)batch * pl::kTreeM;
 }
 
-constexpr int kTreeMinSplit = 2;
+constexpr int kTreeMinSplit = 6;
 
 template <int D, int NT>
 int32_t launch_tree(const CUtensorMap& map, const pl::TreeArgs& a, bool merge, void* stream) {

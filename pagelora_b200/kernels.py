@@ -10,6 +10,7 @@ CUDA graph when its outputs are preallocated.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 
 import torch
 
@@ -796,7 +797,8 @@ def argmax(logits: torch.Tensor, out: torch.Tensor, workspace: torch.Tensor | No
 
 # ----------------------------------------------------- drafted-token trees
 def _need_pool(kv_cache: torch.Tensor) -> None:
-    _need(kv_cache, torch.bfloat16, "kv_cache")
+    if kv_cache.dtype is not torch.bfloat16:
+        raise TypeError(f"kv_cache must be {torch.bfloat16}, got {kv_cache.dtype}")
     if kv_cache.dim() != 5 or kv_cache.size(1) != 2 or not kv_cache.is_contiguous():
         raise ValueError("kv_cache must be a contiguous [pages, 2, page_size, kv_heads, head_dim] tensor")
 
@@ -808,8 +810,18 @@ def _need_vec(t: torch.Tensor, name: str, dtype: torch.dtype = torch.int32, size
         raise ValueError(f"{name} must be contiguous" + ("" if size is None else f" with at least {size} entries"))
 
 
-def _workspace(workspace: torch.Tensor | None, need: int, device: torch.device) -> torch.Tensor:
-    return torch.empty(max(need, 16), dtype=torch.uint8, device=device) if workspace is None else workspace
+def _workspace(workspace: torch.Tensor | None, need: int, like: torch.Tensor) -> torch.Tensor:
+    return like.new_empty(need if need > 16 else 16, dtype=torch.uint8) if workspace is None else workspace
+
+
+def _need_rows(t: torch.Tensor, name: str, rows: int, dtype: torch.dtype = torch.int32) -> tuple[int, int]:
+    """(row stride, width) of a [>= rows, width] matrix with contiguous rows."""
+
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2 or t.shape[0] < rows or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be [{rows}, width] with contiguous rows")
+    return max(t.stride(0), t.shape[1]), t.shape[1]
 
 
 def tree_mask(parents: torch.Tensor, qo_indptr: torch.Tensor, words: int, *, base_positions: torch.Tensor | None = None,
@@ -822,27 +834,30 @@ def tree_mask(parents: torch.Tensor, qo_indptr: torch.Tensor, words: int, *, bas
     receives ``base_positions[request] + depth``."""
 
     _need_cuda(parents, qo_indptr, base_positions, mask, depth, positions)
-    total = parents.numel()
-    batch = qo_indptr.numel() - 1
+    total, batch = parents.numel(), qo_indptr.numel() - 1
     _need_vec(parents, "parents")
     _need_vec(qo_indptr, "qo_indptr")
     if words < 1:
         raise ValueError("words must be at least 1")
     if mask is None:
-        mask = torch.empty(total, words, dtype=torch.int32, device=parents.device)
+        mask = parents.new_empty((total, words))
+    stride, width = _need_rows(mask, "mask", total)
+    if mask.shape[0] != total or width != words:
+        raise ValueError("mask must be [total_q, words]")
     if depth is None:
-        depth = torch.empty(total, dtype=torch.int32, device=parents.device)
-    _need(mask, torch.int32, "mask")
-    if mask.shape != (total, words) or (words > 1 and mask.stride(1) != 1):
-        raise ValueError("mask must be [total_q, words] with contiguous rows")
-    for name, t, n in (("depth", depth, total), ("positions", positions, total), ("base_positions", base_positions, batch)):
-        if t is not None:
-            _need_vec(t, name, size=n)
-    call("pl_tree_mask", ptr(parents), ptr(qo_indptr), ptr(base_positions), int(batch), int(total), int(words),
-         ptr(mask), max(mask.stride(0), words), ptr(depth), ptr(positions), ptr(status), stream_handle())
+        depth = parents.new_empty(total)
+    else:
+        _need_vec(depth, "depth", size=total)
+    if positions is not None:
+        _need_vec(positions, "positions", size=total)
+    if base_positions is not None:
+        _need_vec(base_positions, "base_positions", size=batch)
+    call("pl_tree_mask", parents.data_ptr(), qo_indptr.data_ptr(), ptr(base_positions), batch, total, words,
+         mask.data_ptr(), stride, depth.data_ptr(), ptr(positions), ptr(status), stream_handle())
     return mask, depth
 
 
+@lru_cache(maxsize=256)
 def tree_workspace_bytes(batch: int, total_q: int, num_qo_heads: int, num_kv_heads: int, head_dim: int) -> int:
     """Workspace of :func:`paged_tree_attention` (no initialisation)."""
 
@@ -885,24 +900,23 @@ def paged_tree_attention(
     _need_vec(kv_indptr, "kv_indptr", size=batch + 1)
     _need_vec(kv_indices, "kv_indices")
     _need_vec(kv_last_page_len, "kv_last_page_len", size=batch)
-    _need(tree_mask, torch.int32, "tree_mask")
-    if tree_mask.dim() != 2 or tree_mask.shape[0] != total_q or tree_mask.stride(1) != 1:
-        raise ValueError("tree_mask must be [total_q, words] with contiguous rows")
-    words = tree_mask.shape[1]
+    mask_stride, words = _need_rows(tree_mask, "tree_mask", total_q)
     if out is None:
         out = torch.empty_like(q)
-    _need(out, torch.bfloat16, "out")
-    if out.shape != q.shape or out.stride(-1) != 1:
+    elif out.dtype is not torch.bfloat16:
+        raise TypeError(f"out must be {torch.bfloat16}, got {out.dtype}")
+    elif out.shape != q.shape or out.stride(-1) != 1:
         raise ValueError("out must have q's shape and unit last stride")
     if out_lse is not None:
         _need_vec(out_lse, "out_lse", torch.float32, total_q * hq)
-    workspace = _workspace(workspace, tree_workspace_bytes(batch, total_q, hq, hkv, d), q.device)
-    scale = (1.0 / math.sqrt(d)) if sm_scale is None else float(sm_scale)
-    call("pl_paged_tree_attention", ptr(q), q.stride(0), q.stride(1), ptr(kv_cache), num_pages, ptr(qo_indptr),
-         ptr(kv_indptr), ptr(kv_indices), ptr(kv_last_page_len), kv_indices.numel(), ptr(tree_mask),
-         max(tree_mask.stride(0), words), words, batch, total_q, hq, hkv, d, page_size, scale, ptr(out), out.stride(0),
-         out.stride(1), ptr(out_lse), ptr(workspace), workspace.numel() * workspace.element_size(), ptr(status),
-         stream_handle())
+    workspace = _workspace(workspace, tree_workspace_bytes(batch, total_q, hq, hkv, d), q)
+    q_t, q_h, _ = q.stride()
+    o_t, o_h, _ = out.stride()
+    call("pl_paged_tree_attention", q.data_ptr(), q_t, q_h, kv_cache.data_ptr(), num_pages, qo_indptr.data_ptr(),
+         kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), kv_indices.numel(),
+         tree_mask.data_ptr(), mask_stride, words, batch, total_q, hq, hkv, d, page_size,
+         d ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), o_t, o_h, ptr(out_lse),
+         workspace.data_ptr(), workspace.numel() * workspace.element_size(), ptr(status), stream_handle())
     return out
 
 
@@ -924,12 +938,10 @@ def tree_accept(parents: torch.Tensor, tokens: torch.Tensor, targets: torch.Tens
     _need_vec(base_positions, "base_positions", size=batch)
     _need_vec(keep_count, "keep_count", size=batch)
     _need_vec(next_token, "next_token", torch.int64, batch)
-    _need(keep, torch.int32, "keep")
-    if keep.dim() != 2 or keep.shape[0] < batch or keep.stride(1) != 1:
-        raise ValueError("keep must be [batch, max_keep] with contiguous rows")
-    call("pl_tree_accept", ptr(parents), ptr(tokens), ptr(targets), ptr(qo_indptr), ptr(base_positions), batch, total,
-         keep.shape[1], ptr(keep), max(keep.stride(0), keep.shape[1]), ptr(keep_count), ptr(next_token), ptr(status),
-         stream_handle())
+    stride, width = _need_rows(keep, "keep", batch)
+    call("pl_tree_accept", parents.data_ptr(), tokens.data_ptr(), targets.data_ptr(), qo_indptr.data_ptr(),
+         base_positions.data_ptr(), batch, total, width, keep.data_ptr(), stride, keep_count.data_ptr(),
+         next_token.data_ptr(), ptr(status), stream_handle())
 
 
 # --------------------------------------------------------- pages of a cache
@@ -955,12 +967,27 @@ def _pool_data(pool: torch.Tensor, refcount: torch.Tensor) -> tuple[tuple, int]:
     _need_cuda(pool)
     if pool.dim() < 5 or pool.size(2) != 2 or pool.size(1) != refcount.numel():
         raise ValueError("pool must be [layers, pages, 2, page_size, ...] with one refcount per page")
-    layer = pool[0]
-    if not layer.is_contiguous() or pool.stride(0) < layer.numel():
+    size, shape = pool.element_size(), pool.shape
+    token = math.prod(shape[4:])
+    per_layer = shape[1] * 2 * shape[3] * token
+    if not pool.is_contiguous() and (not pool[0].is_contiguous() or pool.stride(0) < per_layer):
         raise ValueError("every layer of the pool must be contiguous")
-    size = pool.element_size()
-    token = layer.numel() // (layer.size(0) * 2 * layer.size(2)) * size
-    return (ptr(pool), pool.stride(0) * size, pool.size(0), token), layer.size(2)
+    return (pool.data_ptr(), pool.stride(0) * size, shape[0], token * size), shape[3]
+
+
+@lru_cache(maxsize=256)
+def _fork_workspace_bytes(forks: int) -> int:
+    return int(_capi.load_library().pl_page_fork_workspace_bytes(forks))
+
+
+@lru_cache(maxsize=256)
+def _compact_workspace_bytes(rows: int, cap: int) -> int:
+    return int(_capi.load_library().pl_cache_compact_workspace_bytes(rows, cap))
+
+
+@lru_cache(maxsize=256)
+def _sparse_workspace_bytes(batch: int, num_kv_heads: int, max_pages: int) -> int:
+    return int(_capi.load_library().pl_sparse_workspace_bytes(batch, num_kv_heads, max_pages))
 
 
 def page_release(refcount: torch.Tensor, row_pages: torch.Tensor, row_num_pages: torch.Tensor,
@@ -1012,7 +1039,7 @@ def page_fork(pool: torch.Tensor, refcount: torch.Tensor, row_pages: torch.Tenso
     _need_vec(dst_rows, "dst_rows", size=n)
     if dst_rows.numel() != n:
         raise ValueError("src_rows and dst_rows differ in length")
-    workspace = _workspace(workspace, int(_capi.load_library().pl_page_fork_workspace_bytes(n)), pool.device)
+    workspace = _workspace(workspace, _fork_workspace_bytes(n), pool)
     call("pl_page_fork", *data, *tables, page_size, ptr(src_rows), ptr(dst_rows), n, ptr(workspace),
          workspace.numel() * workspace.element_size(), ptr(status), stream_handle())
 
@@ -1030,14 +1057,10 @@ def cache_compact(pool: torch.Tensor, refcount: torch.Tensor, row_pages: torch.T
     rows, cap = row_pages.shape
     _need_vec(keep_from, "keep_from", size=rows)
     _need_vec(keep_count, "keep_count", size=rows)
-    _need(keep, torch.int32, "keep")
-    if keep.dim() != 2 or keep.shape[0] < rows or (keep.shape[1] > 1 and keep.stride(1) != 1):
-        raise ValueError("keep must be [rows, max_keep] with contiguous rows")
-    workspace = _workspace(workspace, int(_capi.load_library().pl_cache_compact_workspace_bytes(rows, cap)),
-                           pool.device)
-    call("pl_cache_compact", *data, *tables, page_size, ptr(keep_from), ptr(keep),
-         max(keep.stride(0), keep.shape[1]), ptr(keep_count), keep.shape[1], ptr(workspace),
-         workspace.numel() * workspace.element_size(), ptr(status), stream_handle())
+    stride, width = _need_rows(keep, "keep", rows)
+    workspace = _workspace(workspace, _compact_workspace_bytes(rows, cap), pool)
+    call("pl_cache_compact", *data, *tables, page_size, ptr(keep_from), ptr(keep), stride, ptr(keep_count), width,
+         ptr(workspace), workspace.numel() * workspace.element_size(), ptr(status), stream_handle())
 
 
 # -------------------------------------------------------- sparse attention
@@ -1055,8 +1078,8 @@ def page_bounds(kv_cache: torch.Tensor, page_ids: torch.Tensor, bounds: torch.Te
     _need_vec(bound_scale, "bound_scale", torch.float32, num_pages * hkv)
     if page_len is not None:
         _need_vec(page_len, "page_len", size=n)
-    call("pl_page_bounds", ptr(kv_cache), num_pages, hkv, d, page_size, ptr(page_ids), ptr(page_len), n, ptr(bounds),
-         ptr(bound_scale), ptr(status), stream_handle())
+    call("pl_page_bounds", kv_cache.data_ptr(), num_pages, hkv, d, page_size, page_ids.data_ptr(), ptr(page_len), n,
+         bounds.data_ptr(), bound_scale.data_ptr(), ptr(status), stream_handle())
 
 
 def paged_sparse_decode(
@@ -1101,8 +1124,9 @@ def paged_sparse_decode(
     _need_vec(bound_scale, "bound_scale", torch.float32, num_pages * hkv)
     if out is None:
         out = torch.empty_like(q)
-    _need(out, torch.bfloat16, "out")
-    if out.shape != q.shape or out.stride(-1) != 1:
+    elif out.dtype is not torch.bfloat16:
+        raise TypeError(f"out must be {torch.bfloat16}, got {out.dtype}")
+    elif out.shape != q.shape or out.stride(-1) != 1:
         raise ValueError("out must have q's shape and unit last stride")
     if out_lse is not None:
         _need_vec(out_lse, "out_lse", torch.float32, batch * hq)
@@ -1112,12 +1136,13 @@ def paged_sparse_decode(
     if max_pages is None:
         max_pages = indices.numel()
     if max_pages > num_select and workspace is None:
-        workspace = _workspace(None, int(_capi.load_library().pl_sparse_workspace_bytes(batch, hkv, int(max_pages))),
-                               q.device)
-    scale = (1.0 / math.sqrt(d)) if sm_scale is None else float(sm_scale)
-    call("pl_paged_sparse_decode", ptr(q), q.stride(0), q.stride(1), ptr(kv_cache), num_pages, ptr(indptr),
-         ptr(indices), ptr(last_page_len), indices.numel(), int(max_pages), ptr(bounds), ptr(bound_scale), batch, hq,
-         hkv, d, page_size, scale, int(num_select), int(sink_pages), int(recent_pages), ptr(out), out.stride(0),
-         out.stride(1), ptr(out_lse), ptr(selected), ptr(workspace),
-         0 if workspace is None else workspace.numel() * workspace.element_size(), ptr(status), stream_handle())
+        workspace = _workspace(None, _sparse_workspace_bytes(batch, hkv, max_pages), q)
+    q_b, q_h, _ = q.stride()
+    o_b, o_h, _ = out.stride()
+    call("pl_paged_sparse_decode", q.data_ptr(), q_b, q_h, kv_cache.data_ptr(), num_pages, indptr.data_ptr(),
+         indices.data_ptr(), last_page_len.data_ptr(), indices.numel(), max_pages, bounds.data_ptr(),
+         bound_scale.data_ptr(), batch, hq, hkv, d, page_size, d ** -0.5 if sm_scale is None else float(sm_scale),
+         num_select, sink_pages, recent_pages, out.data_ptr(), o_b, o_h, ptr(out_lse), selected.data_ptr(),
+         ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), ptr(status),
+         stream_handle())
     return out
