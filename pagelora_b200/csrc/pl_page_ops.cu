@@ -565,9 +565,11 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyCtasPerSm) page_copy_kernel
   const int jobs = *a.job_count;
   if (jobs == 0) return;
   const int PS = a.page_size, halves = 2 * a.layers;
-  // halves of a slice: few jobs are spread over all CTAs, many are read in longer runs
-  const int64_t share = (int64_t)jobs * halves / (2 * gridDim.x);
-  const int slice = (int)max((int64_t)1, min((int64_t)8, share));
+  // halves of a slice: one round of the CTAs when there are few, else at
+  // least two, in runs of at most 8 (jobs of unequal length even out)
+  const int64_t all = (int64_t)jobs * halves;
+  const int64_t share = all <= 2 * (int64_t)gridDim.x ? (all + gridDim.x - 1) / gridDim.x : all / (2 * (int64_t)gridDim.x);
+  const int slice = (int)min((int64_t)8, max((int64_t)1, share));
   const int slices = (halves + slice - 1) / slice;
   const int64_t half = (int64_t)PS * a.token_units;  // 16-byte units
   for (int64_t u = blockIdx.x; u < (int64_t)jobs * slices; u += gridDim.x) {

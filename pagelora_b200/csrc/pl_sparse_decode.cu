@@ -23,7 +23,7 @@ constexpr int kBoundsThreads = 128;
 // ----------------------------------------------------------------- bounds
 // One CTA per (page, kv heads); thread = 8 channels (16 bytes) of one head.
 template <int D>
-__global__ void __launch_bounds__(kBoundsThreads)
+__global__ void __launch_bounds__(kBoundsThreads, 8)
     page_bounds_kernel(const bf16* __restrict__ kv, int64_t num_pages, int hkv, int page_size,
                        const int32_t* __restrict__ page_ids, const int32_t* __restrict__ page_len, int n,
                        int8_t* __restrict__ bounds, float* __restrict__ scale, int32_t* status) {
@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(kBoundsThreads)
   if (ok) {
     const uint4* src = reinterpret_cast<const uint4*>(kv + ((int64_t)pg * 2 * page_size * hkv + h) * D) + u;
     const int64_t step = (int64_t)hkv * D / 8;
-#pragma unroll 8
+#pragma unroll 16
     for (int t = 0; t < len; ++t) {
       const uint4 v = __ldg(src + t * step);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
