@@ -55,6 +55,10 @@ struct TreeArgs {
   int32_t* status;
 };
 
+// Segments between the V producer, which looks them up, and the softmax
+// warps: the ring of K/V tiles keeps the producer at most 3 tiles, hence 4
+// segments, ahead.
+constexpr int kTreeSegs = 8;
 // One segment of an item: K/V tiles [j0, j1).
 struct TreeSeg {
   int q0, n, kv_begin, n_pages, kv_len, kvh, rt, j0, j1, whole;
@@ -80,11 +84,14 @@ struct TreeCfg {
   static constexpr int kSlots = 7 - NT;  // fills the shared memory at D = 128
   static constexpr int kQOff = 0;
   static constexpr int kSlotOff = kQOff + NT * kQBytes;
-  static constexpr int kPairOff = kSlotOff + kSlots * kKVBytes;  // [NT][128] words shared by a row's two threads
-  static constexpr int kBarOff = kPairOff + kRows * 4;
-  static constexpr int kNumBars = 2 * kSlots + 8 + 1;  // full empty | s[2] p[2] o[2] q[2] | fin
-  static constexpr int kMiscOff = kBarOff + kNumBars * 8;  // tmem slot, flags, range, any_bad, 2 segments
-  static constexpr int kSmemBytes = 1024 + kMiscOff + 64 + 2 * (int)sizeof(TreeSeg);
+  // Words shared by a row's two threads.  One row tile: two sets in turn,
+  // since a thread may be a tile ahead of its partner's read.
+  static constexpr int kPairSets = NT == 1 ? 2 : 1;
+  static constexpr int kPairOff = kSlotOff + kSlots * kKVBytes;  // [sets][NT][128]
+  static constexpr int kBarOff = kPairOff + kPairSets * kRows * 4;
+  static constexpr int kNumBars = 2 * kSlots + 8 + 1 + kTreeSegs;  // full empty | s[2] p[2] o[2] q[2] | fin | seg[]
+  static constexpr int kMiscOff = kBarOff + kNumBars * 8;  // tmem slot, flags, range, any_bad, segments
+  static constexpr int kSmemBytes = 1024 + kMiscOff + 64 + kTreeSegs * (int)sizeof(TreeSeg);
   // Scores take 128 columns at 128 * buf (P in their place), O_x at 256 +
   // 128 x.  One row tile: its scores alternate between two buffers, so that
   // the next tile's are computed during this one's softmax.
@@ -262,11 +269,12 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   uint64_t* odone = sready + 4;             // [2] P_x.V of a tile (two row tiles: of a segment) complete
   uint64_t* qready = sready + 6;            // [2] Q_x of a segment staged (8 warps)
   uint64_t* fin = sready + 8;
+  uint64_t* dready = sready + 9;            // [kTreeSegs] segment looked up
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
   volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, K and V tiles issued
   volatile int32_t* range = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 32);  // b, w, w_end, base
   uint32_t* any_bad = reinterpret_cast<uint32_t*>(smem + C::kMiscOff + 48);  // a drafted V held inf or NaN
-  TreeSeg* segs = reinterpret_cast<TreeSeg*>(smem + C::kMiscOff + 64);       // [2] the softmax warps' segment
+  TreeSeg* segs = reinterpret_cast<TreeSeg*>(smem + C::kMiscOff + 64);       // [kTreeSegs], j0 < 0: the end
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
@@ -281,6 +289,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       mbar_init(&qready[x], 8);
     }
     mbar_init(fin, 1);
+    for (int i = 0; i < kTreeSegs; ++i) mbar_init(&dready[i], 1);
     flags[0] = flags[1] = flags[2] = 0;
     any_bad[0] = 0;
     fence_barrier_init();
@@ -335,7 +344,15 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
     int t = 0;
     bool go = true;
     TreeSeg sg;
-    while (go && it.next(a, C::kRows, sg)) {
+    for (int seg = 0;; ++seg) {
+      // the end is published after a timeout too: the softmax warps rely on it
+      const bool some = go && it.next(a, C::kRows, sg);
+      if (kv == 1 && lane == 0) {
+        segs[seg % kTreeSegs] = sg;
+        if (!some) segs[seg % kTreeSegs].j0 = -1;
+        mbar_arrive(&dready[seg % kTreeSegs]);
+      }
+      if (!some) break;
       // This lane's page of tile j (-1: past the row's pages), read two tiles ahead.
       auto page = [&](int j) {
         return lane < boxes && j < sg.j1 && j * ppt + p < sg.n_pages ? a.kv_indices[sg.kv_begin + j * ppt + p] : -1;
@@ -394,43 +411,60 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
                        umma_desc_mn_sw128(vb + kk * 16 * 128, C::kChunkBytes, 1024), idesc_o,
                        (!first || kk > 0) ? 1u : 0u);
       };
+      // One run over all tiles of the CTA: the first scores of a segment are
+      // issued while the last tile of the segment before is worked on.
       bool ok = true;
-      int t = 0;  // tiles of this CTA so far
       TreeSeg sg;
-      for (int seg = 0; ok && it.next(a, C::kRows, sg); ++seg) {
+      const int tiles = it.w_end - it.w;
+      int seg = 0, j = 0;
+      if (tiles > 0) {
+        (void)it.next(a, C::kRows, sg);
+        j = sg.j0;
+        for (int x = 0; x < NT; ++x) ok = ok && tree_wait(&qready[x], 0, flags);
+        ok = ok && wait_item(0);
+        if (ok) {
+          tc_fence_after();
 #pragma unroll
-        for (int x = 0; x < NT; ++x) ok = ok && tree_wait(&qready[x], seg & 1, flags);
-        ok = ok && wait_item(2 * t);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int x = 0; x < NT; ++x) issue_s(x, t);
-        umma_commit(&empty[(2 * t) % C::kSlots]);
-        for (int j = sg.j0; ok && j < sg.j1; ++j, ++t) {
-          const bool more = j + 1 < sg.j1;
-          // K of the next tile and V of this one are waited for in front of
-          // P, whose arrival starts the products
-          if (more) ok = wait_item(2 * t + 2);
+          for (int x = 0; x < NT; ++x) issue_s(x, 0);
+          umma_commit(&empty[0]);
+        }
+      }
+      for (int t = 0; ok && t < tiles; ++t) {
+        const bool more = t + 1 < tiles, last = j + 1 == sg.j1;  // of the CTA, of the segment
+        // K of the next tile and V of this one are waited for in front of
+        // P, whose arrival starts the products
+        if (more) ok = wait_item(2 * t + 2);
+        if (NT == 1 && more) {  // the next scores are computed during this tile's softmax
+          if (last) ok = ok && tree_wait(&qready[0], (seg + 1) & 1, flags);
           if (!ok) break;
-          if (NT == 1 && more) {  // the next scores are computed during this tile's softmax
-            tc_fence_after();
-            issue_s(0, t + 1);
-            umma_commit(&empty[(2 * t + 2) % C::kSlots]);
-          }
-          ok = wait_item(2 * t + 1);
+          tc_fence_after();
+          issue_s(0, t + 1);
+          umma_commit(&empty[(2 * t + 2) % C::kSlots]);
+        }
+        ok = ok && wait_item(2 * t + 1);
 #pragma unroll
-          for (int x = 0; x < NT; ++x) {
-            ok = ok && tree_wait(&pready[C::buf(x, t)], C::phase(t), flags);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(x, t, j == sg.j0);
-            if (NT == 2 && more) {
-              issue_s(x, t + 1);
-              if (x == NT - 1) umma_commit(&empty[(2 * t + 2) % C::kSlots]);
+        for (int x = 0; x < NT; ++x) {
+          ok = ok && tree_wait(&pready[C::buf(x, t)], C::phase(t), flags);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(x, t, j == sg.j0);
+          if (NT == 1 || last) umma_commit(&odone[x]);
+          if (x == NT - 1) umma_commit(&empty[(2 * t + 1) % C::kSlots]);
+          if (NT == 2 && more) {
+            if (last) {
+              ok = tree_wait(&qready[x], (seg + 1) & 1, flags);
+              if (!ok) break;
+              tc_fence_after();
             }
-            if (NT == 1 || !more) umma_commit(&odone[x]);
-            if (x == NT - 1) umma_commit(&empty[(2 * t + 1) % C::kSlots]);
+            issue_s(x, t + 1);
+            if (x == NT - 1) umma_commit(&empty[(2 * t + 2) % C::kSlots]);
           }
+        }
+        ++j;
+        if (last && more) {
+          (void)it.next(a, C::kRows, sg);
+          ++seg;
+          j = sg.j0;
         }
       }
       if (!ok) {
@@ -457,38 +491,45 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
     const uint32_t row_tmem = tmem + ((uint32_t)(32 * quad) << 16);
     const uint32_t o_tmem = row_tmem + (uint32_t)(256 + x * 128 + half * (D / 2));
     const uint32_t pair_bar = 1 + x * 4 + quad;
-    uint32_t* pair = reinterpret_cast<uint32_t*>(smem + C::kPairOff) + x * kTreeM + m;
-    bf16* pair_max = reinterpret_cast<bf16*>(pair);  // [half]
+    uint32_t* pair0 = reinterpret_cast<uint32_t*>(smem + C::kPairOff) + x * kTreeM + m;
     const float sl2 = a.scale_log2;
-    const bool writer = threadIdx.x == 0;
     bool ok = true;
     int t = 0;
+    // First tile of segment `seg`, -1 past the last.  The producer publishes
+    // every segment or, when it gives up, the end, each within a bounded
+    // time; all warps wait for that, so they see the same segments.
+    auto seg_start = [&](int seg) {
+      if (lane == 0)
+        for (int i = 0; i < 8 && !mbar_wait(&dready[seg % kTreeSegs], (seg / kTreeSegs) & 1); ++i) {}
+      __syncwarp();
+      return *const_cast<volatile int*>(&segs[seg % kTreeSegs].j0);
+    };
+    // this thread's half of its q row of segment `seg` (rows outside are zero)
+    auto stage_q = [&](int seg) {
+      const volatile TreeSeg& sg = segs[seg % kTreeSegs];
+      const int row = sg.rt * C::kRows + x * kTreeM + m, tok = row / a.group;
+      const bool row_ok = tok < sg.n;
+      const int head = sg.kvh * a.group + row % a.group;
+      const bf16* src = a.q + (int64_t)(sg.q0 + tok) * a.q_stride_t + (int64_t)head * a.q_stride_h;
+      uint8_t* qs = smem + C::kQOff + x * C::kQBytes;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const int u = half * (D / 16) + i;
+        const uint4 v = row_ok ? __ldg(reinterpret_cast<const uint4*>(src) + u) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(qs + (u >> 3) * C::kChunkBytes + tr_swz(m, u & 7)) = v;
+      }
+      fence_proxy_async_smem();
+      tree_warp_arrive(&qready[x]);
+    };
+    if (seg_start(0) >= 0) stage_q(0);
     for (int seg = 0;; ++seg) {
-      TreeSeg* sp = &segs[seg & 1];
-      if (writer && !it.next(a, C::kRows, *sp)) sp->j0 = -1;
-      named_barrier(15, C::kSoftmaxThreads);
-      const volatile TreeSeg& sg = *sp;
-      const int j0 = sg.j0;
+      const int j0 = seg_start(seg);
       if (j0 < 0) break;
+      const volatile TreeSeg& sg = segs[seg % kTreeSegs];
       // this thread's row of the request, computed where it is needed
       auto row_of = [&]() { return sg.rt * C::kRows + x * kTreeM + m; };
       // else: rows past the request's, nothing to compute
       const bool warp_ok = (sg.rt * C::kRows + x * kTreeM + 32 * quad) / a.group < sg.n;
-      if (ok) {
-        const int row = row_of(), tok = row / a.group;
-        const bool row_ok = tok < sg.n;
-        const int head = sg.kvh * a.group + row % a.group;
-        const bf16* src = a.q + (int64_t)(sg.q0 + tok) * a.q_stride_t + (int64_t)head * a.q_stride_h;
-        uint8_t* qs = smem + C::kQOff + x * C::kQBytes;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const int u = half * (D / 16) + i;
-          const uint4 v = row_ok ? __ldg(reinterpret_cast<const uint4*>(src) + u) : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(qs + (u >> 3) * C::kChunkBytes + tr_swz(m, u & 7)) = v;
-        }
-        fence_proxy_async_smem();
-        tree_warp_arrive(&qready[x]);
-      }
       float m_run = -INFINITY, l_run = 0.f;
       const int j1 = sg.j1;
       // V rows past the last token hold whatever the pool had there, and a
@@ -533,6 +574,9 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         const int sb = C::buf(x, t);
         const uint32_t s_tmem = row_tmem + (uint32_t)(sb * kTreeN + 64 * half);
         ok = ok && tree_warp_wait(&sready[sb], C::phase(t), flags);
+        // the segment's last scores are there: q makes room for the next one's
+        if (ok && j == j1 - 1 && seg_start(seg + 1) >= 0) stage_q(seg + 1);
+        bf16* pair_max = reinterpret_cast<bf16*>(pair0 + (C::kPairSets == 2 ? (t & 1) * C::kRows : 0));  // [half]
         const bool masked = j >= first_masked;  // uniform over the CTA
         if (!warp_ok) {
           if (ok && masked && x == 0) clean_v(j, t);
@@ -639,13 +683,15 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       }
       if (!warp_ok) continue;
       tc_fence_after();
-      float* pair_sum = reinterpret_cast<float*>(pair);
+      // (the partner's read of the last maxima lies behind its P, hence behind O)
+      float* pair_sum = reinterpret_cast<float*>(pair0);
       if (half == 1) *pair_sum = l_run;
       named_barrier(pair_bar, 64);
       if (half == 0) *pair_sum = l_run += *const_cast<volatile float*>(pair_sum);
       named_barrier(pair_bar, 64);
-      if (!ok) continue;
       l_run = *const_cast<volatile float*>(pair_sum);
+      named_barrier(pair_bar, 64);  // read: the next segment's maxima may go there
+      if (!ok) continue;
       const int row = row_of(), tok = row / a.group;
       const bool row_ok = tok < sg.n;
       const int head = sg.kvh * a.group + row % a.group;
