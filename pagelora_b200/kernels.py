@@ -803,11 +803,18 @@ def _need_pool(kv_cache: torch.Tensor) -> None:
         raise ValueError("kv_cache must be a contiguous [pages, 2, page_size, kv_heads, head_dim] tensor")
 
 
-def _need_vec(t: torch.Tensor, name: str, dtype: torch.dtype = torch.int32, size: int | None = None) -> None:
-    if t.dtype is not dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if not t.is_contiguous() or (size is not None and t.numel() < size):
-        raise ValueError(f"{name} must be contiguous" + ("" if size is None else f" with at least {size} entries"))
+def _vecs(dtype: torch.dtype, names: str, tensors: tuple, sizes: tuple) -> None:
+    """Every tensor is a contiguous CUDA tensor of ``dtype`` with at least its
+    size's entries (None: not given).  One pass: these checks are most of what
+    a small launch costs on the host."""
+
+    for t, n in zip(tensors, sizes):
+        if t is None or (t.dtype is dtype and t.is_cuda and t.is_contiguous() and t.numel() >= n):
+            continue
+        name = names.split()[next(i for i, x in enumerate(tensors) if x is t)]
+        _need_cuda(t)
+        _need(t, dtype, name)
+        raise ValueError(f"{name} must be contiguous with at least {n} entries")
 
 
 def _workspace(workspace: torch.Tensor | None, need: int, like: torch.Tensor) -> torch.Tensor:
@@ -817,7 +824,8 @@ def _workspace(workspace: torch.Tensor | None, need: int, like: torch.Tensor) ->
 def _need_rows(t: torch.Tensor, name: str, rows: int, dtype: torch.dtype = torch.int32) -> tuple[int, int]:
     """(row stride, width) of a [>= rows, width] matrix with contiguous rows."""
 
-    if t.dtype is not dtype:
+    if t.dtype is not dtype or not t.is_cuda:
+        _need_cuda(t)
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.dim() != 2 or t.shape[0] < rows or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"{name} must be [{rows}, width] with contiguous rows")
@@ -833,25 +841,19 @@ def tree_mask(parents: torch.Tensor, qo_indptr: torch.Tensor, words: int, *, bas
     (mask int32 [total_q, words], depth int32 [total_q]); ``positions``
     receives ``base_positions[request] + depth``."""
 
-    _need_cuda(parents, qo_indptr, base_positions, mask, depth, positions)
     total, batch = parents.numel(), qo_indptr.numel() - 1
-    _need_vec(parents, "parents")
-    _need_vec(qo_indptr, "qo_indptr")
+    _vecs(torch.int32, "parents qo_indptr base_positions depth positions",
+          (parents, qo_indptr, base_positions, depth, positions), (0, 1, batch, total, total))
     if words < 1:
         raise ValueError("words must be at least 1")
     if mask is None:
-        mask = parents.new_empty((total, words))
-    stride, width = _need_rows(mask, "mask", total)
-    if mask.shape[0] != total or width != words:
-        raise ValueError("mask must be [total_q, words]")
+        mask, stride = parents.new_empty((total, words)), words
+    else:
+        stride, width = _need_rows(mask, "mask", total)
+        if mask.shape[0] != total or width != words:
+            raise ValueError("mask must be [total_q, words]")
     if depth is None:
         depth = parents.new_empty(total)
-    else:
-        _need_vec(depth, "depth", size=total)
-    if positions is not None:
-        _need_vec(positions, "positions", size=total)
-    if base_positions is not None:
-        _need_vec(base_positions, "base_positions", size=batch)
     call("pl_tree_mask", parents.data_ptr(), qo_indptr.data_ptr(), ptr(base_positions), batch, total, words,
          mask.data_ptr(), stride, depth.data_ptr(), ptr(positions), ptr(status), stream_handle())
     return mask, depth
@@ -886,7 +888,7 @@ def paged_tree_attention(
     positions; ``tree_mask`` int32 [total_q, words] from :func:`tree_mask` or
     any bits.  ``out`` bf16 like q, ``out_lse`` fp32 [total_q, Hq]."""
 
-    _need_cuda(q, kv_cache, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, tree_mask, out, out_lse, workspace)
+    _need_cuda(q, kv_cache, out, workspace)
     _need(q, torch.bfloat16, "q")
     _need_pool(kv_cache)
     if q.dim() != 3 or q.stride(-1) != 1:
@@ -896,10 +898,8 @@ def paged_tree_attention(
     if d2 != d:
         raise ValueError("q and kv_cache head_dim differ")
     batch = qo_indptr.numel() - 1
-    _need_vec(qo_indptr, "qo_indptr")
-    _need_vec(kv_indptr, "kv_indptr", size=batch + 1)
-    _need_vec(kv_indices, "kv_indices")
-    _need_vec(kv_last_page_len, "kv_last_page_len", size=batch)
+    _vecs(torch.int32, "qo_indptr kv_indptr kv_indices kv_last_page_len",
+          (qo_indptr, kv_indptr, kv_indices, kv_last_page_len), (1, batch + 1, 0, batch))
     mask_stride, words = _need_rows(tree_mask, "tree_mask", total_q)
     if out is None:
         out = torch.empty_like(q)
@@ -908,7 +908,7 @@ def paged_tree_attention(
     elif out.shape != q.shape or out.stride(-1) != 1:
         raise ValueError("out must have q's shape and unit last stride")
     if out_lse is not None:
-        _need_vec(out_lse, "out_lse", torch.float32, total_q * hq)
+        _vecs(torch.float32, "out_lse", (out_lse,), (total_q * hq,))
     workspace = _workspace(workspace, tree_workspace_bytes(batch, total_q, hq, hkv, d), q)
     q_t, q_h, _ = q.stride()
     o_t, o_h, _ = out.stride()
@@ -929,15 +929,10 @@ def tree_accept(parents: torch.Tensor, tokens: torch.Tensor, targets: torch.Tens
     base_positions[b] + index of its tokens, ``keep_count`` int32 [batch] their
     number, ``next_token`` int64 [batch] the choice after it."""
 
-    _need_cuda(parents, tokens, targets, qo_indptr, base_positions, keep, keep_count, next_token)
     total, batch = parents.numel(), qo_indptr.numel() - 1
-    _need_vec(parents, "parents")
-    _need_vec(qo_indptr, "qo_indptr")
-    for name, t in (("tokens", tokens), ("targets", targets)):
-        _need_vec(t, name, torch.int64, total)
-    _need_vec(base_positions, "base_positions", size=batch)
-    _need_vec(keep_count, "keep_count", size=batch)
-    _need_vec(next_token, "next_token", torch.int64, batch)
+    _vecs(torch.int32, "parents qo_indptr base_positions keep_count", (parents, qo_indptr, base_positions, keep_count),
+          (0, 1, batch, batch))
+    _vecs(torch.int64, "tokens targets next_token", (tokens, targets, next_token), (total, total, batch))
     stride, width = _need_rows(keep, "keep", batch)
     call("pl_tree_accept", parents.data_ptr(), tokens.data_ptr(), targets.data_ptr(), qo_indptr.data_ptr(),
          base_positions.data_ptr(), batch, total, width, keep.data_ptr(), stride, keep_count.data_ptr(),
@@ -949,15 +944,13 @@ def _pool_tables(refcount: torch.Tensor, row_pages: torch.Tensor, row_num_pages:
                  last_page_len: torch.Tensor) -> tuple:
     """Checked arguments (refcount .. row capacity) of the page operations."""
 
-    _need_cuda(refcount, row_pages, row_num_pages, last_page_len)
-    _need_vec(refcount, "refcount")
-    _need_vec(row_pages, "row_pages")
+    rows, cap = row_pages.shape if row_pages.dim() == 2 else (0, 0)
+    _vecs(torch.int32, "refcount row_pages row_num_pages last_page_len",
+          (refcount, row_pages, row_num_pages, last_page_len), (1, 0, rows, rows))
     if row_pages.dim() != 2:
         raise ValueError("row_pages must be [rows, capacity]")
-    rows, cap = row_pages.shape
-    _need_vec(row_num_pages, "row_num_pages", size=rows)
-    _need_vec(last_page_len, "last_page_len", size=rows)
-    return (ptr(refcount), refcount.numel(), ptr(row_pages), ptr(row_num_pages), ptr(last_page_len), rows, cap)
+    return (refcount.data_ptr(), refcount.numel(), row_pages.data_ptr(), row_num_pages.data_ptr(),
+            last_page_len.data_ptr(), rows, cap)
 
 
 def _pool_data(pool: torch.Tensor, refcount: torch.Tensor) -> tuple[tuple, int]:
@@ -995,9 +988,8 @@ def page_release(refcount: torch.Tensor, row_pages: torch.Tensor, row_num_pages:
     """The rows ``rows`` (int32) give their pages back and become empty (pl_page_release)."""
 
     tables = _pool_tables(refcount, row_pages, row_num_pages, last_page_len)
-    _need_cuda(rows)
-    _need_vec(rows, "rows")
-    call("pl_page_release", *tables, ptr(rows), rows.numel(), ptr(status), stream_handle())
+    _vecs(torch.int32, "rows", (rows,), (0,))
+    call("pl_page_release", *tables, rows.data_ptr(), rows.numel(), ptr(status), stream_handle())
 
 
 def page_reserve(refcount: torch.Tensor, row_pages: torch.Tensor, row_num_pages: torch.Tensor,
@@ -1010,15 +1002,10 @@ def page_reserve(refcount: torch.Tensor, row_pages: torch.Tensor, row_num_pages:
     new page table to ``out_indptr`` / ``out_indices`` when given."""
 
     tables = _pool_tables(refcount, row_pages, row_num_pages, last_page_len)
-    _need_cuda(tok_indptr, slot_page, slot_offset, positions, out_indptr, out_indices)
-    rows, total = row_pages.shape[0], slot_page.numel()
-    _need_vec(tok_indptr, "tok_indptr", size=rows + 1)
-    _need_vec(slot_page, "slot_page")
-    _need_vec(slot_offset, "slot_offset", size=total)
-    for name, t, n in (("positions", positions, total), ("out_indptr", out_indptr, rows + 1),
-                       ("out_indices", out_indices, 0)):
-        if t is not None:
-            _need_vec(t, name, size=n)
+    rows, total = tables[5], slot_page.numel()
+    _vecs(torch.int32, "tok_indptr slot_page slot_offset positions out_indptr out_indices",
+          (tok_indptr, slot_page, slot_offset, positions, out_indptr, out_indices),
+          (rows + 1, 0, total, total, rows + 1, 0))
     call("pl_page_reserve", *tables, int(page_size), ptr(tok_indptr), total, ptr(slot_page), ptr(slot_offset),
          ptr(positions), ptr(out_indptr), ptr(out_indices), 0 if out_indices is None else out_indices.numel(),
          ptr(status), stream_handle())
@@ -1033,10 +1020,9 @@ def page_fork(pool: torch.Tensor, refcount: torch.Tensor, row_pages: torch.Tenso
 
     tables = _pool_tables(refcount, row_pages, row_num_pages, last_page_len)
     data, page_size = _pool_data(pool, refcount)
-    _need_cuda(src_rows, dst_rows, workspace)
+    _need_cuda(workspace)
     n = src_rows.numel()
-    _need_vec(src_rows, "src_rows")
-    _need_vec(dst_rows, "dst_rows", size=n)
+    _vecs(torch.int32, "src_rows dst_rows", (src_rows, dst_rows), (0, n))
     if dst_rows.numel() != n:
         raise ValueError("src_rows and dst_rows differ in length")
     workspace = _workspace(workspace, _fork_workspace_bytes(n), pool)
@@ -1053,10 +1039,9 @@ def cache_compact(pool: torch.Tensor, refcount: torch.Tensor, row_pages: torch.T
 
     tables = _pool_tables(refcount, row_pages, row_num_pages, last_page_len)
     data, page_size = _pool_data(pool, refcount)
-    _need_cuda(keep_from, keep, keep_count, workspace)
-    rows, cap = row_pages.shape
-    _need_vec(keep_from, "keep_from", size=rows)
-    _need_vec(keep_count, "keep_count", size=rows)
+    _need_cuda(workspace)
+    rows, cap = tables[5:]
+    _vecs(torch.int32, "keep_from keep_count", (keep_from, keep_count), (rows, rows))
     stride, width = _need_rows(keep, "keep", rows)
     workspace = _workspace(workspace, _compact_workspace_bytes(rows, cap), pool)
     call("pl_cache_compact", *data, *tables, page_size, ptr(keep_from), ptr(keep), stride, ptr(keep_count), width,
@@ -1069,15 +1054,13 @@ def page_bounds(kv_cache: torch.Tensor, page_ids: torch.Tensor, bounds: torch.Te
     """int8 bounds [pages, Hkv, 2, D] and scale [pages, Hkv] of the keys of
     pages ``page_ids`` (pl_page_bounds); ``page_len``: tokens in each (all)."""
 
-    _need_cuda(kv_cache, page_ids, bounds, bound_scale, page_len)
+    _need_cuda(kv_cache)
     _need_pool(kv_cache)
     num_pages, _, page_size, hkv, d = kv_cache.shape
     n = page_ids.numel()
-    _need_vec(page_ids, "page_ids")
-    _need_vec(bounds, "bounds", torch.int8, num_pages * hkv * 2 * d)
-    _need_vec(bound_scale, "bound_scale", torch.float32, num_pages * hkv)
-    if page_len is not None:
-        _need_vec(page_len, "page_len", size=n)
+    _vecs(torch.int32, "page_ids page_len", (page_ids, page_len), (0, n))
+    _vecs(torch.int8, "bounds", (bounds,), (num_pages * hkv * 2 * d,))
+    _vecs(torch.float32, "bound_scale", (bound_scale,), (num_pages * hkv,))
     call("pl_page_bounds", kv_cache.data_ptr(), num_pages, hkv, d, page_size, page_ids.data_ptr(), ptr(page_len), n,
          bounds.data_ptr(), bound_scale.data_ptr(), ptr(status), stream_handle())
 
@@ -1108,7 +1091,7 @@ def paged_sparse_decode(
     ``max_pages``: pages of the longest row (default: all of ``indices``);
     ``selected`` int32 [B, Hkv, num_select] receives the taken pages."""
 
-    _need_cuda(q, kv_cache, indptr, indices, last_page_len, bounds, bound_scale, out, out_lse, selected, workspace)
+    _need_cuda(q, kv_cache, out, workspace)
     _need(q, torch.bfloat16, "q")
     _need_pool(kv_cache)
     if q.dim() != 3 or q.stride(-1) != 1:
@@ -1117,22 +1100,18 @@ def paged_sparse_decode(
     num_pages, _, page_size, hkv, d2 = kv_cache.shape
     if d2 != d:
         raise ValueError("q and kv_cache head_dim differ")
-    _need_vec(indptr, "indptr", size=batch + 1)
-    _need_vec(indices, "indices")
-    _need_vec(last_page_len, "last_page_len", size=batch)
-    _need_vec(bounds, "bounds", torch.int8, num_pages * hkv * 2 * d)
-    _need_vec(bound_scale, "bound_scale", torch.float32, num_pages * hkv)
+    if selected is None:
+        selected = torch.empty(batch, hkv, max(num_select, 1), dtype=torch.int32, device=q.device)
+    _vecs(torch.int32, "indptr indices last_page_len selected", (indptr, indices, last_page_len, selected),
+          (batch + 1, 0, batch, batch * hkv * num_select))
+    _vecs(torch.int8, "bounds", (bounds,), (num_pages * hkv * 2 * d,))
+    _vecs(torch.float32, "bound_scale out_lse", (bound_scale, out_lse), (num_pages * hkv, batch * hq))
     if out is None:
         out = torch.empty_like(q)
     elif out.dtype is not torch.bfloat16:
         raise TypeError(f"out must be {torch.bfloat16}, got {out.dtype}")
     elif out.shape != q.shape or out.stride(-1) != 1:
         raise ValueError("out must have q's shape and unit last stride")
-    if out_lse is not None:
-        _need_vec(out_lse, "out_lse", torch.float32, batch * hq)
-    if selected is None:
-        selected = torch.empty(batch, hkv, max(num_select, 1), dtype=torch.int32, device=q.device)
-    _need_vec(selected, "selected", size=batch * hkv * num_select)
     if max_pages is None:
         max_pages = indices.numel()
     if max_pages > num_select and workspace is None:
