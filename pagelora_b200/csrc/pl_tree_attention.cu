@@ -16,15 +16,26 @@
 // per CTA (one CTA per SM), so ragged contexts fill the device; a CTA takes
 // the one or few item segments of its piece in turn.  A segment that covers
 // its item writes the output; the others leave (O, m, l) in the workspace
-// and tree_merge_kernel joins them.  Within a segment:
-//   warp 0     TMA producer: K_0, V_0, K_1, V_1, ... through a ring of tiles;
-//   warp 1     one lane issues tcgen05.mma: S = Q.K^T into TMEM, O += P.V;
-//   warps 2..  softmax, two threads per row (half of the tile's positions
-//              each): scores from TMEM, mask, online softmax (log2 domain),
-//              P (bf16) into the scores' TMEM columns as the A operand.
-// P is rounded to bf16 as the tensor core's operand; l sums the unrounded
-// fp32 values.  Waits are bounded: on expiry the kernel records
-// PL_ERR_TIMEOUT, drains its copies and returns.
+// and tree_merge_kernel joins them.  Per CTA:
+//   8 * NT warps  softmax, two threads per row (half of the tile's positions
+//                 each): scores from TMEM, mask, online softmax (log2
+//                 domain), P into the scores' TMEM columns as the A operand;
+//   K, V          a TMA producer each, K_0, V_0, K_1, ... through one ring;
+//   MMA           one lane issues tcgen05.mma: S = Q.K^T into TMEM, O += P.V.
+// P is rounded to bf16, as the tensor core's operand (each p by at most 2^-8
+// of itself); l sums the fp32 values before that.  P as two bf16 values,
+// rounded and remainder, would leave no error but the output's rounding and
+// takes 8 to 12 % more time (12 ragged requests with 32 kv heads 210 -> 228
+// us), for a result that is rounded to bf16 in any case.  The maximum that p
+// and l are relative to may lag by 2^8, so O is rescaled in TMEM only when a
+// row's maximum grows past that, which is rare.  Waits are bounded: on expiry
+// the kernel records PL_ERR_TIMEOUT, drains its copies and returns.
+//
+// Few rows read the cache once and are bound by HBM: 16 requests of 20 tokens
+// at 8000 positions (32 / 8 heads of 128) take 203 us in two layers, 5.2 TB/s.
+// Many rows are bound by the tensor core, the exponentials (2^x: 16 a cycle
+// and SM) and the power limit: 8 requests of 64 tokens at 32768 positions take
+// 715 us in two layers, 770 TFLOP/s.
 #include "pl_common.cuh"
 
 namespace pl {
@@ -266,7 +277,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
   uint64_t* empty = bars + C::kSlots;
   uint64_t* sready = bars + 2 * C::kSlots;  // [2] scores of a tile in buffer [i]
   uint64_t* pready = sready + 2;            // [2] P in buffer [i] (8 warps)
-  uint64_t* odone = sready + 4;             // [2] P_x.V of a tile (two row tiles: of a segment) complete
+  uint64_t* odone = sready + 4;             // [2] P.V of a tile from buffer [i] (two row tiles: P_x.V of a segment) complete
   uint64_t* qready = sready + 6;            // [2] Q_x of a segment staged (8 warps)
   uint64_t* fin = sready + 8;
   uint64_t* dready = sready + 9;            // [kTreeSegs] segment looked up
@@ -448,7 +459,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           if (!ok) break;
           tc_fence_after();
           issue_pv(x, t, j == sg.j0);
-          if (NT == 1 || last) umma_commit(&odone[x]);
+          if (NT == 1 || last) umma_commit(&odone[NT == 1 ? t & 1 : x]);
           if (x == NT - 1) umma_commit(&empty[(2 * t + 1) % C::kSlots]);
           if (NT == 2 && more) {
             if (last) {
@@ -630,10 +641,9 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           const bool rescale = m_run != -INFINITY && m_new > m_run + kTreeSlack;
           const float alpha = rescale ? tr_exp2(m_run - m_new) : 1.f;
           if (__any_sync(0xffffffffu, rescale)) {
-            // O_x of the tiles before has to be complete.  Two row tiles: it
-            // is, S was issued after it.  One: S was issued after the P.V of
-            // the tile before the last, so phase t - 1 is the one to wait for.
-            if (NT == 1 && !tree_warp_wait(&odone[x], (t - 1) & 1, flags)) ok = false;
+            // O_x of the tiles before has to be complete (two row tiles: it
+            // is, S was issued after it)
+            if (NT == 1 && !tree_warp_wait(&odone[sb ^ 1], ((t - 1) >> 1) & 1, flags)) ok = false;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -673,10 +683,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         tree_warp_arrive(&pready[sb]);
       }
       // ---- epilogue of the segment: each thread of a row has half of its channels
-      // (one row tile: the last scores only say that the P.V two tiles before
-      // is complete, so the phases are waited for one after the other)
-      if (NT == 1) ok = ok && tree_warp_wait(&odone[x], (t - 2) & 1, flags);
-      ok = ok && tree_warp_wait(&odone[x], (NT == 1 ? t - 1 : seg) & 1, flags);
+      ok = ok && tree_warp_wait(&odone[NT == 1 ? (t - 1) & 1 : x], (NT == 1 ? (t - 1) >> 1 : seg) & 1, flags);
       if (!ok) {
         if (lane == 0) set_status(a.status, PL_ERR_TIMEOUT);
         flags[0] = 1;
@@ -972,11 +979,19 @@ __global__ void __launch_bounds__(128)
 // =================================================================== host
 namespace {
 
-// Two row tiles per CTA when the requests average more rows than one holds.
+// Two row tiles per CTA read a K/V tile once for both, with scores that are
+// not computed ahead: taken when the mean request fills an even number of row
+// tiles, so that no tile is empty.  16 requests at 8000 positions (32 / 8
+// heads of 128), us with one and with two tiles per CTA: 128 rows of a kv
+// head 114, 162; 132 rows 189, 165; 256 rows 205, 192; 384 rows 309, 354.
 bool tree_two_tiles(int total_q, int batch, int group) {
-  return (int64_t)total_q * group > (int64_t)batch * pl::kTreeM;
+  const int64_t tile_rows = (int64_t)batch * pl::kTreeM;
+  return (((int64_t)total_q * group + tile_rows - 1) / tile_rows) % 2 == 0;
 }
 
+// Items of up to this many tiles stay whole, and when all pages together make
+// no more, the merge launch is left out.  8 tokens at 600 positions (5 tiles)
+// take 15.2 us whole and 15.7 us split; 16 tiles gain 5 us from the split.
 constexpr int kTreeMinSplit = 6;
 
 template <int D, int NT>
