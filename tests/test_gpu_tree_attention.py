@@ -171,6 +171,76 @@ def test_inf_and_nan_stay_with_the_rows_that_see_them(K, value, ctx, which):
         assert np.isnan(hit).all()
 
 
+# Requests whose mean fills an even number of 128-row tiles (two per CTA), beside ones that leave a tile or
+# a half of it empty, and without a context or without drafts.
+WIDE = [
+    ([(64, 500)], 8, 2),
+    ([(96, 40), (1, 0), (80, 2000), (40, 300)], 8, 2),
+    ([(200, 3), (0, 77), (256, 900), (60, 129)], 2, 2),
+    ([(37, 700), (33, 0)], 14, 2),
+    ([(130, 1000)], 12, 4),
+    ([(1, 5000), (70, 10), (20, 128), (33, 127)], 32, 2),
+]
+
+
+@pytest.mark.parametrize("d,ps", [(128, 16), (64, 16), (128, 128)])
+@pytest.mark.parametrize("reqs,hq,hkv", WIDE)
+def test_two_row_tiles(K, reqs, hq, hkv, d, ps):
+    mean = -(-sum(n for n, _ in reqs) * (hq // hkv) // (128 * len(reqs)))
+    assert mean % 2 == 0
+    host, dev = _case(reqs, hq, hkv, d, ps, seed=len(reqs) + d)
+    _check(_run(K, dev), host)
+
+
+@pytest.mark.parametrize("value", [np.nan, -np.inf])
+@pytest.mark.parametrize("which", [0, 1])
+def test_two_row_tiles_masks_inf_and_nan(K, value, which):
+    """As above with any bits, rows that see nothing, and a drafted token that only some rows see."""
+
+    rng = np.random.default_rng(12)
+    n, ctx = 72, 200
+    see = [rng.random((n, n)) < 0.4, rng.random((n, n)) < 0.4]
+    see[1][5] = False
+    see[1][70] = False
+    hit = np.flatnonzero(see[0][:, 9])
+
+    def fix(cache, host):
+        pos = ctx + 9
+        cache[host["kv_indices"][pos // host["ps"]], which, pos % host["ps"], :, 5] = value
+
+    host, dev = _case([(n, ctx), (n, 0)], 8, 2, 128, 16, seed=2, see=see, kv_fix=fix)
+    out, lse = _run(K, dev)
+    clean = dict(host, cache=np.nan_to_num(host["cache"], nan=0.0, posinf=0.0, neginf=0.0))
+    _check((out, lse), clean, np.setdiff1d(np.arange(2 * n), hit))
+    assert (out[n + 5] == 0).all() and np.isneginf(lse[n + 70]).all()
+    if which == 1:
+        assert not np.isfinite(out[hit][..., 5]).any() and np.isfinite(np.delete(out[hit], 5, axis=-1)).all()
+    elif np.isnan(value):
+        assert np.isnan(out[hit]).all()
+
+
+@pytest.mark.parametrize("n", [5, 40, 64])
+def test_growing_maxima(K, n):
+    """Scores whose maximum grows by more than 2^8 from tile to tile, not always in order.  A channel adds up to
+    43 to the scores: their fp32 error is at most 128 * 2^-24 * (43 + sum |q k| of the others, about 11)
+    < 2^-11, in place of 2^-12."""
+
+    level = [0, 5, 10, 5, 15, 0, 20, 30, 20, 30, 1]
+
+    def fix(cache, host):
+        for t in range(host["lens"][0]):
+            cache[host["kv_indices"][t // host["ps"]], 0, t % host["ps"], :, 0] = level[t // 128]
+
+    host, dev = _case([(n, 128 * len(level) - n - 20)], 8, 2, 128, 16, seed=n, kv_fix=fix)
+    host["q"][..., 0] = 16.0
+    dev["q"][..., 0] = 16.0
+    out, lse = _run(K, dev)
+    want, wlse, spread = o.tree_attention(host["q"], host["cache"], host["qo"], host["kv_indptr"], host["kv_indices"],
+                                          host["last"], host["see"])
+    assert (np.abs(out - want) <= U * (np.abs(want) + spread) + 2 * F * spread).all()
+    assert (np.abs(lse - wlse) <= 2 * F * (1 + np.abs(wlse))).all()
+
+
 def test_strides_scale_and_streams(K):
     host, dev = _case([(12, 90), (3, 400)], 8, 2, 128, 16, seed=11)
     total = host["qo"][-1]
