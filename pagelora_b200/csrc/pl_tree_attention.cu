@@ -43,6 +43,13 @@ namespace pl {
 constexpr int kTreeM = 128;              // rows of one tile
 constexpr int kTreeN = 128;              // positions of one K/V tile
 constexpr float kTreeSlack = 8.0f;       // log2 growth of a row's maximum that is tolerated before O is rescaled
+// Places on the line that an item takes beside its tiles: its look-up, first
+// scores, masked tiles and epilogue take a CTA about 6300 cycles, a tile 2340.
+// us with 0, 1, 2, 3, 4 places: 12 requests of 5-33 tokens at 300-4100
+// positions, 32 kv heads, two layers 213, 197, 187, 185, 186; 32 of 1-40
+// tokens at 100-9000, 8 kv heads 184, 154, 158, 145, 143-159; 24 of 40-90
+// tokens 337, 308, 278, 251, 245; requests of equal length do not change.
+constexpr int kTreeItemCost = 3;
 constexpr int kTreeMaxTokens = 1024;     // drafted tokens of one request (tree_mask / tree_accept)
 
 struct TreeArgs {
@@ -139,8 +146,10 @@ struct TreeReq {
     rts = (int)(((int64_t)n * a.group + rows - 1) / rows);
     ntiles = max(1, (kv_len + kTreeN - 1) / kTreeN);  // an empty context still writes its zero rows
   }
-  // tiles of the request (the host bounds the total of all requests)
-  __device__ __forceinline__ int work(int hkv) const { return rts * hkv * ntiles; }
+  // length of an item on the line: its tiles and what it costs besides
+  __device__ __forceinline__ int span() const { return ntiles + kTreeItemCost; }
+  // of the request (the host bounds the total of all requests)
+  __device__ __forceinline__ int work(int hkv) const { return rts * hkv * span(); }
 };
 
 // Inclusive prefix sum over a warp.
@@ -154,7 +163,7 @@ __device__ __forceinline__ int tree_scan(int v) {
   return v;
 }
 
-// Tiles of all requests (one warp).
+// Length of the line (one warp).
 __device__ __forceinline__ int tree_total(const TreeArgs& a, int rows) {
   int t = 0;
   for (int b = threadIdx.x & 31; b < a.batch; b += 32) {
@@ -167,13 +176,13 @@ __device__ __forceinline__ int tree_total(const TreeArgs& a, int rows) {
   return t;
 }
 
-// Tiles per CTA.
+// Its part of a CTA.
 __device__ __forceinline__ int tree_share(int total, int ctas) { return max(1, (total + ctas - 1) / ctas); }
 
-// The requests that hold tiles w0 and w1 of the line (batch: past the end)
-// and their first tiles.  A cut that falls inside an item of at most
-// min_split tiles moves to the item's start, so short items are never split
-// (and never merged).  One warp.
+// The requests that hold places w0 and w1 of the line (batch: past the end)
+// and where they begin.  A cut in front of an item's second tile, or inside an
+// item of at most min_split tiles, moves to the item's start, so short items
+// are never split (and never merged).  One warp.
 struct TreeAt {
   int b, base, w;
 };
@@ -185,7 +194,7 @@ __device__ __forceinline__ void tree_locate(const TreeArgs& a, int rows, TreeAt&
   for (int b0 = 0; b0 < a.batch && at1.b == a.batch; b0 += 32) {
     TreeReq r;
     int n = 0;
-    r.ntiles = 1;
+    r.ntiles = 1;  // lanes past the batch
     if (b0 + lane < a.batch) {
       r.load(a, b0 + lane, rows);
       n = r.work(a.num_kv_heads);
@@ -199,15 +208,17 @@ __device__ __forceinline__ void tree_locate(const TreeArgs& a, int rows, TreeAt&
       at[i]->b = b0 + l;
       at[i]->base = __shfl_sync(0xffffffffu, inc - n, l);
       const int nt = __shfl_sync(0xffffffffu, r.ntiles, l);
-      if (nt <= a.min_split) at[i]->w -= (at[i]->w - at[i]->base) % nt;
+      const int off = (at[i]->w - at[i]->base) % (nt + kTreeItemCost);
+      if (nt <= a.min_split || off <= kTreeItemCost) at[i]->w -= off;
     }
     base = __shfl_sync(0xffffffffu, inc, 31);
   }
 }
 
-// Walks the item segments of the tile range [w, w_end).
+// Walks the item segments of the range [w, w_end) of the line.
 struct TreeIter {
-  int b, w, w_end, base;  // base: first tile of request b
+  int b, w, w_end, base;  // base: where request b begins
+  __device__ __forceinline__ bool more() const { return w < w_end; }
   __device__ __forceinline__ bool next(const TreeArgs& a, int rows, TreeSeg& s) {
     if (w >= w_end) return false;
     TreeReq r;
@@ -217,19 +228,20 @@ struct TreeIter {
       ++b;
       r.load(a, b, rows);
     }
-    const int off = w - base;
-    const int item = off / r.ntiles;
+    const int item = (w - base) / r.span();
+    const int off = w - base - item * r.span();
+    const int end = min(off + (w_end - w), r.span());
     s.q0 = r.q0;
     s.n = r.n;
     s.kv_begin = r.kv_begin;
     s.n_pages = r.n_pages;
     s.kv_len = r.kv_len;
-    s.j0 = off - item * r.ntiles;
-    s.j1 = min(s.j0 + (w_end - w), r.ntiles);
+    s.j0 = max(0, off - kTreeItemCost);
+    s.j1 = end - kTreeItemCost;
     s.rt = item % r.rts;
     s.kvh = item / r.rts;
     s.whole = s.j0 == 0 && s.j1 == r.ntiles;
-    w += s.j1 - s.j0;
+    w += end - off;
     return true;
   }
 };
@@ -426,10 +438,9 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       // issued while the last tile of the segment before is worked on.
       bool ok = true;
       TreeSeg sg;
-      const int tiles = it.w_end - it.w;
       int seg = 0, j = 0;
-      if (tiles > 0) {
-        (void)it.next(a, C::kRows, sg);
+      bool more = it.next(a, C::kRows, sg);
+      if (more) {
         j = sg.j0;
         for (int x = 0; x < NT; ++x) ok = ok && tree_wait(&qready[x], 0, flags);
         ok = ok && wait_item(0);
@@ -440,8 +451,9 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           umma_commit(&empty[0]);
         }
       }
-      for (int t = 0; ok && t < tiles; ++t) {
-        const bool more = t + 1 < tiles, last = j + 1 == sg.j1;  // of the CTA, of the segment
+      for (int t = 0; ok && more; ++t) {
+        const bool last = j + 1 == sg.j1;  // tile of the segment
+        more = !last || it.more();         // tiles in this CTA
         // K of the next tile and V of this one are waited for in front of
         // P, whose arrival starts the products
         if (more) ok = wait_item(2 * t + 2);
@@ -789,7 +801,7 @@ template <int D>
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArgs a, int rows) {
   const int lane = threadIdx.x & 31;
   const int tok_g = blockIdx.x;
-  // the request of this token, the tiles in front of it, and all tiles
+  // the request of this token, where it begins on the line, and the line's length
   int q0 = 0, rts = 0, nt = 0, base = 0, total = 0;
   bool found = false;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
@@ -811,9 +823,9 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
   const int share = tree_share(total, a.ctas);
   const int head = blockIdx.y * (kMergeThreads / 32) + threadIdx.x / 32;
   const int row = (tok_g - q0) * a.group + head % a.group;
-  const int w = base + ((head / a.group) * rts + row / rows) * nt;
+  const int w = base + ((head / a.group) * rts + row / rows) * (nt + kTreeItemCost);
   const int m = row % rows;
-  const int ca = w / share, cb = (w + nt - 1) / share;
+  const int ca = (w + kTreeItemCost) / share, cb = (w + kTreeItemCost + nt - 1) / share;
   pdl_wait();
   pdl_launch_dependents();
   if (!found || nt <= a.min_split || head >= a.num_qo_heads || ca == cb) return;  // not split
@@ -1062,7 +1074,7 @@ extern "C" int32_t pl_paged_tree_attention(
   const bool two = tree_two_tiles(total_q, batch, group);
   // the line of tiles is indexed in 32 bits; an upper bound of its length
   const int64_t most_rts = (int64_t)total_q * group / pl::kTreeM + batch;
-  if (most_rts * num_kv_heads > 0x7FFFFFFFll / (total_pages * page_size / pl::kTreeN + 1)) return PL_ERR_UNSUPPORTED;
+  if (most_rts * num_kv_heads > 0x7FFFFFFFll / (total_pages * page_size / pl::kTreeN + 1 + pl::kTreeItemCost)) return PL_ERR_UNSUPPORTED;
   pl::TreeArgs a;
   a.q = static_cast<const pl::bf16*>(q);
   a.kv = static_cast<const pl::bf16*>(kv_cache);
