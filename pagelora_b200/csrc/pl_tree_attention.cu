@@ -32,10 +32,12 @@
 // the kernel records PL_ERR_TIMEOUT, drains its copies and returns.
 //
 // Few rows read the cache once and are bound by HBM: 16 requests of 20 tokens
-// at 8000 positions (32 / 8 heads of 128) take 203 us in two layers, 5.2 TB/s.
-// Many rows are bound by the tensor core, the exponentials (2^x: 16 a cycle
-// and SM) and the power limit: 8 requests of 64 tokens at 32768 positions take
-// 715 us in two layers, 770 TFLOP/s.
+// at 8000 positions (32 / 8 heads of 128) take 205 us in two layers, 5.2 TB/s;
+// 89 us of a layer are this kernel, where a plain copy of the bytes takes 81.
+// Many rows are bound by the chain softmax (2200 cycles) -> P.V -> next scores
+// (2800, half of it the issue) of each of two row tiles in turn, and by the
+// power limit: 8 requests of 64 tokens at 32768 positions take 740 us in two
+// layers, 745 TFLOP/s (660 us before the clock falls from 1.8 to 1.6 GHz).
 #include "pl_common.cuh"
 
 namespace pl {
