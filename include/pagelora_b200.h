@@ -875,6 +875,8 @@ int32_t pl_argmax(const void *logits, int64_t stride, int32_t vocab,
  *              natural log, nullable
  *   workspace  16-byte aligned, pl_tree_workspace_bytes; needs no
  *              initialisation and keeps nothing between calls
+ * Arrays without entries (no drafted token, no page) may be NULL, here and in
+ * pl_tree_mask, pl_tree_accept and pl_paged_sparse_decode.
  * Supported: head_dim 64 or 128, page_size 16 / 32 / 64 / 128, any group up
  * to 128.  A request with n_b > its cached tokens or > 32 * mask_words, or
  * with a table outside kv_indices, writes PL_ERR_INVALID_ARGUMENT to

@@ -966,8 +966,10 @@ extern "C" int32_t pl_paged_sparse_decode(
     int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float sm_scale, int32_t num_select,
     int32_t sink_pages, int32_t recent_pages, void* out, int64_t o_stride_b, int64_t o_stride_h, float* out_lse,
     int32_t* selected, void* workspace, int64_t workspace_bytes, int32_t* status_dev, void* stream) {
-  if (q == nullptr || kv_cache == nullptr || indptr == nullptr || indices == nullptr || last_page_len == nullptr ||
-      bounds == nullptr || bound_scale == nullptr || out == nullptr || selected == nullptr || batch < 0 ||
+  // what has no entries may be null
+  if (kv_cache == nullptr || indptr == nullptr || (total_pages > 0 && indices == nullptr) || bounds == nullptr ||
+      bound_scale == nullptr || batch < 0 ||
+      (batch > 0 && (q == nullptr || last_page_len == nullptr || out == nullptr || selected == nullptr)) ||
       num_pages <= 0 || num_pages > 0x3FFFFFFF || total_pages < 0 || max_pages < 0 || max_pages > 0x7FFFFFF0 || num_kv_heads <= 0 ||
       num_qo_heads <= 0 || num_qo_heads % num_kv_heads != 0 || !(sm_scale > 0.f) || sink_pages < 0 || recent_pages < 1 || num_select < 1 ||
       (int64_t)sink_pages + recent_pages > num_select)

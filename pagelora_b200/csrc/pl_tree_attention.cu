@@ -1047,8 +1047,10 @@ extern "C" int32_t pl_paged_tree_attention(
     int32_t total_q, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float sm_scale,
     void* out, int64_t out_stride_t, int64_t out_stride_h, float* out_lse, void* workspace, int64_t workspace_bytes,
     int32_t* status_dev, void* stream) {
-  if (q == nullptr || kv_cache == nullptr || qo_indptr == nullptr || kv_indptr == nullptr || kv_indices == nullptr ||
-      kv_last_page_len == nullptr || tree_mask == nullptr || out == nullptr || batch < 0 || total_q < 0 ||
+  // what has no entries may be null
+  if (kv_cache == nullptr || qo_indptr == nullptr || kv_indptr == nullptr || kv_last_page_len == nullptr ||
+      (total_pages > 0 && kv_indices == nullptr) ||
+      (total_q > 0 && (q == nullptr || tree_mask == nullptr || out == nullptr)) || batch < 0 || total_q < 0 ||
       num_pages <= 0 || num_pages > 0x3FFFFFFF || total_pages < 0 || mask_words <= 0 || mask_stride < mask_words ||
       num_kv_heads <= 0 || num_qo_heads <= 0 || num_qo_heads % num_kv_heads != 0 || !(sm_scale > 0.f))
     return PL_ERR_INVALID_ARGUMENT;
@@ -1114,7 +1116,8 @@ extern "C" int32_t pl_paged_tree_attention(
 extern "C" int32_t pl_tree_mask(const int32_t* parents, const int32_t* qo_indptr, const int32_t* base_positions,
                                 int32_t batch, int32_t total_q, int32_t mask_words, int32_t* mask, int64_t mask_stride,
                                 int32_t* depth, int32_t* positions, int32_t* status_dev, void* stream) {
-  if (parents == nullptr || qo_indptr == nullptr || mask == nullptr || batch < 0 || total_q < 0 || mask_words <= 0 ||
+  if (qo_indptr == nullptr || (total_q > 0 && (parents == nullptr || mask == nullptr)) || batch < 0 ||
+      total_q < 0 || mask_words <= 0 ||
       mask_stride < mask_words)
     return PL_ERR_INVALID_ARGUMENT;
   if (batch == 0 || total_q == 0) return PL_OK;
@@ -1129,7 +1132,7 @@ extern "C" int32_t pl_tree_accept(const int32_t* parents, const int64_t* tokens,
                                   const int32_t* qo_indptr, const int32_t* base_positions, int32_t batch,
                                   int32_t total_q, int32_t max_keep, int32_t* keep, int64_t keep_stride,
                                   int32_t* keep_count, int64_t* next_token, int32_t* status_dev, void* stream) {
-  if (parents == nullptr || tokens == nullptr || targets == nullptr || qo_indptr == nullptr ||
+  if ((total_q > 0 && (parents == nullptr || tokens == nullptr || targets == nullptr)) || qo_indptr == nullptr ||
       base_positions == nullptr || keep == nullptr || keep_count == nullptr || next_token == nullptr || batch < 0 ||
       total_q < 0 || max_keep <= 0 || keep_stride < max_keep)
     return PL_ERR_INVALID_ARGUMENT;

@@ -113,6 +113,9 @@ def test_empty_calls_do_nothing(capi):
                              ("pl_paged_tree_attention", TREE, dict(batch=0)),
                              ("pl_paged_sparse_decode", SPARSE, dict(batch=0)), ("pl_page_bounds", BOUNDS, dict(n=0)),
                              ("pl_tree_mask", MASK, dict(total_q=0)), ("pl_tree_accept", ACCEPT, dict(batch=0)),
+                             ("pl_paged_tree_attention", TREE, dict(total_q=0, q=None, mask=None, out=None)),
+                             ("pl_tree_mask", MASK, dict(total_q=0, parents=None, mask=None)),
+                             ("pl_paged_sparse_decode", SPARSE, dict(batch=0, q=None, last=None, out=None, selected=None)),
                              ("pl_page_release", RELEASE, dict(n=0, released=None)),
                              ("pl_page_fork", FORK, dict(n=0, ws=None))):
         assert getattr(lib, fn)(*dict(args, **change).values()) == 0, fn

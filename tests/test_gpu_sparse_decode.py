@@ -248,3 +248,12 @@ def test_refusals(K):
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     K.page_bounds(dev["cache"], _i32([10 ** 6]), dev["bounds"], dev["scale"], status=status)
     assert int(status.item()) == _capi.PL_ERR_PAGE_OUT_OF_RANGE
+
+
+def test_rows_without_pages(K):
+    """Every row is empty and the page list has no entries."""
+
+    _, dev = _case(K, [0, 0], 4, 2, 64, 16, seed=3)
+    dev["indices"] = dev["indices"][:0]
+    out, lse, sel = _run(K, dev, 4, 1, 1, max_pages=8)
+    assert (out == 0).all() and np.isneginf(lse).all() and (sel == -1).all()

@@ -421,3 +421,20 @@ def test_tree_accept_refusals(K):
     assert int(status.item()) == _capi.PL_ERR_INVALID_ARGUMENT and int(count.item()) == 0
     with pytest.raises(TypeError):
         K.tree_accept(_i32([-1]), one.int(), one, _i32([0, 1]), _i32([0]), keep=keep, keep_count=count, next_token=nxt)
+
+
+def test_calls_without_entries(K):
+    """No drafted token in any row: nothing to mask or attend to, every row keeps nothing."""
+
+    host, dev = _case([(3, 20), (2, 0)], 8, 2, 128, 16, seed=14)
+    none = _i32([0, 0, 0])
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    mask, depth = K.tree_mask(none[:0], none, 1, status=status)
+    assert mask.shape == (0, 1) and depth.numel() == 0
+    out = K.paged_tree_attention(dev["q"][:0], dev["cache"], none, dev["kv_indptr"], dev["kv_indices"], dev["last"], mask,
+                                 status=status)
+    assert out.shape == (0, 8, 128)
+    keep, count = torch.full((2, 4), 9, dtype=torch.int32, device="cuda"), none[:2].clone() + 9
+    nxt = torch.zeros(2, dtype=torch.int64, device="cuda")
+    K.tree_accept(none[:0], nxt[:0], nxt[:0], none, none[:2], keep=keep, keep_count=count, next_token=nxt, status=status)
+    assert count.tolist() == [0, 0] and int(status.item()) == 0
