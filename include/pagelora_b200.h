@@ -1058,8 +1058,8 @@ int32_t pl_page_bounds(const void *kv_cache, int64_t num_pages,
  *            row (index in its page list), ascending, then -1
  *   workspace 16-byte aligned, pl_sparse_workspace_bytes, no initialisation
  *            (unused, nullable, when max_pages <= num_select)
- * Supported: head_dim 64 or 128, page_size 16 or 32, group <= 16.  No
- * reference counterpart.
+ * Supported: head_dim 64 or 128, page_size 16 or 32, group <= 16, and
+ * num_select up to 24576 where max_pages is larger.  No reference counterpart.
  */
 int64_t pl_sparse_workspace_bytes(int32_t batch, int32_t num_kv_heads,
                                   int32_t max_pages);

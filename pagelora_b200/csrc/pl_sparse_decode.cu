@@ -635,10 +635,8 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
     else
       sparse_select<0>(a, keys, r.pages, hist, lo, hi, list, all);
   } else {
-    for (int i = threadIdx.x; i < hi - lo; i += kSparseThreads) list[i] = lo + i;
     if (all != nullptr)
       for (int i = threadIdx.x; i < a.select; i += kSparseThreads) all[i] = i < taken ? i : -1;
-    __syncthreads();
   }
 
   // the selection's use of the ring's bytes, before the copies'
@@ -652,10 +650,11 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
   uint8_t* ring = smem + warp * C::kRing * C::kTile;
   uint64_t* full = bars + warp * C::kRing;
   // page id of a unit (looked at when it is loaded), -1 past the last
-  auto page_of = [&](int u) { return u < units ? a.indices[r.begin + list[u >> ushift]] : -1; };
+  auto nth = [&](int i) { return r.pages <= a.select ? lo + i : list[i]; };  // taken page of the row
+  auto page_of = [&](int u) { return u < units ? a.indices[r.begin + nth(u >> ushift)] : -1; };
   auto live_of = [&](int u) {  // its tokens
     if (u >= units) return 0;
-    const int len = list[u >> ushift] == r.pages - 1 ? r.last : PS;
+    const int len = nth(u >> ushift) == r.pages - 1 ? r.last : PS;
     return min(kSparseUnit, max(0, len - (u & (upp - 1)) * kSparseUnit));
   };
   // Tile into a slot: 16-byte unit c of token t at (c / 8) * kHalfBytes +
@@ -917,10 +916,14 @@ constexpr int kScoreSteps = 4;  // steps of a warp when rows differ in length
 
 int32_t sparse_key_stride(int32_t max_pages) { return (int32_t)(((int64_t)max_pages + 3) & ~int64_t(3)); }
 
+constexpr int kSparseMostListed = 24576;  // selected pages of a row, kept in shared memory
+
 template <int D, int NH>
 int32_t launch_attend_nh(const CUtensorMap& map, const pl::SparseArgs& a, int batch, void* stream) {
   auto kern = pl::sparse_attend_kernel<D, NH>;
-  const int list = 4 * ((a.select < a.max_pages ? a.select : a.max_pages) / a.splits + 2);
+  // rows that take all their pages need no list
+  const int list = a.select < a.max_pages ? 4 * (a.select / a.splits + 2) : 0;
+  static_assert(1024 + pl::SparseCfg<D>::kListOff + 4 * (kSparseMostListed + 2) + 16 <= 232448, "the list must fit");
   const int smem = 1024 + pl::SparseCfg<D>::kListOff + ((list + 15) & ~15);
   int32_t st = pl_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
   if (st != PL_OK) return st;
@@ -982,6 +985,7 @@ extern "C" int32_t pl_paged_sparse_decode(
       (reinterpret_cast<uintptr_t>(q) & 15) != 0 || (reinterpret_cast<uintptr_t>(out) & 15) != 0 ||
       (q_stride_b % 8) != 0 || (q_stride_h % 8) != 0 || (o_stride_b % 8) != 0 || (o_stride_h % 8) != 0)
     return PL_ERR_INVALID_ARGUMENT;
+  if (max_pages > num_select && num_select > kSparseMostListed) return PL_ERR_UNSUPPORTED;
   if (batch == 0) return PL_OK;
   if (max_pages > num_select &&
       (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||

@@ -83,7 +83,7 @@ def test_invalid_arguments(capi, fn):
     ("pl_paged_tree_attention", TREE, dict(d=96)), ("pl_paged_tree_attention", TREE, dict(ps=24)),
     ("pl_paged_tree_attention", TREE, dict(hq=258)), ("pl_paged_sparse_decode", SPARSE, dict(ps=64)),
     ("pl_paged_sparse_decode", SPARSE, dict(hq=34)), ("pl_paged_sparse_decode", SPARSE, dict(d=80)),
-    ("pl_page_bounds", BOUNDS, dict(d=96)),
+    ("pl_page_bounds", BOUNDS, dict(d=96)), ("pl_paged_sparse_decode", SPARSE, dict(select=24577, max_pages=30000)),
 ])
 def test_unsupported_shapes(capi, fn, args, change):
     c, lib = capi

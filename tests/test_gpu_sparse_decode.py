@@ -257,3 +257,16 @@ def test_rows_without_pages(K):
     dev["indices"] = dev["indices"][:0]
     out, lse, sel = _run(K, dev, 4, 1, 1, max_pages=8)
     assert (out == 0).all() and np.isneginf(lse).all() and (sel == -1).all()
+
+
+@pytest.mark.parametrize("select", [2900, 3044, 30000])
+def test_many_selected_pages(K, select):
+    """A list of thousands of pages, and budgets that hold all pages of every row (3000 + 44 in the table)."""
+
+    host, dev = _case(K, [48000, 700], 4, 1, 64, 16, seed=31)
+    out, lse, sel = _run(K, dev, select, 1, 1)
+    want, wlse, spread, chosen = o.sparse_decode(host["q"], host["cache"], host["indptr"], host["indices"], host["last"],
+                                                 host["bounds"], host["scale"], num_select=select, sink=1, recent=1)
+    assert (sel == chosen).all()
+    assert (np.abs(out - want) <= U * (np.abs(want) + spread) + F * spread).all()
+    assert (np.abs(lse - wlse) <= F * (1 + np.abs(wlse))).all()
