@@ -23,13 +23,18 @@
 //   K, V          a TMA producer each, K_0, V_0, K_1, ... through one ring;
 //   MMA           one lane issues tcgen05.mma: S = Q.K^T into TMEM, O += P.V.
 // P is rounded to bf16, as the tensor core's operand (each p by at most 2^-8
-// of itself); l sums the fp32 values before that.  P as two bf16 values,
-// rounded and remainder, would leave no error but the output's rounding and
-// takes 8 to 12 % more time (12 ragged requests with 32 kv heads 210 -> 228
-// us), for a result that is rounded to bf16 in any case.  The maximum that p
-// and l are relative to may lag by 2^8, so O is rescaled in TMEM only when a
-// row's maximum grows past that, which is rare.  Waits are bounded: on expiry
-// the kernel records PL_ERR_TIMEOUT, drains its copies and returns.
+// of itself).  One row tile: O is divided by the sum of the rounded values, so
+// that a row of few positions is nearly exact (of one: exact) and the error
+// of a long one stays about that of the output's own rounding; lse takes the
+// sum of the fp32 values.  Two row tiles have no registers for a second sum
+// (8 requests of 64 tokens at 32768 positions 750 -> 790 us) and divide by
+// that one.  P as two bf16 values, rounded and remainder, would leave the
+// output's rounding alone and takes 5 to 18 % more time (16 requests of 20
+// tokens 209 -> 225 us, the 8 above 745 -> 880).
+// The maximum that p and the sums are relative to may lag by 2^8, so O is
+// rescaled in TMEM only when a row's maximum grows past that, which is rare.
+// Waits are bounded: on expiry the kernel records PL_ERR_TIMEOUT, drains its
+// copies and returns.
 //
 // Few rows read the cache once and are bound by HBM: 16 requests of 20 tokens
 // at 8000 positions (32 / 8 heads of 128) take 205 us in two layers, 5.2 TB/s;
@@ -71,7 +76,7 @@ struct TreeArgs {
   int64_t out_stride_t, out_stride_h;
   float* lse;      // optional [total_q, Hq], natural log
   float* part_o;   // [2 * ctas][128 * NT][D]
-  float* part_ml;  // [2 * ctas][2][128 * NT]
+  float* part_ml;  // [2 * ctas][3][128 * NT]: m, l, the sum of the rounded p
   int32_t* status;
 };
 
@@ -555,7 +560,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       auto row_of = [&]() { return sg.rt * C::kRows + x * kTreeM + m; };
       // else: rows past the request's, nothing to compute
       const bool warp_ok = (sg.rt * C::kRows + x * kTreeM + 32 * quad) / a.group < sg.n;
-      float m_run = -INFINITY, l_run = 0.f;
+      float m_run = -INFINITY, l_run = 0.f, n_run = 0.f;  // sums of p, of p as rounded
       const int j1 = sg.j1;
       // V rows past the last token hold whatever the pool had there, and a
       // drafted token's V may hold inf or NaN that a row which masks the
@@ -668,14 +673,15 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
               tmem_st16_wait(o_tmem + 16 * c, o);
             }
             l_run *= alpha;
+            if constexpr (NT == 1) n_run *= alpha;
           }
           if (rescale || m_run == -INFINITY) m_run = m_new;
         }
         const float nb = m_run == -INFINITY ? 0.f : -m_run;
         const float2 sl2_2 = make_float2(sl2, sl2), nb_2 = make_float2(nb, nb);
-        float2 sm[4];
+        float2 sm[2], sn[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sm[k] = make_float2(0.f, 0.f);
+        for (int k = 0; k < 2; ++k) sm[k] = sn[k] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t pk[16];
@@ -684,13 +690,18 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
             float2 e = fma_f32x2(make_float2(v[32 * c + i], v[32 * c + i + 1]), sl2_2, nb_2);
             e.x = tr_exp2(e.x);
             e.y = tr_exp2(e.y);
-            sm[(i >> 1) & 3] = add_f32x2(sm[(i >> 1) & 3], e);
+            sm[(i >> 1) & 1] = add_f32x2(sm[(i >> 1) & 1], e);
             pk[i / 2] = pack_bf16x2(e.x, e.y);
+            if constexpr (NT == 1) sn[(i >> 1) & 1] = add_f32x2(sn[(i >> 1) & 1], unpack_bf16x2(pk[i / 2]));
           }
           tmem_st16_u32(s_tmem + 16 * c, pk);
         }
-        sm[0] = add_f32x2(add_f32x2(sm[0], sm[1]), add_f32x2(sm[2], sm[3]));
+        sm[0] = add_f32x2(sm[0], sm[1]);
         l_run += sm[0].x + sm[0].y;
+        if constexpr (NT == 1) {
+          sn[0] = add_f32x2(sn[0], sn[1]);
+          n_run += sn[0].x + sn[0].y;
+        }
         tmem_st_wait();
         if (masked && x == 0 && quads == 4) clean_v(j, t);
         tc_fence_before();
@@ -706,11 +717,17 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       tc_fence_after();
       // (the partner's read of the last maxima lies behind its P, hence behind O)
       float* pair_sum = reinterpret_cast<float*>(pair0);
+      // half 0 gets the row's l, both halves its n
+      if constexpr (NT == 2) n_run = l_run;
       if (half == 1) *pair_sum = l_run;
       named_barrier(pair_bar, 64);
-      if (half == 0) *pair_sum = l_run += *const_cast<volatile float*>(pair_sum);
+      if (half == 0) l_run += *const_cast<volatile float*>(pair_sum);
       named_barrier(pair_bar, 64);
-      l_run = *const_cast<volatile float*>(pair_sum);
+      if (half == 1) *pair_sum = n_run;
+      named_barrier(pair_bar, 64);
+      if (half == 0) *pair_sum = n_run += *const_cast<volatile float*>(pair_sum);
+      named_barrier(pair_bar, 64);
+      n_run = *const_cast<volatile float*>(pair_sum);
       named_barrier(pair_bar, 64);  // read: the next segment's maxima may go there
       if (!ok) continue;
       const int row = row_of(), tok = row / a.group;
@@ -720,7 +737,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
       const bool whole = sg.whole != 0;
       // any_bad is final: every P of the segment was waited for by its P.V
       const bool check_bad = *const_cast<volatile uint32_t*>(any_bad) != 0 && j1 * kTreeN > ctx;
-      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+      const float inv = n_run == 0.f ? 0.f : 1.f / n_run;
       const int slot = 2 * (int)blockIdx.x + (j0 > 0 ? 0 : 1);
       bf16* dst = a.out + (int64_t)(sg.q0 + tok) * a.out_stride_t + (int64_t)head * a.out_stride_h + half * (D / 2);
       float* pdst = a.part_o + ((int64_t)slot * C::kRows + x * kTreeM + m) * D + half * (D / 2);
@@ -768,9 +785,10 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
             a.lse[(int64_t)(sg.q0 + tok) * a.num_qo_heads + head] =
                 l_run == 0.f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
         } else {
-          float* ml = a.part_ml + (int64_t)slot * 2 * C::kRows + x * kTreeM + m;
+          float* ml = a.part_ml + (int64_t)slot * 3 * C::kRows + x * kTreeM + m;
           ml[0] = m_run;
           ml[C::kRows] = l_run;
+          ml[2 * C::kRows] = n_run;
         }
       }
       tc_fence_before();  // O was read: the next segment's first P.V (issued after its P arrives) may overwrite it
@@ -833,21 +851,23 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
   if (!found || nt <= a.min_split || head >= a.num_qo_heads || ca == cb) return;  // not split
   auto slot = [&](int c) { return (int64_t)(2 * c + (c == ca ? 1 : 0)); };
   constexpr int E = D / 32;
-  float acc[E], L = 0.f, M = -INFINITY;
+  float acc[E], L = 0.f, N = 0.f, M = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   for (int c0 = ca; c0 <= cb; c0 += 32) {
     // a lane per state: its maximum and sum; then all lanes add the states up
-    float mc = -INFINITY, lc = 0.f;
+    float mc = -INFINITY, lc = 0.f, nc = 0.f;
     if (c0 + lane <= cb) {
-      const float* ml = a.part_ml + slot(c0 + lane) * 2 * rows + m;
+      const float* ml = a.part_ml + slot(c0 + lane) * 3 * rows + m;
       mc = ml[0];
       lc = ml[rows];
+      nc = ml[2 * rows];
     }
     const float m_new = fmaxf(M, warp_max(mc));
     const float old = M == -INFINITY ? 0.f : exp2f(M - m_new);
     const float wt = mc == -INFINITY ? 0.f : exp2f(mc - m_new);
     L = L * old + warp_sum(mc == -INFINITY ? 0.f : wt * lc);
+    N = N * old + warp_sum(mc == -INFINITY ? 0.f : wt * nc);
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= old;
     M = m_new;
@@ -869,7 +889,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
       for (int e = 0; e < E; ++e) acc[e] += saw ? wi * v[e] : 0.f;
     }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const float inv = N == 0.f ? 0.f : 1.f / N;
   bf16* dst = a.out + (int64_t)tok_g * a.out_stride_t + (int64_t)head * a.out_stride_h + lane * E;
   if constexpr (E == 4) {
     *reinterpret_cast<uint2*>(dst) =
@@ -1037,7 +1057,7 @@ extern "C" int64_t pl_tree_workspace_bytes(int32_t batch, int32_t total_q, int32
     return 0;
   const int sms = pl_host::sm_count();
   const int64_t rows = pl::kTreeM * (tree_two_tiles(total_q, batch, num_qo_heads / num_kv_heads) ? 2 : 1);
-  return 2 * (int64_t)(sms > 0 ? sms : 148) * rows * (head_dim + 2) * 4;
+  return 2 * (int64_t)(sms > 0 ? sms : 148) * rows * (head_dim + 3) * 4;
 }
 
 extern "C" int32_t pl_paged_tree_attention(

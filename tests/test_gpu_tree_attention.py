@@ -438,3 +438,15 @@ def test_calls_without_entries(K):
     nxt = torch.zeros(2, dtype=torch.int64, device="cuda")
     K.tree_accept(none[:0], nxt[:0], nxt[:0], none, none[:2], keep=keep, keep_count=count, next_token=nxt, status=status)
     assert count.tolist() == [0, 0] and int(status.item()) == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_row_of_one_position_is_exact(K, d):
+    """Tokens without a context that see themselves alone: the output is their V, the LSE their score."""
+
+    n = 20
+    host, dev = _case([(n, 0), (1, 0)], 8, 2, d, 16, seed=5, see=[np.eye(n, dtype=bool), np.eye(1, dtype=bool)])
+    out, _ = _run(K, dev)
+    want, _, _ = o.tree_attention(host["q"], host["cache"], host["qo"], host["kv_indptr"], host["kv_indices"],
+                                  host["last"], host["see"])
+    assert (out == np.float64(np.float32(want))).all()
