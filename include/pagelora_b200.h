@@ -727,8 +727,10 @@ int32_t pl_linear_gemm_lora_precompute(int32_t num_tokens, int32_t k_in,
  *               beyond fp32 summation order, and is deterministic for a
  *               given value
  *   workspace   256-byte aligned, pl_linear_gemm_plan's workspace_bytes for
- *               the same num_ctas; its first 4 * ceil(n_out / 128) bytes
- *               are arrival counters: zero before the first call, left zero.
+ *               the same num_ctas; its first 4096 bytes (4 * num_ctas
+ *               where that is more) are arrival counters: zero before the
+ *               first call, left zero.  Calls of different shapes, each of
+ *               at most 1024 CTAs, may use one workspace in turn.
  *   flags       PL_FLAG_WEIGHTS_STATIC as for the GEMV; PL_FLAG_SILU_PAIRS:
  *               w is a gate/up stack interleaved in blocks of 64 rows (rows
  *               128j .. 128j+63 = gate rows 64j .. 64j+63, the next 64 = the

@@ -33,6 +33,13 @@ constexpr int kGemmM = 128;      // weight rows per tile (UMMA M)
 constexpr int kGemmKC = 64;      // K per chunk: one 128-byte swizzled row of bf16
 constexpr int kGemmThreads = 192;
 constexpr int kGemmIssue = 4;    // units per producer TMA instruction
+// Arrival tickets at the start of the workspace.  A shared tile's is that of
+// the first CTA that contributes to it: that CTA's range goes on in the next
+// CTA's, so the tile is its last and no other tile has the same one.  The
+// partials begin behind 1024 tickets whatever the shape, so that calls of
+// different shapes may follow one another in one workspace and none writes
+// partials over the tickets of another.
+constexpr int kGemmTickets = 1024;
 
 struct GemmArgs {
   GemvArgs e;          // epilogue fields: n_out, bias, LoRA, residual, y, status; T, K
@@ -41,7 +48,7 @@ struct GemmArgs {
   int32_t stages;
   int32_t max_slots;   // partial slots per tile
   float* partial;      // [m_tiles][max_slots][N][128] fp32
-  int32_t* counters;   // [m_tiles] arrival tickets, zero between calls
+  int32_t* counters;   // [ctas] arrival tickets of shared tiles, zero between calls
   int32_t lora_stage;  // bytes of shared memory holding the rank-16 LoRA down rows and adapter ids (0: none)
   int32_t lora_delta;  // bytes holding the precomputed LoRA terms of the CTA's last tile (0: none)
 };
@@ -384,7 +391,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         __threadfence();
         named_barrier(1, kEpiThreads);
         if (ew == 0 && lane == 0) {
-          const int32_t ticket = atomicAdd(&g.counters[t], 1);
+          const int32_t ticket = atomicAdd(&g.counters[c_first], 1);
           flags[1] = ticket == c_last - c_first ? 1 : 0;
         }
         named_barrier(1, kEpiThreads);
@@ -434,7 +441,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                                   (int64_t)t * kGemmM);
             }
           }
-          if (ew == 0 && lane == 0) g.counters[t] = 0;
+          if (ew == 0 && lane == 0) g.counters[c_first] = 0;
         }
         named_barrier(1, kEpiThreads);  // flags[1] is reused by the next segment
       }
@@ -656,8 +663,13 @@ GemmShape gemm_shape(int tokens, int k_in, int n_out, int ctas, bool allow_3d) {
   return s;
 }
 
+// Bytes of the arrival tickets, in front of the partials.
+int64_t gemm_ticket_bytes(const GemmShape& s) {
+  return align256(4 * (int64_t)(s.ctas > pl::kGemmTickets ? s.ctas : pl::kGemmTickets));
+}
+
 int64_t gemm_workspace_bytes(const GemmShape& s) {
-  int64_t b = align256((int64_t)s.m_tiles * 4);
+  int64_t b = gemm_ticket_bytes(s);
   if (s.max_slots > 1) b += (int64_t)s.m_tiles * s.max_slots * s.n * pl::kGemmM * 4;
   return b;
 }
@@ -801,7 +813,7 @@ extern "C" int32_t pl_linear_lora_gemm(const void* x, int64_t x_stride, int32_t 
   g.max_slots = sh.max_slots;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   g.counters = reinterpret_cast<int32_t*>(ws);
-  g.partial = sh.max_slots > 1 ? reinterpret_cast<float*>(ws + align256((int64_t)sh.m_tiles * 4)) : nullptr;
+  g.partial = sh.max_slots > 1 ? reinterpret_cast<float*>(ws + gemm_ticket_bytes(sh)) : nullptr;
   // Rank-16 LoRA: stage the (small) down rows and adapter ids in shared
   // memory so the epilogue reads them once per CTA instead of per element.
   if (lora_b != nullptr)
