@@ -33,6 +33,7 @@
 // tokens 209 -> 225 us, the 8 above 745 -> 880).
 // The maximum that p and the sums are relative to may lag by 2^8, so O is
 // rescaled in TMEM only when a row's maximum grows past that, which is rare.
+// It lies within 2 of a maximum whatever the scores' size (kTreeNearMax).
 // Waits are bounded: on expiry the kernel records PL_ERR_TIMEOUT, drains its
 // copies and returns.
 //
@@ -50,6 +51,17 @@ namespace pl {
 constexpr int kTreeM = 128;              // rows of one tile
 constexpr int kTreeN = 128;              // positions of one K/V tile
 constexpr float kTreeSlack = 8.0f;       // log2 growth of a row's maximum that is tolerated before O is rescaled
+// The two threads of a row tell each other their maxima in bf16, one word in
+// all, which shared memory has room for.  Below this size that is off by at
+// most 2; from here on the row takes the fp32 maxima, in three more barriers.
+constexpr float kTreeNearMax = 1024.0f;
+// From this size on the fp32 product score * scale is itself off by more than
+// 2 from the exact one that a fused multiply-add takes: the scores are scaled
+// before the maximum is subtracted, so that the highest gives p = 1.
+constexpr float kTreeScaledMax = 67108864.0f;
+// What a warp that gave up tells in place of its maximum (a NaN that no
+// rounding gives): its partner does not go on to the fp32 exchange.
+constexpr uint16_t kTreeGaveUp = 0xffff;
 // Places on the line that an item takes beside its tiles: its look-up, first
 // scores, masked tiles and epilogue take a CTA about 6300 cycles, a tile 2340.
 // us with 0, 1, 2, 3, 4 places: 12 requests of 5-33 tokens at 300-4100
@@ -512,8 +524,9 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
     // Per row tile two groups of four warps; group `half` has the positions
     // 64 half .. 64 half + 63 of every K/V tile, so a row's two threads share
     // its running maximum (through shared memory) and keep a sum each.  A
-    // warp whose wait ran out does no further work but still meets its named
-    // barriers, so that no other warp is left in one.
+    // warp whose wait ran out does no further work but still meets the one
+    // named barrier of every tile and says so there (kTreeGaveUp), so that no
+    // other warp is left in one.
     const int x = warp / 8;
     const int half = (warp / 4) & 1;
     const int quad = warp & 3;
@@ -614,6 +627,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           continue;
         }
         if (!ok) {
+          pair_max[half] = __ushort_as_bfloat16(kTreeGaveUp);
           named_barrier(pair_bar, 64);
           continue;
         }
@@ -650,12 +664,33 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
 #pragma unroll
         for (int i = 8; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
         // both threads of the row take the larger of the two maxima, as
-        // rounded to bf16 (any common reference near the maximum serves)
+        // rounded to bf16: a common reference within 2 of the maximum serves
         const bf16 mine = f2bf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
         pair_max[half] = mine;
         named_barrier(pair_bar, 64);
-        const float tmax = fmaxf(bf2f(mine), bf2f(*const_cast<volatile bf16*>(&pair_max[half ^ 1])));
-        if (__any_sync(0xffffffffu, tmax > m_run + kTreeSlack || m_run == -INFINITY)) {
+        const uint16_t theirs = *reinterpret_cast<volatile uint16_t*>(&pair_max[half ^ 1]);
+        float tmax = theirs == kTreeGaveUp ? -INFINITY : fmaxf(bf2f(mine), bf2f(__ushort_as_bfloat16(theirs)));
+        float sl = sl2;
+        // (the votes of a row's two warps agree: tmax and m_run are the same)
+        if (__any_sync(0xffffffffu, tmax > m_run + kTreeSlack || m_run == -INFINITY || fabsf(tmax) >= kTreeNearMax)) {
+          if (__any_sync(0xffffffffu, fabsf(tmax) >= kTreeNearMax && tmax != -INFINITY)) {
+            volatile float* word = reinterpret_cast<float*>(pair_max);
+            float top = v[0];
+#pragma unroll
+            for (int i = 1; i < 64; ++i) top = fmaxf(top, v[i]);
+            top *= sl2;
+            named_barrier(pair_bar, 64);  // both have read the rounded maxima
+            if (half == 1) *word = top;
+            named_barrier(pair_bar, 64);
+            if (half == 0) *word = tmax = fmaxf(top, *word);
+            named_barrier(pair_bar, 64);
+            if (half == 1) tmax = *word;
+            if (__any_sync(0xffffffffu, fabsf(tmax) >= kTreeScaledMax && tmax != -INFINITY)) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) v[i] *= sl2;
+              sl = 1.f;
+            }
+          }
           const float m_new = fmaxf(m_run, tmax);
           const bool rescale = m_run != -INFINITY && m_new > m_run + kTreeSlack;
           const float alpha = rescale ? tr_exp2(m_run - m_new) : 1.f;
@@ -678,7 +713,7 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
           if (rescale || m_run == -INFINITY) m_run = m_new;
         }
         const float nb = m_run == -INFINITY ? 0.f : -m_run;
-        const float2 sl2_2 = make_float2(sl2, sl2), nb_2 = make_float2(nb, nb);
+        const float2 sl2_2 = make_float2(sl, sl), nb_2 = make_float2(nb, nb);
         float2 sm[2], sn[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) sm[k] = sn[k] = make_float2(0.f, 0.f);
