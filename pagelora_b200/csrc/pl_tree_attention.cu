@@ -848,7 +848,9 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
 }
 
 // Joins the partial states of the items that several CTAs shared: one warp
-// per (query token, head), the states weighted by 2^(m - max m).  The tables
+// per (query token, head), the states weighted by 2^(m - max m).  A state that
+// saw nothing has the sum 0 and is left out; one whose scores are all NaN also
+// has no maximum (m = -inf), but a sum of NaN, which reaches the row.  The tables
 // are read before the wait for the attention's grid (which lets this one
 // start only once they are complete).
 constexpr int kMergeThreads = 128;
@@ -900,9 +902,10 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
     }
     const float m_new = fmaxf(M, warp_max(mc));
     const float old = M == -INFINITY ? 0.f : exp2f(M - m_new);
-    const float wt = mc == -INFINITY ? 0.f : exp2f(mc - m_new);
-    L = L * old + warp_sum(mc == -INFINITY ? 0.f : wt * lc);
-    N = N * old + warp_sum(mc == -INFINITY ? 0.f : wt * nc);
+    const bool any = lc != 0.f;
+    const float wt = mc == -INFINITY ? 1.f : exp2f(mc - m_new);
+    L = L * old + warp_sum(any ? wt * lc : 0.f);
+    N = N * old + warp_sum(any ? wt * nc : 0.f);
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= old;
     M = m_new;
@@ -919,7 +922,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
         v[0] = f.x; v[1] = f.y;
       }
       const float wi = __shfl_sync(0xffffffffu, wt, i);
-      const bool saw = __shfl_sync(0xffffffffu, mc, i) != -INFINITY;  // else the state holds no values
+      const bool saw = __shfl_sync(0xffffffffu, any ? 1 : 0, i) != 0;  // else the state holds no values
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] += saw ? wi * v[e] : 0.f;
     }
