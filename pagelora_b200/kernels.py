@@ -829,7 +829,12 @@ def _need_rows(t: torch.Tensor, name: str, rows: int, dtype: torch.dtype = torch
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.dim() != 2 or t.shape[0] < rows or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"{name} must be [{rows}, width] with contiguous rows")
-    return max(t.stride(0), t.shape[1]), t.shape[1]
+    stride, width = t.stride(0), t.shape[1]
+    if stride < width:
+        if t.shape[0] > 1:  # an expanded tensor has fewer entries than the kernel would touch
+            raise ValueError(f"{name} must have rows of its own (row stride {stride}, width {width})")
+        stride = width
+    return stride, width
 
 
 def tree_mask(parents: torch.Tensor, qo_indptr: torch.Tensor, words: int, *, base_positions: torch.Tensor | None = None,
