@@ -818,7 +818,11 @@ def _vecs(dtype: torch.dtype, names: str, tensors: tuple, sizes: tuple) -> None:
 
 
 def _workspace(workspace: torch.Tensor | None, need: int, like: torch.Tensor) -> torch.Tensor:
-    return like.new_empty(need if need > 16 else 16, dtype=torch.uint8) if workspace is None else workspace
+    if workspace is None:
+        return like.new_empty(need if need > 16 else 16, dtype=torch.uint8)
+    if not workspace.is_contiguous():  # its size is taken from its entries
+        raise ValueError("workspace must be contiguous")
+    return workspace
 
 
 def _need_rows(t: torch.Tensor, name: str, rows: int, dtype: torch.dtype = torch.int32) -> tuple[int, int]:
@@ -1119,8 +1123,8 @@ def paged_sparse_decode(
         raise ValueError("out must have q's shape and unit last stride")
     if max_pages is None:
         max_pages = indices.numel()
-    if max_pages > num_select and workspace is None:
-        workspace = _workspace(None, _sparse_workspace_bytes(batch, hkv, max_pages), q)
+    if max_pages > num_select:
+        workspace = _workspace(workspace, _sparse_workspace_bytes(batch, hkv, max_pages), q)
     q_b, q_h, _ = q.stride()
     o_b, o_h, _ = out.stride()
     call("pl_paged_sparse_decode", q.data_ptr(), q_b, q_h, kv_cache.data_ptr(), num_pages, indptr.data_ptr(),

@@ -59,3 +59,15 @@ def test_calls_with_overlapping_rows(cuda_device):
     tables = torch.zeros(4, **i32), torch.zeros(2, 3, **i32), torch.zeros(2, **i32), torch.zeros(2, **i32)
     with pytest.raises(ValueError):
         K.cache_compact(pool, *tables, torch.zeros(2, **i32), row.expand(2, 3), torch.zeros(2, **i32))
+
+
+def test_workspaces_that_are_not_contiguous():
+    """A workspace's size is that of its entries, which a view may share."""
+
+    from pagelora_b200.kernels import _workspace
+
+    ws = torch.empty(64, dtype=torch.uint8)
+    assert _workspace(ws, 16, ws) is ws and _workspace(None, 99, ws).numel() == 99
+    for view in (ws[:1].expand(1 << 20), ws[::2], ws.view(8, 8).t()):
+        with pytest.raises(ValueError, match="contiguous"):
+            _workspace(view, 16, ws)
