@@ -964,7 +964,9 @@ int32_t pl_tree_accept(const int32_t *parents, const int64_t *tokens,
  * slot_page / slot_offset [total_tokens] and, when given, whose positions in
  * the row go to positions_out.  out_indptr [num_rows+1] / out_indices
  * [max_indices] (nullable) receive the new page table.  A row's partial last
- * page has to be its own (PL_ERR_PAGE_SHARED).
+ * page has to be its own (PL_ERR_PAGE_SHARED).  A refused call fills
+ * slot_page and slot_offset with -1, which pl_kv_append and
+ * pl_qkv_rope_append reject, and positions_out with 0.
  *
  * pl_page_fork: row dst_rows[i] (empty, listed once) becomes a copy of
  * src_rows[i]: full pages are shared, a partial last page is copied (its

@@ -307,7 +307,13 @@ __global__ void __launch_bounds__(kPoolThreads, 1)
     p.refcount[page] = 1;
   });
   if (!enough && threadIdx.x == 0) set_status(p.status, PL_ERR_POOL_EXHAUSTED);
-  if (refused || !enough) return;
+  if (refused || !enough) {  // no slots: the appends that follow reject these, whatever the buffers held
+    for (int64_t i = rank * kPoolThreads + (int)threadIdx.x; i < total; i += CTAS * kPoolThreads) {
+      slot_page[i] = slot_off[i] = -1;
+      if (positions != nullptr) positions[i] = 0;
+    }
+    return;
+  }
   // slots of the new tokens and the page table, rows dealt over the warps
   const int lane = threadIdx.x & 31;
   for (int r = rank * kPoolWarps + (threadIdx.x >> 5); r < p.rows; r += CTAS * kPoolWarps) {
@@ -712,7 +718,7 @@ extern "C" int32_t pl_page_reserve(int32_t *refcount, int64_t num_pages, int32_t
   if (tok_indptr == nullptr || total_tokens < 0 || max_indices < 0 ||
       (total_tokens > 0 && (slot_page == nullptr || slot_offset == nullptr)))
     return PL_ERR_INVALID_ARGUMENT;
-  if (num_rows == 0) return PL_OK;
+  if (num_rows == 0) return total_tokens == 0 ? PL_OK : PL_ERR_INVALID_ARGUMENT;
   return launch_pool(pl::page_reserve_kernel<1>, pl::page_reserve_kernel<pl::kPoolCtas>, p, stream, tok_indptr,
                      (int)total_tokens, slot_page, slot_offset, positions_out, out_indptr, out_indices, max_indices);
 }

@@ -1007,8 +1007,9 @@ def page_reserve(refcount: torch.Tensor, row_pages: torch.Tensor, row_num_pages:
                  out_indptr: torch.Tensor | None = None, out_indices: torch.Tensor | None = None,
                  status: torch.Tensor | None = None) -> None:
     """Row r grows by tok_indptr[r+1] - tok_indptr[r] tokens (pl_page_reserve):
-    their slots go to ``slot_page`` / ``slot_offset`` (one entry per token), the
-    new page table to ``out_indptr`` / ``out_indices`` when given."""
+    their slots go to ``slot_page`` / ``slot_offset`` (one entry per token; -1
+    when the call is refused), the new page table to ``out_indptr`` /
+    ``out_indices`` when given."""
 
     tables = _pool_tables(refcount, row_pages, row_num_pages, last_page_len)
     rows, total = tables[5], slot_page.numel()
