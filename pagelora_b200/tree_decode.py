@@ -11,7 +11,8 @@ bookkeeping on the device.  One verification step of drafted trees is
     move together, the rest of the drafts' pages go back to the pool)
 
 with no host synchronisation; rows fork and end with :meth:`fork` and
-:meth:`release`.  With ``sparse`` the decoder also keeps the int8 key bounds of
+:meth:`release`.  What the device refuses (a row or the pool without room) changes
+no row and accepts no token; :meth:`check` says why.  With ``sparse`` the decoder also keeps the int8 key bounds of
 every page, and :meth:`step_sparse` decodes one token per row over the pages
 that their score selects.  No reference counterpart: the reference decodes one
 token per row and step (model/flashinfer/generation.py:188-247).
@@ -40,7 +41,9 @@ class SparsePages:
 
 @dataclass
 class TreeStep:
-    """Result of :meth:`TreeDecoder.verify` (device tensors)."""
+    """Result of :meth:`TreeDecoder.verify` (device tensors).  A step that was
+    refused keeps nothing: keep -1, keep_count 0, next_token -1, and targets and
+    logits without meaning."""
 
     targets: torch.Tensor     # int64 [tokens]: the model's choice after each drafted token
     keep: torch.Tensor        # int32 [rows, max]: positions of the accepted path, then -1
@@ -69,6 +72,7 @@ class TreeDecoder:
         self.lens = torch.tensor(engine.context_len, dtype=torch.int32, device=dev)
         self.indptr = torch.zeros(self.rows + 1, dtype=torch.int32, device=dev)
         self.indices = torch.zeros(self.rows * self.cap, dtype=torch.int32, device=dev)
+        self._none = torch.zeros(self.rows, dtype=torch.int32, device=dev)
         self.one_each = torch.arange(self.rows + 1, dtype=torch.int32, device=dev)
         self._gemm_ws: dict[int, torch.Tensor] = {}
         self.sparse = sparse
@@ -152,6 +156,11 @@ class TreeDecoder:
                        out_indices=self.indices, status=self.status)
         return slot_page, slot_off, positions
 
+    def _row_lens(self) -> torch.Tensor:
+        """Cached tokens of every row, from its pages."""
+
+        return ((self.num - 1) * self.e.page_size + self.last).clamp_(min=0)
+
     # --------------------------------------------------------------- steps
     @torch.no_grad()
     def verify(self, tokens: torch.Tensor, parents: torch.Tensor, qo_indptr: torch.Tensor, max_tokens: int) -> TreeStep:
@@ -179,8 +188,16 @@ class TreeDecoder:
         nxt = torch.empty(self.rows, dtype=torch.int64, device=tokens.device)
         K.tree_accept(parents, tokens, targets, qo_indptr, self.lens, keep=keep, keep_count=count, next_token=nxt,
                       status=self.status)
-        K.cache_compact(self.e.kv, self.refcount, self.table, self.num, self.last, self.lens, keep, count,
-                        status=self.status)
+        tables = (self.e.kv, self.refcount, self.table, self.num, self.last)
+        K.cache_compact(*tables, self.lens, keep, count, status=self.status)
+        # A refused reservation or compaction left the rows as they were before
+        # it: the step keeps nothing, and the drafts' pages are given back.
+        # (Cutting rows to the length that they have changes nothing.)
+        done = (self._row_lens() == self.lens + count).all()
+        count.mul_(done)
+        keep.masked_fill_(~done, -1)
+        nxt.masked_fill_(~done, -1)
+        K.cache_compact(*tables, self.lens + count, keep, self._none, status=self.status)
         if self.sparse is not None:
             self._refresh_bounds(self.lens // self.e.page_size, (max_tokens - 1) // self.e.page_size + 2)
         self.lens.add_(count)
@@ -189,7 +206,7 @@ class TreeDecoder:
     @torch.no_grad()
     def step_sparse(self, tokens: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """One token per row (int64 [rows]) over the selected pages; returns
-        (next tokens, logits)."""
+        (next tokens, logits).  A step that was refused returns -1 for every row."""
 
         if self.sparse is None:
             raise ValueError("the decoder was built without a page budget (sparse)")
@@ -207,8 +224,10 @@ class TreeDecoder:
 
         logits = self._forward(tokens, positions, torch.arange(self.rows, device=tokens.device), slot_page, slot_off,
                                attend)
-        self.lens.add_(1)
-        return K.argmax(logits, torch.empty_like(tokens)), logits
+        lens = self._row_lens()
+        grown = (lens != self.lens).any()  # the reservation is for all rows or for none
+        self.lens.copy_(lens)
+        return K.argmax(logits, torch.empty_like(tokens)).masked_fill_(~grown, -1), logits
 
     # ---------------------------------------------------------------- rows
     def fork(self, src: list[int], dst: list[int]) -> None:
@@ -218,7 +237,7 @@ class TreeDecoder:
             raise ValueError("a row forks into a row with the same adapter")
         s, d = (torch.tensor(r, dtype=torch.int32, device=self.lens.device) for r in (src, dst))
         K.page_fork(self.e.kv, self.refcount, self.table, self.num, self.last, s, d, status=self.status)
-        self.lens[d.long()] = self.lens[s.long()]
+        self.lens.copy_(self._row_lens())
         if self.sparse is not None:  # the copied last pages
             self._refresh_bounds((self.num - 1).clamp(min=0), 1)
 
@@ -227,12 +246,16 @@ class TreeDecoder:
 
         r = torch.tensor(rows, dtype=torch.int32, device=self.lens.device)
         K.page_release(self.refcount, self.table, self.num, self.last, r, status=self.status)
-        self.lens[r.long()] = 0
+        self.lens.copy_(self._row_lens())
 
     def check(self) -> None:
-        """Raises when a step reported a device status."""
+        """Raises when a step reported a device status (the first one since the
+        last call, which this one clears)."""
 
-        self.e._check_status()
+        try:
+            self.e._check_status()
+        finally:
+            self.status.zero_()
 
     def _refresh_bounds(self, first: torch.Tensor, most: int) -> None:
         """Bounds of the pages first[r] .. of every row (at most ``most``)."""
