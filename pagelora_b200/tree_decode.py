@@ -73,7 +73,9 @@ class TreeDecoder:
         self.indptr = torch.zeros(self.rows + 1, dtype=torch.int32, device=dev)
         self.indices = torch.zeros(self.rows * self.cap, dtype=torch.int32, device=dev)
         self._none = torch.zeros(self.rows, dtype=torch.int32, device=dev)
-        self.one_each = torch.arange(self.rows + 1, dtype=torch.int32, device=dev)
+        # the rows that step_sparse advances: (row ids, their slots' indptr); None: not known
+        self._live = None
+        self._ended = 0 in engine.context_len  # some row may be without a context
         self._gemm_ws: dict[int, torch.Tensor] = {}
         self.sparse = sparse
         if sparse is not None:
@@ -169,6 +171,8 @@ class TreeDecoder:
         r's tree at qo_indptr[r]:qo_indptr[r+1], at most ``max_tokens`` each;
         a row without tokens stays as it is."""
 
+        if self._ended:  # a draft may begin an empty row
+            self._live = None
         total = tokens.numel()
         tok_row = torch.searchsorted(qo_indptr[1:], torch.arange(total, device=tokens.device, dtype=torch.int32),
                                      right=True)
@@ -203,14 +207,39 @@ class TreeDecoder:
         self.lens.add_(count)
         return TreeStep(targets, keep, count, nxt, logits)
 
+    def _live_rows(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """The rows that hold a context, ascending, and the indptr of one token
+        each.  Waits for the device when rows may have ended or begun since."""
+
+        if self._live is None:
+            dev = self.lens.device
+            live = torch.ones(self.rows, dtype=torch.int32)
+            if self._ended:
+                live = (self.num > 0).to("cpu", torch.int32)
+                self._ended = not live.all()
+            indptr = torch.cat([live.new_zeros(1), live.cumsum(0, dtype=torch.int32)])
+            self._live = live.nonzero().flatten().to(dev), indptr.to(dev)
+        return self._live
+
     @torch.no_grad()
     def step_sparse(self, tokens: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """One token per row (int64 [rows]) over the selected pages; returns
-        (next tokens, logits).  A step that was refused returns -1 for every row."""
+        (next tokens [rows], logits [rows, vocab]).  Rows without a context take
+        no part: their next token is -1 and their logits are 0.  A step that was
+        refused returns -1 for every row."""
 
         if self.sparse is None:
             raise ValueError("the decoder was built without a page budget (sparse)")
-        slot_page, slot_off, positions = self._reserve(self.one_each, self.rows)
+        rows, tok_indptr = self._live_rows()
+        n, some = rows.numel(), rows.numel() < self.rows
+        nxt = torch.full((self.rows,), -1, dtype=torch.int64, device=rows.device)
+        if n == 0:
+            return nxt, torch.zeros(self.rows, self.e.lm_head.shape[0], dtype=torch.bfloat16, device=rows.device)
+        slot_page, slot_off, positions = self._reserve(tok_indptr, n)
+        indptr, last = self.indptr, self.last
+        if some:  # (rows without a context have no pages between those of the others)
+            tokens, last = tokens[rows], last[rows]
+            indptr = torch.cat([indptr[rows], indptr[-1:]])
         sp = self.sparse
 
         def attend(li, q):
@@ -218,16 +247,19 @@ class TreeDecoder:
             # the page that takes the token is among the recent ones, whose
             # bounds are not read; they are kept current for when it is not
             K.page_bounds(kv, slot_page, bounds, scale, page_len=slot_off + 1, status=self.status)
-            return K.paged_sparse_decode(q, kv, self.indptr, self.indices, self.last, bounds, scale,
-                                         num_select=sp.select, sink_pages=sp.sink, recent_pages=sp.recent,
-                                         max_pages=self.cap, status=self.status)
+            return K.paged_sparse_decode(q, kv, indptr, self.indices, last, bounds, scale, num_select=sp.select,
+                                         sink_pages=sp.sink, recent_pages=sp.recent, max_pages=self.cap,
+                                         status=self.status)
 
-        logits = self._forward(tokens, positions, torch.arange(self.rows, device=tokens.device), slot_page, slot_off,
-                               attend)
+        logits = self._forward(tokens, positions, rows, slot_page, slot_off, attend)
         lens = self._row_lens()
         grown = (lens != self.lens).any()  # the reservation is for all rows or for none
         self.lens.copy_(lens)
-        return K.argmax(logits, torch.empty_like(tokens)).masked_fill_(~grown, -1), logits
+        nxt[rows] = K.argmax(logits, torch.empty_like(tokens))
+        nxt.masked_fill_(~grown, -1)
+        if some:
+            logits = logits.new_zeros(self.rows, logits.shape[1]).index_copy_(0, rows, logits)
+        return nxt, logits
 
     # ---------------------------------------------------------------- rows
     def fork(self, src: list[int], dst: list[int]) -> None:
@@ -235,6 +267,7 @@ class TreeDecoder:
 
         if any(self.e.row_adapter[a] != self.e.row_adapter[b] for a, b in zip(src, dst)):
             raise ValueError("a row forks into a row with the same adapter")
+        self._live = None
         s, d = (torch.tensor(r, dtype=torch.int32, device=self.lens.device) for r in (src, dst))
         K.page_fork(self.e.kv, self.refcount, self.table, self.num, self.last, s, d, status=self.status)
         self.lens.copy_(self._row_lens())
@@ -242,8 +275,10 @@ class TreeDecoder:
             self._refresh_bounds((self.num - 1).clamp(min=0), 1)
 
     def release(self, rows: list[int]) -> None:
-        """The rows end: their pages go back to the pool."""
+        """The rows end: their pages go back to the pool, and they stay empty
+        until a fork or a draft begins them anew."""
 
+        self._live, self._ended = None, True
         r = torch.tensor(rows, dtype=torch.int32, device=self.lens.device)
         K.page_release(self.refcount, self.table, self.num, self.last, r, status=self.status)
         self.lens.copy_(self._row_lens())
