@@ -1035,7 +1035,8 @@ int32_t pl_cache_compact(void *pool, int64_t layer_stride_bytes,
  * s), within +-127, and bound_scale[page][head] = s.  A page with an inf or
  * NaN key gets bounds 0 and scale +inf.  bounds int8 [num_pages][num_kv_heads]
  * [2][head_dim] (16-byte aligned), bound_scale fp32 [num_pages][num_kv_heads];
- * only the listed pages are written.  head_dim 64 or 128.  No reference
+ * only the listed pages are written.  An entry of page -1 and length 0 is left
+ * out, so that a list may keep its size.  head_dim 64 or 128.  No reference
  * counterpart.
  */
 int32_t pl_page_bounds(const void *kv_cache, int64_t num_pages,

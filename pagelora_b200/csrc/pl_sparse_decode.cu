@@ -48,7 +48,6 @@ __global__ void __launch_bounds__(kBoundsThreads, 8)
   const int i = live ? (int)(unit / hkv) : 0, h = live ? (int)(unit % hkv) : 0;
   const int pg = page_ids[i];
   const bool ok = live && pg >= 0 && pg < num_pages;
-  if (live && !ok) set_status(status, PL_ERR_PAGE_OUT_OF_RANGE);
   int len = page_size;
   if (page_len != nullptr && live) {
     len = page_len[i];
@@ -57,6 +56,7 @@ __global__ void __launch_bounds__(kBoundsThreads, 8)
       len = len < 0 ? 0 : page_size;
     }
   }
+  if (live && !ok && !(pg == -1 && len == 0)) set_status(status, PL_ERR_PAGE_OUT_OF_RANGE);
   float lo[8], hi[8];
   bool finite = true;
 #pragma unroll

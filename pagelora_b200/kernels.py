@@ -1062,7 +1062,8 @@ def cache_compact(pool: torch.Tensor, refcount: torch.Tensor, row_pages: torch.T
 def page_bounds(kv_cache: torch.Tensor, page_ids: torch.Tensor, bounds: torch.Tensor, bound_scale: torch.Tensor, *,
                 page_len: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
     """int8 bounds [pages, Hkv, 2, D] and scale [pages, Hkv] of the keys of
-    pages ``page_ids`` (pl_page_bounds); ``page_len``: tokens in each (all)."""
+    pages ``page_ids`` (pl_page_bounds); ``page_len``: tokens in each (all).
+    Entries of page -1 and length 0 are left out."""
 
     _need_cuda(kv_cache)
     _need_pool(kv_cache)

@@ -299,8 +299,8 @@ class TreeDecoder:
         at = torch.minimum(at, (self.num - 1).clamp(min=0)[:, None])
         ids = torch.gather(self.table, 1, at.long())
         length = torch.where(at == self.num[:, None] - 1, self.last[:, None], self.e.page_size)
-        live = (self.num > 0)[:, None].expand_as(ids)
-        ids, length = ids[live].contiguous(), length[live].contiguous()
+        live = (self.num > 0)[:, None]  # rows without pages: entries that page_bounds leaves out
+        ids, length = torch.where(live, ids, -1), torch.where(live, length, 0)
         for li in range(self.e.kv.shape[0]):
             K.page_bounds(self.e.kv[li], ids, self.bounds[li], self.bound_scale[li], page_len=length,
                           status=self.status)
