@@ -882,7 +882,8 @@ int32_t pl_argmax(const void *logits, int64_t stride, int32_t vocab,
  * Supported: head_dim 64 or 128, page_size 16 / 32 / 64 / 128, any group up
  * to 128.  A request with n_b > its cached tokens or > 32 * mask_words, or
  * with a table outside kv_indices, writes PL_ERR_INVALID_ARGUMENT to
- * *status_dev.
+ * *status_dev.  A call of more than 2^30 pairs of 128 or 256 query rows of a
+ * kv head and 128 positions writes PL_ERR_UNSUPPORTED and no output.
  */
 int64_t pl_tree_workspace_bytes(int32_t batch, int32_t total_q,
                                 int32_t num_qo_heads, int32_t num_kv_heads,

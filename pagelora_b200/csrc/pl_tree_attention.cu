@@ -69,6 +69,8 @@ constexpr uint16_t kTreeGaveUp = 0xffff;
 // tokens at 100-9000, 8 kv heads 184, 154, 158, 145, 143-159; 24 of 40-90
 // tokens 337, 308, 278, 251, 245; requests of equal length do not change.
 constexpr int kTreeItemCost = 3;
+// Places of the line: positions on it, and sums of two, are 32-bit.
+constexpr int64_t kTreeMostPlaces = 1 << 30;
 constexpr int kTreeMaxTokens = 1024;     // drafted tokens of one request (tree_mask / tree_accept)
 
 struct TreeArgs {
@@ -155,10 +157,12 @@ struct TreeReq {
     const int q1 = a.qo_indptr[b + 1];
     const bool ok = q0 >= 0 && q1 >= q0 && q1 <= a.total_q;
     n = ok ? q1 - q0 : 0;
-    // a table that leaves [0, total_pages) counts as empty (and is reported)
+    // a table that leaves [0, total_pages), or has 2^31 positions, counts as
+    // empty (and is reported)
     kv_begin = a.kv_indptr[b];
     const int kv_end = a.kv_indptr[b + 1];
     n_pages = kv_begin >= 0 && kv_end >= kv_begin && kv_end <= a.total_pages ? kv_end - kv_begin : 0;
+    if ((int64_t)n_pages * a.page_size > 0x7FFFFFFF) n_pages = 0;
     int last = a.kv_last[b];
     last = last < 0 ? 0 : (last > a.page_size ? a.page_size : last);
     kv_len = n_pages > 0 ? (n_pages - 1) * a.page_size + last : 0;
@@ -167,8 +171,9 @@ struct TreeReq {
   }
   // length of an item on the line: its tiles and what it costs besides
   __device__ __forceinline__ int span() const { return ntiles + kTreeItemCost; }
-  // of the request (the host bounds the total of all requests)
+  // of the request (kTreeMostPlaces bounds the total of all requests)
   __device__ __forceinline__ int work(int hkv) const { return rts * hkv * span(); }
+  __device__ __forceinline__ int64_t work64(int hkv) const { return (int64_t)rts * hkv * span(); }
 };
 
 // Inclusive prefix sum over a warp.
@@ -182,17 +187,25 @@ __device__ __forceinline__ int tree_scan(int v) {
   return v;
 }
 
-// Length of the line (one warp).
+__device__ __forceinline__ int64_t tree_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, (long long)v, o);
+  return v;
+}
+
+// Length of the line (one warp), 0 when it has more than kTreeMostPlaces (more
+// than hours of work, or a qo_indptr that goes back and names tokens often).
 __device__ __forceinline__ int tree_total(const TreeArgs& a, int rows) {
-  int t = 0;
+  int64_t t = 0;
   for (int b = threadIdx.x & 31; b < a.batch; b += 32) {
     TreeReq r;
     r.load(a, b, rows);
-    t += r.work(a.num_kv_heads);
+    t += r.work64(a.num_kv_heads);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  return t;
+  t = tree_sum64(t);
+  if (t <= kTreeMostPlaces) return (int)t;
+  if (blockIdx.x == 0) set_status(a.status, PL_ERR_UNSUPPORTED);
+  return 0;
 }
 
 // Its part of a CTA.
@@ -860,10 +873,11 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
   const int tok_g = blockIdx.x;
   // the request of this token, where it begins on the line, and the line's length
   int q0 = 0, rts = 0, nt = 0, base = 0, total = 0;
+  int64_t places = 0;
   bool found = false;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     TreeReq r;
-    r.n = r.rts = r.ntiles = r.q0 = 0;
+    r.n = r.rts = r.ntiles = r.q0 = 0;  // lanes past the batch
     if (b0 + lane < a.batch) r.load(a, b0 + lane, rows);
     const int w = r.work(a.num_kv_heads), inc = total + tree_scan(w);
     const uint32_t hit = __ballot_sync(0xffffffffu, r.q0 <= tok_g && tok_g < r.q0 + r.n);
@@ -876,7 +890,9 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
       base = __shfl_sync(0xffffffffu, inc - w, l);
     }
     total = __shfl_sync(0xffffffffu, inc, 31);
+    places += tree_sum64(r.work64(a.num_kv_heads));
   }
+  if (places > kTreeMostPlaces) found = false;  // refused: there is nothing to join
   const int share = tree_share(total, a.ctas);
   const int head = blockIdx.y * (kMergeThreads / 32) + threadIdx.x / 32;
   const int row = (tok_g - q0) * a.group + head % a.group;
@@ -1134,9 +1150,6 @@ extern "C" int32_t pl_paged_tree_attention(
   if (sms <= 0) return PL_ERR_NO_DEVICE;
 
   const bool two = tree_two_tiles(total_q, batch, group);
-  // the line of tiles is indexed in 32 bits; an upper bound of its length
-  const int64_t most_rts = (int64_t)total_q * group / pl::kTreeM + batch;
-  if (most_rts * num_kv_heads > 0x7FFFFFFFll / (total_pages * page_size / pl::kTreeN + 1 + pl::kTreeItemCost)) return PL_ERR_UNSUPPORTED;
   pl::TreeArgs a;
   a.q = static_cast<const pl::bf16*>(q);
   a.kv = static_cast<const pl::bf16*>(kv_cache);
