@@ -682,11 +682,12 @@ __global__ void __launch_bounds__(TreeCfg<D, NT>::kThreads, 1)
         pair_max[half] = mine;
         named_barrier(pair_bar, 64);
         const uint16_t theirs = *reinterpret_cast<volatile uint16_t*>(&pair_max[half ^ 1]);
-        float tmax = theirs == kTreeGaveUp ? -INFINITY : fmaxf(bf2f(mine), bf2f(__ushort_as_bfloat16(theirs)));
+        float tmax = fmaxf(bf2f(mine), bf2f(__ushort_as_bfloat16(theirs)));
         float sl = sl2;
+        const bool large = fabsf(tmax) >= kTreeNearMax && tmax != -INFINITY && theirs != kTreeGaveUp;
         // (the votes of a row's two warps agree: tmax and m_run are the same)
-        if (__any_sync(0xffffffffu, tmax > m_run + kTreeSlack || m_run == -INFINITY || fabsf(tmax) >= kTreeNearMax)) {
-          if (__any_sync(0xffffffffu, fabsf(tmax) >= kTreeNearMax && tmax != -INFINITY)) {
+        if (__builtin_expect(__any_sync(0xffffffffu, tmax > m_run + kTreeSlack || m_run == -INFINITY || large), 0)) {
+          if (__builtin_expect(__any_sync(0xffffffffu, large), 0)) {
             volatile float* word = reinterpret_cast<float*>(pair_max);
             float top = v[0];
 #pragma unroll
