@@ -113,7 +113,8 @@ struct TreeCfg {
   static constexpr int kThreads = NT == 2 ? 640 : 96 + kSoftmaxThreads;
   // NT = 2: 20 warps are launched with 96 registers a thread (5 warps per
   // scheduler); the softmax threads (4 warpgroups) take 104, the rest 64:
-  // 512 * 104 + 128 * 64 = 640 * 96.  The host refuses another launch count.
+  // 512 * 104 + 128 * 64 = 640 * 96.  The host takes one row tile when the
+  // kernel does not start with 96.
   static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 104, kOtherRegs = 64;
   static constexpr int kRows = kTreeM * NT;
   static constexpr int kChunks = D / 64;
@@ -1083,19 +1084,25 @@ bool tree_two_tiles(int total_q, int batch, int group) {
 // take 15.2 us whole and 15.7 us split; 16 tiles gain 5 us from the split.
 constexpr int kTreeMinSplit = 6;
 
+// Whether the kernel for two row tiles starts with the registers that its
+// warps' shares add up to.  A compiler that gives it another count leaves the
+// wide calls to the form with one row tile, which takes the same arguments.
+template <int D>
+bool tree_split_adds_up() {
+  static const bool ok = [] {
+    cudaFuncAttributes f;
+    return cudaFuncGetAttributes(&f, pl::paged_tree_kernel<D, 2>) == cudaSuccess &&
+           (f.numRegs + 7) / 8 * 8 == pl::TreeCfg<D, 2>::kLaunchRegs;
+  }();
+  return ok;
+}
+
 template <int D, int NT>
 int32_t launch_tree(const CUtensorMap& map, const pl::TreeArgs& a, bool merge, void* stream) {
   using C = pl::TreeCfg<D, NT>;
   auto kern = pl::paged_tree_kernel<D, NT>;
   int32_t st = pl_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (st != PL_OK) return st;
-  if (NT == 2) {  // the register split only adds up for this launch count
-    static const int regs = [&] {
-      cudaFuncAttributes f;
-      return cudaFuncGetAttributes(&f, kern) == cudaSuccess ? f.numRegs : -1;
-    }();
-    if (regs != C::kLaunchRegs) return PL_ERR_UNSUPPORTED;
-  }
   st = pl_host::launch_pdl(kern, dim3(a.ctas), dim3(C::kThreads), C::kSmemBytes, stream, map, a);
   if (st != PL_OK || !merge) return st;
   constexpr int warps = pl::kMergeThreads / 32;
@@ -1150,7 +1157,8 @@ extern "C" int32_t pl_paged_tree_attention(
   const int sms = pl_host::sm_count();
   if (sms <= 0) return PL_ERR_NO_DEVICE;
 
-  const bool two = tree_two_tiles(total_q, batch, group);
+  const bool two = tree_two_tiles(total_q, batch, group) &&
+                   (head_dim == 128 ? tree_split_adds_up<128>() : tree_split_adds_up<64>());
   pl::TreeArgs a;
   a.q = static_cast<const pl::bf16*>(q);
   a.kv = static_cast<const pl::bf16*>(kv_cache);
