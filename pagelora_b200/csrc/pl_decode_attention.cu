@@ -763,12 +763,15 @@ struct MapKey {
   }
 };
 
-constexpr int kMapCache = 128;
+// Two maps a layer (boxes of a page, and of 16 tokens for the sparse decode)
+// of models of up to 256 layers.  The layers of a step follow one another, so
+// a look-up begins behind the last hit.
+constexpr int kMapCache = 512;
 struct MapCache {
   std::mutex mu;
   MapKey key[kMapCache];
   CUtensorMap map[kMapCache];
-  int used = 0, next = 0;
+  int used = 0, next = 0, hint = 0;
 };
 MapCache g_maps;
 
@@ -782,11 +785,14 @@ int32_t kv_tensor_map_rows(const void* cache, int64_t pages, int hkv, int d, int
   cudaGetDevice(&dev);
   MapKey k{cache, pages, hkv, d, ps, rows, dev};
   std::lock_guard<std::mutex> lock(g_maps.mu);
-  for (int i = 0; i < g_maps.used; ++i)
-    if (g_maps.key[i] == k) {
-      *out = g_maps.map[i];
+  for (int i = 0; i < g_maps.used; ++i) {
+    const int at = (g_maps.hint + i) % g_maps.used;
+    if (g_maps.key[at] == k) {
+      *out = g_maps.map[at];
+      g_maps.hint = at + 1;
       return PL_OK;
     }
+  }
   pl_host::EncodeTiledFn enc = pl_host::encode_tiled_fn();
   if (enc == nullptr) return PL_ERR_CUDA;
   cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)hkv, (cuuint64_t)ps, (cuuint64_t)(2 * pages)};
