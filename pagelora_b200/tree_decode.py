@@ -60,8 +60,14 @@ class TreeDecoder:
     def __init__(self, engine: BatchDecodeEngine, *, sparse: SparsePages | None = None) -> None:
         if engine.world != 1 or engine.cascade is not None:
             raise ValueError("the engine's rows must hold their whole context (no split-KV, no shared prefix)")
-        if engine.lora_rank and engine.spec.hidden > K.SHRINK_ROWS_MAX_K:
-            raise ValueError(f"LoRA rows need hidden <= {K.SHRINK_ROWS_MAX_K}")
+        spec = engine.spec
+        if engine.lora_rank and max(spec.hidden, spec.q_dim) > K.SHRINK_ROWS_MAX_K:
+            raise ValueError(f"LoRA rows need hidden and query features <= {K.SHRINK_ROWS_MAX_K}")
+        if sparse is not None:
+            if sparse.sink < 0 or sparse.recent < 1 or sparse.sink + sparse.recent > sparse.select:
+                raise ValueError("a page budget needs sink >= 0, recent >= 1 and sink + recent <= select")
+            if engine.page_size not in (16, 32) or spec.num_qo_heads > 16 * spec.num_kv_heads:
+                raise ValueError("sparse decode needs pages of 16 or 32 tokens and at most 16 query heads per kv head")
         self.e = engine
         dev = engine.device
         self.table, self.num, self.last = engine.row_pages, engine.row_num_pages, engine.last_page_len
@@ -163,6 +169,17 @@ class TreeDecoder:
 
         return ((self.num - 1) * self.e.page_size + self.last).clamp_(min=0)
 
+    @staticmethod
+    def _need_tokens(tokens: torch.Tensor, n: int) -> None:
+        K._vecs(torch.int64, "tokens", (tokens,), (n,))
+        if tokens.dim() != 1 or tokens.numel() != n:
+            raise ValueError(f"tokens must be [{n}]")
+
+    def _row_ids(self, rows: list[int]) -> torch.Tensor:
+        if any(not 0 <= r < self.rows for r in rows):
+            raise ValueError(f"rows are 0 .. {self.rows - 1}")
+        return torch.tensor(rows, dtype=torch.int32, device=self.lens.device)
+
     # --------------------------------------------------------------- steps
     @torch.no_grad()
     def verify(self, tokens: torch.Tensor, parents: torch.Tensor, qo_indptr: torch.Tensor, max_tokens: int) -> TreeStep:
@@ -171,9 +188,17 @@ class TreeDecoder:
         r's tree at qo_indptr[r]:qo_indptr[r+1], at most ``max_tokens`` each;
         a row without tokens stays as it is."""
 
+        total = tokens.numel()
+        self._need_tokens(tokens, total)
+        K._vecs(torch.int32, "parents qo_indptr", (parents, qo_indptr), (total, self.rows + 1))
+        if parents.numel() != total or qo_indptr.numel() != self.rows + 1 or max_tokens < 1:
+            raise ValueError("parents needs an entry per token, qo_indptr one per row and one more, max_tokens >= 1")
+        if total == 0:
+            logits = torch.empty(0, self.e.lm_head.shape[0], dtype=torch.bfloat16, device=tokens.device)
+            return TreeStep(tokens.clone(), self._none.new_full((self.rows, max_tokens), -1), self._none.clone(),
+                            tokens.new_full((self.rows,), -1), logits)
         if self._ended:  # a draft may begin an empty row
             self._live = None
-        total = tokens.numel()
         tok_row = torch.searchsorted(qo_indptr[1:], torch.arange(total, device=tokens.device, dtype=torch.int32),
                                      right=True)
         slot_page, slot_off, _ = self._reserve(qo_indptr, total)
@@ -230,6 +255,7 @@ class TreeDecoder:
 
         if self.sparse is None:
             raise ValueError("the decoder was built without a page budget (sparse)")
+        self._need_tokens(tokens, self.rows)
         rows, tok_indptr = self._live_rows()
         n, some = rows.numel(), rows.numel() < self.rows
         nxt = torch.full((self.rows,), -1, dtype=torch.int64, device=rows.device)
@@ -265,10 +291,12 @@ class TreeDecoder:
     def fork(self, src: list[int], dst: list[int]) -> None:
         """Empty rows ``dst`` continue as copies of ``src`` (same adapters)."""
 
+        s, d = self._row_ids(src), self._row_ids(dst)
+        if len(src) != len(dst):
+            raise ValueError("src and dst differ in length")
         if any(self.e.row_adapter[a] != self.e.row_adapter[b] for a, b in zip(src, dst)):
             raise ValueError("a row forks into a row with the same adapter")
         self._live = None
-        s, d = (torch.tensor(r, dtype=torch.int32, device=self.lens.device) for r in (src, dst))
         K.page_fork(self.e.kv, self.refcount, self.table, self.num, self.last, s, d, status=self.status)
         self.lens.copy_(self._row_lens())
         if self.sparse is not None:  # the copied last pages
@@ -278,8 +306,8 @@ class TreeDecoder:
         """The rows end: their pages go back to the pool, and they stay empty
         until a fork or a draft begins them anew."""
 
+        r = self._row_ids(rows)
         self._live, self._ended = None, True
-        r = torch.tensor(rows, dtype=torch.int32, device=self.lens.device)
         K.page_release(self.refcount, self.table, self.num, self.last, r, status=self.status)
         self.lens.copy_(self._row_lens())
 
