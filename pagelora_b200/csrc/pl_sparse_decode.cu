@@ -893,12 +893,12 @@ __global__ void __launch_bounds__(kSparseThreads, 2) sparse_attend_kernel(const 
     float L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c = 0; c < S; ++c) {
-      const float mc = recv_ml[c * 32 + row], lc = recv_ml[c * 32 + 16 + row];
-      if (lc == 0.f) continue;  // a CTA without pages
-      // no maximum, but a sum: the scores are NaN, and so is the sum
+      // without a maximum: a CTA without pages, whose state is 0, or NaN scores,
+      // whose sum is NaN
+      const float mc = recv_ml[c * 32 + row];
       const float f = mc == -INFINITY ? 1.f : exp2f(mc - M);
       const float4 v = recv[i * S + c];
-      L += f * lc;
+      L += f * recv_ml[c * 32 + 16 + row];
       acc.x += f * v.x;
       acc.y += f * v.y;
       acc.z += f * v.z;
