@@ -70,7 +70,7 @@ constexpr uint16_t kTreeGaveUp = 0xffff;
 // tokens 337, 308, 278, 251, 245; requests of equal length do not change.
 constexpr int kTreeItemCost = 3;
 // Places of the line: positions on it, and sums of two, are 32-bit.
-constexpr int64_t kTreeMostPlaces = 1 << 30;
+constexpr uint32_t kTreeMostPlaces = 1u << 30;
 constexpr int kTreeMaxTokens = 1024;     // drafted tokens of one request (tree_mask / tree_accept)
 
 struct TreeArgs {
@@ -174,7 +174,10 @@ struct TreeReq {
   __device__ __forceinline__ int span() const { return ntiles + kTreeItemCost; }
   // of the request (kTreeMostPlaces bounds the total of all requests)
   __device__ __forceinline__ int work(int hkv) const { return rts * hkv * span(); }
-  __device__ __forceinline__ int64_t work64(int hkv) const { return (int64_t)rts * hkv * span(); }
+  // the same, or kTreeMostPlaces + 1 where it is more than that
+  __device__ __forceinline__ uint32_t places(int hkv) const {
+    return (uint32_t)min((int64_t)rts * hkv * span(), (int64_t)kTreeMostPlaces + 1);
+  }
 };
 
 // Inclusive prefix sum over a warp.
@@ -188,22 +191,24 @@ __device__ __forceinline__ int tree_scan(int v) {
   return v;
 }
 
-__device__ __forceinline__ int64_t tree_sum64(int64_t v) {
+// Sums of places stay at kTreeMostPlaces + 1 from there on.
+__device__ __forceinline__ uint32_t tree_add(uint32_t a, uint32_t b) { return min(a + b, kTreeMostPlaces + 1); }
+__device__ __forceinline__ uint32_t tree_add_warp(uint32_t v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, (long long)v, o);
+  for (int o = 16; o > 0; o >>= 1) v = tree_add(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
 // Length of the line (one warp), 0 when it has more than kTreeMostPlaces (more
 // than hours of work, or a qo_indptr that goes back and names tokens often).
 __device__ __forceinline__ int tree_total(const TreeArgs& a, int rows) {
-  int64_t t = 0;
+  uint32_t t = 0;
   for (int b = threadIdx.x & 31; b < a.batch; b += 32) {
     TreeReq r;
     r.load(a, b, rows);
-    t += r.work64(a.num_kv_heads);
+    t = tree_add(t, r.places(a.num_kv_heads));
   }
-  t = tree_sum64(t);
+  t = tree_add_warp(t);
   if (t <= kTreeMostPlaces) return (int)t;
   if (blockIdx.x == 0) set_status(a.status, PL_ERR_UNSUPPORTED);
   return 0;
@@ -875,7 +880,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
   const int tok_g = blockIdx.x;
   // the request of this token, where it begins on the line, and the line's length
   int q0 = 0, rts = 0, nt = 0, base = 0, total = 0;
-  int64_t places = 0;
+  uint32_t places = 0;
   bool found = false;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     TreeReq r;
@@ -892,7 +897,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
       base = __shfl_sync(0xffffffffu, inc - w, l);
     }
     total = __shfl_sync(0xffffffffu, inc, 31);
-    places += tree_sum64(r.work64(a.num_kv_heads));
+    places = tree_add(places, tree_add_warp(r.places(a.num_kv_heads)));
   }
   if (places > kTreeMostPlaces) found = false;  // refused: there is nothing to join
   const int share = tree_share(total, a.ctas);
