@@ -167,7 +167,8 @@ class TreeDecoder:
     def _row_lens(self) -> torch.Tensor:
         """Cached tokens of every row, from its pages."""
 
-        return ((self.num - 1) * self.e.page_size + self.last).clamp_(min=0)
+        ps = self.e.page_size
+        return torch.add(self.last, self.num, alpha=ps).sub_(ps).clamp_(min=0)
 
     @staticmethod
     def _need_tokens(tokens: torch.Tensor, n: int) -> None:
@@ -222,14 +223,14 @@ class TreeDecoder:
         # A refused reservation or compaction left the rows as they were before
         # it: the step keeps nothing, and the drafts' pages are given back.
         # (Cutting rows to the length that they have changes nothing.)
-        done = (self._row_lens() == self.lens + count).all()
-        count.mul_(done)
-        keep.masked_fill_(~done, -1)
-        nxt.masked_fill_(~done, -1)
-        K.cache_compact(*tables, self.lens + count, keep, self._none, status=self.status)
-        if self.sparse is not None:
-            self._refresh_bounds(self.lens // self.e.page_size, (max_tokens - 1) // self.e.page_size + 2)
+        undone = (self._row_lens() != self.lens + count).any()
+        for t, nothing in ((count, 0), (keep, -1), (nxt, -1)):
+            t.masked_fill_(undone, nothing)
+        first = self.lens // self.e.page_size if self.sparse is not None else None
         self.lens.add_(count)
+        K.cache_compact(*tables, self.lens, keep, self._none, status=self.status)
+        if first is not None:
+            self._refresh_bounds(first, (max_tokens - 1) // self.e.page_size + 2)
         return TreeStep(targets, keep, count, nxt, logits)
 
     def _live_rows(self) -> tuple[torch.Tensor, torch.Tensor]:
@@ -258,9 +259,9 @@ class TreeDecoder:
         self._need_tokens(tokens, self.rows)
         rows, tok_indptr = self._live_rows()
         n, some = rows.numel(), rows.numel() < self.rows
-        nxt = torch.full((self.rows,), -1, dtype=torch.int64, device=rows.device)
         if n == 0:
-            return nxt, torch.zeros(self.rows, self.e.lm_head.shape[0], dtype=torch.bfloat16, device=rows.device)
+            logits = torch.zeros(self.rows, self.e.lm_head.shape[0], dtype=torch.bfloat16, device=rows.device)
+            return torch.full_like(tokens, -1), logits
         slot_page, slot_off, positions = self._reserve(tok_indptr, n)
         indptr, last = self.indptr, self.last
         if some:  # (rows without a context have no pages between those of the others)
@@ -278,12 +279,12 @@ class TreeDecoder:
                                          status=self.status)
 
         logits = self._forward(tokens, positions, rows, slot_page, slot_off, attend)
+        nxt = K.argmax(logits, torch.empty_like(tokens))
         lens = self._row_lens()
-        grown = (lens != self.lens).any()  # the reservation is for all rows or for none
+        nxt.masked_fill_((lens == self.lens).all(), -1)  # the reservation is for all rows or for none
         self.lens.copy_(lens)
-        nxt[rows] = K.argmax(logits, torch.empty_like(tokens))
-        nxt.masked_fill_(~grown, -1)
         if some:
+            nxt = nxt.new_full((self.rows,), -1).index_copy_(0, rows, nxt)
             logits = logits.new_zeros(self.rows, logits.shape[1]).index_copy_(0, rows, logits)
         return nxt, logits
 
