@@ -38,12 +38,13 @@
 // copies and returns.
 //
 // Few rows read the cache once and are bound by HBM: 16 requests of 20 tokens
-// at 8000 positions (32 / 8 heads of 128) take 205 us in two layers, 5.2 TB/s;
+// at 8000 positions (32 / 8 heads of 128) take 210 us in two layers, 5.0 TB/s;
 // 89 us of a layer are this kernel, where a plain copy of the bytes takes 81.
-// Many rows are bound by the chain softmax (2200 cycles) -> P.V -> next scores
-// (2800, half of it the issue) of each of two row tiles in turn, and by the
-// power limit: 8 requests of 64 tokens at 32768 positions take 740 us in two
-// layers, 745 TFLOP/s (660 us before the clock falls from 1.8 to 1.6 GHz).
+// Many rows are bound by the chain maximum -> its exchange -> exponentials ->
+// P.V -> next scores of each of two row tiles in turn: 8 requests of 64 tokens
+// at 32768 positions take 737 us in two layers, 747 TFLOP/s (660 us before the
+// power limit lowers the clock from 1.8 to 1.6 GHz).  The prefill kernel, which
+// does not wait for the maximum, does the same products at 916 TFLOP/s.
 #include "pl_common.cuh"
 
 namespace pl {

@@ -11,11 +11,12 @@ bookkeeping on the device.  One verification step of drafted trees is
     move together, the rest of the drafts' pages go back to the pool)
 
 with no host synchronisation; rows fork and end with :meth:`fork` and
-:meth:`release`.  What the device refuses (a row or the pool without room) changes
-no row and accepts no token; :meth:`check` says why.  With ``sparse`` the decoder also keeps the int8 key bounds of
-every page, and :meth:`step_sparse` decodes one token per row over the pages
-that their score selects.  No reference counterpart: the reference decodes one
-token per row and step (model/flashinfer/generation.py:188-247).
+:meth:`release`.  What the device refuses (a row or the pool without room)
+changes no row and accepts no token; :meth:`check` says why.  With ``sparse``
+the decoder also keeps the int8 key bounds of every page, and
+:meth:`step_sparse` decodes one token per row over the pages that their score
+selects.  No reference counterpart: the reference decodes one token per row and
+step (model/flashinfer/generation.py:188-247).
 """
 
 from __future__ import annotations
