@@ -1086,6 +1086,185 @@ int32_t pl_paged_sparse_decode(const void *q, int64_t q_stride_b,
                                void *workspace, int64_t workspace_bytes,
                                int32_t *status_dev, void *stream);
 
+/* ------------------------------------------------- sliding window and sinks */
+
+/*
+ * Attention with a sliding window and a few first tokens that stay visible:
+ * a query at position p sees the positions j <= p with j > p - window or
+ * j < sinks (window >= 1, sinks >= 0).  A query that sees nothing yields O =
+ * 0 and LSE = -inf.  What a query does not see does not reach it, inf and NaN
+ * included.  sm_scale > 0.  No reference counterpart.
+ *
+ * pl_paged_window_decode: one token per row, at the row's last cached
+ * position.  q, kv_cache, indptr, indices, last_page_len, out, out_lse as
+ * pl_paged_decode; total_pages = entries of indices; a table outside them
+ * writes PL_ERR_INVALID_ARGUMENT and counts as empty.  Pages without a visible
+ * position are not looked up.  workspace: 16-byte aligned, no
+ * initialisation, of a size that does not depend on the batch.  Supported:
+ * head_dim 64 or 128, page_size 16 / 32 / 64 / 128, group <= 16, batch <=
+ * 65535, total_pages * page_size < 2^31.
+ *
+ * pl_paged_window_prefill: ragged prompts; everything else as
+ * pl_paged_prefill (causal).  Pages that no query of 2 * (128 / group)
+ * neighbouring tokens sees are not looked up.
+ */
+int64_t pl_window_decode_workspace_bytes(int32_t num_qo_heads,
+                                         int32_t num_kv_heads,
+                                         int32_t head_dim);
+int32_t pl_paged_window_decode(const void *q, int64_t q_stride_b,
+                               int64_t q_stride_h, const void *kv_cache,
+                               int64_t num_pages, const int32_t *indptr,
+                               const int32_t *indices,
+                               const int32_t *last_page_len,
+                               int64_t total_pages, int32_t batch,
+                               int32_t num_qo_heads, int32_t num_kv_heads,
+                               int32_t head_dim, int32_t page_size,
+                               float sm_scale, int32_t window, int32_t sinks,
+                               void *out, int64_t o_stride_b,
+                               int64_t o_stride_h, float *out_lse,
+                               void *workspace, int64_t workspace_bytes,
+                               int32_t *status_dev, void *stream);
+int32_t pl_paged_window_prefill(const void *q, int64_t q_stride_t,
+                                int64_t q_stride_h, const void *kv_cache,
+                                int64_t num_pages, const int32_t *qo_indptr,
+                                const int32_t *kv_indptr,
+                                const int32_t *kv_indices,
+                                const int32_t *kv_last_page_len, int32_t batch,
+                                int32_t total_q, int32_t num_qo_heads,
+                                int32_t num_kv_heads, int32_t head_dim,
+                                int32_t page_size, float sm_scale,
+                                int32_t window, int32_t sinks, void *out,
+                                int64_t out_stride_t, int64_t out_stride_h,
+                                float *out_lse, int32_t *status_dev,
+                                void *stream);
+
+/* ------------------------------------------------------ a cache in 4 bits */
+
+/*
+ * A paged K/V cache of 4-bit records, uint8 [num_pages][2][page_size]
+ * [num_kv_heads][head_dim / 2 + 16] (16-byte aligned).  The record of one
+ * head of one token's K (or V): head_dim / 2 bytes of codes, channel 2i in
+ * the low half of byte i; four scales, then four minima, bf16.  Channel c
+ * belongs to group c % 4 and stands for min + scale * code; min is the
+ * group's smallest value, scale = bf16((max - min) / 15), code = rint((x -
+ * min) / scale) within 0 .. 15.  A group with inf or NaN stands for NaN.
+ * head_dim 64 or 128.  The page operations move records as token_bytes =
+ * num_kv_heads * (head_dim / 2 + 16).  No reference counterpart.
+ *
+ * pl_kv4_append: K and V bf16 [num_tokens][num_kv_heads][head_dim] (heads
+ * contiguous, 16-byte aligned rows) go to (page_id[t], page_offset[t]); a
+ * slot outside the pool writes PL_ERR_PAGE_OUT_OF_RANGE and is left out.
+ *
+ * pl_kv4_expand: out[i], bf16 [2][page_size][num_kv_heads][head_dim], receives
+ * the values of page page_ids[i], rounded once; an entry of -1 is left out.
+ *
+ * pl_paged_kv4_decode: one query token per row over the records (their values
+ * are not rounded); arguments as pl_paged_window_decode, window 0: the whole
+ * context.
+ */
+int32_t pl_kv4_append(const void *k, int64_t k_stride, const void *v,
+                      int64_t v_stride, void *kv4_cache, int64_t num_pages,
+                      const int32_t *page_id, const int32_t *page_offset,
+                      int32_t num_tokens, int32_t num_kv_heads,
+                      int32_t head_dim, int32_t page_size, int32_t *status_dev,
+                      void *stream);
+int32_t pl_kv4_expand(const void *kv4_cache, int64_t num_pages,
+                      const int32_t *page_ids, int32_t n, int32_t num_kv_heads,
+                      int32_t head_dim, int32_t page_size, void *out,
+                      int32_t *status_dev, void *stream);
+int64_t pl_kv4_decode_workspace_bytes(int32_t num_qo_heads,
+                                      int32_t num_kv_heads, int32_t head_dim);
+int32_t pl_paged_kv4_decode(const void *q, int64_t q_stride_b,
+                            int64_t q_stride_h, const void *kv4_cache,
+                            int64_t num_pages, const int32_t *indptr,
+                            const int32_t *indices,
+                            const int32_t *last_page_len, int64_t total_pages,
+                            int32_t batch, int32_t num_qo_heads,
+                            int32_t num_kv_heads, int32_t head_dim,
+                            int32_t page_size, float sm_scale, int32_t window,
+                            int32_t sinks, void *out, int64_t o_stride_b,
+                            int64_t o_stride_h, float *out_lse,
+                            void *workspace, int64_t workspace_bytes,
+                            int32_t *status_dev, void *stream);
+
+/* ------------------------------------- eviction by accumulated attention weight */
+
+/*
+ * weight fp32 [batch][weight_capacity] (row stride weight_stride) holds what
+ * every cached position has received; position j of row b is weight[b][j].
+ * Positions from weight_capacity on write PL_ERR_ROW_CAPACITY and are left
+ * out.  Sums have a fixed order.  No reference counterpart.
+ *
+ * pl_paged_decode_weights: pl_paged_decode over the whole context (limits as
+ * pl_paged_window_decode) that adds to weight[b][j] the sum of the softmax
+ * weight of position j over all query heads.  workspace: 16-byte aligned, no
+ * initialisation (num_qo_heads <= 8192).
+ *
+ * pl_paged_prefill_weights: adds to weight[b][j] the sum over the request's
+ * query tokens i and heads h of exp(sm_scale q_ih . k_j - lse[i][h]) where i
+ * sees j (causal: the request's tokens are its last cached positions).  lse
+ * fp32 [total_q][num_qo_heads] as an attention of the same q and cache wrote
+ * it (-inf: the query gives nothing).  q (positive strides), kv_cache and the
+ * tables as pl_paged_prefill; a request with more tokens than cached positions
+ * or with tables outside kv_indices or q writes PL_ERR_INVALID_ARGUMENT and is
+ * left out.
+ *
+ * pl_evict_select: what row r of lens[r] cached positions keeps.  A row of at
+ * most budget positions keeps all: keep_from = lens[r], keep_count = 0.
+ * Another keeps its first `sinks` and last `recent` positions and, of the
+ * others, those of the highest weight up to `budget` in all, the lower position
+ * first among equals (-0 equals 0, NaN is above all): keep_from = sinks,
+ * keep[r] = the other positions, ascending, keep_count = budget - sinks.  Rest
+ * of keep[r]: -1.  These are pl_cache_compact's arguments.  out_weight
+ * [num_rows][capacity] (not overlapping weight) receives the kept positions'
+ * weights in their new order, then 0.  keep_width >= budget - sinks, sinks +
+ * recent <= budget.  A row with lens < 0 or > capacity writes
+ * PL_ERR_INVALID_ARGUMENT and keeps all.
+ */
+int64_t pl_decode_weights_workspace_bytes(int32_t batch, int32_t num_qo_heads,
+                                          int32_t num_kv_heads,
+                                          int32_t head_dim, int32_t page_size,
+                                          int64_t total_pages);
+int32_t pl_paged_decode_weights(const void *q, int64_t q_stride_b,
+                                int64_t q_stride_h, const void *kv_cache,
+                                int64_t num_pages, const int32_t *indptr,
+                                const int32_t *indices,
+                                const int32_t *last_page_len,
+                                int64_t total_pages, int32_t batch,
+                                int32_t num_qo_heads, int32_t num_kv_heads,
+                                int32_t head_dim, int32_t page_size,
+                                float sm_scale, void *out, int64_t o_stride_b,
+                                int64_t o_stride_h, float *out_lse,
+                                float *weight, int64_t weight_stride,
+                                int32_t weight_capacity, void *workspace,
+                                int64_t workspace_bytes, int32_t *status_dev,
+                                void *stream);
+int64_t pl_prefill_weights_workspace_bytes(int32_t num_kv_heads,
+                                           int32_t page_size,
+                                           int64_t total_pages);
+int32_t pl_paged_prefill_weights(const void *q, int64_t q_stride_t,
+                                 int64_t q_stride_h, const void *kv_cache,
+                                 int64_t num_pages, const int32_t *qo_indptr,
+                                 const int32_t *kv_indptr,
+                                 const int32_t *kv_indices,
+                                 const int32_t *kv_last_page_len,
+                                 int64_t total_pages, int32_t batch,
+                                 int32_t total_q, int32_t num_qo_heads,
+                                 int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t page_size, float sm_scale,
+                                 const float *lse, float *weight,
+                                 int64_t weight_stride,
+                                 int32_t weight_capacity, void *workspace,
+                                 int64_t workspace_bytes, int32_t *status_dev,
+                                 void *stream);
+int32_t pl_evict_select(const float *weight, int64_t weight_stride,
+                        int32_t capacity, const int32_t *lens,
+                        int32_t num_rows, int32_t budget, int32_t sinks,
+                        int32_t recent, int32_t *keep_from, int32_t *keep,
+                        int64_t keep_stride, int32_t keep_width,
+                        int32_t *keep_count, float *out_weight,
+                        int64_t out_stride, int32_t *status_dev, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -197,6 +197,43 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _F, _I32, _I32,
          _I32, _P, _I64, _I64, _P, _P, _P, _I64, _P, _P],
     ),
+    "pl_window_decode_workspace_bytes": (_I64, [_I32, _I32, _I32]),
+    "pl_paged_window_decode": (
+        _I32,
+        [_P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F, _I32, _I32, _P, _I64, _I64, _P,
+         _P, _I64, _P, _P],
+    ),
+    "pl_paged_window_prefill": (
+        _I32,
+        [_P, _I64, _I64, _P, _I64, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _F, _I32, _I32, _P, _I64, _I64,
+         _P, _P, _P],
+    ),
+    "pl_kv4_append": (
+        _I32, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _I32, _I32, _I32, _I32, _P, _P],
+    ),
+    "pl_kv4_expand": (_I32, [_P, _I64, _P, _I32, _I32, _I32, _I32, _P, _P, _P]),
+    "pl_kv4_decode_workspace_bytes": (_I64, [_I32, _I32, _I32]),
+    "pl_paged_kv4_decode": (
+        _I32,
+        [_P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F, _I32, _I32, _P, _I64, _I64, _P,
+         _P, _I64, _P, _P],
+    ),
+    "pl_decode_weights_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I64]),
+    "pl_paged_decode_weights": (
+        _I32,
+        [_P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F, _P, _I64, _I64, _P, _P, _I64,
+         _I32, _P, _I64, _P, _P],
+    ),
+    "pl_prefill_weights_workspace_bytes": (_I64, [_I32, _I32, _I64]),
+    "pl_paged_prefill_weights": (
+        _I32,
+        [_P, _I64, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _F, _P, _P, _I64, _I32,
+         _P, _I64, _P, _P],
+    ),
+    "pl_evict_select": (
+        _I32,
+        [_P, _I64, _I32, _P, _I32, _I32, _I32, _I32, _P, _P, _I64, _I32, _P, _P, _I64, _P, _P],
+    ),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -1,0 +1,686 @@
+// Eviction by accumulated attention weight: the weights that a prompt's
+// tokens give the cached positions (pl_paged_prefill_weights), and the choice
+// of the positions to keep (pl_evict_select).  The decode step's weights come
+// with its attention (pl_window_decode.cu); pl_cache_compact moves what stays.
+#include "pl_line_decode.cuh"
+
+namespace pl {
+
+// ------------------------------------------------------- weights of a prompt
+// weight[b][j] += sum over query tokens i and heads h of exp(scale q_ih.k_j -
+// lse_ih), i at position p_i >= j.  The attention that gave lse has read V and
+// written O; this is its score product alone, transposed: one CTA takes a
+// (request, tile of 128 positions, kv head), keeps K in shared memory and
+// streams the query tiles (128 rows = tq tokens x group heads) that see it.
+//   warp 0     TMA: K once, then the query tiles through a ring;
+//   warp 1     tcgen05.mma S^T = K.Q^T into one of four TMEM buffers;
+//   warps 2-9  two groups of four take the tiles in turn: a thread is a
+//              position, reads its 128 scores, and adds 2^(s - lse) into one
+//              register, so nothing is exchanged between threads; the columns'
+//              log sums stand in shared memory.
+// The kv heads' sums go to the workspace and are added in head order by
+// prompt_weight_add_kernel, so two runs give the same bits.  Bound by the
+// exponentials: a tile has 16384 of them (1024 cycles at 16 a cycle) and 512
+// cycles of products at head_dim 128.
+constexpr int kPwThreads = 320;
+constexpr int kPwM = 128;      // positions, and rows of a query tile
+constexpr int kPwSlots = 4;    // query tiles in flight
+constexpr int kPwBufs = 4;     // score buffers
+
+struct PromptWeightArgs {
+  const int32_t* qo_indptr;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_last;
+  int64_t num_pages, total_pages;
+  int32_t batch, total_q, num_qo_heads, group, tq, page_size;
+  float scale_log2;
+  const float* lse;   // [total_q, Hq]
+  float* partial;     // [Hkv][total_pages * page_size]
+  int32_t* status;
+};
+
+template <int D>
+struct PromptWeightCfg {
+  static constexpr int kChunks = D / 64;
+  static constexpr int kChunkBytes = kPwM * 128;
+  static constexpr int kTileBytes = kChunks * kChunkBytes;
+  static constexpr int kSlotOff = kTileBytes;                      // behind K
+  static constexpr int kLseOff = kSlotOff + kPwSlots * kTileBytes; // [2 groups][2][128]
+  static constexpr int kSumOff = kLseOff + 4 * kPwM * 4;           // [128]
+  static constexpr int kBarOff = kSumOff + kPwM * 4;               // kfull qfull[4] qempty[4] sready[4] sfree[4] fin
+  static constexpr int kMiscOff = kBarOff + (2 + 2 * kPwSlots + 2 * kPwBufs) * 8;
+  static constexpr int kSmemBytes = 1024 + kMiscOff + 64;
+  static_assert(kSmemBytes <= 232448, "tiles exceed the shared-memory limit");
+};
+
+// Request and tile of positions that block `x` of the line of tiles takes; a
+// table outside kv_indices has none.  One warp; false past the last tile.
+struct PwSpan {
+  int req, tile, kv_begin, n_pages, kv_len, q0, qlen;
+};
+
+__device__ __forceinline__ int pw_kv_len(const PromptWeightArgs& a, int b, bool report) {
+  const int k0 = a.kv_indptr[b], k1 = a.kv_indptr[b + 1];
+  const int q0 = a.qo_indptr[b], q1 = a.qo_indptr[b + 1];
+  int last = a.kv_last[b];
+  last = last < 0 ? 0 : (last > a.page_size ? a.page_size : last);
+  const int len = k1 > k0 ? (k1 - k0 - 1) * a.page_size + last : 0;
+  if (k0 < 0 || k1 < k0 || (int64_t)k1 > a.total_pages || q0 < 0 || q1 < q0 || q1 > a.total_q || q1 - q0 > len) {
+    if (report) set_status(a.status, PL_ERR_INVALID_ARGUMENT);
+    return 0;
+  }
+  return q1 > q0 ? len : 0;
+}
+
+__device__ __forceinline__ bool pw_find(const PromptWeightArgs& a, int x, PwSpan& s) {
+  const int lane = threadIdx.x % 32;
+  int before = 0;
+  for (int base = 0; base < a.batch; base += 32) {
+    const int b = base + lane;
+    const int len = b < a.batch ? pw_kv_len(a, b, x == 0) : 0;
+    const int n = (len + kPwM - 1) / kPwM;
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > x);
+    if (hit != 0) {
+      const int src = __ffs(hit) - 1;
+      s.req = base + src;
+      s.tile = x - (before + __shfl_sync(0xffffffffu, incl - n, src));
+      s.kv_len = __shfl_sync(0xffffffffu, len, src);
+      s.kv_begin = a.kv_indptr[s.req];
+      s.n_pages = a.kv_indptr[s.req + 1] - s.kv_begin;
+      s.q0 = a.qo_indptr[s.req];
+      s.qlen = a.qo_indptr[s.req + 1] - s.q0;
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPwThreads, 1)
+    prompt_weight_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map,
+                         const PromptWeightArgs a) {
+  using C = PromptWeightCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+  uint64_t* qfull = kfull + 1;              // [slots] query tile landed
+  uint64_t* qempty = qfull + kPwSlots;      // [slots] query tile read
+  uint64_t* sready = qempty + kPwSlots;     // [bufs] scores in TMEM
+  uint64_t* sfree = sready + kPwBufs;       // [bufs] scores read (4 warps)
+  uint64_t* fin = sfree + kPwBufs;          // every tensor-core op finished
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
+  volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, issued, consumed
+  PwSpan* span = reinterpret_cast<PwSpan*>(smem + C::kMiscOff + 32);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int kvh = blockIdx.y;
+
+  if (threadIdx.x == 0) {
+    mbar_init(kfull, 1);
+    for (int i = 0; i < kPwSlots; ++i) {
+      mbar_init(&qfull[i], 1);
+      mbar_init(&qempty[i], 1);
+    }
+    for (int i = 0; i < kPwBufs; ++i) {
+      mbar_init(&sready[i], 1);
+      mbar_init(&sfree[i], 4);
+    }
+    mbar_init(fin, 1);
+    flags[0] = flags[1] = flags[2] = 0;
+    fence_barrier_init();
+  }
+  if (threadIdx.x == 32) {
+    prefetch_tensormap(&kv_map);
+    prefetch_tensormap(&q_map);
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  if (warp == 0) {
+    PwSpan s = {};
+    s.req = -1;
+    pw_find(a, blockIdx.x, s);
+    if (lane == 0) *span = s;
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const PwSpan sp = *span;
+  const int PS = a.page_size;
+  const int kv0 = sp.tile * kPwM;
+  const int p_first = sp.kv_len - sp.qlen;                       // position of the request's first query
+  const int j0 = sp.req >= 0 && kv0 > p_first ? (kv0 - p_first) / a.tq : 0;  // first query tile that sees the tile
+  const int j1 = sp.req >= 0 ? (sp.qlen + a.tq - 1) / a.tq : 0;
+  const int n = j1 > j0 ? j1 - j0 : 0;
+  const int rows = a.tq * a.group;                               // rows of a query tile in use
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    int i = 0;
+    if (n > 0) {
+      const int ppt = kPwM / PS, boxes = ppt * C::kChunks;  // <= 16
+      const int p = lane / C::kChunks, hh = lane % C::kChunks;
+      if (lane == 0) mbar_arrive_expect_tx(kfull, C::kTileBytes);
+      __syncwarp();
+      if (lane < boxes) {
+        const int page = sp.tile * ppt + p;
+        int32_t coord = (int32_t)(2 * a.num_pages);  // out of range: zeros
+        if (page < sp.n_pages) {
+          const int32_t pid = a.kv_indices[sp.kv_begin + page];
+          if (pid >= 0 && (int64_t)pid < a.num_pages)
+            coord = 2 * pid;
+          else
+            set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
+        }
+        tma_load_4d(smem + hh * C::kChunkBytes + p * PS * 128, &kv_map, hh * 64, kvh, 0, coord, kfull);
+      }
+      for (; i < n; ++i) {
+        const int s = i % kPwSlots;
+        bool ok = true;
+        if (i >= kPwSlots) ok = mbar_wait(&qempty[s], ((i / kPwSlots) - 1) & 1);
+        if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) {
+          if (lane == 0 && !__all_sync(0xffffffffu, ok)) set_status(a.status, PL_ERR_TIMEOUT);
+          flags[0] = 1;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&qfull[s], C::kChunks * rows * 128);
+        __syncwarp();
+        if (lane < C::kChunks)
+          tma_load_4d(smem + C::kSlotOff + s * C::kTileBytes + lane * C::kChunkBytes, &q_map, lane * 64, 0, kvh,
+                      sp.q0 + (j0 + i) * a.tq, &qfull[s]);
+      }
+    }
+    if (lane == 0) flags[1] = i;
+  } else if (warp == 1) {
+    // ---------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_bf16(kPwM, kPwM);
+      int consumed = 0;
+      bool ok = n == 0 || mbar_wait(kfull, 0);
+      const uint32_t kb = smem_u32(smem);
+      for (int i = 0; ok && i < n; ++i) {
+        const int s = i % kPwSlots, b = i % kPwBufs;
+        ok = mbar_wait(&qfull[s], (i / kPwSlots) & 1) && !flags[0];
+        if (!ok) break;
+        consumed = i + 1;
+        if (i >= kPwBufs) ok = mbar_wait(&sfree[b], ((i / kPwBufs) - 1) & 1) && !flags[0];
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t qs = smem_u32(smem + C::kSlotOff + s * C::kTileBytes);
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16(tmem + (uint32_t)(b * kPwM), umma_desc_k_sw128(kb + c * C::kChunkBytes + 32 * k),
+                      umma_desc_k_sw128(qs + c * C::kChunkBytes + 32 * k), idesc, (c | k) ? 1u : 0u);
+        umma_commit(&sready[b]);
+        umma_commit(&qempty[s]);
+      }
+      if (!ok) {
+        set_status(a.status, PL_ERR_TIMEOUT);
+        flags[0] = 1;
+      }
+      flags[2] = consumed;
+      umma_commit(fin);
+      if (!mbar_wait(fin, 0)) set_status(a.status, PL_ERR_TIMEOUT);
+    }
+  } else {
+    // -------------------------------------------------------- exponentials
+    const int x = warp < 6 ? 0 : 1, quad = warp & 3;
+    const int m = 32 * quad + lane;  // position within the tile == TMEM lane
+    const uint32_t row_tmem = tmem + ((uint32_t)(32 * quad) << 16);
+    float* lse_s = reinterpret_cast<float*>(smem + C::kLseOff) + x * 2 * kPwM;
+    const int pos = kv0 + m;
+    // -log2 sum of column m of query tile j; columns without a query give 2^-inf
+    auto lse_of = [&](int j) -> float {
+      const int tok = j * a.tq + m / a.group;
+      if (m >= rows || tok >= sp.qlen) return -INFINITY;
+      const float v = a.lse[(int64_t)(sp.q0 + tok) * a.num_qo_heads + kvh * a.group + m % a.group];
+      return v == -INFINITY ? -INFINITY : -v * kLog2e;
+    };
+    const float sl2 = a.scale_log2;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    bool ok = true;
+    float next = x < n ? lse_of(j0 + x) : 0.f;
+    for (int i = x; i < n; i += 2) {
+      float* ls = lse_s + ((i >> 1) & 1) * kPwM;
+      ls[m] = next;
+      if (i + 2 < n) next = lse_of(j0 + i + 2);
+      named_barrier(1 + x, 128);
+      const int b = i % kPwBufs;
+      ok = flags[0] == 0 && mbar_wait(&sready[b], (i / kPwBufs) & 1);
+      if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) ok = false;
+      if (ok) {
+        tc_fence_after();
+        // column c is a query at position first + c / group: seen from column `from` on
+        const int first = p_first + (j0 + i) * a.tq;
+        const int from = pos > first ? (pos - first) * a.group : 0;
+        const bool masked = kv0 + kPwM - 1 > first;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          float v[64];
+          tmem_ld64(row_tmem + (uint32_t)(b * kPwM + 64 * h), v);
+          const float4* l4 = reinterpret_cast<const float4*>(ls + 64 * h);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float4 l = l4[c];
+            float p0 = line_exp2(fmaf(v[4 * c], sl2, l.x)), p1 = line_exp2(fmaf(v[4 * c + 1], sl2, l.y));
+            float p2 = line_exp2(fmaf(v[4 * c + 2], sl2, l.z)), p3 = line_exp2(fmaf(v[4 * c + 3], sl2, l.w));
+            if (masked) {
+              const int col = 64 * h + 4 * c;
+              p0 = col >= from ? p0 : 0.f;
+              p1 = col + 1 >= from ? p1 : 0.f;
+              p2 = col + 2 >= from ? p2 : 0.f;
+              p3 = col + 3 >= from ? p3 : 0.f;
+            }
+            sum[0] += p0;
+            sum[1] += p1;
+            sum[2] += p2;
+            sum[3] += p3;
+          }
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sfree[b]);
+      if (!ok) flags[0] = 1;  // nobody waits any more; the loop goes on for the barrier's count
+    }
+    if (!ok && lane == 0) set_status(a.status, PL_ERR_TIMEOUT);
+    // the two groups' sums, in this order
+    float* sums = reinterpret_cast<float*>(smem + C::kSumOff);
+    const float mine = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    if (x == 1) sums[m] = mine;
+    named_barrier(3, 256);
+    if (x == 0 && sp.req >= 0 && pos < sp.kv_len && flags[0] == 0)
+      a.partial[(int64_t)kvh * a.total_pages * PS + (int64_t)sp.kv_begin * PS + pos] = mine + sums[m];
+  }
+
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int issued = flags[1], consumed = flags[2];
+    for (int i = consumed; i < issued; ++i) (void)mbar_wait(&qfull[i % kPwSlots], (i / kPwSlots) & 1);
+    if (n > 0) (void)mbar_wait(kfull, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// weight[b][pos] += the kv heads' sums, in head order; a thread per position
+// of the page table's line.
+__global__ void __launch_bounds__(256)
+    prompt_weight_add_kernel(const PromptWeightArgs a, int32_t hkv, float* weight, int64_t weight_stride,
+                             int32_t capacity) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t all = a.total_pages * a.page_size;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= all) return;
+  const int32_t entry = (int32_t)(at / a.page_size);
+  int lo = 0, hi = a.batch;  // the row that holds the entry
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (a.kv_indptr[mid + 1] > entry) hi = mid; else lo = mid + 1;
+  }
+  if (lo >= a.batch || a.kv_indptr[lo] > entry) return;
+  const int len = pw_kv_len(a, lo, false);
+  const int64_t pos = at - (int64_t)a.kv_indptr[lo] * a.page_size;
+  if (pos >= len) return;
+  if (pos >= capacity) {
+    set_status(a.status, PL_ERR_ROW_CAPACITY);
+    return;
+  }
+  float sum = 0.f;
+#pragma unroll 8
+  for (int h = 0; h < hkv; ++h) sum += __ldcg(a.partial + h * all + at);
+  weight[(int64_t)lo * weight_stride + pos] += sum;
+}
+
+// ------------------------------------------------------------------ select
+// The positions that a row of len > budget keeps: the first `sinks`, the last
+// `recent`, and the k = budget - sinks - recent others of the highest weight,
+// the lowest position first among equals.  Weights compare as numbers (-0 as
+// 0; a NaN above all).  A radix select over the bits finds the k-th largest:
+// 11, 11 and 10 bits in three passes, each a histogram in shared memory; then
+// every warp counts what its run of positions keeps, and after a scan of the
+// counts writes it in ascending order.  A row is one CTA, or (kCluster) eight
+// that share its positions and read each other's histograms through
+// distributed shared memory.  The weights come from L2 after the first pass.
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelBins = 2048;
+constexpr int kSelCluster = 8;
+
+struct SelectArgs {
+  const float* weight;
+  int64_t weight_stride;
+  int32_t capacity;     // columns of weight and out_weight
+  const int32_t* lens;
+  int32_t budget, sinks, recent;
+  int32_t* keep_from;
+  int32_t* keep;
+  int64_t keep_stride;
+  int32_t keep_width;
+  int32_t* keep_count;
+  float* out_weight;
+  int64_t out_stride;
+  int32_t* status;
+};
+
+__device__ __forceinline__ uint32_t select_key(float w) {
+  if (w != w) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(w + 0.f);
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+template <bool kCluster>
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const SelectArgs a) {
+  __shared__ __align__(16) int32_t hist[kSelBins];
+  __shared__ int32_t scan[kSelWarps];
+  __shared__ int32_t pick[2];                    // digit, count above it
+  __shared__ int32_t counts[2 * kSelWarps + 2];  // per warp: above, equal; then the CTA's sums
+  constexpr int nr = kCluster ? kSelCluster : 1;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = kCluster ? blockIdx.x % kSelCluster : 0;
+  const int row = kCluster ? blockIdx.x / kSelCluster : blockIdx.x;
+  auto sync = [&]() {
+    if constexpr (kCluster) cluster_sync_all(); else __syncthreads();
+  };
+  pdl_launch_dependents();
+  pdl_wait();
+  int len = a.lens[row];
+  const float* w = a.weight + (int64_t)row * a.weight_stride;
+  float* ow = a.out_weight + (int64_t)row * a.out_stride;
+  int32_t* keep = a.keep + (int64_t)row * a.keep_stride;
+  const bool cut = len > a.budget && len <= a.capacity;
+  if (rank == 0 && threadIdx.x == 0) {
+    if (len < 0 || len > a.capacity) set_status(a.status, PL_ERR_INVALID_ARGUMENT);
+    a.keep_from[row] = cut ? a.sinks : (len < 0 ? 0 : len);
+    a.keep_count[row] = cut ? a.budget - a.sinks : 0;
+  }
+  len = len < 0 ? 0 : (len > a.capacity ? a.capacity : len);
+  const int kept = cut ? a.budget : len;
+  const int tid = rank * kSelThreads + threadIdx.x;
+  constexpr int all = nr * kSelThreads;
+  // what does not depend on the choice
+  const int listed = cut ? a.budget - a.sinks : 0;
+  for (int i = listed + tid; i < a.keep_width; i += all) keep[i] = -1;
+  for (int i = kept + tid; i < a.capacity; i += all) ow[i] = 0.f;
+  if (!cut) {
+    for (int i = tid; i < len; i += all) ow[i] = w[i];
+    return;  // the whole row's CTAs alike
+  }
+  const int k = a.budget - a.sinks - a.recent;
+  for (int i = tid; i < a.sinks; i += all) ow[i] = w[i];
+  for (int i = tid; i < a.recent; i += all) {
+    const int pos = len - a.recent + i;
+    keep[k + i] = pos;
+    ow[a.sinks + k + i] = w[pos];
+  }
+  // this warp's run of the candidates [sinks, len - recent)
+  const int c0 = a.sinks, n = len - a.recent - a.sinks;
+  const int runs = nr * kSelWarps, per = ((n + runs - 1) / runs + 31) / 32 * 32;
+  const int b = min(n, (rank * kSelWarps + warp) * per), e = min(n, b + per);
+
+  uint32_t prefix = 0, mask = 0;
+  int want = k;  // still to be found among the keys with this prefix
+  if (k > 0) {
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
+      for (int i = threadIdx.x; i < kSelBins; i += kSelThreads) hist[i] = 0;
+      __syncthreads();
+#pragma unroll 4
+      for (int i = b + lane; i < e; i += 32) {
+        const uint32_t key = select_key(w[c0 + i]);
+        if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1);
+      }
+      sync();
+      // four bins a thread, from the highest down
+      const int bin = kSelBins - 4 - 4 * threadIdx.x;
+      int4 h = make_int4(0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < nr; ++r) {
+        int4 o;
+        if constexpr (kCluster) {
+          const float4 f = dsmem_ld_f32x4(dsmem_map(smem_u32(hist + bin), r));
+          o = make_int4(__float_as_int(f.x), __float_as_int(f.y), __float_as_int(f.z), __float_as_int(f.w));
+        } else {
+          o = *reinterpret_cast<const int4*>(hist + bin);
+        }
+        h.x += o.x;
+        h.y += o.y;
+        h.z += o.z;
+        h.w += o.w;
+      }
+      const int mine = h.x + h.y + h.z + h.w;
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+      }
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      int above = incl - mine;
+      for (int i = 0; i < warp; ++i) above += scan[i];
+      if (above < want && want <= above + mine) {
+        int d = bin + 3;
+        if (want > above + h.w) { above += h.w; --d;
+          if (want > above + h.z) { above += h.z; --d;
+            if (want > above + h.y) { above += h.y; --d; } } }
+        pick[0] = d;
+        pick[1] = above;
+      }
+      sync();  // the digit is known, and every CTA has read the histograms
+      prefix |= (uint32_t)pick[0] << shift;
+      mask |= ((1u << bits) - 1) << shift;
+      want -= pick[1];
+    }
+  } else {
+    prefix = 0xffffffffu;
+  }
+  // counts of every warp's run: above the key, equal to it
+  int gt = 0, eq = 0;
+#pragma unroll 4
+  for (int i = b + lane; i < e; i += 32) {
+    const uint32_t key = select_key(w[c0 + i]);
+    gt += key > prefix;
+    eq += key == prefix;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    gt += __shfl_xor_sync(0xffffffffu, gt, o);
+    eq += __shfl_xor_sync(0xffffffffu, eq, o);
+  }
+  if (lane == 0) {
+    counts[2 * warp] = gt;
+    counts[2 * warp + 1] = eq;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int g = 0, q = 0;
+    for (int i = 0; i < kSelWarps; ++i) {
+      g += counts[2 * i];
+      q += counts[2 * i + 1];
+    }
+    counts[2 * kSelWarps] = g;
+    counts[2 * kSelWarps + 1] = q;
+  }
+  sync();
+  gt = eq = 0;  // in front of this warp's run
+  if constexpr (kCluster) {
+    for (int r = 0; r < rank; ++r) {
+      gt += __float_as_int(dsmem_ld_f32(dsmem_map(smem_u32(&counts[2 * kSelWarps]), r)));
+      eq += __float_as_int(dsmem_ld_f32(dsmem_map(smem_u32(&counts[2 * kSelWarps + 1]), r)));
+    }
+  }
+  for (int i = 0; i < warp; ++i) {
+    gt += counts[2 * i];
+    eq += counts[2 * i + 1];
+  }
+  const unsigned below = (1u << lane) - 1;
+  for (int i0 = b; i0 < e; i0 += 32) {
+    const int i = i0 + lane;
+    const float v = i < e ? w[c0 + i] : 0.f;
+    const uint32_t key = select_key(v);
+    const unsigned bg = __ballot_sync(0xffffffffu, i < e && key > prefix);
+    const unsigned bq = __ballot_sync(0xffffffffu, i < e && key == prefix);
+    const int g = gt + __popc(bg & below), q = eq + __popc(bq & below);
+    const bool take = i < e && (key > prefix || (key == prefix && q < want));
+    if (take) {
+      const int at = g + min(q, want);
+      keep[at] = c0 + i;
+      ow[a.sinks + at] = v;
+    }
+    gt += __popc(bg);
+    eq += __popc(bq);
+  }
+  if constexpr (kCluster) cluster_sync_all();  // the counts are read before a CTA ends
+}
+
+}  // namespace pl
+
+// =================================================================== host
+namespace {
+
+int64_t align256(int64_t v) { return (v + 255) & ~int64_t(255); }
+
+template <int D>
+int32_t launch_prompt_weights(const CUtensorMap& kv_map, const CUtensorMap& q_map, const pl::PromptWeightArgs& a,
+                              int64_t tiles, int hkv, void* stream) {
+  using C = pl::PromptWeightCfg<D>;
+  auto kern = pl::prompt_weight_kernel<D>;
+  const int32_t st = pl_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
+  if (st != PL_OK) return st;
+  return pl_host::launch_pdl(kern, dim3((unsigned)tiles, hkv), dim3(pl::kPwThreads), C::kSmemBytes, stream, kv_map,
+                             q_map, a);
+}
+
+}  // namespace
+
+extern "C" int64_t pl_prefill_weights_workspace_bytes(int32_t num_kv_heads, int32_t page_size, int64_t total_pages) {
+  if (num_kv_heads <= 0 || page_size <= 0 || total_pages < 0) return 0;
+  return align256(total_pages * page_size * num_kv_heads * 4);
+}
+
+extern "C" int32_t pl_paged_prefill_weights(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv_cache,
+                                            int64_t num_pages, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                            const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                                            int64_t total_pages, int32_t batch, int32_t total_q, int32_t num_qo_heads,
+                                            int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float sm_scale,
+                                            const float* lse, float* weight, int64_t weight_stride,
+                                            int32_t weight_capacity, void* workspace, int64_t workspace_bytes,
+                                            int32_t* status_dev, void* stream) {
+  if (batch < 0 || total_q < 0 || num_pages <= 0 || total_pages < 0 || num_kv_heads <= 0 || num_qo_heads <= 0 ||
+      num_qo_heads % num_kv_heads != 0 || kv_cache == nullptr || !(sm_scale > 0.f) || weight_capacity < 0 ||
+      weight_stride < weight_capacity || (weight == nullptr && weight_capacity > 0))
+    return PL_ERR_INVALID_ARGUMENT;
+  const int group = num_qo_heads / num_kv_heads;
+  if (group > pl::kPwM || (head_dim != 64 && head_dim != 128) ||
+      (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) || num_kv_heads > 65535 ||
+      total_pages * page_size > 0x7FFFFFFFll || num_pages > 0x3FFFFFFFll)
+    return PL_ERR_UNSUPPORTED;
+  if (batch == 0 || total_q == 0 || total_pages == 0) return PL_OK;
+  if (q == nullptr || qo_indptr == nullptr || kv_indptr == nullptr || kv_indices == nullptr ||
+      kv_last_page_len == nullptr || lse == nullptr)
+    return PL_ERR_INVALID_ARGUMENT;
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv_cache)) & 15) != 0 || q_stride_t <= 0 || q_stride_h <= 0 || q_stride_t % 8 != 0 || q_stride_h % 8 != 0)
+    return PL_ERR_INVALID_ARGUMENT;
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
+      workspace_bytes < pl_prefill_weights_workspace_bytes(num_kv_heads, page_size, total_pages))
+    return PL_ERR_WORKSPACE_TOO_SMALL;
+
+  pl::PromptWeightArgs a = {};
+  a.qo_indptr = qo_indptr;
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.kv_last = kv_last_page_len;
+  a.num_pages = num_pages;
+  a.total_pages = total_pages;
+  a.batch = batch;
+  a.total_q = total_q;
+  a.num_qo_heads = num_qo_heads;
+  a.group = group;
+  a.tq = pl::kPwM / group;
+  a.page_size = page_size;
+  a.scale_log2 = sm_scale * pl::kLog2e;
+  a.lse = lse;
+  a.partial = static_cast<float*>(workspace);
+  a.status = status_dev;
+
+  CUtensorMap kv_map, q_map;
+  int32_t st = pl_host::kv_tensor_map(kv_cache, num_pages, num_kv_heads, head_dim, page_size, &kv_map);
+  if (st != PL_OK) return st;
+  pl_host::EncodeTiledFn enc = pl_host::encode_tiled_fn();
+  if (enc == nullptr) return PL_ERR_CUDA;
+  // q as {head_dim, heads of a group, kv heads, tokens}; a box is tq tokens of one group, 64 channels
+  const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)group, (cuuint64_t)num_kv_heads, (cuuint64_t)total_q};
+  const cuuint64_t strides[3] = {(cuuint64_t)q_stride_h * 2, (cuuint64_t)q_stride_h * 2 * group,
+                                 (cuuint64_t)q_stride_t * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)group, 1, (cuuint32_t)a.tq};
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  if (enc(&q_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(q), dims, strides, box, ones,
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return PL_ERR_INVALID_ARGUMENT;
+  // a row of n positions has ceil(n / 128) <= n / 128 + 1 tiles
+  const int64_t tiles = total_pages * page_size / pl::kPwM + batch;
+  if (tiles > 0x7FFFFFFF) return PL_ERR_UNSUPPORTED;
+  st = head_dim == 128 ? launch_prompt_weights<128>(kv_map, q_map, a, tiles, num_kv_heads, stream)
+                       : launch_prompt_weights<64>(kv_map, q_map, a, tiles, num_kv_heads, stream);
+  if (st != PL_OK) return st;
+  const int64_t blocks = (total_pages * page_size + 255) / 256;
+  return pl_host::launch_pdl(pl::prompt_weight_add_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a,
+                             num_kv_heads, weight, weight_stride, weight_capacity);
+}
+
+extern "C" int32_t pl_evict_select(const float* weight, int64_t weight_stride, int32_t capacity, const int32_t* lens,
+                                   int32_t num_rows, int32_t budget, int32_t sinks, int32_t recent, int32_t* keep_from,
+                                   int32_t* keep, int64_t keep_stride, int32_t keep_width, int32_t* keep_count,
+                                   float* out_weight, int64_t out_stride, int32_t* status_dev, void* stream) {
+  if (num_rows < 0 || capacity < 0 || budget < 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget ||
+      keep_width < budget - sinks || keep_stride < keep_width || weight_stride < capacity || out_stride < capacity)
+    return PL_ERR_INVALID_ARGUMENT;
+  if (num_rows > 0x7FFFFFFF / pl::kSelCluster) return PL_ERR_UNSUPPORTED;
+  if (num_rows == 0) return PL_OK;
+  if (lens == nullptr || keep_from == nullptr || keep_count == nullptr || (keep == nullptr && keep_width > 0) ||
+      (capacity > 0 && (weight == nullptr || out_weight == nullptr || weight == out_weight)))
+    return PL_ERR_INVALID_ARGUMENT;
+  pl::SelectArgs a;
+  a.weight = weight;
+  a.weight_stride = weight_stride;
+  a.capacity = capacity;
+  a.lens = lens;
+  a.budget = budget;
+  a.sinks = sinks;
+  a.recent = recent;
+  a.keep_from = keep_from;
+  a.keep = keep;
+  a.keep_stride = keep_stride;
+  a.keep_width = keep_width;
+  a.keep_count = keep_count;
+  a.out_weight = out_weight;
+  a.out_stride = out_stride;
+  a.status = status_dev;
+  // A CTA reads 4096 positions a pass in about the time of a cluster's exchange.
+  if (capacity > 8192)
+    return pl_host::launch_pdl_cluster(pl::evict_select_kernel<true>, dim3((unsigned)num_rows * pl::kSelCluster),
+                                       dim3(pl::kSelThreads), 0, stream, pl::kSelCluster, a);
+  return pl_host::launch_pdl(pl::evict_select_kernel<false>, dim3((unsigned)num_rows), dim3(pl::kSelThreads), 0, stream,
+                             a);
+}

@@ -30,6 +30,15 @@
 //              first tile) takes a max pass first and rescales O.
 // Waits are bounded; on expiry the kernel records PL_ERR_TIMEOUT, lets its
 // copies and tensor-core work drain (bounded) and returns.
+//
+// kWindow (pl_paged_window_prefill): a query at position p sees j <= p with
+// j > p - window or j < sinks.  A pair of query tiles visits the tiles of the
+// sinks and those from its first query's window on, so the work is bounded by
+// the window; only tiles that the borders cross pay for masks.  Pages that no
+// query of the pair sees are not looked up (a cache may have given them
+// away), positions that none sees are cleared in V, and where a border of the
+// pair's masks crosses a tile, inf and NaN elements of V are replaced by zero
+// and added at the end for the rows that do see them (0 x NaN is NaN).
 #include "pl_common.cuh"
 
 namespace pl {
@@ -54,6 +63,8 @@ struct PrefillArgs {
   int64_t out_stride_t, out_stride_h;
   float* lse;  // optional [total_q, Hq], natural log
   int32_t* status;
+  int32_t window, sinks;  // kWindow only
+  const bf16* kv;         // kWindow only: the pool, read for inf / NaN elements of V
 };
 
 template <int D>
@@ -85,7 +96,7 @@ __device__ __forceinline__ float pf_exp2(float x) {
   return y;
 }
 
-template <int D>
+template <int D, bool kWindow>
 __global__ void __launch_bounds__(kPrefillThreads, 1)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap kv_map, const PrefillArgs a) {
   using C = PrefillCfg<D>;
@@ -100,7 +111,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   uint64_t* qready = sready + 6;                  // [2] Q_X staged (128 arrivals)
   uint64_t* fin = sready + 8;                     // every tensor-core op of the CTA finished
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
-  volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, issued, consumed
+  volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, issued, consumed, bad V
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int kvh = blockIdx.y;
@@ -116,7 +127,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       mbar_init(&qready[x], 128);
     }
     mbar_init(fin, 1);
-    flags[0] = flags[1] = flags[2] = 0;
+    flags[0] = flags[1] = flags[2] = flags[3] = 0;
     fence_barrier_init();
   }
   if (threadIdx.x == 32) prefetch_tensormap(&kv_map);
@@ -160,12 +171,23 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   const int t1 = min(t0 + tq2, qlen);
   int n_vis = a.causal ? kv_len - qlen + t1 : kv_len;  // kv positions the pair's queries may see
   n_vis = n_vis < 0 ? 0 : (n_vis > kv_len ? kv_len : n_vis);
-  const int ntiles = (n_vis + kPrefillN - 1) / kPrefillN;
+  // Tiles of the pair: the sinks' in front (early), then from tile `first` on.
+  int first = 0, early = 0, wlo = 0;
+  if constexpr (kWindow) {
+    const int64_t lo = (int64_t)kv_len - qlen + t0 - a.window + 1;  // first position that the first query's window holds
+    wlo = lo > 0 && n_vis > 0 ? (int)lo : 0;
+    first = wlo / kPrefillN;
+    early = min((int)(((int64_t)a.sinks + kPrefillN - 1) / kPrefillN), first);
+  }
+  const int ntiles = (n_vis + kPrefillN - 1) / kPrefillN - first + early;
   // The CTAs resident at one time mostly share a kv head and would walk the
   // same K/V tiles in lock-step, all hitting the same L2 lines; each starts
   // at its own tile instead (online softmax is order-free).
   const int rot = ntiles > 1 ? (int)(((unsigned)pair * 7u + (unsigned)kvh * 3u) % (unsigned)ntiles) : 0;
-  auto tile_of = [&](int it) { return it + rot < ntiles ? it + rot : it + rot - ntiles; };
+  auto tile_of = [&](int it) {
+    const int u = it + rot < ntiles ? it + rot : it + rot - ntiles;
+    return kWindow && u >= early ? u - early + first : u;
+  };
 
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::kTmemCols);
@@ -197,7 +219,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       if (lane < boxes) {
         const int kv = i & 1, page_idx = tile_of(i >> 1) * ppt + p;
         int32_t coord = (int32_t)(2 * a.num_pages);  // out of range: the copy writes zeros
-        if (page_idx < n_pages) {
+        bool wanted = page_idx < n_pages;
+        if constexpr (kWindow)
+          wanted = wanted && page_idx * PS < n_vis && ((page_idx + 1) * PS > wlo || page_idx * PS < a.sinks);
+        if (wanted) {
           const int32_t pid = a.kv_indices[kv_begin + page_idx];
           if (pid >= 0 && (int64_t)pid < a.num_pages)
             coord = 2 * pid + kv;
@@ -307,6 +332,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
 
     // last kv position this row may see (rows outside the tile see all)
     const int lim = (a.causal && row_ok) ? kv_len - qlen + tok : kv_len - 1;
+    // first position of this row's window (kWindow)
+    const int wl = kWindow && row_ok ? (int)max((int64_t)0, (int64_t)lim - a.window + 1) : 0;
+    auto sees = [&](int col) { return col <= lim && (!kWindow || col >= wl || col < a.sinks); };
     const float sl2 = a.scale_log2;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
@@ -318,7 +346,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       }
       tc_fence_after();
       const int kv0 = tile_of(j) * kPrefillN;
-      const bool masked = kv0 + kPrefillN - 1 > lim;  // some column of this row is masked
+      // some column of this row is masked
+      const bool masked =
+          kv0 + kPrefillN - 1 > lim || (kWindow && kv0 < wl && kv0 + kPrefillN > a.sinks);
       // P_X and O_X are free once P_X(j-1).V_{j-1} has run (S_X(j) was issued
       // after it, so this wait returns at once)
       if (j >= 1) ok = mbar_wait(&odone[x], (j - 1) & 1);
@@ -352,7 +382,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             float p1 = pf_exp2(fmaf(v[i + 1], sl2, nb));
             float s0 = v[i], s1 = v[i + 1];
             if (masked) {
-              const bool k0 = col <= lim, k1 = col + 1 <= lim;
+              const bool k0 = sees(col), k1 = sees(col + 1);
               p0 = k0 ? p0 : 0.f;
               p1 = k1 ? p1 : 0.f;
               s0 = k0 ? s0 : -INFINITY;
@@ -384,7 +414,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           tmem_ld64(s_tmem + 64 * h, v);
           if (masked) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) mx[i & 7] = fmaxf(mx[i & 7], kv0 + 64 * h + i <= lim ? v[i] : -INFINITY);
+            for (int i = 0; i < 64; ++i) mx[i & 7] = fmaxf(mx[i & 7], sees(kv0 + 64 * h + i) ? v[i] : -INFINITY);
           } else {
 #pragma unroll
             for (int i = 0; i < 64; ++i) mx[i & 7] = fmaxf(mx[i & 7], v[i]);
@@ -425,8 +455,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             float p0 = pf_exp2(fmaf(v[i], sl2, nb));
             float p1 = pf_exp2(fmaf(v[i + 1], sl2, nb));
             if (masked) {
-              p0 = col <= lim ? p0 : 0.f;
-              p1 = col + 1 <= lim ? p1 : 0.f;
+              p0 = sees(col) ? p0 : 0.f;
+              p1 = sees(col + 1) ? p1 : 0.f;
             }
             sm[(i >> 1) & 7] += p0 + p1;
             pk[i / 2] = pack_bf16x2(p0, p1);
@@ -443,7 +473,44 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       // the pool had there (0 * NaN is NaN): tile A's threads clear those V
       // rows (P_A.V_j runs first, after this tile's arrival).
       const int tail0 = kv_len - kv0, tail1 = min(kPrefillN, n_pages * PS - kv0);
-      if (x == 0 && tail0 >= 0 && tail0 < tail1) {
+      if constexpr (kWindow) {
+        // Positions hidden from the whole pair: below wlo (sinks aside) and
+        // from n_vis on.  Hidden from some of its rows: the pair's other
+        // window starts [wlo, wlo1) and its own tokens (p0, n_vis).
+        const int p0 = kv_len - qlen + t0;
+        const int wlo1 = (int)max((int64_t)wlo, (int64_t)n_vis - a.window);
+        const bool lower = kv0 < wlo1 && kv0 + kPrefillN > a.sinks, upper = kv0 + kPrefillN > p0 + 1;
+        if (x == 0 && (lower || upper)) {
+          const int item = 2 * j + 1;
+          if (mbar_wait(&full[item % kPrefillSlots], (item / kPrefillSlots) & 1)) {
+            uint8_t* vt = smem + C::kSlotOff + (item % kPrefillSlots) * C::kKVBytes;
+            const int r0 = lower ? 0 : max(0, p0 + 1 - kv0), r1 = upper ? kPrefillN : min(kPrefillN, wlo1 - kv0);
+            const int units = C::kChunks * 8;
+            for (int idx = m; idx < (r1 - r0) * units; idx += 128) {
+              const int r = r0 + idx / units, hh = (idx / 8) % C::kChunks, u = idx % 8, pos = kv0 + r;
+              const bool below = pos < wlo1 && pos >= a.sinks;
+              if (!below && pos <= p0) continue;  // every row sees it
+              uint4* at = reinterpret_cast<uint4*>(vt + hh * C::kChunkBytes + r * 128 + u * 16);
+              if (pos >= n_vis || (below && pos < wlo)) {
+                *at = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              uint4 e = *at;
+              uint32_t* w = reinterpret_cast<uint32_t*>(&e);
+              bool hit = false;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if ((w[k] & 0x7f80u) == 0x7f80u) { w[k] &= 0xffff0000u; hit = true; }
+                if ((w[k] & 0x7f800000u) == 0x7f800000u) { w[k] &= 0x0000ffffu; hit = true; }
+              }
+              if (hit) {
+                *at = e;
+                flags[3] = 1;
+              }
+            }
+          }
+        }
+      } else if (x == 0 && tail0 >= 0 && tail0 < tail1) {
         const int item = 2 * j + 1;
         if (mbar_wait(&full[item % kPrefillSlots], (item / kPrefillSlots) & 1)) {
           uint8_t* vt = smem + C::kSlotOff + (item % kPrefillSlots) * C::kKVBytes;
@@ -483,6 +550,28 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = 0.f;
       }
+      if constexpr (kWindow) {
+        if (flags[3] != 0 && row_ok) {
+          // the inf / NaN elements that were taken out of the pair's border positions, where this row sees them
+          const int p0 = kv_len - qlen + t0;
+          const int wlo1 = (int)max((int64_t)wlo, (int64_t)n_vis - a.window);
+          auto add = [&](int from, int to, int keep) {
+            for (int pos = max(from, 0); pos < to; ++pos) {
+              if (pos < keep || !sees(pos)) continue;
+              const int32_t pid = a.kv_indices[kv_begin + pos / PS];
+              if (pid < 0 || (int64_t)pid >= a.num_pages) continue;
+              const bf16* vrow = a.kv + ((((int64_t)pid * 2 + 1) * PS + pos % PS) * gridDim.y + kvh) * D + 32 * c;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float e = bf2f(vrow[i]);
+                if (!isfinite(e)) v[i] += e;
+              }
+            }
+          };
+          add(wlo, min(wlo1, p0 + 1), a.sinks);
+          add(p0 + 1, n_vis, 0);
+        }
+      }
       if (row_ok && !flags[0]) {
         uint32_t pk[16];
 #pragma unroll
@@ -517,24 +606,22 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
 // =================================================================== host
 namespace {
 
-template <int D>
+template <int D, bool kWindow>
 int32_t launch_prefill(const CUtensorMap& map, const pl::PrefillArgs& a, int grid_x, int hkv, void* stream) {
   using C = pl::PrefillCfg<D>;
-  auto kern = pl::paged_prefill_kernel<D>;
+  auto kern = pl::paged_prefill_kernel<D, kWindow>;
   int32_t st = pl_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (st != PL_OK) return st;
   return pl_host::launch_pdl(kern, dim3(grid_x, hkv), dim3(pl::kPrefillThreads), C::kSmemBytes, stream, map, a);
 }
 
-}  // namespace
-
-extern "C" int32_t pl_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv_cache,
-                                    int64_t num_pages, const int32_t* qo_indptr, const int32_t* kv_indptr,
-                                    const int32_t* kv_indices, const int32_t* kv_last_page_len, int32_t batch,
-                                    int32_t total_q, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
-                                    int32_t page_size, float sm_scale, int32_t causal, void* out,
-                                    int64_t out_stride_t, int64_t out_stride_h, float* out_lse, int32_t* status_dev,
-                                    void* stream) {
+// window 0: none (pl_paged_prefill)
+int32_t run_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv_cache, int64_t num_pages,
+                    const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                    const int32_t* kv_last_page_len, int32_t batch, int32_t total_q, int32_t num_qo_heads,
+                    int32_t num_kv_heads, int32_t head_dim, int32_t page_size, float sm_scale, int32_t causal,
+                    int32_t window, int32_t sinks, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                    float* out_lse, int32_t* status_dev, void* stream) {
   if (q == nullptr || kv_cache == nullptr || qo_indptr == nullptr || kv_indptr == nullptr || kv_indices == nullptr ||
       kv_last_page_len == nullptr || out == nullptr || batch < 0 || total_q < 0 || num_pages <= 0 ||
       num_kv_heads <= 0 || num_qo_heads <= 0 || num_qo_heads % num_kv_heads != 0)
@@ -578,6 +665,39 @@ extern "C" int32_t pl_paged_prefill(const void* q, int64_t q_stride_t, int64_t q
   // every request contributes ceil(len / 2tq) <= len / 2tq + 1 tile pairs
   const int64_t grid_x = ((int64_t)total_q + 2 * a.tq - 1) / (2 * a.tq) + batch;
   if (grid_x > 0x7FFFFFFF) return PL_ERR_INVALID_ARGUMENT;
-  if (head_dim == 128) return launch_prefill<128>(map, a, (int)grid_x, num_kv_heads, stream);
-  return launch_prefill<64>(map, a, (int)grid_x, num_kv_heads, stream);
+  a.window = window;
+  a.sinks = sinks;
+  a.kv = static_cast<const pl::bf16*>(kv_cache);
+  if (window > 0)
+    return head_dim == 128 ? launch_prefill<128, true>(map, a, (int)grid_x, num_kv_heads, stream)
+                           : launch_prefill<64, true>(map, a, (int)grid_x, num_kv_heads, stream);
+  if (head_dim == 128) return launch_prefill<128, false>(map, a, (int)grid_x, num_kv_heads, stream);
+  return launch_prefill<64, false>(map, a, (int)grid_x, num_kv_heads, stream);
+}
+
+}  // namespace
+
+extern "C" int32_t pl_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv_cache,
+                                    int64_t num_pages, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                    const int32_t* kv_indices, const int32_t* kv_last_page_len, int32_t batch,
+                                    int32_t total_q, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                                    int32_t page_size, float sm_scale, int32_t causal, void* out,
+                                    int64_t out_stride_t, int64_t out_stride_h, float* out_lse, int32_t* status_dev,
+                                    void* stream) {
+  return run_prefill(q, q_stride_t, q_stride_h, kv_cache, num_pages, qo_indptr, kv_indptr, kv_indices, kv_last_page_len,
+                     batch, total_q, num_qo_heads, num_kv_heads, head_dim, page_size, sm_scale, causal, 0, 0, out,
+                     out_stride_t, out_stride_h, out_lse, status_dev, stream);
+}
+
+extern "C" int32_t pl_paged_window_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv_cache,
+                                           int64_t num_pages, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                           const int32_t* kv_indices, const int32_t* kv_last_page_len, int32_t batch,
+                                           int32_t total_q, int32_t num_qo_heads, int32_t num_kv_heads,
+                                           int32_t head_dim, int32_t page_size, float sm_scale, int32_t window,
+                                           int32_t sinks, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                                           float* out_lse, int32_t* status_dev, void* stream) {
+  if (window < 1 || sinks < 0 || !(sm_scale > 0.f)) return PL_ERR_INVALID_ARGUMENT;
+  return run_prefill(q, q_stride_t, q_stride_h, kv_cache, num_pages, qo_indptr, kv_indptr, kv_indices, kv_last_page_len,
+                     batch, total_q, num_qo_heads, num_kv_heads, head_dim, page_size, sm_scale, 1, window, sinks, out,
+                     out_stride_t, out_stride_h, out_lse, status_dev, stream);
 }

@@ -1136,3 +1136,342 @@ def paged_sparse_decode(
          ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), ptr(status),
          stream_handle())
     return out
+
+
+# ------------------------------------------------ sliding window and sinks
+def _need_out(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(q)
+    if out.dtype is not torch.bfloat16:
+        raise TypeError(f"out must be {torch.bfloat16}, got {out.dtype}")
+    if out.shape != q.shape or out.stride(-1) != 1:
+        raise ValueError("out must have q's shape and unit last stride")
+    return out
+
+
+def _need_queries(q: torch.Tensor, rows: str = "tokens") -> None:
+    _need(q, torch.bfloat16, "q")
+    if q.dim() != 3 or q.stride(-1) != 1:
+        raise ValueError(f"q must be [{rows}, qo_heads, head_dim] with unit last stride")
+
+
+def _need_window(window: int, sinks: int) -> None:
+    if window < 1 or sinks < 0:
+        raise ValueError("window must be at least 1 and sinks at least 0")
+
+
+@lru_cache(maxsize=256)
+def _window_decode_workspace_bytes(num_qo_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    return int(_capi.load_library().pl_window_decode_workspace_bytes(num_qo_heads, num_kv_heads, head_dim))
+
+
+@lru_cache(maxsize=256)
+def _kv4_decode_workspace_bytes(num_qo_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    return int(_capi.load_library().pl_kv4_decode_workspace_bytes(num_qo_heads, num_kv_heads, head_dim))
+
+
+def paged_window_prefill(
+    q: torch.Tensor,
+    kv_cache: torch.Tensor,
+    qo_indptr: torch.Tensor,
+    kv_indptr: torch.Tensor,
+    kv_indices: torch.Tensor,
+    kv_last_page_len: torch.Tensor,
+    *,
+    window: int,
+    sinks: int = 0,
+    sm_scale: float | None = None,
+    out: torch.Tensor | None = None,
+    out_lse: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Ragged causal prefill where a query at position p sees the last
+    ``window`` positions up to p and the first ``sinks`` of its request
+    (pl_paged_window_prefill); arguments as :func:`paged_prefill`."""
+
+    _need_cuda(q, kv_cache, out)
+    _need_queries(q)
+    _need_pool(kv_cache)
+    _need_window(window, sinks)
+    total_q, hq, d = q.shape
+    num_pages, _, page_size, hkv, d2 = kv_cache.shape
+    if d2 != d:
+        raise ValueError("q and kv_cache head_dim differ")
+    batch = qo_indptr.numel() - 1
+    _vecs(torch.int32, "qo_indptr kv_indptr kv_indices kv_last_page_len",
+          (qo_indptr, kv_indptr, kv_indices, kv_last_page_len), (1, batch + 1, 0, batch))
+    out = _need_out(out, q)
+    if out_lse is not None:
+        _vecs(torch.float32, "out_lse", (out_lse,), (total_q * hq,))
+    if batch == 0 or total_q == 0:
+        return out
+    if kv_indices.numel() == 0:  # no request has a cached position: nothing to see
+        if out_lse is not None:
+            out_lse.fill_(-math.inf)
+        return out.zero_()
+    call("pl_paged_window_prefill", q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), num_pages,
+         qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), batch,
+         total_q, hq, hkv, d, page_size, d ** -0.5 if sm_scale is None else float(sm_scale), window, sinks,
+         out.data_ptr(), out.stride(0), out.stride(1), ptr(out_lse), ptr(status), stream_handle())
+    return out
+
+
+def _line_decode(fn: str, q, kv_cache, d, indptr, indices, last_page_len, window, sinks, sm_scale, out, out_lse,
+                 workspace, need, status) -> torch.Tensor:
+    """The checks and the call that the window and the 4-bit decode share."""
+
+    batch, hq, _ = q.shape
+    num_pages, _, page_size, hkv, _ = kv_cache.shape
+    _vecs(torch.int32, "indptr indices last_page_len", (indptr, indices, last_page_len), (batch + 1, 0, batch))
+    out = _need_out(out, q)
+    if out_lse is not None:
+        _vecs(torch.float32, "out_lse", (out_lse,), (batch * hq,))
+    workspace = _workspace(workspace, need(hq, hkv, d), q)
+    call(fn, q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), num_pages, indptr.data_ptr(),
+         indices.data_ptr(), last_page_len.data_ptr(), indices.numel(), batch, hq, hkv, d, page_size,
+         d ** -0.5 if sm_scale is None else float(sm_scale), window, sinks, out.data_ptr(), out.stride(0),
+         out.stride(1), ptr(out_lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(), ptr(status),
+         stream_handle())
+    return out
+
+
+def paged_window_decode(
+    q: torch.Tensor,
+    kv_cache: torch.Tensor,
+    indptr: torch.Tensor,
+    indices: torch.Tensor,
+    last_page_len: torch.Tensor,
+    *,
+    window: int,
+    sinks: int = 0,
+    sm_scale: float | None = None,
+    out: torch.Tensor | None = None,
+    out_lse: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Paged decode of one token per row over its last ``window`` cached
+    positions and the first ``sinks`` (pl_paged_window_decode): q [B, Hq, D]
+    bf16, ``out`` bf16 like q, ``out_lse`` fp32 [B, Hq]."""
+
+    _need_cuda(q, kv_cache, out, workspace)
+    _need_queries(q, "batch")
+    _need_pool(kv_cache)
+    _need_window(window, sinks)
+    if kv_cache.size(4) != q.size(2):
+        raise ValueError("q and kv_cache head_dim differ")
+    return _line_decode("pl_paged_window_decode", q, kv_cache, q.size(2), indptr, indices, last_page_len, window, sinks,
+                        sm_scale, out, out_lse, workspace, _window_decode_workspace_bytes, status)
+
+
+# -------------------------------------------------------- a cache in 4 bits
+def kv4_record_bytes(head_dim: int) -> int:
+    """Bytes of one head of one token's K (or V) in a 4-bit cache: its last
+    dimension, uint8 [pages, 2, page_size, kv_heads, record] (pl_kv4_append)."""
+
+    return head_dim // 2 + 16
+
+
+def _need_kv4(cache: torch.Tensor, head_dim: int) -> None:
+    if cache.dtype is not torch.uint8:
+        raise TypeError(f"kv4_cache must be {torch.uint8}, got {cache.dtype}")
+    if cache.dim() != 5 or cache.size(1) != 2 or not cache.is_contiguous():
+        raise ValueError("kv4_cache must be a contiguous [pages, 2, page_size, kv_heads, record] tensor")
+    if cache.size(4) != kv4_record_bytes(head_dim):
+        raise ValueError(f"a record of head_dim {head_dim} has {kv4_record_bytes(head_dim)} bytes, "
+                         f"kv4_cache has {cache.size(4)}")
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, kv4_cache: torch.Tensor, page_id: torch.Tensor,
+               page_offset: torch.Tensor, status: torch.Tensor | None = None) -> None:
+    """Quantise k, v [T, Hkv, D] bf16 into the 4-bit pool at (page_id[t],
+    page_offset[t]) (pl_kv4_append)."""
+
+    _need_cuda(k, v, kv4_cache)
+    _need(k, torch.bfloat16, "k")
+    _need(v, torch.bfloat16, "v")
+    if k.dim() != 3 or v.shape != k.shape:
+        raise ValueError("k and v must be [T, Hkv, D]")
+    t, hkv, d = k.shape
+    _need_kv4(kv4_cache, d)
+    if kv4_cache.size(3) != hkv:
+        raise ValueError("k and kv4_cache kv heads differ")
+    _vecs(torch.int32, "page_id page_offset", (page_id, page_offset), (t, t))
+    for x in (k, v):
+        if t and (x.stride(2) != 1 or (hkv > 1 and x.stride(1) != d)):
+            raise ValueError("k/v must be [T, Hkv, D] with contiguous heads")
+    call("pl_kv4_append", ptr(k), k.stride(0), ptr(v), v.stride(0), ptr(kv4_cache), kv4_cache.size(0), ptr(page_id),
+         ptr(page_offset), t, hkv, d, kv4_cache.size(2), ptr(status), stream_handle())
+
+
+def kv4_expand(kv4_cache: torch.Tensor, page_ids: torch.Tensor, *, out: torch.Tensor,
+               status: torch.Tensor | None = None) -> torch.Tensor:
+    """Pages ``page_ids`` (int32 [n]; -1: left out) of a 4-bit pool as bf16 pages
+    ``out`` [n, 2, page_size, Hkv, D] (pl_kv4_expand), a pool that the prompt's
+    attention reads."""
+
+    _need_cuda(kv4_cache, out)
+    _need_pool(out)
+    _need_kv4(kv4_cache, out.size(4))
+    n = page_ids.numel()
+    _vecs(torch.int32, "page_ids", (page_ids,), (0,))
+    if out.size(0) < n or out.shape[1:4] != kv4_cache.shape[1:4]:
+        raise ValueError("out must be [n, 2, page_size, kv_heads, head_dim] of kv4_cache's page")
+    call("pl_kv4_expand", ptr(kv4_cache), kv4_cache.size(0), ptr(page_ids), n, out.size(3), out.size(4), out.size(2),
+         ptr(out), ptr(status), stream_handle())
+    return out
+
+
+def paged_kv4_decode(
+    q: torch.Tensor,
+    kv4_cache: torch.Tensor,
+    indptr: torch.Tensor,
+    indices: torch.Tensor,
+    last_page_len: torch.Tensor,
+    *,
+    window: int | None = None,
+    sinks: int = 0,
+    sm_scale: float | None = None,
+    out: torch.Tensor | None = None,
+    out_lse: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Paged decode of one token per row straight over a 4-bit pool
+    (pl_paged_kv4_decode): q [B, Hq, D] bf16; ``window`` and ``sinks`` as
+    :func:`paged_window_decode` (None: the whole context)."""
+
+    _need_cuda(q, kv4_cache, out, workspace)
+    _need_queries(q, "batch")
+    _need_kv4(kv4_cache, q.size(2))
+    if window is None:
+        window, sinks = 0, 0
+    else:
+        _need_window(window, sinks)
+    return _line_decode("pl_paged_kv4_decode", q, kv4_cache, q.size(2), indptr, indices, last_page_len, window, sinks,
+                        sm_scale, out, out_lse, workspace, _kv4_decode_workspace_bytes, status)
+
+
+# ------------------------------------------- eviction by attention weight
+@lru_cache(maxsize=256)
+def _decode_weights_workspace_bytes(batch: int, num_qo_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
+                                    total_pages: int) -> int:
+    return int(_capi.load_library().pl_decode_weights_workspace_bytes(batch, num_qo_heads, num_kv_heads, head_dim,
+                                                                      page_size, total_pages))
+
+
+@lru_cache(maxsize=256)
+def _prefill_weights_workspace_bytes(num_kv_heads: int, page_size: int, total_pages: int) -> int:
+    return int(_capi.load_library().pl_prefill_weights_workspace_bytes(num_kv_heads, page_size, total_pages))
+
+
+def paged_decode_weights(
+    q: torch.Tensor,
+    kv_cache: torch.Tensor,
+    indptr: torch.Tensor,
+    indices: torch.Tensor,
+    last_page_len: torch.Tensor,
+    weight: torch.Tensor,
+    *,
+    sm_scale: float | None = None,
+    out: torch.Tensor | None = None,
+    out_lse: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Paged decode of one token per row that also adds, over all query heads,
+    the softmax weight of every cached position to ``weight`` fp32
+    [B, capacity] (pl_paged_decode_weights)."""
+
+    _need_cuda(q, kv_cache, out, workspace)
+    _need_queries(q, "batch")
+    _need_pool(kv_cache)
+    batch, hq, d = q.shape
+    num_pages, _, page_size, hkv, d2 = kv_cache.shape
+    if d2 != d:
+        raise ValueError("q and kv_cache head_dim differ")
+    _vecs(torch.int32, "indptr indices last_page_len", (indptr, indices, last_page_len), (batch + 1, 0, batch))
+    w_stride, w_cap = _need_rows(weight, "weight", batch, torch.float32)
+    out = _need_out(out, q)
+    if out_lse is not None:
+        _vecs(torch.float32, "out_lse", (out_lse,), (batch * hq,))
+    total = indices.numel()
+    workspace = _workspace(workspace, _decode_weights_workspace_bytes(batch, hq, hkv, d, page_size, total), q)
+    call("pl_paged_decode_weights", q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), num_pages,
+         indptr.data_ptr(), indices.data_ptr(), last_page_len.data_ptr(), total, batch, hq, hkv, d, page_size,
+         d ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), out.stride(0), out.stride(1),
+         ptr(out_lse), weight.data_ptr(), w_stride, w_cap, workspace.data_ptr(),
+         workspace.numel() * workspace.element_size(), ptr(status), stream_handle())
+    return out
+
+
+def paged_prefill_weights(
+    q: torch.Tensor,
+    kv_cache: torch.Tensor,
+    qo_indptr: torch.Tensor,
+    kv_indptr: torch.Tensor,
+    kv_indices: torch.Tensor,
+    kv_last_page_len: torch.Tensor,
+    lse: torch.Tensor,
+    weight: torch.Tensor,
+    *,
+    sm_scale: float | None = None,
+    workspace: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Adds to ``weight`` fp32 [requests, capacity] what the tokens q
+    [total_q, Hq, D] (the last positions of their requests) give every cached
+    position, over tokens and heads, from the log sums ``lse`` fp32
+    [total_q, Hq] of their causal attention (pl_paged_prefill_weights)."""
+
+    _need_cuda(q, kv_cache, workspace)
+    _need_queries(q)
+    _need_pool(kv_cache)
+    total_q, hq, d = q.shape
+    num_pages, _, page_size, hkv, d2 = kv_cache.shape
+    if d2 != d:
+        raise ValueError("q and kv_cache head_dim differ")
+    batch = qo_indptr.numel() - 1
+    _vecs(torch.int32, "qo_indptr kv_indptr kv_indices kv_last_page_len",
+          (qo_indptr, kv_indptr, kv_indices, kv_last_page_len), (1, batch + 1, 0, batch))
+    _vecs(torch.float32, "lse", (lse,), (total_q * hq,))
+    w_stride, w_cap = _need_rows(weight, "weight", batch, torch.float32)
+    total = kv_indices.numel()
+    workspace = _workspace(workspace, _prefill_weights_workspace_bytes(hkv, page_size, total), q)
+    call("pl_paged_prefill_weights", q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), num_pages,
+         qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), total, batch,
+         total_q, hq, hkv, d, page_size, d ** -0.5 if sm_scale is None else float(sm_scale), lse.data_ptr(),
+         weight.data_ptr(), w_stride, w_cap, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+         ptr(status), stream_handle())
+    return weight
+
+
+def evict_select(weight: torch.Tensor, lens: torch.Tensor, budget: int, *, sinks: int, recent: int,
+                 keep_from: torch.Tensor, keep: torch.Tensor, keep_count: torch.Tensor, out_weight: torch.Tensor,
+                 status: torch.Tensor | None = None) -> None:
+    """The ``budget`` positions that every row of ``lens`` (int32 [rows]) cached
+    positions keeps (pl_evict_select): its first ``sinks``, its last
+    ``recent`` and the others of the highest ``weight`` fp32 [rows, capacity].
+    ``keep_from``, ``keep`` int32 [rows, >= budget - sinks] and ``keep_count``
+    are :func:`cache_compact`'s arguments; ``out_weight`` like weight, a
+    buffer of its own, receives the moved weights."""
+
+    rows = lens.numel()
+    _vecs(torch.int32, "lens keep_from keep_count", (lens, keep_from, keep_count), (rows, rows, rows))
+    if sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError("a budget needs sinks >= 0, recent >= 0 and sinks + recent <= budget")
+    w_stride, w_cap = _need_rows(weight, "weight", rows, torch.float32)
+    o_stride, o_cap = _need_rows(out_weight, "out_weight", rows, torch.float32)
+    k_stride, k_width = _need_rows(keep, "keep", rows)
+    if o_cap != w_cap:
+        raise ValueError("weight and out_weight differ in width")
+    if k_width < budget - sinks:
+        raise ValueError("keep needs budget - sinks columns")
+    if w_cap and rows:
+        w0, o0 = weight.data_ptr(), out_weight.data_ptr()
+        span = 4 * ((rows - 1) * max(w_stride, o_stride) + w_cap)
+        if w0 < o0 + span and o0 < w0 + span:
+            raise ValueError("weight and out_weight must not overlap")
+    call("pl_evict_select", weight.data_ptr(), w_stride, w_cap, lens.data_ptr(), rows, budget, sinks, recent,
+         keep_from.data_ptr(), keep.data_ptr(), k_stride, k_width, keep_count.data_ptr(), out_weight.data_ptr(),
+         o_stride, ptr(status), stream_handle())
