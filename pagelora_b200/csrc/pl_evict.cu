@@ -2,6 +2,8 @@
 // tokens give the cached positions (pl_paged_prefill_weights), and the choice
 // of the positions to keep (pl_evict_select).  The decode step's weights come
 // with its attention (pl_window_decode.cu); pl_cache_compact moves what stays.
+#include <type_traits>
+
 #include "pl_line_decode.cuh"
 
 namespace pl {
@@ -9,23 +11,33 @@ namespace pl {
 // ------------------------------------------------------- weights of a prompt
 // weight[b][j] += sum over query tokens i and heads h of exp(scale q_ih.k_j -
 // lse_ih), i at position p_i >= j.  The attention that gave lse has read V and
-// written O; this is its score product alone, transposed: one CTA takes a
-// (request, tile of 128 positions, kv head), keeps K in shared memory and
-// streams the query tiles (128 rows = tq tokens x group heads) that see it.
-//   warp 0     TMA: K once, then the query tiles through a ring;
-//   warp 1     tcgen05.mma S^T = K.Q^T into one of four TMEM buffers;
-//   warps 2-9  two groups of four take the tiles in turn: a thread is a
-//              position, reads its 128 scores, and adds 2^(s - lse) into one
-//              register, so nothing is exchanged between threads; the columns'
-//              log sums stand in shared memory.
-// The kv heads' sums go to the workspace and are added in head order by
-// prompt_weight_add_kernel, so two runs give the same bits.  Bound by the
-// exponentials: a tile has 16384 of them (1024 cycles at 16 a cycle) and 512
-// cycles of products at head_dim 128.
-constexpr int kPwThreads = 320;
-constexpr int kPwM = 128;      // positions, and rows of a query tile
-constexpr int kPwSlots = 4;    // query tiles in flight
-constexpr int kPwBufs = 4;     // score buffers
+// written O; this is its score product alone, transposed.  One CTA takes a
+// (request, run of 256 positions, kv head, chunk of the query tiles), keeps
+// the run's K in shared memory and streams the query tiles (128 rows = tq
+// tokens x the group's heads) that see it.
+//   warp 0     TMA: K once, then the query tiles through a ring, and the log
+//              sums of their columns;
+//   warp 1     tcgen05.mma S^T = K.Q^T, two products of 128 positions a query
+//              tile, each into one of two TMEM buffers;
+//   warps 2-17 four groups of four, one for each buffer: a thread is a
+//              position, reads its 128 scores, and adds 2^(s - lse) into its
+//              own sums, so nothing is exchanged between threads.
+// The sums of the kv heads and chunks go to the workspace and are added in
+// this order by prompt_weight_add_kernel, so two runs give the same bits.
+// 128 x 128 scores have 1024 cycles of exponentials on the multi-function
+// units (16 a cycle) beside 512 cycles of products at head_dim 128, so a
+// quarter of the pairs is computed on the FMA pipe instead (pw_exp2_pair, nine
+// cycles an element; none 393, a quarter 381, half 421 us at 8192 tokens, 32
+// heads).  Measured 374 us there, 0.73 PFLOP/s: 1250 cycles a product, of
+// which the chain product -> commit -> read -> exponentials of a buffer and
+// its successor's is what is left; tensor memory holds no third one.
+constexpr int kPwM = 128;                   // positions of a product
+constexpr int kPwTiles = 2;                 // products a CTA: 256 positions
+constexpr int kPwN = 128;                   // rows of a query tile
+constexpr int kPwThreads = 32 * (2 + 8 * kPwTiles);
+constexpr int kPwSlots = 4;                 // query tiles in flight
+constexpr int kPwLse = kPwSlots + 4;        // log sums: of tiles whose scores are not added yet
+constexpr int kPwChunks = 4;                // at most as many chunks of a request's query tiles
 
 struct PromptWeightArgs {
   const int32_t* qo_indptr;
@@ -33,32 +45,61 @@ struct PromptWeightArgs {
   const int32_t* kv_indices;
   const int32_t* kv_last;
   int64_t num_pages, total_pages;
-  int32_t batch, total_q, num_qo_heads, group, tq, page_size;
+  int32_t batch, total_q, num_qo_heads, num_kv_heads, group, page_size;
+  int32_t tq;            // tokens of a tile
+  int32_t chunk;         // token tiles of a chunk
   float scale_log2;
   const float* lse;   // [total_q, Hq]
-  float* partial;     // [Hkv][total_pages * page_size]
+  float* partial;     // [kPwChunks][Hkv][total_pages * page_size]
   int32_t* status;
 };
 
 template <int D>
 struct PromptWeightCfg {
   static constexpr int kChunks = D / 64;
-  static constexpr int kChunkBytes = kPwM * 128;
-  static constexpr int kTileBytes = kChunks * kChunkBytes;
-  static constexpr int kSlotOff = kTileBytes;                      // behind K
-  static constexpr int kLseOff = kSlotOff + kPwSlots * kTileBytes; // [2 groups][2][128]
-  static constexpr int kSumOff = kLseOff + 4 * kPwM * 4;           // [128]
-  static constexpr int kBarOff = kSumOff + kPwM * 4;               // kfull qfull[4] qempty[4] sready[4] sfree[4] fin
-  static constexpr int kMiscOff = kBarOff + (2 + 2 * kPwSlots + 2 * kPwBufs) * 8;
-  static constexpr int kSmemBytes = 1024 + kMiscOff + 64;
+  static constexpr int kKChunkBytes = kPwM * 128;                   // 64 channels of 128 positions
+  static constexpr int kKBytes = kChunks * kKChunkBytes;
+  static constexpr int kQChunkBytes = kPwN * 128;
+  static constexpr int kQBytes = kChunks * kQChunkBytes;
+  static constexpr int kSlotOff = kPwTiles * kKBytes;               // behind K
+  static constexpr int kLseOff = kSlotOff + kPwSlots * kQBytes;     // [kPwLse][128]
+  static constexpr int kBarOff = kLseOff + kPwLse * kPwN * 4;       // kfull qfull[] qempty[] sready[][2] sfree[][2] fin
+  static constexpr int kSumOff = kBarOff + (2 + 2 * kPwSlots + 4 * kPwTiles) * 8;  // [tiles][128]
+  static constexpr int kMiscOff = kSumOff + kPwTiles * kPwM * 4;
+  static constexpr int kSmemBytes = 1024 + kMiscOff + 80;
   static_assert(kSmemBytes <= 232448, "tiles exceed the shared-memory limit");
 };
 
-// Request and tile of positions that block `x` of the line of tiles takes; a
-// table outside kv_indices has none.  One warp; false past the last tile.
+// 2^x of a pair by range reduction to [-1/2, 1/2] and a polynomial of degree 5
+// of least relative error there, 1 at 0 (9.2e-8; 1.9e-7 with fp32's roundings,
+// where the multi-function unit has 2.4e-7).  x below -127 counts as -127,
+// whose bits come out as 0; NaN stays NaN.
+__device__ __forceinline__ float2 pw_exp2_pair(float2 x) {
+  auto clamp = [](float v) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(r) : "f"(v));  // -127
+    return r;
+  };
+  auto both = [](float v) { return make_float2(v, v); };
+  x = make_float2(clamp(x.x), clamp(x.y));
+  const float2 r = add_f32x2(x, both(12582912.f));  // the nearest whole number, in the low bits
+  const float2 n = add_f32x2(r, both(-12582912.f));
+  const float2 f = fma_f32x2(n, both(-1.f), x);
+  float2 p = fma_f32x2(both(0.001326458528637886f), f, both(0.0096714673563838f));
+  p = fma_f32x2(p, f, both(0.05550733581185341f));
+  p = fma_f32x2(p, f, both(0.24022242426872253f));
+  p = fma_f32x2(p, f, both(0.6931470036506653f));
+  p = fma_f32x2(p, f, both(1.f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
+}
+
+// Request and run of positions that block `x` of the line of runs takes; a
+// table outside kv_indices has none.  One warp; false past the last run.
 struct PwSpan {
-  int req, tile, kv_begin, n_pages, kv_len, q0, qlen;
+  int req, run, kv_begin, n_pages, kv_len, q0, qlen;
 };
+constexpr int kPwRun = kPwTiles * kPwM;
 
 __device__ __forceinline__ int pw_kv_len(const PromptWeightArgs& a, int b, bool report) {
   const int k0 = a.kv_indptr[b], k1 = a.kv_indptr[b + 1];
@@ -73,13 +114,19 @@ __device__ __forceinline__ int pw_kv_len(const PromptWeightArgs& a, int b, bool 
   return q1 > q0 ? len : 0;
 }
 
+// First token tile whose queries see position `pos` of a request.
+__device__ __forceinline__ int pw_first(const PromptWeightArgs& a, int pos, int kv_len, int qlen) {
+  const int p0 = kv_len - qlen;
+  return pos > p0 ? (pos - p0) / a.tq : 0;
+}
+
 __device__ __forceinline__ bool pw_find(const PromptWeightArgs& a, int x, PwSpan& s) {
   const int lane = threadIdx.x % 32;
   int before = 0;
   for (int base = 0; base < a.batch; base += 32) {
     const int b = base + lane;
     const int len = b < a.batch ? pw_kv_len(a, b, x == 0) : 0;
-    const int n = (len + kPwM - 1) / kPwM;
+    const int n = (len + kPwRun - 1) / kPwRun;
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -90,7 +137,7 @@ __device__ __forceinline__ bool pw_find(const PromptWeightArgs& a, int x, PwSpan
     if (hit != 0) {
       const int src = __ffs(hit) - 1;
       s.req = base + src;
-      s.tile = x - (before + __shfl_sync(0xffffffffu, incl - n, src));
+      s.run = x - (before + __shfl_sync(0xffffffffu, incl - n, src));
       s.kv_len = __shfl_sync(0xffffffffu, len, src);
       s.kv_begin = a.kv_indptr[s.req];
       s.n_pages = a.kv_indptr[s.req + 1] - s.kv_begin;
@@ -111,24 +158,24 @@ __global__ void __launch_bounds__(kPwThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
-  uint64_t* qfull = kfull + 1;              // [slots] query tile landed
+  uint64_t* qfull = kfull + 1;              // [slots] query tile and log sums landed
   uint64_t* qempty = qfull + kPwSlots;      // [slots] query tile read
-  uint64_t* sready = qempty + kPwSlots;     // [bufs] scores in TMEM
-  uint64_t* sfree = sready + kPwBufs;       // [bufs] scores read (4 warps)
-  uint64_t* fin = sfree + kPwBufs;          // every tensor-core op finished
+  uint64_t* sready = qempty + kPwSlots;     // [tiles][2] scores in TMEM
+  uint64_t* sfree = sready + 2 * kPwTiles;  // [tiles][2] scores read (4 warps)
+  uint64_t* fin = sfree + 2 * kPwTiles;     // every tensor-core op finished
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
   volatile int32_t* flags = reinterpret_cast<volatile int32_t*>(smem + C::kMiscOff + 16);  // abort, issued, consumed
   PwSpan* span = reinterpret_cast<PwSpan*>(smem + C::kMiscOff + 32);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int kvh = blockIdx.y;
+  const int kvh = blockIdx.x % a.num_kv_heads, chunk = blockIdx.x / a.num_kv_heads % kPwChunks;
 
   if (threadIdx.x == 0) {
     mbar_init(kfull, 1);
     for (int i = 0; i < kPwSlots; ++i) {
-      mbar_init(&qfull[i], 1);
+      mbar_init(&qfull[i], 33);  // the copies, and the lanes' log sums
       mbar_init(&qempty[i], 1);
     }
-    for (int i = 0; i < kPwBufs; ++i) {
+    for (int i = 0; i < 2 * kPwTiles; ++i) {
       mbar_init(&sready[i], 1);
       mbar_init(&sfree[i], 4);
     }
@@ -145,172 +192,231 @@ __global__ void __launch_bounds__(kPwThreads, 1)
   if (warp == 0) {
     PwSpan s = {};
     s.req = -1;
-    pw_find(a, blockIdx.x, s);
+    pw_find(a, blockIdx.x / a.num_kv_heads / kPwChunks, s);
     if (lane == 0) *span = s;
   }
+  __syncthreads();
+  const PwSpan sp = *span;
+  const int PS = a.page_size, kv0 = sp.run * kPwRun;
+  // token tiles [j0, j1) of this chunk see the run
+  const int j0 = max(chunk * a.chunk, pw_first(a, kv0, sp.kv_len, sp.qlen));
+  const int j1 = min((chunk + 1) * a.chunk, (sp.qlen + a.tq - 1) / a.tq);
+  if (sp.req < 0 || j0 >= j1) return;  // nothing was started
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  const int rows = a.tq * a.group;  // rows of a query tile in use; the others are 0
+  for (int i = threadIdx.x; i < kPwSlots * C::kChunks * (kPwN - rows) * 8; i += kPwThreads) {
+    const int c = i / ((kPwN - rows) * 8), u = i % ((kPwN - rows) * 8);
+    reinterpret_cast<uint4*>(smem + C::kSlotOff + c * C::kQChunkBytes + rows * 128)[u] = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const PwSpan sp = *span;
-  const int PS = a.page_size;
-  const int kv0 = sp.tile * kPwM;
-  const int p_first = sp.kv_len - sp.qlen;                       // position of the request's first query
-  const int j0 = sp.req >= 0 && kv0 > p_first ? (kv0 - p_first) / a.tq : 0;  // first query tile that sees the tile
-  const int j1 = sp.req >= 0 ? (sp.qlen + a.tq - 1) / a.tq : 0;
-  const int n = j1 > j0 ? j1 - j0 : 0;
-  const int rows = a.tq * a.group;                               // rows of a query tile in use
+  const int n = j1 - j0;
+  const int p_first = sp.kv_len - sp.qlen;
+  const int tiles = min(kPwTiles, (sp.kv_len - kv0 + kPwM - 1) / kPwM);
+  // the first of this CTA's tiles that sees product x
+  auto first_of = [&](int x) { return max(0, pw_first(a, kv0 + x * kPwM, sp.kv_len, sp.qlen) - j0); };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    int i = 0;
-    if (n > 0) {
-      const int ppt = kPwM / PS, boxes = ppt * C::kChunks;  // <= 16
+    const int ppt = kPwM / PS, boxes = ppt * C::kChunks;  // <= 16
+    {
       const int p = lane / C::kChunks, hh = lane % C::kChunks;
-      if (lane == 0) mbar_arrive_expect_tx(kfull, C::kTileBytes);
+      if (lane == 0) mbar_arrive_expect_tx(kfull, tiles * C::kKBytes);
       __syncwarp();
-      if (lane < boxes) {
-        const int page = sp.tile * ppt + p;
-        int32_t coord = (int32_t)(2 * a.num_pages);  // out of range: zeros
-        if (page < sp.n_pages) {
-          const int32_t pid = a.kv_indices[sp.kv_begin + page];
-          if (pid >= 0 && (int64_t)pid < a.num_pages)
-            coord = 2 * pid;
-          else
-            set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
+      for (int x = 0; x < tiles; ++x) {
+        if (lane < boxes) {
+          const int page = (kv0 / kPwM + x) * ppt + p;
+          int32_t coord = (int32_t)(2 * a.num_pages);  // out of range: zeros
+          if (page < sp.n_pages) {
+            const int32_t pid = a.kv_indices[sp.kv_begin + page];
+            if (pid >= 0 && (int64_t)pid < a.num_pages)
+              coord = 2 * pid;
+            else
+              set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
+          }
+          tma_load_4d(smem + x * C::kKBytes + hh * C::kKChunkBytes + p * PS * 128, &kv_map, hh * 64, kvh, 0, coord,
+                      kfull);
         }
-        tma_load_4d(smem + hh * C::kChunkBytes + p * PS * 128, &kv_map, hh * 64, kvh, 0, coord, kfull);
       }
-      for (; i < n; ++i) {
-        const int s = i % kPwSlots;
-        bool ok = true;
-        if (i >= kPwSlots) ok = mbar_wait(&qempty[s], ((i / kPwSlots) - 1) & 1);
-        if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) {
-          if (lane == 0 && !__all_sync(0xffffffffu, ok)) set_status(a.status, PL_ERR_TIMEOUT);
-          flags[0] = 1;
-          break;
-        }
-        if (lane == 0) mbar_arrive_expect_tx(&qfull[s], C::kChunks * rows * 128);
-        __syncwarp();
-        if (lane < C::kChunks)
-          tma_load_4d(smem + C::kSlotOff + s * C::kTileBytes + lane * C::kChunkBytes, &q_map, lane * 64, 0, kvh,
-                      sp.q0 + (j0 + i) * a.tq, &qfull[s]);
+    }
+    // log sums of columns 4 lane .. 4 lane + 3; columns without a query: inf
+    int tok[4], off[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      tok[e] = 4 * lane + e < rows ? (4 * lane + e) / a.group : 0x3fffffff;
+      off[e] = (4 * lane + e) / a.group * a.num_qo_heads + (4 * lane + e) % a.group;
+    }
+    auto lse_of = [&](int j, float* v) {
+      const float* src = a.lse + (int64_t)(sp.q0 + j * a.tq) * a.num_qo_heads + kvh * a.group;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = j * a.tq + tok[e] < sp.qlen ? __ldg(src + off[e]) : INFINITY;
+    };
+    int i = 0;
+    float next[4];
+    lse_of(j0, next);
+    for (; i < n; ++i) {
+      const int s = i % kPwSlots;
+      bool ok = true;
+      // (the products of tile i - 4 waited until tile i - 6 was read, and so tile i - 8 added, whose log sums'
+      // place tile i takes)
+      if (i >= kPwSlots) ok = mbar_wait(&qempty[s], ((i / kPwSlots) - 1) & 1);
+      if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) {
+        if (lane == 0 && !__all_sync(0xffffffffu, ok)) set_status(a.status, PL_ERR_TIMEOUT);
+        flags[0] = 1;
+        break;
       }
+      if (lane == 0) mbar_arrive_expect_tx(&qfull[s], C::kChunks * rows * 128);
+      __syncwarp();
+      if (lane < C::kChunks)
+        tma_load_4d(smem + C::kSlotOff + s * C::kQBytes + lane * C::kQChunkBytes, &q_map, lane * 64, 0, kvh,
+                    sp.q0 + (j0 + i) * a.tq, &qfull[s]);
+      float l[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) l[e] = next[e] == -INFINITY ? -INFINITY : -next[e] * kLog2e;
+      if (i + 1 < n) lse_of(j0 + i + 1, next);
+      reinterpret_cast<float4*>(smem + C::kLseOff + i % kPwLse * kPwN * 4)[lane] = make_float4(l[0], l[1], l[2], l[3]);
+      mbar_arrive(&qfull[s]);
     }
     if (lane == 0) flags[1] = i;
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc = umma_idesc_bf16(kPwM, kPwM);
-      int consumed = 0;
-      bool ok = n == 0 || mbar_wait(kfull, 0);
-      const uint32_t kb = smem_u32(smem);
-      for (int i = 0; ok && i < n; ++i) {
-        const int s = i % kPwSlots, b = i % kPwBufs;
-        ok = mbar_wait(&qfull[s], (i / kPwSlots) & 1) && !flags[0];
-        if (!ok) break;
-        consumed = i + 1;
-        if (i >= kPwBufs) ok = mbar_wait(&sfree[b], ((i / kPwBufs) - 1) & 1) && !flags[0];
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t qs = smem_u32(smem + C::kSlotOff + s * C::kTileBytes);
+    // The whole warp walks the loop, with counts that are uniform by
+    // construction, and one lane issues: descriptors then stay in uniform
+    // registers.  (With one lane alone in the loop every product's operands
+    // went through the vector registers: about 125 cycles an instruction,
+    // where 128 columns take 64.)
+    constexpr uint32_t idesc = umma_idesc_bf16(kPwM, kPwN);
+    const uint32_t leader = elect_one();
+    const int nu = uniform(n), tu = uniform(tiles);
+    int done[kPwTiles], from[kPwTiles];  // products issued, first token tile
 #pragma unroll
-        for (int c = 0; c < C::kChunks; ++c)
+    for (int x = 0; x < kPwTiles; ++x) {
+      done[x] = 0;
+      from[x] = uniform(first_of(x));
+    }
+    const uint32_t tm = uniform((int)tmem), base = smem_u32(smem);
+    int consumed = 0;
+    bool ok = __all_sync(0xffffffffu, mbar_wait(kfull, 0));
+    for (int i = 0; ok && i < nu; ++i) {
+      const int s = i % kPwSlots;
+      ok = __all_sync(0xffffffffu, mbar_wait(&qfull[s], (i / kPwSlots) & 1) && !flags[0]);
+      if (!ok) break;
+      consumed = i + 1;
+      const uint32_t qs = base + C::kSlotOff + s * C::kQBytes;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16(tmem + (uint32_t)(b * kPwM), umma_desc_k_sw128(kb + c * C::kChunkBytes + 32 * k),
-                      umma_desc_k_sw128(qs + c * C::kChunkBytes + 32 * k), idesc, (c | k) ? 1u : 0u);
-        umma_commit(&sready[b]);
-        umma_commit(&qempty[s]);
+      for (int x = 0; x < kPwTiles; ++x) {
+        if (x < tu && i >= from[x] && ok) {
+          const int k = done[x]++, b = 2 * x + (k & 1);
+          if (k >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&sfree[b], ((k >> 1) - 1) & 1));
+          tc_fence_after();
+          if (ok) {
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                umma_bf16_if(leader, tm + (uint32_t)(b * kPwN),
+                             umma_desc_k_sw128(base + x * C::kKBytes + c * C::kKChunkBytes + 32 * e),
+                             umma_desc_k_sw128(qs + c * C::kQChunkBytes + 32 * e), idesc, (c | e) ? 1u : 0u);
+            umma_commit_if(leader, &sready[b]);
+          }
+        }
       }
+      umma_commit_if(leader, &qempty[s]);
+    }
+    if (lane == 0) {
       if (!ok) {
         set_status(a.status, PL_ERR_TIMEOUT);
         flags[0] = 1;
       }
       flags[2] = consumed;
-      umma_commit(fin);
-      if (!mbar_wait(fin, 0)) set_status(a.status, PL_ERR_TIMEOUT);
     }
+    umma_commit_if(leader, fin);
+    if (!mbar_wait(fin, 0)) set_status(a.status, PL_ERR_TIMEOUT);
+    __syncwarp();
   } else {
     // -------------------------------------------------------- exponentials
-    const int x = warp < 6 ? 0 : 1, quad = warp & 3;
-    const int m = 32 * quad + lane;  // position within the tile == TMEM lane
+    const int x = (warp - 2) / 8, b = (warp - 2) / 4, quad = warp & 3;  // product, buffer
+    const int m = 32 * quad + lane;  // position within the product == TMEM lane
     const uint32_t row_tmem = tmem + ((uint32_t)(32 * quad) << 16);
-    float* lse_s = reinterpret_cast<float*>(smem + C::kLseOff) + x * 2 * kPwM;
-    const int pos = kv0 + m;
-    // -log2 sum of column m of query tile j; columns without a query give 2^-inf
-    auto lse_of = [&](int j) -> float {
-      const int tok = j * a.tq + m / a.group;
-      if (m >= rows || tok >= sp.qlen) return -INFINITY;
-      const float v = a.lse[(int64_t)(sp.q0 + tok) * a.num_qo_heads + kvh * a.group + m % a.group];
-      return v == -INFINITY ? -INFINITY : -v * kLog2e;
-    };
-    const float sl2 = a.scale_log2;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const int pos = kv0 + x * kPwM + m;
+    const float2 sl2 = make_float2(a.scale_log2, a.scale_log2);
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     bool ok = true;
-    float next = x < n ? lse_of(j0 + x) : 0.f;
-    for (int i = x; i < n; i += 2) {
-      float* ls = lse_s + ((i >> 1) & 1) * kPwM;
-      ls[m] = next;
-      if (i + 2 < n) next = lse_of(j0 + i + 2);
-      named_barrier(1 + x, 128);
-      const int b = i % kPwBufs;
-      ok = flags[0] == 0 && mbar_wait(&sready[b], (i / kPwBufs) & 1);
-      if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) ok = false;
-      if (ok) {
-        tc_fence_after();
-        // column c is a query at position first + c / group: seen from column `from` on
-        const int first = p_first + (j0 + i) * a.tq;
-        const int from = pos > first ? (pos - first) * a.group : 0;
-        const bool masked = kv0 + kPwM - 1 > first;
+    const int first_tile = first_of(x) + (b & 1);
+    for (int i = first_tile, k = 0; x < tiles && i < n; i += 2, ++k) {
+      ok = mbar_wait(&sready[b], k & 1);
+      if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      // column c is a query at position first + c / group: seen from column `from` on
+      const int first = p_first + (j0 + i) * a.tq;
+      const int from = pos > first ? (pos - first) * a.group : 0;
+      const int to = (sp.qlen - (j0 + i) * a.tq) * a.group;  // columns behind are another request's queries
+      const float4* lse4 = reinterpret_cast<const float4*>(smem + C::kLseOff + i % kPwLse * kPwN * 4);
+      auto add_tile = [&](auto masked_t) {
+        constexpr bool kMasked = decltype(masked_t)::value;
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          float v[64];
-          tmem_ld64(row_tmem + (uint32_t)(b * kPwM + 64 * h), v);
-          const float4* l4 = reinterpret_cast<const float4*>(ls + 64 * h);
+        for (int h = 0; h < kPwN / 32; ++h) {
+          float v[32];
+          tmem_ld32(row_tmem + (uint32_t)(b * kPwN + 32 * h), v);
+          if (h == kPwN / 32 - 1) {  // read: the next product may come while these are added
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sfree[b]);
+          }
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const float4 l = l4[c];
-            float p0 = line_exp2(fmaf(v[4 * c], sl2, l.x)), p1 = line_exp2(fmaf(v[4 * c + 1], sl2, l.y));
-            float p2 = line_exp2(fmaf(v[4 * c + 2], sl2, l.z)), p3 = line_exp2(fmaf(v[4 * c + 3], sl2, l.w));
-            if (masked) {
-              const int col = 64 * h + 4 * c;
-              p0 = col >= from ? p0 : 0.f;
-              p1 = col + 1 >= from ? p1 : 0.f;
-              p2 = col + 2 >= from ? p2 : 0.f;
-              p3 = col + 3 >= from ? p3 : 0.f;
+          for (int c = 0; c < 8; ++c) {
+            const float4 l = lse4[8 * h + c];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int col = 4 * c + 2 * e, pair = 2 * c + e;
+              float2 p = fma_f32x2(make_float2(v[col], v[col + 1]), sl2,
+                                   e == 0 ? make_float2(l.x, l.y) : make_float2(l.z, l.w));
+              if (pair % 4 == 1)
+                p = pw_exp2_pair(p);
+              else
+                p = make_float2(line_exp2(p.x), line_exp2(p.y));
+              if constexpr (kMasked) {
+                p.x = 32 * h + col >= from && 32 * h + col < to ? p.x : 0.f;
+                p.y = 32 * h + col + 1 >= from && 32 * h + col + 1 < to ? p.y : 0.f;
+              }
+              sum[e] = add_f32x2(sum[e], p);
             }
-            sum[0] += p0;
-            sum[1] += p1;
-            sum[2] += p2;
-            sum[3] += p3;
           }
         }
-        tc_fence_before();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sfree[b]);
-      if (!ok) flags[0] = 1;  // nobody waits any more; the loop goes on for the barrier's count
+      };
+      if (kv0 + (x + 1) * kPwM - 1 > first || to < rows)
+        add_tile(std::true_type{});
+      else
+        add_tile(std::false_type{});
     }
-    if (!ok && lane == 0) set_status(a.status, PL_ERR_TIMEOUT);
-    // the two groups' sums, in this order
-    float* sums = reinterpret_cast<float*>(smem + C::kSumOff);
-    const float mine = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    if (x == 1) sums[m] = mine;
-    named_barrier(3, 256);
-    if (x == 0 && sp.req >= 0 && pos < sp.kv_len && flags[0] == 0)
-      a.partial[(int64_t)kvh * a.total_pages * PS + (int64_t)sp.kv_begin * PS + pos] = mine + sums[m];
+    if (!ok) {
+      set_status(a.status, PL_ERR_TIMEOUT);
+      flags[0] = 1;
+    }
+    // the sums of a product's two buffers
+    float* sums = reinterpret_cast<float*>(smem + C::kSumOff) + x * kPwM;
+    const float mine = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+    if (b & 1) sums[m] = mine;
+    named_barrier(1 + x, 256);
+    if (!(b & 1) && flags[0] == 0 && pos < sp.kv_len)
+      a.partial[((int64_t)chunk * a.num_kv_heads + kvh) * a.total_pages * PS + (int64_t)sp.kv_begin * PS + pos] =
+          mine + sums[m];
   }
 
   __syncthreads();
   if (threadIdx.x == 0) {
     const int issued = flags[1], consumed = flags[2];
     for (int i = consumed; i < issued; ++i) (void)mbar_wait(&qfull[i % kPwSlots], (i / kPwSlots) & 1);
-    if (n > 0) (void)mbar_wait(kfull, 0);
+    (void)mbar_wait(kfull, 0);
   }
   tc_fence_before();
   __syncthreads();
@@ -320,8 +426,9 @@ __global__ void __launch_bounds__(kPwThreads, 1)
   }
 }
 
-// weight[b][pos] += the kv heads' sums, in head order; a thread per position
-// of the page table's line.
+// weight[b][pos] += the sums of the kv heads and of the chunks whose queries see
+// the position's run, in this order; a thread per position of the page
+// table's line.
 __global__ void __launch_bounds__(256)
     prompt_weight_add_kernel(const PromptWeightArgs a, int32_t hkv, float* weight, int64_t weight_stride,
                              int32_t capacity) {
@@ -344,9 +451,12 @@ __global__ void __launch_bounds__(256)
     set_status(a.status, PL_ERR_ROW_CAPACITY);
     return;
   }
+  const int qlen = a.qo_indptr[lo + 1] - a.qo_indptr[lo];
+  const int c0 = pw_first(a, (int)pos / kPwRun * kPwRun, len, qlen) / a.chunk, c1 = ((qlen + a.tq - 1) / a.tq - 1) / a.chunk;
   float sum = 0.f;
+  for (int c = c0; c <= c1; ++c)
 #pragma unroll 8
-  for (int h = 0; h < hkv; ++h) sum += __ldcg(a.partial + h * all + at);
+    for (int h = 0; h < hkv; ++h) sum += __ldcg(a.partial + ((int64_t)c * hkv + h) * all + at);
   weight[(int64_t)lo * weight_stride + pos] += sum;
 }
 
@@ -562,12 +672,12 @@ int64_t align256(int64_t v) { return (v + 255) & ~int64_t(255); }
 
 template <int D>
 int32_t launch_prompt_weights(const CUtensorMap& kv_map, const CUtensorMap& q_map, const pl::PromptWeightArgs& a,
-                              int64_t tiles, int hkv, void* stream) {
+                              int64_t blocks, void* stream) {
   using C = pl::PromptWeightCfg<D>;
   auto kern = pl::prompt_weight_kernel<D>;
   const int32_t st = pl_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (st != PL_OK) return st;
-  return pl_host::launch_pdl(kern, dim3((unsigned)tiles, hkv), dim3(pl::kPwThreads), C::kSmemBytes, stream, kv_map,
+  return pl_host::launch_pdl(kern, dim3((unsigned)blocks), dim3(pl::kPwThreads), C::kSmemBytes, stream, kv_map,
                              q_map, a);
 }
 
@@ -575,7 +685,7 @@ int32_t launch_prompt_weights(const CUtensorMap& kv_map, const CUtensorMap& q_ma
 
 extern "C" int64_t pl_prefill_weights_workspace_bytes(int32_t num_kv_heads, int32_t page_size, int64_t total_pages) {
   if (num_kv_heads <= 0 || page_size <= 0 || total_pages < 0) return 0;
-  return align256(total_pages * page_size * num_kv_heads * 4);
+  return align256(pl::kPwChunks * total_pages * page_size * num_kv_heads * 4);
 }
 
 extern "C" int32_t pl_paged_prefill_weights(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv_cache,
@@ -591,7 +701,7 @@ extern "C" int32_t pl_paged_prefill_weights(const void* q, int64_t q_stride_t, i
       weight_stride < weight_capacity || (weight == nullptr && weight_capacity > 0))
     return PL_ERR_INVALID_ARGUMENT;
   const int group = num_qo_heads / num_kv_heads;
-  if (group > pl::kPwM || (head_dim != 64 && head_dim != 128) ||
+  if (group > 128 || (head_dim != 64 && head_dim != 128) ||
       (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) || num_kv_heads > 65535 ||
       total_pages * page_size > 0x7FFFFFFFll || num_pages > 0x3FFFFFFFll)
     return PL_ERR_UNSUPPORTED;
@@ -615,8 +725,12 @@ extern "C" int32_t pl_paged_prefill_weights(const void* q, int64_t q_stride_t, i
   a.batch = batch;
   a.total_q = total_q;
   a.num_qo_heads = num_qo_heads;
+  a.num_kv_heads = num_kv_heads;
   a.group = group;
-  a.tq = pl::kPwM / group;
+  a.tq = pl::kPwN / group;
+  // chunks share long prompts out (the first run of positions is seen by all queries, the last by few)
+  a.chunk = ((total_q + a.tq - 1) / a.tq + pl::kPwChunks - 1) / pl::kPwChunks;
+  if (a.chunk < 16) a.chunk = 16;
   a.page_size = page_size;
   a.scale_log2 = sm_scale * pl::kLog2e;
   a.lse = lse;
@@ -628,7 +742,7 @@ extern "C" int32_t pl_paged_prefill_weights(const void* q, int64_t q_stride_t, i
   if (st != PL_OK) return st;
   pl_host::EncodeTiledFn enc = pl_host::encode_tiled_fn();
   if (enc == nullptr) return PL_ERR_CUDA;
-  // q as {head_dim, heads of a group, kv heads, tokens}; a box is tq tokens of one group, 64 channels
+  // q as {head_dim, heads of a group, kv heads, tokens}; a box is 64 channels of tq tokens
   const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)group, (cuuint64_t)num_kv_heads, (cuuint64_t)total_q};
   const cuuint64_t strides[3] = {(cuuint64_t)q_stride_h * 2, (cuuint64_t)q_stride_h * 2 * group,
                                  (cuuint64_t)q_stride_t * 2};
@@ -638,14 +752,14 @@ extern "C" int32_t pl_paged_prefill_weights(const void* q, int64_t q_stride_t, i
           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return PL_ERR_INVALID_ARGUMENT;
-  // a row of n positions has ceil(n / 128) <= n / 128 + 1 tiles
-  const int64_t tiles = total_pages * page_size / pl::kPwM + batch;
-  if (tiles > 0x7FFFFFFF) return PL_ERR_UNSUPPORTED;
-  st = head_dim == 128 ? launch_prompt_weights<128>(kv_map, q_map, a, tiles, num_kv_heads, stream)
-                       : launch_prompt_weights<64>(kv_map, q_map, a, tiles, num_kv_heads, stream);
+  // a row of n positions has ceil(n / 256) <= n / 256 + 1 runs
+  const int64_t blocks = (total_pages * page_size / pl::kPwRun + batch) * pl::kPwChunks * num_kv_heads;
+  if (blocks > 0x7FFFFFFF) return PL_ERR_UNSUPPORTED;
+  st = head_dim == 128 ? launch_prompt_weights<128>(kv_map, q_map, a, blocks, stream)
+                       : launch_prompt_weights<64>(kv_map, q_map, a, blocks, stream);
   if (st != PL_OK) return st;
-  const int64_t blocks = (total_pages * page_size + 255) / 256;
-  return pl_host::launch_pdl(pl::prompt_weight_add_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a,
+  const int64_t add = (total_pages * page_size + 255) / 256;
+  return pl_host::launch_pdl(pl::prompt_weight_add_kernel, dim3((unsigned)add), dim3(256), 0, stream, a,
                              num_kv_heads, weight, weight_stride, weight_capacity);
 }
 

@@ -39,6 +39,8 @@
 // away), positions that none sees are cleared in V, and where a border of the
 // pair's masks crosses a tile, inf and NaN elements of V are replaced by zero
 // and added at the end for the rows that do see them (0 x NaN is NaN).
+#include <type_traits>
+
 #include "pl_common.cuh"
 
 namespace pl {
@@ -335,6 +337,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     // first position of this row's window (kWindow)
     const int wl = kWindow && row_ok ? (int)max((int64_t)0, (int64_t)lim - a.window + 1) : 0;
     auto sees = [&](int col) { return col <= lim && (!kWindow || col >= wl || col < a.sinks); };
+    // bit i: the row sees position col + i
+    auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1); };  // the first n bits
+    auto seen_bits = [&](int col) -> uint32_t {
+      uint32_t w = below(lim + 1 - col);
+      if constexpr (kWindow) w &= ~below(wl - col) | below(a.sinks - col);
+      return w;
+    };
     const float sl2 = a.scale_log2;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
@@ -358,117 +367,129 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       }
       tc_fence_after();
       uint8_t* pt = smem + C::kPOff + x * C::kPBytes;
-      // One pass against the running maximum; a row whose maximum grows by
-      // more than 2^kRescaleSlack (and the first tile) takes the two-pass path.
-      // Max and sum run as 8 independent chains each.
-      bool two_pass = __any_sync(0xffffffffu, m_run == -INFINITY);
-      if (!two_pass) {
-        const float nb = -m_run;
-        float sm[8], mx[8];
+      // Tiles that no border of the warp's rows crosses run without masks.
+      auto softmax_tile = [&](auto masked_t) {
+        constexpr bool kMasked = decltype(masked_t)::value;
+        // One pass against the running maximum; a row whose maximum grows by
+        // more than 2^kRescaleSlack (and the first tile) takes the two-pass path.
+        // Max and sum run as 8 independent chains each.
+        bool two_pass = __any_sync(0xffffffffu, m_run == -INFINITY);
+        if (!two_pass) {
+          const float nb = -m_run;
+          float sm[8], mx[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          sm[k] = 0.f;
-          mx[k] = -INFINITY;
-        }
+          for (int k = 0; k < 8; ++k) {
+            sm[k] = 0.f;
+            mx[k] = -INFINITY;
+          }
 #pragma unroll 1
-        for (int h = 0; h < kPrefillN / 64; ++h) {
-          float v[64];
-          tmem_ld64(s_tmem + 64 * h, v);
-          uint32_t pk[32];
+          for (int h = 0; h < kPrefillN / 64; ++h) {
+            float v[64];
+            tmem_ld64(s_tmem + 64 * h, v);
+            const uint32_t see0 = kMasked ? seen_bits(kv0 + 64 * h) : 0u, see1 = kMasked ? seen_bits(kv0 + 64 * h + 32) : 0u;
+            auto seen = [&](int c) { return (((c < 32 ? see0 : see1) >> (c & 31)) & 1u) != 0; };
+            uint32_t pk[32];
 #pragma unroll
-          for (int i = 0; i < 64; i += 2) {
-            const int col = kv0 + 64 * h + i;
-            float p0 = pf_exp2(fmaf(v[i], sl2, nb));
-            float p1 = pf_exp2(fmaf(v[i + 1], sl2, nb));
-            float s0 = v[i], s1 = v[i + 1];
-            if (masked) {
-              const bool k0 = sees(col), k1 = sees(col + 1);
-              p0 = k0 ? p0 : 0.f;
-              p1 = k1 ? p1 : 0.f;
-              s0 = k0 ? s0 : -INFINITY;
-              s1 = k1 ? s1 : -INFINITY;
+            for (int i = 0; i < 64; i += 2) {
+              float p0 = pf_exp2(fmaf(v[i], sl2, nb));
+              float p1 = pf_exp2(fmaf(v[i + 1], sl2, nb));
+              float s0 = v[i], s1 = v[i + 1];
+              if constexpr (kMasked) {
+                const bool k0 = seen(i), k1 = seen(i + 1);
+                p0 = k0 ? p0 : 0.f;
+                p1 = k1 ? p1 : 0.f;
+                s0 = k0 ? s0 : -INFINITY;
+                s1 = k1 ? s1 : -INFINITY;
+              }
+              mx[(i >> 1) & 7] = fmaxf(mx[(i >> 1) & 7], fmaxf(s0, s1));
+              sm[(i >> 1) & 7] += p0 + p1;
+              pk[i / 2] = pack_bf16x2(p0, p1);
             }
-            mx[(i >> 1) & 7] = fmaxf(mx[(i >> 1) & 7], fmaxf(s0, s1));
-            sm[(i >> 1) & 7] += p0 + p1;
-            pk[i / 2] = pack_bf16x2(p0, p1);
+            uint8_t* chunk = pt + h * C::kChunkBytes;
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              *reinterpret_cast<uint4*>(chunk + pf_swz(m, u)) =
+                  make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
           }
-          uint8_t* chunk = pt + h * C::kChunkBytes;
-#pragma unroll
-          for (int u = 0; u < 8; ++u)
-            *reinterpret_cast<uint4*>(chunk + pf_swz(m, u)) =
-                make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
+          const float vmax =
+              fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+          two_pass = __any_sync(0xffffffffu, vmax * sl2 > m_run + kRescaleSlack);
+          if (!two_pass) l_run += ((sm[0] + sm[1]) + (sm[2] + sm[3])) + ((sm[4] + sm[5]) + (sm[6] + sm[7]));
         }
-        const float vmax =
-            fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-        two_pass = __any_sync(0xffffffffu, vmax * sl2 > m_run + kRescaleSlack);
-        if (!two_pass) l_run += ((sm[0] + sm[1]) + (sm[2] + sm[3])) + ((sm[4] + sm[5]) + (sm[6] + sm[7]));
-      }
-      if (two_pass) {
-        // pass 1: row maximum of the masked scores
-        float mx[8];
+        if (two_pass) {
+          // pass 1: row maximum of the masked scores
+          float mx[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mx[k] = -INFINITY;
+          for (int k = 0; k < 8; ++k) mx[k] = -INFINITY;
 #pragma unroll 1
-        for (int h = 0; h < kPrefillN / 64; ++h) {
-          float v[64];
-          tmem_ld64(s_tmem + 64 * h, v);
-          if (masked) {
+          for (int h = 0; h < kPrefillN / 64; ++h) {
+            float v[64];
+            tmem_ld64(s_tmem + 64 * h, v);
+            const uint32_t see0 = kMasked ? seen_bits(kv0 + 64 * h) : 0u, see1 = kMasked ? seen_bits(kv0 + 64 * h + 32) : 0u;
+            auto seen = [&](int c) { return (((c < 32 ? see0 : see1) >> (c & 31)) & 1u) != 0; };
+            if constexpr (kMasked) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) mx[i & 7] = fmaxf(mx[i & 7], sees(kv0 + 64 * h + i) ? v[i] : -INFINITY);
-          } else {
+              for (int i = 0; i < 64; ++i) mx[i & 7] = fmaxf(mx[i & 7], seen(i) ? v[i] : -INFINITY);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) mx[i & 7] = fmaxf(mx[i & 7], v[i]);
-          }
-        }
-        float tmax =
-            fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-        tmax *= sl2;  // sl2 > 0: the max commutes with the scaling
-        const float m_new = fmaxf(m_run, tmax);
-        const bool rescale = m_run != -INFINITY && m_new > m_run + kRescaleSlack;
-        const float m_use = (m_run == -INFINITY || rescale) ? m_new : m_run;
-        if (__any_sync(0xffffffffu, rescale)) {
-          const float alpha = rescale ? pf_exp2(m_run - m_use) : 1.f;
-#pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
-            float v[16];
-            tmem_ld16(o_tmem + 16 * c, v);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] *= alpha;
-            tmem_st16_wait(o_tmem + 16 * c, v);
-          }
-          l_run *= alpha;
-        }
-        m_run = m_use;
-        // pass 2: P = exp2(s * scale - m), row sum, bf16 P into the swizzled tile
-        const float nb = m_use == -INFINITY ? 0.f : -m_use;
-        float sm[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sm[k] = 0.f;
-#pragma unroll 1
-        for (int h = 0; h < kPrefillN / 64; ++h) {
-          float v[64];
-          tmem_ld64(s_tmem + 64 * h, v);
-          uint32_t pk[32];
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) {
-            const int col = kv0 + 64 * h + i;
-            float p0 = pf_exp2(fmaf(v[i], sl2, nb));
-            float p1 = pf_exp2(fmaf(v[i + 1], sl2, nb));
-            if (masked) {
-              p0 = sees(col) ? p0 : 0.f;
-              p1 = sees(col + 1) ? p1 : 0.f;
+              for (int i = 0; i < 64; ++i) mx[i & 7] = fmaxf(mx[i & 7], v[i]);
             }
-            sm[(i >> 1) & 7] += p0 + p1;
-            pk[i / 2] = pack_bf16x2(p0, p1);
           }
-          uint8_t* chunk = pt + h * C::kChunkBytes;
+          float tmax =
+              fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+          tmax *= sl2;  // sl2 > 0: the max commutes with the scaling
+          const float m_new = fmaxf(m_run, tmax);
+          const bool rescale = m_run != -INFINITY && m_new > m_run + kRescaleSlack;
+          const float m_use = (m_run == -INFINITY || rescale) ? m_new : m_run;
+          if (__any_sync(0xffffffffu, rescale)) {
+            const float alpha = rescale ? pf_exp2(m_run - m_use) : 1.f;
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              float v[16];
+              tmem_ld16(o_tmem + 16 * c, v);
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            *reinterpret_cast<uint4*>(chunk + pf_swz(m, u)) =
-                make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
+              for (int i = 0; i < 16; ++i) v[i] *= alpha;
+              tmem_st16_wait(o_tmem + 16 * c, v);
+            }
+            l_run *= alpha;
+          }
+          m_run = m_use;
+          // pass 2: P = exp2(s * scale - m), row sum, bf16 P into the swizzled tile
+          const float nb = m_use == -INFINITY ? 0.f : -m_use;
+          float sm[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sm[k] = 0.f;
+#pragma unroll 1
+          for (int h = 0; h < kPrefillN / 64; ++h) {
+            float v[64];
+            tmem_ld64(s_tmem + 64 * h, v);
+            const uint32_t see0 = kMasked ? seen_bits(kv0 + 64 * h) : 0u, see1 = kMasked ? seen_bits(kv0 + 64 * h + 32) : 0u;
+            auto seen = [&](int c) { return (((c < 32 ? see0 : see1) >> (c & 31)) & 1u) != 0; };
+            uint32_t pk[32];
+#pragma unroll
+            for (int i = 0; i < 64; i += 2) {
+              float p0 = pf_exp2(fmaf(v[i], sl2, nb));
+              float p1 = pf_exp2(fmaf(v[i + 1], sl2, nb));
+              if constexpr (kMasked) {
+                p0 = seen(i) ? p0 : 0.f;
+                p1 = seen(i + 1) ? p1 : 0.f;
+              }
+              sm[(i >> 1) & 7] += p0 + p1;
+              pk[i / 2] = pack_bf16x2(p0, p1);
+            }
+            uint8_t* chunk = pt + h * C::kChunkBytes;
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              *reinterpret_cast<uint4*>(chunk + pf_swz(m, u)) =
+                  make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
+          }
+          l_run += ((sm[0] + sm[1]) + (sm[2] + sm[3])) + ((sm[4] + sm[5]) + (sm[6] + sm[7]));
         }
-        l_run += ((sm[0] + sm[1]) + (sm[2] + sm[3])) + ((sm[4] + sm[5]) + (sm[6] + sm[7]));
-      }
+      };
+      if (__any_sync(0xffffffffu, masked))
+        softmax_tile(std::true_type{});
+      else
+        softmax_tile(std::false_type{});
       // Slots past the request's last token in its last page hold whatever
       // the pool had there (0 * NaN is NaN): tile A's threads clear those V
       // rows (P_A.V_j runs first, after this tile's arrival).
@@ -488,10 +509,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             const int units = C::kChunks * 8;
             for (int idx = m; idx < (r1 - r0) * units; idx += 128) {
               const int r = r0 + idx / units, hh = (idx / 8) % C::kChunks, u = idx % 8, pos = kv0 + r;
-              const bool below = pos < wlo1 && pos >= a.sinks;
-              if (!below && pos <= p0) continue;  // every row sees it
+              const bool lower_part = pos < wlo1 && pos >= a.sinks;
+              if (!lower_part && pos <= p0) continue;  // every row sees it
               uint4* at = reinterpret_cast<uint4*>(vt + hh * C::kChunkBytes + r * 128 + u * 16);
-              if (pos >= n_vis || (below && pos < wlo)) {
+              if (pos >= n_vis || (lower_part && pos < wlo)) {
                 *at = make_uint4(0, 0, 0, 0);
                 continue;
               }

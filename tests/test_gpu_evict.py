@@ -237,3 +237,35 @@ def test_a_cache_that_evicts(K):
         weight, spare = spare, weight
     assert int(status.item()) == 0
     assert [len(x) for x in ref] == [92, 48, 92]
+
+
+def test_prompt_weights_stay_apart(K):
+    """A request's weights do not depend on its neighbours' queries or on unused memory."""
+
+    def edit(q, cache, indptr, indices, lens):
+        q[70:130] = np.nan  # request 1, beside tiles of requests 0 and 2
+
+    host, dev = _case([200, 90, 77], [70, 60, 37], 14, 2, 64, 16, 6, edit)
+    tables = [dev["qo"], dev["indptr"], dev["indices"], dev["last"]]
+    lse = torch.empty(167, 14, device="cuda")
+    K.paged_prefill(dev["q"], dev["cache"], *tables, out_lse=lse)
+    weight = torch.zeros(3, 200, device="cuda")
+    K.paged_prefill_weights(dev["q"], dev["cache"], *tables, lse, weight)
+    added = o.paged(host["q"][:70], host["cache"], host["qo"][:2], host["indptr"], host["indices"], host["last"][:1],
+                    64 ** -0.5)[2]
+    _weights_ok(weight[:1], torch.zeros(1, 200), added, [200])
+    assert torch.isnan(weight[1, :90]).all() and torch.isfinite(weight[2]).all() and (weight[2, :77] > 0).all()
+
+
+@pytest.mark.parametrize("n,length,hq,hkv", [(1500, 1500, 4, 2), (700, 1300, 6, 1), (40, 3000, 8, 2)])
+def test_prompt_weights_over_many_runs(K, n, length, hq, hkv):
+    host, dev = _case([length], [n], hq, hkv, 64, 16, n)
+    tables = [dev["qo"], dev["indptr"], dev["indices"], dev["last"]]
+    lse = torch.empty(n, hq, device="cuda")
+    K.paged_prefill(dev["q"], dev["cache"], *tables, out_lse=lse)
+    weight = torch.zeros(1, length, device="cuda")
+    ws = torch.full((K._prefill_weights_workspace_bytes(hkv, 16, dev["indices"].numel()),), 255, dtype=torch.uint8,
+                    device="cuda")
+    K.paged_prefill_weights(dev["q"], dev["cache"], *tables, lse, weight, workspace=ws)
+    added = o.paged(host["q"], host["cache"], host["qo"], host["indptr"], host["indices"], host["last"], 64 ** -0.5)[2]
+    _weights_ok(weight, torch.zeros(1, length), added, [length])
