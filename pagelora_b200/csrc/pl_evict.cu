@@ -468,12 +468,16 @@ __global__ void __launch_bounds__(256)
 // 11, 11 and 10 bits in three passes, each a histogram in shared memory; then
 // every warp counts what its run of positions keeps, and after a scan of the
 // counts writes it in ascending order.  A row is one CTA, or (kCluster) eight
-// that share its positions and read each other's histograms through
-// distributed shared memory.  The weights come from L2 after the first pass.
-constexpr int kSelThreads = 512;
+// that share its positions; each adds up a slice of their histograms' bins through
+// distributed shared memory, and all read the slices.  The ordered bits stay in shared memory from the
+// first pass on (12 rows of 131072 positions: 49 us when every pass read the
+// weights again); runs longer than fit there read the rest again.
+constexpr int kSelThreads = 1024;
+constexpr int kSelHeld = 49152;   // positions a CTA holds at most (192 KB)
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelBins = 2048;
 constexpr int kSelCluster = 8;
+constexpr int kSelSlice = kSelBins / kSelCluster;  // bins that a CTA of a cluster adds up
 
 struct SelectArgs {
   const float* weight;
@@ -488,6 +492,7 @@ struct SelectArgs {
   int32_t* keep_count;
   float* out_weight;
   int64_t out_stride;
+  int32_t held;         // keys that a warp holds in shared memory
   int32_t* status;
 };
 
@@ -500,9 +505,11 @@ __device__ __forceinline__ uint32_t select_key(float w) {
 template <bool kCluster>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const SelectArgs a) {
   __shared__ __align__(16) int32_t hist[kSelBins];
+  __shared__ __align__(16) int32_t slice[kCluster ? kSelSlice : 4];
   __shared__ int32_t scan[kSelWarps];
   __shared__ int32_t pick[2];                    // digit, count above it
   __shared__ int32_t counts[2 * kSelWarps + 2];  // per warp: above, equal; then the CTA's sums
+  extern __shared__ uint32_t held[];             // [warps][a.held]: keys of the first positions of a warp's run
   constexpr int nr = kCluster ? kSelCluster : 1;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rank = kCluster ? blockIdx.x % kSelCluster : 0;
@@ -527,24 +534,38 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const SelectA
   const int tid = rank * kSelThreads + threadIdx.x;
   constexpr int all = nr * kSelThreads;
   // what does not depend on the choice
-  const int listed = cut ? a.budget - a.sinks : 0;
-  for (int i = listed + tid; i < a.keep_width; i += all) keep[i] = -1;
-  for (int i = kept + tid; i < a.capacity; i += all) ow[i] = 0.f;
-  if (!cut) {
-    for (int i = tid; i < len; i += all) ow[i] = w[i];
-    return;  // the whole row's CTAs alike
-  }
   const int k = a.budget - a.sinks - a.recent;
-  for (int i = tid; i < a.sinks; i += all) ow[i] = w[i];
-  for (int i = tid; i < a.recent; i += all) {
-    const int pos = len - a.recent + i;
-    keep[k + i] = pos;
-    ow[a.sinks + k + i] = w[pos];
+  auto fill = [&]() {
+    const int listed = cut ? a.budget - a.sinks : 0, front = cut ? a.sinks : len;
+    for (int i = listed + tid; i < a.keep_width; i += all) keep[i] = -1;
+    for (int i = kept + tid; i < a.capacity; i += all) ow[i] = 0.f;
+    for (int i = tid; i < front; i += all) ow[i] = w[i];
+    if (cut)
+      for (int i = tid; i < a.recent; i += all) {
+        const int pos = len - a.recent + i;
+        keep[k + i] = pos;
+        ow[a.sinks + k + i] = w[pos];
+      }
+  };
+  if (!cut) {
+    fill();
+    return;  // the whole row's CTAs alike
   }
   // this warp's run of the candidates [sinks, len - recent)
   const int c0 = a.sinks, n = len - a.recent - a.sinks;
   const int runs = nr * kSelWarps, per = ((n + runs - 1) / runs + 31) / 32 * 32;
   const int b = min(n, (rank * kSelWarps + warp) * per), e = min(n, b + per);
+  uint32_t* mine_held = held + warp * a.held;
+  const int eh = min(e, b + a.held);
+  // f(key) of every candidate of the run
+  auto walk = [&](auto f) {
+#pragma unroll 8
+    for (int i = b + lane; i < eh; i += 32) f(mine_held[i - b]);
+#pragma unroll 4
+    for (int i = eh + lane; i < e; i += 32) f(select_key(w[c0 + i]));
+  };
+#pragma unroll 8
+  for (int i = b + lane; i < eh; i += 32) mine_held[i - b] = select_key(w[c0 + i]);
 
   uint32_t prefix = 0, mask = 0;
   int want = k;  // still to be found among the keys with this prefix
@@ -554,28 +575,30 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const SelectA
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
       for (int i = threadIdx.x; i < kSelBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-#pragma unroll 4
-      for (int i = b + lane; i < e; i += 32) {
-        const uint32_t key = select_key(w[c0 + i]);
+      walk([&](uint32_t key) {
         if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1);
-      }
+      });
       sync();
-      // four bins a thread, from the highest down
+      if constexpr (kCluster) {
+        if (threadIdx.x < kSelSlice) {
+          const uint32_t at = smem_u32(hist + rank * kSelSlice + threadIdx.x);
+          int sum = 0;
+#pragma unroll
+          for (int r = 0; r < nr; ++r) sum += __float_as_int(dsmem_ld_f32(dsmem_map(at, r)));
+          slice[threadIdx.x] = sum;
+        }
+        cluster_sync_all();
+      }
+      // four bins a thread of the first half of the block, from the highest down
       const int bin = kSelBins - 4 - 4 * threadIdx.x;
       int4 h = make_int4(0, 0, 0, 0);
-#pragma unroll
-      for (int r = 0; r < nr; ++r) {
-        int4 o;
+      if (bin >= 0) {
         if constexpr (kCluster) {
-          const float4 f = dsmem_ld_f32x4(dsmem_map(smem_u32(hist + bin), r));
-          o = make_int4(__float_as_int(f.x), __float_as_int(f.y), __float_as_int(f.z), __float_as_int(f.w));
+          const float4 f = dsmem_ld_f32x4(dsmem_map(smem_u32(slice + bin % kSelSlice), bin / kSelSlice));
+          h = make_int4(__float_as_int(f.x), __float_as_int(f.y), __float_as_int(f.z), __float_as_int(f.w));
         } else {
-          o = *reinterpret_cast<const int4*>(hist + bin);
+          h = *reinterpret_cast<const int4*>(hist + bin);
         }
-        h.x += o.x;
-        h.y += o.y;
-        h.z += o.z;
-        h.w += o.w;
       }
       const int mine = h.x + h.y + h.z + h.w;
       int incl = mine;
@@ -596,7 +619,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const SelectA
         pick[0] = d;
         pick[1] = above;
       }
-      sync();  // the digit is known, and every CTA has read the histograms
+      __syncthreads();  // the digit is known (another CTA writes its slice again behind the next cluster barrier only)
       prefix |= (uint32_t)pick[0] << shift;
       mask |= ((1u << bits) - 1) << shift;
       want -= pick[1];
@@ -606,12 +629,10 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const SelectA
   }
   // counts of every warp's run: above the key, equal to it
   int gt = 0, eq = 0;
-#pragma unroll 4
-  for (int i = b + lane; i < e; i += 32) {
-    const uint32_t key = select_key(w[c0 + i]);
+  walk([&](uint32_t key) {
     gt += key > prefix;
     eq += key == prefix;
-  }
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     gt += __shfl_xor_sync(0xffffffffu, gt, o);
@@ -643,11 +664,12 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const SelectA
     gt += counts[2 * i];
     eq += counts[2 * i + 1];
   }
+  if constexpr (kCluster) cluster_sync_all();  // the counts are read; no CTA's shared memory is needed by another now
+  fill();  // (behind the barriers, which would wait for the stores)
   const unsigned below = (1u << lane) - 1;
   for (int i0 = b; i0 < e; i0 += 32) {
     const int i = i0 + lane;
-    const float v = i < e ? w[c0 + i] : 0.f;
-    const uint32_t key = select_key(v);
+    const uint32_t key = i < eh ? mine_held[i - b] : (i < e ? select_key(w[c0 + i]) : 0u);
     const unsigned bg = __ballot_sync(0xffffffffu, i < e && key > prefix);
     const unsigned bq = __ballot_sync(0xffffffffu, i < e && key == prefix);
     const int g = gt + __popc(bg & below), q = eq + __popc(bq & below);
@@ -655,12 +677,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const SelectA
     if (take) {
       const int at = g + min(q, want);
       keep[at] = c0 + i;
-      ow[a.sinks + at] = v;
+      ow[a.sinks + at] = w[c0 + i];
     }
     gt += __popc(bg);
     eq += __popc(bq);
   }
-  if constexpr (kCluster) cluster_sync_all();  // the counts are read before a CTA ends
 }
 
 }  // namespace pl
@@ -791,10 +812,17 @@ extern "C" int32_t pl_evict_select(const float* weight, int64_t weight_stride, i
   a.out_weight = out_weight;
   a.out_stride = out_stride;
   a.status = status_dev;
-  // A CTA reads 4096 positions a pass in about the time of a cluster's exchange.
-  if (capacity > 8192)
-    return pl_host::launch_pdl_cluster(pl::evict_select_kernel<true>, dim3((unsigned)num_rows * pl::kSelCluster),
-                                       dim3(pl::kSelThreads), 0, stream, pl::kSelCluster, a);
-  return pl_host::launch_pdl(pl::evict_select_kernel<false>, dim3((unsigned)num_rows), dim3(pl::kSelThreads), 0, stream,
-                             a);
+  // One CTA walks 8192 positions in about the time that a cluster's exchanges take.
+  const bool cluster = capacity > 8192;
+  const int64_t runs = pl::kSelWarps * (cluster ? pl::kSelCluster : 1);
+  const int64_t per = ((capacity + runs - 1) / runs + 31) / 32 * 32;
+  a.held = (int32_t)(per < pl::kSelHeld / pl::kSelWarps ? per : pl::kSelHeld / pl::kSelWarps);
+  const size_t smem = (size_t)a.held * pl::kSelWarps * 4;
+  auto kern = cluster ? pl::evict_select_kernel<true> : pl::evict_select_kernel<false>;
+  const int32_t st = pl_host::ensure_smem_attr(reinterpret_cast<const void*>(kern), pl::kSelHeld * 4);
+  if (st != PL_OK) return st;
+  if (cluster)
+    return pl_host::launch_pdl_cluster(kern, dim3((unsigned)num_rows * pl::kSelCluster), dim3(pl::kSelThreads), smem,
+                                       stream, pl::kSelCluster, a);
+  return pl_host::launch_pdl(kern, dim3((unsigned)num_rows), dim3(pl::kSelThreads), smem, stream, a);
 }

@@ -21,12 +21,41 @@ namespace pl {
 __device__ __forceinline__ float bf_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// The smaller and the larger of packed pairs; NaN where one is NaN.
+__device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
 // ----------------------------------------------------------------- append
 // Eight lanes take one record (K or V of one head of one token): D / 8
 // channels a lane, a group's extremes by three exchanges.  Differences are
 // taken between halves of the values, which neither overflow nor round, so
 // every finite bf16 input has finite scales.  A group with inf or NaN
-// decodes to NaN.  Bound by HBM: 2 D bytes in, D / 2 + 16 out.
+// decodes to NaN.  A code comes from a product with 1 / scale; where its
+// remainder is within 2^-18 of half a step the quotients are divided out.
+// Bound by HBM: 2 D bytes in, D / 2 + 16 out.
 template <int D>
 __global__ void __launch_bounds__(256)
     kv4_append_kernel(const bf16* k, int64_t k_stride, const bf16* v, int64_t v_stride, uint8_t* cache,
@@ -35,65 +64,79 @@ __global__ void __launch_bounds__(256)
   constexpr int E = D / 8, kRecord = D / 2 + 16;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t rec = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 8;
+  // record (token, K / V, head) of the line; the host keeps their number below 2^31
+  const uint32_t rec = blockIdx.x * 32 + threadIdx.x / 8;
   const int sub = threadIdx.x % 8;
-  const bool on = rec < (int64_t)tokens * 2 * hkv;
-  const int h = on ? (int)(rec % hkv) : 0, kv = on ? (int)(rec / hkv % 2) : 0, tok = on ? (int)(rec / hkv / 2) : 0;
+  const bool on = rec < (uint32_t)tokens * 2 * hkv;
+  const uint32_t part = on ? rec / hkv : 0;
+  const int h = on ? (int)(rec - part * hkv) : 0, kv = part & 1, tok = (int)(part >> 1);
   const bf16* src = (kv ? v + (int64_t)tok * v_stride : k + (int64_t)tok * k_stride) + (int64_t)h * D + sub * E;
-  float x[E];
+  uint32_t x[E / 2];  // pairs of channels: groups 0, 1 and 2, 3 in turn
 #pragma unroll
   for (int u = 0; u < E / 8; ++u) {
     const uint4 w = on ? __ldg(reinterpret_cast<const uint4*>(src) + u) : make_uint4(0, 0, 0, 0);
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[8 * u + 2 * i] = 0.5f * bf_lo(ws[i]);
-      x[8 * u + 2 * i + 1] = 0.5f * bf_hi(ws[i]);
-    }
+    x[4 * u] = w.x;
+    x[4 * u + 1] = w.y;
+    x[4 * u + 2] = w.z;
+    x[4 * u + 3] = w.w;
   }
-  float lo[4], hi[4], bad[4];
+  uint32_t lo2[2] = {x[0], x[1]}, hi2[2] = {x[0], x[1]};
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    lo[c] = hi[c] = x[c];
-    bad[c] = 0.f;
-#pragma unroll
-    for (int i = c; i < E; i += 4) {
-      lo[c] = fminf(lo[c], x[i]);
-      hi[c] = fmaxf(hi[c], x[i]);
-      bad[c] += 0.f * x[i];  // NaN for an inf or NaN
-    }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      lo[c] = fminf(lo[c], __shfl_xor_sync(0xffffffffu, lo[c], o));
-      hi[c] = fmaxf(hi[c], __shfl_xor_sync(0xffffffffu, hi[c], o));
-      bad[c] += __shfl_xor_sync(0xffffffffu, bad[c], o);
-    }
+  for (int i = 2; i < E / 2; ++i) {
+    lo2[i & 1] = min_bf16x2(lo2[i & 1], x[i]);
+    hi2[i & 1] = max_bf16x2(hi2[i & 1], x[i]);
   }
-  uint32_t tail[4];  // scales 0 1, 2 3, minima 0 1, 2 3
-  float step[4];
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      lo2[c] = min_bf16x2(lo2[c], __shfl_xor_sync(0xffffffffu, lo2[c], o));
+      hi2[c] = max_bf16x2(hi2[c], __shfl_xor_sync(0xffffffffu, hi2[c], o));
+    }
+  // lane `sub` has group sub % 4's scale and minimum, and tells the others
+  float lo[4], step[4], inv[4];
+  uint32_t tail;  // (scale, minimum) of the lane's group
   {
-    float sc[4], mn[4];
+    const uint32_t lw = (sub & 2) ? lo2[1] : lo2[0], hw = (sub & 2) ? hi2[1] : hi2[0];
+    const float l = 0.5f * ((sub & 1) ? bf_hi(lw) : bf_lo(lw)), h = 0.5f * ((sub & 1) ? bf_hi(hw) : bf_lo(hw));
+    const bool good = l > -INFINITY && h < INFINITY;  // (NaN is neither)
+    const float s = bfr((h - l) / 7.5f);
+    tail = good ? pack_bf16x2(s, 2.f * l) : 0x7FFF7FFFu;
+    const float st = good && s > 0.f ? 0.5f * s : 1.f, iv = 1.f / st;  // a constant group: all codes 0
+    const int from = threadIdx.x & 24;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const float s = bfr((hi[c] - lo[c]) / 7.5f);
-      sc[c] = bad[c] == 0.f ? s : NAN;
-      mn[c] = bad[c] == 0.f ? 2.f * lo[c] : NAN;
-      step[c] = s > 0.f ? 0.5f * s : INFINITY;  // a constant group: all codes 0
+      lo[c] = __shfl_sync(0xffffffffu, l, from + c);
+      step[c] = __shfl_sync(0xffffffffu, st, from + c);
+      inv[c] = __shfl_sync(0xffffffffu, iv, from + c);
     }
-    tail[0] = pack_bf16x2(sc[0], sc[1]);
-    tail[1] = pack_bf16x2(sc[2], sc[3]);
-    tail[2] = pack_bf16x2(mn[0], mn[1]);
-    tail[3] = pack_bf16x2(mn[2], mn[3]);
   }
+  constexpr float kWhole = 12582912.f;  // adding it leaves the nearest whole number in the low bits
+  auto half_of = [&](int i) { return 0.5f * ((i & 1) ? bf_hi(x[i / 2]) : bf_lo(x[i / 2])); };
   uint32_t code[E / 8];
+  bool near_tie = false;
 #pragma unroll
   for (int u = 0; u < E / 8; ++u) {
     code[u] = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int c = i % 4;
-      const float q = rintf((x[8 * u + i] - lo[c]) / step[c]);
-      code[u] |= (uint32_t)fminf(fmaxf(q, 0.f), 15.f) << (4 * i);
+      const float d = half_of(8 * u + i) - lo[c], w = fmaf(d, inv[c], kWhole), q = w - kWhole;
+      const float r = fabsf(fmaf(-q, step[c], d));  // of a right code at most step / 2
+      near_tie |= !(r < 0.499996f * step[c]);
+      code[u] |= (__float_as_uint(w) & 15u) << (4 * i);
+    }
+  }
+  if (near_tie) {
+#pragma unroll
+    for (int u = 0; u < E / 8; ++u) {
+      code[u] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = i % 4;
+        const float q = rintf((half_of(8 * u + i) - lo[c]) / step[c]);
+        code[u] |= (uint32_t)fminf(fmaxf(q, 0.f), 15.f) << (4 * i);
+      }
     }
   }
   if (!on) return;
@@ -108,8 +151,8 @@ __global__ void __launch_bounds__(256)
   else
     *reinterpret_cast<uint32_t*>(dst + 4 * sub) = code[0];
   if (sub < 4) {
-    const uint32_t w = sub == 0 ? tail[0] : sub == 1 ? tail[1] : sub == 2 ? tail[2] : tail[3];
-    *reinterpret_cast<uint32_t*>(dst + D / 2 + 4 * sub) = w;
+    reinterpret_cast<uint16_t*>(dst + D / 2)[sub] = (uint16_t)tail;
+    reinterpret_cast<uint16_t*>(dst + D / 2)[4 + sub] = (uint16_t)(tail >> 16);
   }
 }
 
@@ -118,21 +161,20 @@ __global__ void __launch_bounds__(256)
 // record.  Bound by HBM: D / 2 + 16 bytes in, 2 D out.
 template <int D>
 __global__ void __launch_bounds__(256)
-    kv4_expand_kernel(const uint8_t* cache, int64_t num_pages, const int32_t* page_ids, int32_t n, int32_t per_page,
-                      bf16* out, int32_t* status) {
+    kv4_expand_kernel(const uint8_t* cache, int64_t num_pages, const int32_t* page_ids, int32_t per_page, bf16* out,
+                      int32_t* status) {
   constexpr int E = D / 8, kRecord = D / 2 + 16;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t rec = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 8;
-  const int sub = threadIdx.x % 8;
-  if (rec >= (int64_t)n * per_page) return;
-  const int i = (int)(rec / per_page);
+  // 32 records of page i (per_page, K and V, is a multiple of 32 for pages of 16 tokens)
+  const int blocks = per_page / 32, i = blockIdx.x / blocks;
+  const int at = (blockIdx.x - i * blocks) * 32 + threadIdx.x / 8, sub = threadIdx.x % 8;
   const int32_t pid = page_ids[i];
   if (pid < 0 || (int64_t)pid >= num_pages) {
-    if (pid != -1 && sub == 0 && rec % per_page == 0) set_status(status, PL_ERR_PAGE_OUT_OF_RANGE);
+    if (pid != -1 && threadIdx.x == 0) set_status(status, PL_ERR_PAGE_OUT_OF_RANGE);
     return;
   }
-  const uint8_t* src = cache + ((int64_t)pid * per_page + rec % per_page) * kRecord;
+  const uint8_t* src = cache + ((int64_t)pid * per_page + at) * kRecord;
   const uint4 tail = __ldg(reinterpret_cast<const uint4*>(src + D / 2));
   uint32_t code[E / 8];
   if constexpr (E == 16) {
@@ -142,19 +184,24 @@ __global__ void __launch_bounds__(256)
   } else {
     code[0] = __ldg(reinterpret_cast<const uint32_t*>(src + 4 * sub));
   }
-  const float sc[4] = {bf_lo(tail.x), bf_hi(tail.x), bf_lo(tail.y), bf_hi(tail.y)};
-  const float mn[4] = {bf_lo(tail.z), bf_hi(tail.z), bf_lo(tail.w), bf_hi(tail.w)};
-  uint4* dst = reinterpret_cast<uint4*>(out + rec * D + sub * E);
+  // Pairs of channels G and G + 4 of a word: 128 + code as bf16 bits, less 128, and one packed fma, which rounds
+  // min + scale * code once.
+  uint32_t sc[4], mn[4];
+  const uint32_t ts[4] = {tail.x, tail.x, tail.y, tail.y}, tm[4] = {tail.z, tail.z, tail.w, tail.w};
+#pragma unroll
+  for (int G = 0; G < 4; ++G) {
+    sc[G] = __byte_perm(ts[G], 0, (G & 1) ? 0x3232 : 0x1010);
+    mn[G] = __byte_perm(tm[G], 0, (G & 1) ? 0x3232 : 0x1010);
+  }
+  uint4* dst = reinterpret_cast<uint4*>(out + ((int64_t)i * per_page + at) * D + sub * E);
 #pragma unroll
   for (int u = 0; u < E / 8; ++u) {
-    uint32_t w[4];
+    uint32_t v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c0 = (2 * j) % 4, c1 = (2 * j + 1) % 4;
-      w[j] = pack_bf16x2(fmaf(sc[c0], (float)((code[u] >> (8 * j)) & 15), mn[c0]),
-                         fmaf(sc[c1], (float)((code[u] >> (8 * j + 4)) & 15), mn[c1]));
-    }
-    dst[u] = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int G = 0; G < 4; ++G)
+      v[G] = fma_bf16x2(sub_bf16x2(((code[u] >> (4 * G)) & 0x000F000Fu) | 0x43004300u, 0x43004300u), sc[G], mn[G]);
+    dst[u] = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
+                        __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
   }
 }
 
@@ -203,7 +250,8 @@ struct Kv4Cfg {
   static constexpr int kPartBytes = kTile * kRecord;      // K (or V) of a tile
   static constexpr int kCopies = 2 * kPartBytes / 512;    // copies of 16 bytes a lane and tile
   static constexpr int kStages = 4;                       // tiles of a warp's ring
-  static constexpr int kRingBytes = kStages * 2 * kPartBytes;
+  static constexpr int kStageBytes = 2 * kPartBytes;
+  static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kSteps = D / 64;                   // k16 steps of a group
   static constexpr int kTiles = D / 16;                   // output tiles
   static constexpr int kState = kTiles * 4 + 4;           // a lane's O, m and l of one column block
@@ -222,17 +270,6 @@ constexpr float kKv4Score = 590295810358705651712.f;      // 2^69
 constexpr float kKv4P = 60.f;                             // exponent of p's factor
 constexpr float kKv4Unp = 8.673617379884035e-19f;         // 2^-60
 constexpr float kKv4Out = 9444732965739290427392.f;       // 2^73 = 2^(133 - 60)
-
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 
 struct Kv4Plan {
   int32_t heads;   // kv heads of an item
@@ -275,6 +312,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
   const int log_per = __ffs(a.page_size) - 5;  // tiles of a page, a power of two
   const int tile_bytes = (int)token_bytes * kTile;
   const uint32_t ring_at = smem_u32(ring) + 16 * lane;
+  const uint32_t tails_at = smem_u32(ring) + C::kPartBytes + (lane % kTile) * C::kRecord + D / 2;
   uint32_t src_off[C::kCopies];
 #pragma unroll
   for (int i = 0; i < C::kCopies; ++i) {
@@ -342,7 +380,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
       return -1;
     };
     int32_t now = places(lane), next = places(32 + lane);
-    auto issue = [&](int k) {
+    auto issue = [&](int k, uint32_t stage) {
       if (k < n) {
         if (k != 0 && (k & 31) == 0) {
           now = next;
@@ -351,49 +389,57 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
         const int32_t place = __shfl_sync(0xffffffffu, now, k & 31);
         const uint32_t bytes = place >= 0 ? 16 : 0;  // else zeros
         const uint8_t* src = head_base + (int64_t)max(place, 0) * tile_bytes;
-        const uint32_t dst = ring_at + (k % C::kStages) * 2 * C::kPartBytes;
+        const uint32_t dst = ring_at + stage;
 #pragma unroll
         for (int i = 0; i < C::kCopies; ++i) cp_async16(dst + 512 * i, src + src_off[i], bytes);
       }
       cp_async_commit();  // (an empty group past the last tile keeps the count)
     };
 #pragma unroll
-    for (int k = 0; k < C::kStages - 1; ++k) issue(k);
+    for (int k = 0; k < C::kStages - 1; ++k) issue(k, k * C::kStageBytes);
+    uint32_t here = 0, freed = (C::kStages - 1) * C::kStageBytes;  // stages of tile k, of tile k - 1 and k + 3
+    int u = lo + turn;                                  // tile k's place among the visible ones
+    const int window_edge = sp.wlo > 0 ? sp.early : -1;  // (the sinks' tiles and the window's first)
 #pragma unroll 1
     for (int k = 0; k < n; ++k) {
       cp_async_wait<C::kStages - 2>();
       __syncwarp();  // tile k is there for all lanes, and all have done with tile k - 1
-      issue(k + C::kStages - 1);
-      const int base = tile_at(k) * kTile;
-      uint32_t* kt = reinterpret_cast<uint32_t*>(ring + (k % C::kStages) * 2 * C::kPartBytes);
-      uint32_t* vt = kt + C::kPartBytes / 4;
-      // positions of this tile may be hidden
-      const bool edge = base + kTile > sp.len || base < sp.wlo;
-      auto sees = [&](int pos) { return pos < sp.len && (pos >= sp.wlo || pos < a.sinks); };
+      issue(k + C::kStages - 1, freed);
+      const uint8_t* kg = ring + here + g * C::kRecord;                          // K of position g
+      const uint8_t* vt = ring + here + C::kPartBytes + 2 * t * C::kRecord;      // V of position 2t
+      const uint32_t tails = tails_at + here;
+      uint8_t* v_tile = ring + here + C::kPartBytes;
+      freed = here;
+      here = here == (C::kStages - 1) * C::kStageBytes ? 0 : here + C::kStageBytes;
+      // positions of this tile may be hidden: in front of the window, or behind the last one
+      const bool edge = u <= window_edge || u == sp.n - 1;
+      const int u_here = u;
+      u += pl.share;
+      auto sees = [&](int i) {
+        const int pos = sp.tile(u_here) * kTile + i;
+        return pos < sp.len && (pos >= sp.wlo || pos < a.sinks);
+      };
       if (edge) {  // p is 0 there, but 0 x NaN is NaN, so their V tails are cleared
-        if (lane < kTile && !sees(base + lane))
-          *reinterpret_cast<uint4*>(vt + lane * C::kWords + D / 8) = make_uint4(0, 0, 0, 0);
+        if (lane < kTile && !sees(lane))
+          *reinterpret_cast<uint4*>(v_tile + lane * C::kRecord + D / 2) = make_uint4(0, 0, 0, 0);
         __syncwarp();
       }
       // ---- scores of 16 positions x 8 heads, x 2^-69
       float sc[NT][4];
       {
-        const uint32_t* k0 = kt + g * C::kWords;
-        const uint32_t* k1 = k0 + 8 * C::kWords;
+        const uint32_t* k0 = reinterpret_cast<const uint32_t*>(kg) + t;
         uint32_t w0[2 * C::kSteps], w1[2 * C::kSteps];
 #pragma unroll
         for (int w = 0; w < 2 * C::kSteps; ++w) {
-          w0[w] = k0[t + 4 * w];
-          w1[w] = k1[t + 4 * w];
+          w0[w] = k0[4 * w];
+          w1[w] = k0[8 * C::kWords + 4 * w];
         }
-        const uint2 s0 = *reinterpret_cast<const uint2*>(k0 + D / 8), s1 = *reinterpret_cast<const uint2*>(k1 + D / 8);
-        const uint32_t mm0 = k0[D / 8 + 2 + (t & 1)], mm1 = k1[D / 8 + 2 + (t & 1)];
+        const uint4 s0 = *reinterpret_cast<const uint4*>(kg + D / 2);
+        const uint4 s1 = *reinterpret_cast<const uint4*>(kg + 8 * C::kRecord + D / 2);
+        const uint32_t mm0 = (t & 1) ? s0.w : s0.z, mm1 = (t & 1) ? s1.w : s1.z;
         const uint32_t ma[4] = {mm0, mm1, mm0, mm1};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-          mma_bf16_16816(sc[nt], ma, mq[nt]);
-        }
+        for (int nt = 0; nt < NT; ++nt) mma_bf16_16816_zero(sc[nt], ma, mq[nt]);
 #pragma unroll
         for (int G = 0; G < 4; ++G) {
           if (G == 2) {
@@ -408,13 +454,16 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
           const float f1 = (G & 1) ? bf_hi(G < 2 ? s1.x : s1.y) : bf_lo(G < 2 ? s1.x : s1.y);
           float acc[NT][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-#pragma unroll
           for (int st = 0; st < C::kSteps; ++st) {
             const uint32_t ka[4] = {w0[2 * st] & mask, w1[2 * st] & mask, w0[2 * st + 1] & mask,
                                     w1[2 * st + 1] & mask};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(acc[nt], ka, qb[nt][G][st]);
+            for (int nt = 0; nt < NT; ++nt) {
+              if (st == 0)
+                mma_bf16_16816_zero(acc[nt], ka, qb[nt][G][st]);
+              else
+                mma_bf16_16816(acc[nt], ka, qb[nt][G][st]);
+            }
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -434,7 +483,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
 #pragma unroll
           for (int c = 0; c < 4; ++c) x[nt][c] = fmaf(sc[nt][c], sl2, ref[nt][c & 1]);
         if (edge) {
-          const bool see0 = sees(base + g), see1 = sees(base + g + 8);
+          const bool see0 = sees(g), see1 = sees(g + 8);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -447,7 +496,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
 #pragma unroll
         for (int c = 0; c < 4; ++c) grow |= x[nt][c] > kKv4P + kLineSlack;
       if (__any_sync(0xffffffffu, grow)) {
-        const bool see0 = sees(base + g), see1 = sees(base + g + 8);
+        const bool see0 = !edge || sees(g), see1 = !edge || sees(g + 8);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -486,11 +535,11 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
         uint32_t ta[4] = {0u, 0u, 0u, 0u};
         asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
                      : "=r"(ta[0]), "=r"(ta[2])
-                     : "r"(smem_u32(vt + (lane % kTile) * C::kWords + D / 8)));
+                     : "r"(tails));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(pt[nt], ta, pp[nt][0]);
       }
-      const uint32_t* va = vt + 2 * t * C::kWords;
+      const uint32_t* va = reinterpret_cast<const uint32_t*>(vt);
       // ---- p x scale
       uint32_t pb[NT][4][2];
 #pragma unroll
@@ -776,8 +825,8 @@ extern "C" int32_t pl_kv4_append(const void* k, int64_t k_stride, const void* v,
   if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(kv4_cache)) & 15) !=
           0 || k_stride % 8 != 0 || v_stride % 8 != 0)
     return PL_ERR_INVALID_ARGUMENT;
-  const int64_t blocks = ((int64_t)num_tokens * 2 * num_kv_heads + 31) / 32;
-  if (blocks > 0x7FFFFFFF) return PL_ERR_UNSUPPORTED;
+  const int64_t records = (int64_t)num_tokens * 2 * num_kv_heads, blocks = (records + 31) / 32;
+  if (records > 0x7FFFFFFF) return PL_ERR_UNSUPPORTED;
   auto kern = head_dim == 128 ? pl::kv4_append_kernel<128> : pl::kv4_append_kernel<64>;
   return pl_host::launch_pdl(kern, dim3((unsigned)blocks), dim3(256), 0, stream, static_cast<const pl::bf16*>(k),
                              k_stride, static_cast<const pl::bf16*>(v), v_stride, static_cast<uint8_t*>(kv4_cache),
@@ -789,16 +838,16 @@ extern "C" int32_t pl_kv4_expand(const void* kv4_cache, int64_t num_pages, const
                                  int32_t* status_dev, void* stream) {
   if (n < 0 || num_kv_heads <= 0 || page_size <= 0 || num_pages <= 0 || kv4_cache == nullptr)
     return PL_ERR_INVALID_ARGUMENT;
-  if (head_dim != 64 && head_dim != 128) return PL_ERR_UNSUPPORTED;
+  if ((head_dim != 64 && head_dim != 128) || page_size % 16 != 0) return PL_ERR_UNSUPPORTED;
   if (n == 0) return PL_OK;
   if (page_ids == nullptr || out == nullptr ||
       ((reinterpret_cast<uintptr_t>(kv4_cache) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
     return PL_ERR_INVALID_ARGUMENT;
   const int64_t per_page = 2ll * page_size * num_kv_heads;
-  const int64_t blocks = (n * per_page + 31) / 32;
+  const int64_t blocks = n * (per_page / 32);
   if (blocks > 0x7FFFFFFF || per_page > 0x7FFFFFFF) return PL_ERR_UNSUPPORTED;
   auto kern = head_dim == 128 ? pl::kv4_expand_kernel<128> : pl::kv4_expand_kernel<64>;
   return pl_host::launch_pdl(kern, dim3((unsigned)blocks), dim3(256), 0, stream,
-                             static_cast<const uint8_t*>(kv4_cache), num_pages, page_ids, n, (int32_t)per_page,
+                             static_cast<const uint8_t*>(kv4_cache), num_pages, page_ids, (int32_t)per_page,
                              static_cast<pl::bf16*>(out), status_dev);
 }
