@@ -4,9 +4,12 @@
 // weight of every cached token accumulated (pl_paged_decode_weights).
 //
 // A CTA walks its piece of the line tile by tile (16 positions of one kv
-// head): warp 0 brings K and V by TMA (16 positions x 64 channels a box,
-// 128B-swizzled, eight tiles an instruction) through a ring that runs on
-// across items; tile i belongs to consumer warp i % 8.  Positions are the
+// head): warp 0 brings K and warp 1 V by TMA (16 positions x 64 channels a
+// box, 128B-swizzled, 32 KB an instruction) through a ring that runs on across
+// items.  (A warp's instruction takes about 0.4 us beside 0.7 for 32 KB of
+// rows: one warp for both, 64 KB at a time, 140 us for 48 windows of 4096
+// positions, 32 KB at a time 171.)  Tile i belongs to consumer warp i % 8.
+// Positions are the
 // rows of S^T = K.Q^T (mma m16n8k16: eight query heads side by side, so a
 // group of up to 8 wastes no row) and channels the rows of O^T = V^T.P^T; P
 // goes from the one's result layout to the other's operand layout by an 8x8
@@ -24,7 +27,7 @@
 namespace pl {
 
 constexpr int kLineWarps = 8;                          // consumer warps
-constexpr int kLineThreads = 32 * (1 + kLineWarps);
+constexpr int kLineThreads = 32 * (2 + kLineWarps);
 constexpr int kLineAccum = 256;                        // positions per block of the accumulation
 
 template <int D, int NT>
@@ -33,13 +36,14 @@ struct LineCfg {
   static constexpr int kHalfBytes = kTile * 128;             // one box
   static constexpr int kTileBytes = kHalves * kHalfBytes;    // K (or V) of a tile
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kBoxes = 2 * kHalves;
-  static constexpr int kBatch = 32 / kBoxes;                 // tiles per producer instruction
-  static constexpr int kStages = 2 * kBatch;                 // a multiple of kLineWarps
+  static constexpr int kBatch = 8 * (128 / D);               // tiles per producer instruction: 32 KB of K or of V
+  // Three batches make the ring (48 windows: 126 us, two 130); two where the
+  // join of two column blocks takes the room.
+  static constexpr int kStages = (NT == 1 ? 3 : 2) * kBatch;  // a multiple of kLineWarps
   static constexpr int kHeads = 8 * NT;
-  static constexpr int kRow = D + 4;                         // floats of a head's O in the join scratch
-  static constexpr int kJoinOff = kStages * kStageBytes;     // [warps][kHeads][kRow]
-  static constexpr int kMlOff = kJoinOff + kLineWarps * kHeads * kRow * 4;  // [warps][kHeads] (m, l)
+  static constexpr int kPiece = D + 4;                       // floats of a head's piece in the workspace
+  static constexpr int kJoinOff = kStages * kStageBytes;     // [warps][kHeads][D], swizzled
+  static constexpr int kMlOff = kJoinOff + kLineWarps * kHeads * D * 4;  // [warps][kHeads] (m, l)
   static constexpr int kBarOff = kMlOff + kLineWarps * kHeads * 8;
   static constexpr int kOkOff = kBarOff + 2 * kStages * 8;   // [stages] the tile's page exists
   static constexpr int kFindOff = (kOkOff + kStages * 4 + 15) & ~15;  // 36 int64
@@ -65,13 +69,13 @@ __global__ void __launch_bounds__(kLineThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 2);  // K's and V's copies
       mbar_init(&empty[s], 1);
     }
     flags[0] = 0;
     fence_barrier_init();
   }
-  if (threadIdx.x == 32) prefetch_tensormap(&kv_map);
+  if (threadIdx.x == 64) prefetch_tensormap(&kv_map);
   pdl_launch_dependents();
   pdl_wait();  // q, the page table and the cache come from upstream kernels
   int row0;
@@ -81,22 +85,24 @@ __global__ void __launch_bounds__(kLineThreads, 1)
   if ((int64_t)blockIdx.x >= cut.ctas) return;  // fewer pieces than CTAs: nothing was started
   const int64_t begin = cut.begin(blockIdx.x), end = cut.begin((int64_t)blockIdx.x + 1);
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    const int box = lane % C::kBoxes, kv = box / C::kHalves, hh = box % C::kHalves;
+  if (warp < 2) {
+    // ----------------------------------------------------------- producers
+    const int kv = warp, hh = lane % C::kHalves;
     int i0 = 0;  // tiles of this CTA so far
     for_each_segment(a, row0, row_start, begin, end, [&](int, const RowSpan& sp, int kvh, int lo, int hi) {
       const int n = hi - lo;
-      auto entry = [&](int u) {
-        return u < n ? a.indices[sp.begin + sp.tile(lo + u) * kTile / a.page_size] : -1;
-      };
-      int32_t next = entry(lane / C::kBoxes);
+      // page ids of 32 tiles a load, one load ahead: its latency would else bound every batch
+      auto entry = [&](int u) { return u < n ? a.indices[sp.begin + sp.tile(lo + u) * kTile / a.page_size] : -1; };
+      int32_t now = entry(lane), next = entry(32 + lane);
       for (int u0 = 0; u0 < n; u0 += C::kBatch) {
-        const int u = u0 + lane / C::kBoxes;
-        const bool on = u < n;
+        if (u0 != 0 && u0 % 32 == 0) {
+          now = next;
+          next = entry(u0 + 32 + lane);
+        }
+        const int u = u0 + lane / C::kHalves;
+        const bool on = lane < C::kBatch * C::kHalves && u < n;
         const int i = i0 + u, s = i % C::kStages;
-        const int32_t pid = next;
-        next = entry(u + C::kBatch);
+        const int32_t pid = __shfl_sync(0xffffffffu, now, u % 32);
         bool ok = true;
         if (on && i >= C::kStages) ok = mbar_wait(&empty[s], ((i / C::kStages) - 1) & 1);
         if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) {
@@ -110,10 +116,10 @@ __global__ void __launch_bounds__(kLineThreads, 1)
           return false;
         }
         const bool valid = on && pid >= 0 && (int64_t)pid < a.num_pages;
-        if (on && box == 0) {
-          page_ok[s] = valid;
+        if (on && hh == 0) {
+          if (kv == 0) page_ok[s] = valid;
           if (valid) {
-            mbar_arrive_expect_tx(&full[s], C::kStageBytes);
+            mbar_arrive_expect_tx(&full[s], C::kTileBytes);
           } else {
             set_status(a.status, PL_ERR_PAGE_OUT_OF_RANGE);
             mbar_arrive(&full[s]);
@@ -129,7 +135,7 @@ __global__ void __launch_bounds__(kLineThreads, 1)
     });
   } else {
     // ----------------------------------------------------------- consumers
-    const int cw = warp - 1, ctid = threadIdx.x - 32;
+    const int cw = warp - 2, ctid = threadIdx.x - 64;
     const int g = lane >> 2, t = lane & 3;
     float* join = reinterpret_cast<float*>(smem + C::kJoinOff);
     float2* ml = reinterpret_cast<float2*>(smem + C::kMlOff);
@@ -269,14 +275,15 @@ __global__ void __launch_bounds__(kLineThreads, 1)
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
-      float* mine = join + cw * C::kHeads * C::kRow;
+      // channel d of head h at d ^ 8 (h / 2 % 4): the lanes of a store differ in bank
+      float* mine = join + cw * C::kHeads * D;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int j = 0; j < D / 16; ++j)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            mine[(8 * nt + 2 * t + (c & 1)) * C::kRow + 16 * j + g + 8 * (c >> 1)] = o[nt][j][c];
+            mine[(8 * nt + 2 * t + (c & 1)) * D + ((16 * j + g + 8 * (c >> 1)) ^ (8 * t))] = o[nt][j][c];
         if (g == 0) {
           ml[cw * C::kHeads + 8 * nt + 2 * t] = make_float2(m[nt][0], l[nt][0]);
           ml[cw * C::kHeads + 8 * nt + 2 * t + 1] = make_float2(m[nt][1], l[nt][1]);
@@ -284,7 +291,7 @@ __global__ void __launch_bounds__(kLineThreads, 1)
       }
       named_barrier(1, 32 * kLineWarps);
       const bool whole = lo == 0 && hi == sp.n;
-      float* piece = a.partial + ((int64_t)blockIdx.x * 2 + (lo == 0 ? 1 : 0)) * a.group * C::kRow;
+      float* piece = a.partial + ((int64_t)blockIdx.x * 2 + (lo == 0 ? 1 : 0)) * a.group * C::kPiece;
       for (int idx = ctid; idx < a.group * (D / 4); idx += 32 * kLineWarps) {
         const int h = idx / (D / 4), d = 4 * (idx % (D / 4));
         float M = -INFINITY, L = 0.f;
@@ -295,7 +302,7 @@ __global__ void __launch_bounds__(kLineThreads, 1)
         for (int w = 0; w < kLineWarps; ++w) {
           const float2 x = ml[w * C::kHeads + h];
           const float wt = x.x == -INFINITY ? 0.f : exp2f(x.x - M);  // 0 x NaN stays NaN: a query of NaN
-          const float4 v = *reinterpret_cast<const float4*>(join + (w * C::kHeads + h) * C::kRow + d);
+          const float4 v = *reinterpret_cast<const float4*>(join + (w * C::kHeads + h) * D + (d ^ (8 * (h / 2 % 4))));
           L += wt * x.y;
           acc.x += wt * v.x;
           acc.y += wt * v.y;
@@ -312,8 +319,8 @@ __global__ void __launch_bounds__(kLineThreads, 1)
           if (a.out_lse != nullptr && d == 0)
             a.out_lse[(int64_t)row * a.num_qo_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
         } else {
-          *reinterpret_cast<float4*>(piece + h * C::kRow + d) = acc;
-          if (d == 0) *reinterpret_cast<float2*>(piece + h * C::kRow + D) = make_float2(M, L);
+          *reinterpret_cast<float4*>(piece + h * C::kPiece + d) = acc;
+          if (d == 0) *reinterpret_cast<float2*>(piece + h * C::kPiece + D) = make_float2(M, L);
         }
       }
       if (ctid == 0) flags[1] = flags[0];  // one decision for all warps
@@ -336,11 +343,13 @@ __global__ void __launch_bounds__(kLineAccum)
   const int64_t t0 = (int64_t)blockIdx.x * (kLineAccum / kTile);
   const int64_t t1 = t0 + kLineAccum / kTile < tiles ? t0 + kLineAccum / kTile : tiles;
   // first row whose pages end behind this block's first tile
-  int lo = 0, hi = a.batch;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if ((int64_t)a.indptr[mid + 1] * per > t0) hi = mid; else lo = mid + 1;
-  }
+  __shared__ int first_row;
+  if (threadIdx.x == 0) first_row = a.batch;
+  __syncthreads();
+  for (int r = threadIdx.x; r < a.batch; r += kLineAccum)
+    if ((int64_t)a.indptr[r + 1] * per > t0 && (r == 0 || (int64_t)a.indptr[r] * per <= t0)) atomicMin(&first_row, r);
+  __syncthreads();
+  const int lo = first_row;
   for (int r = lo; r < a.batch; ++r) {
     const RowSpan sp = row_span(a, r, false);
     const int64_t first = (int64_t)sp.begin * per;
@@ -361,8 +370,15 @@ __global__ void __launch_bounds__(kLineAccum)
     float* dst = weight + (int64_t)r * weight_stride + pos;
     const float old = *dst;
     float sum = 0.f;
-#pragma unroll 8
-    for (int h = 0; h < a.num_qo_heads; ++h) sum += line_exp2(__ldcg(sc + h * kTile) - lse2[h]);
+    constexpr int kLoads = 16;  // in flight
+    for (int h0 = 0; h0 < a.num_qo_heads; h0 += kLoads) {
+      float v[kLoads];
+#pragma unroll
+      for (int h = 0; h < kLoads; ++h) v[h] = h0 + h < a.num_qo_heads ? __ldcg(sc + (h0 + h) * kTile) : -INFINITY;
+#pragma unroll
+      for (int h = 0; h < kLoads; ++h)
+        if (h0 + h < a.num_qo_heads) sum += line_exp2(v[h] - lse2[h0 + h]);
+    }
     *dst = old + sum;
   }
 }
