@@ -249,7 +249,7 @@ struct Kv4Cfg {
   static constexpr int kWords = kRecord / 4;
   static constexpr int kPartBytes = kTile * kRecord;      // K (or V) of a tile
   static constexpr int kCopies = 2 * kPartBytes / 512;    // copies of 16 bytes a lane and tile
-  static constexpr int kStages = 4;                       // tiles of a warp's ring
+  static constexpr int kStages = 5;                       // tiles of a warp's ring
   static constexpr int kStageBytes = 2 * kPartBytes;
   static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kSteps = D / 64;                   // k16 steps of a group
@@ -257,8 +257,8 @@ struct Kv4Cfg {
   static constexpr int kState = kTiles * 4 + 4;           // a lane's O, m and l of one column block
   static constexpr int kRegs = NT * kState;
   static constexpr int kRingOff = 36 * 8;                 // behind line_find's scratch
-  static constexpr int kJoinOff = kRingOff + kWarps * kRingBytes;  // [warps - 1] states (warps that share a head)
-  static constexpr int kSmemBytes = kJoinOff + (kWarps - 1) * kRegs * 128;
+  static constexpr int kSmemBytes = kRingOff + kWarps * kRingBytes;
+  static_assert(kRegs * 128 <= kRingBytes, "a warp's state joins through its ring");
   static_assert(2 * kPartBytes % 512 == 0, "whole copies");
   static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "the rings exceed the shared memory");
 };
@@ -305,7 +305,6 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
   const int g = lane >> 2, t = lane & 3;
   const int sharers = pl.heads * pl.share * 32;  // threads at the join's barriers
   const float sl2 = a.scale_log2 * kKv4Score;    // scores come x 2^-69
-  float* join = reinterpret_cast<float*>(smem + C::kJoinOff);
   uint8_t* ring = smem + C::kRingOff + warp * C::kRingBytes;
   // a lane's copies of a tile: 16-byte unit lane + 32 i of [K, V][position][record]
   const int64_t token_bytes = (int64_t)a.num_kv_heads * C::kRecord;
@@ -397,20 +396,72 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
     };
 #pragma unroll
     for (int k = 0; k < C::kStages - 1; ++k) issue(k, k * C::kStageBytes);
-    uint32_t here = 0, freed = (C::kStages - 1) * C::kStageBytes;  // stages of tile k, of tile k - 1 and k + 3
+    // Scores of a tile: the groups' products one by one (step), so that they
+    // can stand between those of another tile's V.
+    float sc[NT][4];  // 16 positions x 8 heads, x 2^-69
+    uint32_t w0[2 * C::kSteps], w1[2 * C::kSteps];
+    uint2 s0, s1;
+    auto scores_begin = [&](uint32_t stage) {
+      const uint8_t* kg = ring + stage + g * C::kRecord;  // K of position g
+      const uint32_t* k0 = reinterpret_cast<const uint32_t*>(kg) + t;
+#pragma unroll
+      for (int w = 0; w < 2 * C::kSteps; ++w) {
+        w0[w] = k0[4 * w];
+        w1[w] = k0[8 * C::kWords + 4 * w];
+      }
+      const uint4 t0 = *reinterpret_cast<const uint4*>(kg + D / 2);
+      const uint4 t1 = *reinterpret_cast<const uint4*>(kg + 8 * C::kRecord + D / 2);
+      const uint32_t mm0 = (t & 1) ? t0.w : t0.z, mm1 = (t & 1) ? t1.w : t1.z;
+      const uint32_t ma[4] = {mm0, mm1, mm0, mm1};
+      s0 = make_uint2(t0.x, t0.y);
+      s1 = make_uint2(t1.x, t1.y);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma_bf16_16816_zero(sc[nt], ma, mq[nt]);
+    };
+    auto scores_step = [&](int G) {
+      if (G == 2) {
+#pragma unroll
+        for (int w = 0; w < 2 * C::kSteps; ++w) {
+          w0[w] >>= 8;
+          w1[w] >>= 8;
+        }
+      }
+      const uint32_t mask = (G & 1) ? kOdd : kEven;
+      const float f0 = (G & 1) ? bf_hi(G < 2 ? s0.x : s0.y) : bf_lo(G < 2 ? s0.x : s0.y);
+      const float f1 = (G & 1) ? bf_hi(G < 2 ? s1.x : s1.y) : bf_lo(G < 2 ? s1.x : s1.y);
+      float acc[NT][4];
+#pragma unroll
+      for (int st = 0; st < C::kSteps; ++st) {
+        const uint32_t ka[4] = {w0[2 * st] & mask, w1[2 * st] & mask, w0[2 * st + 1] & mask, w1[2 * st + 1] & mask};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (st == 0)
+            mma_bf16_16816_zero(acc[nt], ka, qb[nt][G][st]);
+          else
+            mma_bf16_16816(acc[nt], ka, qb[nt][G][st]);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        sc[nt][0] = fmaf(acc[nt][0], f0, sc[nt][0]);
+        sc[nt][1] = fmaf(acc[nt][1], f0, sc[nt][1]);
+        sc[nt][2] = fmaf(acc[nt][2], f1, sc[nt][2]);
+        sc[nt][3] = fmaf(acc[nt][3], f1, sc[nt][3]);
+      }
+    };
+    uint32_t here = 0, freed = (C::kStages - 1) * C::kStageBytes;  // stages of tile k, of tile k - 1 (and k + 4)
     int u = lo + turn;                                  // tile k's place among the visible ones
     const int window_edge = sp.wlo > 0 ? sp.early : -1;  // (the sinks' tiles and the window's first)
+    cp_async_wait<C::kStages - 2>();
+    __syncwarp();
+    scores_begin(0);
+#pragma unroll
+    for (int G = 0; G < 4; ++G) scores_step(G);
 #pragma unroll 1
     for (int k = 0; k < n; ++k) {
-      cp_async_wait<C::kStages - 2>();
-      __syncwarp();  // tile k is there for all lanes, and all have done with tile k - 1
-      issue(k + C::kStages - 1, freed);
-      const uint8_t* kg = ring + here + g * C::kRecord;                          // K of position g
-      const uint8_t* vt = ring + here + C::kPartBytes + 2 * t * C::kRecord;      // V of position 2t
+      const uint8_t* vt = ring + here + C::kPartBytes + 2 * t * C::kRecord;  // V of position 2t
       const uint32_t tails = tails_at + here;
       uint8_t* v_tile = ring + here + C::kPartBytes;
-      freed = here;
-      here = here == (C::kStages - 1) * C::kStageBytes ? 0 : here + C::kStageBytes;
       // positions of this tile may be hidden: in front of the window, or behind the last one
       const bool edge = u <= window_edge || u == sp.n - 1;
       const int u_here = u;
@@ -423,56 +474,6 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
         if (lane < kTile && !sees(lane))
           *reinterpret_cast<uint4*>(v_tile + lane * C::kRecord + D / 2) = make_uint4(0, 0, 0, 0);
         __syncwarp();
-      }
-      // ---- scores of 16 positions x 8 heads, x 2^-69
-      float sc[NT][4];
-      {
-        const uint32_t* k0 = reinterpret_cast<const uint32_t*>(kg) + t;
-        uint32_t w0[2 * C::kSteps], w1[2 * C::kSteps];
-#pragma unroll
-        for (int w = 0; w < 2 * C::kSteps; ++w) {
-          w0[w] = k0[4 * w];
-          w1[w] = k0[8 * C::kWords + 4 * w];
-        }
-        const uint4 s0 = *reinterpret_cast<const uint4*>(kg + D / 2);
-        const uint4 s1 = *reinterpret_cast<const uint4*>(kg + 8 * C::kRecord + D / 2);
-        const uint32_t mm0 = (t & 1) ? s0.w : s0.z, mm1 = (t & 1) ? s1.w : s1.z;
-        const uint32_t ma[4] = {mm0, mm1, mm0, mm1};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_bf16_16816_zero(sc[nt], ma, mq[nt]);
-#pragma unroll
-        for (int G = 0; G < 4; ++G) {
-          if (G == 2) {
-#pragma unroll
-            for (int w = 0; w < 2 * C::kSteps; ++w) {
-              w0[w] >>= 8;
-              w1[w] >>= 8;
-            }
-          }
-          const uint32_t mask = (G & 1) ? kOdd : kEven;
-          const float f0 = (G & 1) ? bf_hi(G < 2 ? s0.x : s0.y) : bf_lo(G < 2 ? s0.x : s0.y);
-          const float f1 = (G & 1) ? bf_hi(G < 2 ? s1.x : s1.y) : bf_lo(G < 2 ? s1.x : s1.y);
-          float acc[NT][4];
-#pragma unroll
-          for (int st = 0; st < C::kSteps; ++st) {
-            const uint32_t ka[4] = {w0[2 * st] & mask, w1[2 * st] & mask, w0[2 * st + 1] & mask,
-                                    w1[2 * st + 1] & mask};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if (st == 0)
-                mma_bf16_16816_zero(acc[nt], ka, qb[nt][G][st]);
-              else
-                mma_bf16_16816(acc[nt], ka, qb[nt][G][st]);
-            }
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            sc[nt][0] = fmaf(acc[nt][0], f0, sc[nt][0]);
-            sc[nt][1] = fmaf(acc[nt][1], f0, sc[nt][1]);
-            sc[nt][2] = fmaf(acc[nt][2], f1, sc[nt][2]);
-            sc[nt][3] = fmaf(acc[nt][3], f1, sc[nt][3]);
-          }
-        }
       }
       // exponents of p; one above 60 + the slack moves the reference (at first it is -inf)
       float x[NT][4];
@@ -553,6 +554,13 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
 #pragma unroll
           for (int G = 0; G < 4; ++G) pb[nt][G][y] = mul_bf16x2(pp[nt][G & 1][y], ss[G]);
       }
+      // ---- tile k + 1 is there for all lanes, and all have done with tile k - 1
+      cp_async_wait<C::kStages - 3>();
+      __syncwarp();
+      issue(k + C::kStages - 1, freed);
+      freed = here;
+      here = here == (C::kStages - 1) * C::kStageBytes ? 0 : here + C::kStageBytes;
+      scores_begin(here);  // (behind the last tile: of a stage that nobody reads again)
       // ---- O^T += (codes - 8)^T . (P scale)^T; the two halves of a word in turn
       uint32_t lo01[C::kSteps], hi01[C::kSteps], lo89[C::kSteps], hi89[C::kSteps];
 #pragma unroll
@@ -596,6 +604,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][j], wa, pb[nt][G]);
         }
+        scores_step(G);
       }
     }
     cp_async_wait<0>();
@@ -625,7 +634,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
       }
     // ---- join the warps that share the head, in turn order
     if (pl.share > 1) {
-      float* slot = join + (hh * (pl.share - 1) + turn - 1) * C::kRegs * 32 + lane;  // (turn 0 keeps its own)
+      float* slot = reinterpret_cast<float*>(ring) + lane;  // (turn 0 keeps its own)
       if (turn != 0) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -646,7 +655,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
         for (int other = 1; other < pl.share; ++other)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const float* p = slot + other * C::kRegs * 32 + nt * C::kState * 32;
+            const float* p = slot + other * (C::kRingBytes / 4) + nt * C::kState * 32;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const float mo = p[(C::kTiles * 4 + e) * 32], lo_ = p[(C::kTiles * 4 + 2 + e) * 32];
