@@ -140,9 +140,10 @@ class TreeDecoder:
                 qkv = self._linear(xn, L["w_qkv"])
             else:
                 qkv = self._linear(x, L["w_qkv"], prologue=PL_PROLOGUE_RMSNORM, norm_weight=L["input_norm"])
+            kv, kv_page, kv_off = self._kv_target(li, slot_page, slot_off)
             K.qkv_rope_append(qkv, num_qo_heads=s.num_qo_heads, num_kv_heads=s.num_kv_heads, head_dim=s.head_dim,
-                              positions=positions, rope_theta=s.rope_theta, kv_cache=e.kv[li], page_id=slot_page,
-                              page_offset=slot_off, q_out=q, lora_down=down, lora_b=L["b_qkv"] if lora else None,
+                              positions=positions, rope_theta=s.rope_theta, kv_cache=kv, page_id=kv_page,
+                              page_offset=kv_off, q_out=q, lora_down=down, lora_b=L["b_qkv"] if lora else None,
                               lora_scale=e.qkv_lora_scale, tok_adapter=adapter, q_norm_weight=L["q_norm"],
                               k_norm_weight=L["k_norm"], norm_eps=s.rms_eps, status=self.status)
             attn = attend(li, q).view(n, s.q_dim)
@@ -156,6 +157,11 @@ class TreeDecoder:
                 gate_up = self._linear(x, L["w_gate_up"], prologue=PL_PROLOGUE_RMSNORM, norm_weight=L["post_norm"])
                 x = self._linear(gate_up, L["w_down"], prologue=PL_PROLOGUE_SILU_MUL, residual=x)
         return self._linear(x, e.lm_head, prologue=PL_PROLOGUE_RMSNORM, norm_weight=e.final_norm)
+
+    def _kv_target(self, li, slot_page, slot_off):
+        """(pool, pages, offsets) that a layer's new K/V are written to."""
+
+        return self.e.kv[li], slot_page, slot_off
 
     def _reserve(self, tok_indptr, total):
         slot_page = torch.empty(total, dtype=torch.int32, device=self.lens.device)
