@@ -1099,7 +1099,8 @@ int32_t pl_paged_sparse_decode(const void *q, int64_t q_stride_b,
  * position.  q, kv_cache, indptr, indices, last_page_len, out, out_lse as
  * pl_paged_decode; total_pages = entries of indices; a table outside them
  * writes PL_ERR_INVALID_ARGUMENT and counts as empty.  Pages without a visible
- * position are not looked up.  workspace: 16-byte aligned, no
+ * position are not looked up; a looked up entry outside the pool writes
+ * PL_ERR_PAGE_OUT_OF_RANGE and its positions are not seen.  workspace: 16-byte aligned, no
  * initialisation, of a size that does not depend on the batch.  Supported:
  * head_dim 64 or 128, page_size 16 / 32 / 64 / 128, group <= 16, batch <=
  * 65535, total_pages * page_size < 2^31.
@@ -1160,7 +1161,8 @@ int32_t pl_paged_window_prefill(const void *q, int64_t q_stride_t,
  *
  * pl_paged_kv4_decode: one query token per row over the records (their values
  * are not rounded); arguments as pl_paged_window_decode, window 0: the whole
- * context.
+ * context.  Elements of q and scales are below 2^56 in size.  An entry outside
+ * the pool writes PL_ERR_PAGE_OUT_OF_RANGE and counts as a page of zeros.
  */
 int32_t pl_kv4_append(const void *k, int64_t k_stride, const void *v,
                       int64_t v_stride, void *kv4_cache, int64_t num_pages,

@@ -48,6 +48,13 @@ __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t 
   return r;
 }
 
+// a b - c
+__device__ __forceinline__ uint32_t fms_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 n;\n\tneg.bf16x2 n, %3;\n\tfma.rn.bf16x2 %0, %1, %2, n;\n\t}" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
 // ----------------------------------------------------------------- append
 // Eight lanes take one record (K or V of one head of one token): D / 8
 // channels a lane, a group's extremes by three exchanges.  Differences are
@@ -227,19 +234,23 @@ __global__ void __launch_bounds__(256)
 //   S_jh = sum_G s_jG (sum_{d in G} q_hd c_jd) + sum_G m_jG Q_hG,
 //   O_dh = sum_j (p_jh s_jG)(c_jd - 8) + sum_j p_jh m_jG + 8 sum_j p_jh s_jG.
 // sum_G m Q is one product with Q in three bf16 parts (exact to 2^-24); the
-// last two sums are the rows of one product with the tile's tails.  Codes of
-// V are centred (one subtraction for two) since rounding p s to bf16 and the
-// tensor core's truncating sums err in proportion to the operand: uncentred
-// codes measured a relative error of 0.0045 at 600 positions and, with an
-// offset of 128 in place of the subnormals, 0.039 at 8192, where this form
-// has 0.003.  K is exact; p is rounded to bf16 and so is p s (2^-9 each).
+// last two sums are the rows of one product with the tile's tails.  K is
+// exact.  p is rounded to bf16 (2^-9, as elsewhere); p s enters as a bf16 value
+// and its exact remainder, since a group's spread can exceed a channel's: one
+// rounded p s gave a relative error of 0.0031 in place of 0.0023 (and 616 us
+// in place of 697, for 64 rows of 8192 positions and 32 kv heads; remainders
+// of p too: 0.0017 and 740).  Codes of V are centred (one subtraction for two)
+// since the tensor core's sums truncate in proportion to what they hold: an
+// offset of 128 in place of the subnormals measured 0.039 at 8192 positions.
 // P^T is turned into the operand layout before the scales go on, as packed
-// pairs: two transposes and eight products instead of eight and sixteen.
+// pairs.
 //
-// Bound by HBM in bytes (160 a position and head at head_dim 128 where bf16
-// has 512), and near it by the logic pipe: about 130 of its half-rate
-// instructions a tile and head.  Two CTAs share an SM where a group fits one
-// column block, so that one's latencies are the other's issue slots.
+// The bytes (160 a position and head at head_dim 128 where bf16 has 512) are
+// within reach of HBM, 412 us there; what bounds it is issue: about 390
+// instructions a tile and head, half of them on the half-rate logic pipe, and
+// 26 products.  Two CTAs share an SM where a group fits one column block (128
+// registers a thread), and the next tile's scores stand between this one's
+// values (646 -> 616 us), so that one's latencies are the other's issue slots.
 template <int D, int NT>
 struct Kv4Cfg {
   static constexpr int kWarps = 8;
@@ -519,17 +530,15 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
         exponents();
       }
       // ---- P, its sums, and P^T (lane (g, t): head g, positions 2t, 2t+1 and 2t+8, 2t+9)
-      uint32_t pp[NT][2][2];  // [even, odd groups][pair]
+      uint32_t ph[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float p0 = line_exp2(x[nt][0]), p1 = line_exp2(x[nt][1]);
         const float p2 = line_exp2(x[nt][2]), p3 = line_exp2(x[nt][3]);
         l[nt][0] += p0 + p2;
         l[nt][1] += p1 + p3;
-        pp[nt][0][0] = movmatrix_trans(pack_bf16x2(p0, p1));
-        pp[nt][0][1] = movmatrix_trans(pack_bf16x2(p2, p3));
-#pragma unroll
-        for (int y = 0; y < 2; ++y) pp[nt][1][y] = mul_bf16x2(pp[nt][0][y], 0x3D803D80u);  // / 16
+        ph[nt][0] = movmatrix_trans(pack_bf16x2(p0, p1));
+        ph[nt][1] = movmatrix_trans(pack_bf16x2(p2, p3));
       }
       // ---- sum p scale and sum p min: rows of one product with the tails, turned as they are read
       {
@@ -538,21 +547,19 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
                      : "=r"(ta[0]), "=r"(ta[2])
                      : "r"(tails));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(pt[nt], ta, pp[nt][0]);
+        for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(pt[nt], ta, ph[nt]);
       }
       const uint32_t* va = reinterpret_cast<const uint32_t*>(vt);
-      // ---- p x scale
-      uint32_t pb[NT][4][2];
+      // ---- scales of the positions, in pairs; those of odd groups / 16
+      uint32_t ss[4][2];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         const uint2 s0 = *reinterpret_cast<const uint2*>(va + 8 * y * C::kWords + D / 8);
         const uint2 s1 = *reinterpret_cast<const uint2*>(va + (8 * y + 1) * C::kWords + D / 8);
-        const uint32_t ss[4] = {__byte_perm(s0.x, s1.x, 0x5410), __byte_perm(s0.x, s1.x, 0x7632),
-                                __byte_perm(s0.y, s1.y, 0x5410), __byte_perm(s0.y, s1.y, 0x7632)};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int G = 0; G < 4; ++G) pb[nt][G][y] = mul_bf16x2(pp[nt][G & 1][y], ss[G]);
+        ss[0][y] = __byte_perm(s0.x, s1.x, 0x5410);
+        ss[1][y] = mul_bf16x2(__byte_perm(s0.x, s1.x, 0x7632), 0x3D803D80u);
+        ss[2][y] = __byte_perm(s0.y, s1.y, 0x5410);
+        ss[3][y] = mul_bf16x2(__byte_perm(s0.y, s1.y, 0x7632), 0x3D803D80u);
       }
       // ---- tile k + 1 is there for all lanes, and all have done with tile k - 1
       cp_async_wait<C::kStages - 3>();
@@ -585,26 +592,40 @@ __global__ void __launch_bounds__(Kv4Cfg<D, NT>::kThreads, Kv4Cfg<D, NT>::kCtas)
           }
         }
         const uint32_t mask = (G & 1) ? kOdd : kEven, mid = (G & 1) ? 0x00800080u : 0x00080008u;
+        // p scale as a bf16 value and its (exact) remainder
+        uint32_t hi[NT][2], lo_part[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            hi[nt][y] = mul_bf16x2(ph[nt][y], ss[G][y]);
+            lo_part[nt][y] = fms_bf16x2(ph[nt][y], ss[G][y], hi[nt][y]);
+          }
+        uint32_t wa[C::kTiles / 4][4];
 #pragma unroll
         for (int j = G; j < C::kTiles; j += 4) {
-          uint32_t wa[4];
+          uint32_t* w = wa[j / 4];
           if constexpr (D == 128) {
-            wa[0] = j < 4 ? lo01[0] : hi01[0];
-            wa[1] = j < 4 ? lo01[C::kSteps - 1] : hi01[C::kSteps - 1];
-            wa[2] = j < 4 ? lo89[0] : hi89[0];
-            wa[3] = j < 4 ? lo89[C::kSteps - 1] : hi89[C::kSteps - 1];
+            w[0] = j < 4 ? lo01[0] : hi01[0];
+            w[1] = j < 4 ? lo01[C::kSteps - 1] : hi01[C::kSteps - 1];
+            w[2] = j < 4 ? lo89[0] : hi89[0];
+            w[3] = j < 4 ? lo89[C::kSteps - 1] : hi89[C::kSteps - 1];
           } else {
-            wa[0] = lo01[0];
-            wa[1] = hi01[0];
-            wa[2] = lo89[0];
-            wa[3] = hi89[0];
+            w[0] = lo01[0];
+            w[1] = hi01[0];
+            w[2] = lo89[0];
+            w[3] = hi89[0];
           }
 #pragma unroll
-          for (int c = 0; c < 4; ++c) wa[c] = sub_bf16x2(wa[c] & mask, mid);
+          for (int c = 0; c < 4; ++c) w[c] = sub_bf16x2(w[c] & mask, mid);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][j], wa, pb[nt][G]);
+          for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][j], w, hi[nt]);
         }
-        scores_step(G);
+        scores_step(G);  // (between the two products of an accumulator)
+#pragma unroll
+        for (int j = G; j < C::kTiles; j += 4)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][j], wa[j / 4], lo_part[nt]);
       }
     }
     cp_async_wait<0>();
