@@ -1156,8 +1156,8 @@ def _need_queries(q: torch.Tensor, rows: str = "tokens") -> None:
 
 
 def _need_window(window: int, sinks: int) -> None:
-    if window < 1 or sinks < 0:
-        raise ValueError("window must be at least 1 and sinks at least 0")
+    if not 1 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31:
+        raise ValueError("window must be at least 1 and sinks at least 0, both below 2**31")
 
 
 @lru_cache(maxsize=256)
@@ -1458,8 +1458,8 @@ def evict_select(weight: torch.Tensor, lens: torch.Tensor, budget: int, *, sinks
 
     rows = lens.numel()
     _vecs(torch.int32, "lens keep_from keep_count", (lens, keep_from, keep_count), (rows, rows, rows))
-    if sinks < 0 or recent < 0 or sinks + recent > budget:
-        raise ValueError("a budget needs sinks >= 0, recent >= 0 and sinks + recent <= budget")
+    if sinks < 0 or recent < 0 or sinks + recent > budget or budget >= 2 ** 31:
+        raise ValueError("a budget needs sinks >= 0, recent >= 0 and sinks + recent <= budget < 2**31")
     w_stride, w_cap = _need_rows(weight, "weight", rows, torch.float32)
     o_stride, o_cap = _need_rows(out_weight, "out_weight", rows, torch.float32)
     k_stride, k_width = _need_rows(keep, "keep", rows)
