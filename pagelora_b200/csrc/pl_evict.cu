@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kPwThreads, 1)
       // place tile i takes)
       if (i >= kPwSlots) ok = mbar_wait(&qempty[s], ((i / kPwSlots) - 1) & 1);
       if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) {
-        if (lane == 0 && !__all_sync(0xffffffffu, ok)) set_status(a.status, PL_ERR_TIMEOUT);
+        if (!ok) set_status(a.status, PL_ERR_TIMEOUT);
         flags[0] = 1;
         break;
       }

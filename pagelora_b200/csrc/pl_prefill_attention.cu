@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       bool ok = true;
       if (i >= kPrefillSlots) ok = mbar_wait(&empty[s], ((i / kPrefillSlots) - 1) & 1);
       if (__any_sync(0xffffffffu, !ok || flags[0] != 0)) {  // one decision for the whole warp
-        if (lane == 0 && !__all_sync(0xffffffffu, ok)) set_status(a.status, PL_ERR_TIMEOUT);
+        if (!ok) set_status(a.status, PL_ERR_TIMEOUT);
         flags[0] = 1;
         break;
       }
