@@ -1147,8 +1147,9 @@ int32_t pl_paged_window_prefill(const void *q, int64_t q_stride_t,
  * head of one token's K (or V): head_dim / 2 bytes of codes, channel 2i in
  * the low half of byte i; four scales, then four minima, bf16.  Channel c
  * belongs to group c % 4 and stands for min + scale * code; min is the
- * group's smallest value, scale = bf16((max - min) / 15), code = rint((x -
- * min) / scale) within 0 .. 15.  A group with inf or NaN stands for NaN.
+ * group's smallest value, scale = bf16((max - min) / 15), 0 where that is below
+ * 2^-120, code = rint((x - min) / scale) within 0 .. 15 (scale 0: code 0).  A
+ * group with inf or NaN stands for NaN.
  * head_dim 64 or 128.  The page operations move records as token_bytes =
  * num_kv_heads * (head_dim / 2 + 16).  No reference counterpart.
  *

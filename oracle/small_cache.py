@@ -79,6 +79,7 @@ def pack4(x):
     grp = half.reshape(*half.shape[:-1], half.shape[-1] // 4, 4)
     lo, hi = grp.min(-2), grp.max(-2)
     scale = to_bf16((hi - lo) / np.float32(7.5))
+    scale = np.where(scale >= 2.0 ** -120, scale, 0).astype(np.float32)
     step = np.where(scale > 0, np.float32(0.5) * scale, np.float32(np.inf))
     code = np.clip(np.rint((grp - lo[..., None, :]) / step[..., None, :]), 0, 15)
     return code.reshape(half.shape).astype(np.int64), scale, lo * np.float32(2)

@@ -269,3 +269,12 @@ def test_prompt_weights_over_many_runs(K, n, length, hq, hkv):
     K.paged_prefill_weights(dev["q"], dev["cache"], *tables, lse, weight, workspace=ws)
     added = o.paged(host["q"], host["cache"], host["qo"], host["indptr"], host["indices"], host["last"], 64 ** -0.5)[2]
     _weights_ok(weight, torch.zeros(1, length), added, [length])
+
+
+def test_select_of_more_positions_than_shared_memory_holds(K):
+    rng = np.random.default_rng(77)
+    w = (rng.random((2, 500_000)) ** 6).astype(np.float32)
+    w[1, ::2] = 0.5
+    weight = torch.as_tensor(w).cuda()
+    lens = [500_000, 450_001]
+    _check_select(_select(K, weight, lens, 30_000, 7, 1000), weight, lens, 30_000, 7, 1000)

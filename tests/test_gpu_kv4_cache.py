@@ -44,6 +44,8 @@ def test_append(K, d, ps, hkv, t):
     x[1, t // 2] = -1.5          # constant groups
     x[0, t // 3, :, 5] = 3e38    # a difference that fp32 does not hold
     x[0, t // 3, :, 9] = -3e38
+    x[1, 0] = rng.normal(size=(hkv, d)) * 2.0 ** -125  # a spread that no scale is given for
+    x[1, t - 1] = rng.normal(size=(hkv, d)) * 2.0 ** -110
     xt = _bf16(x)
     wide = torch.zeros(t, 2, hkv * d, dtype=torch.bfloat16, device="cuda")  # strided rows
     wide[:, 0].copy_(xt[0].reshape(t, -1))
@@ -62,7 +64,7 @@ def test_append(K, d, ps, hkv, t):
         rec = o.record_bytes(*o.pack4(xs))
         want[slots // ps, kv, slots % ps] = rec
         val, scale, _ = o.unpack4(rec)
-        assert (np.abs(val - xs) <= scale * (0.5 + 15 * 2.0 ** -9)).all()
+        assert (np.abs(val - xs) <= scale * (0.5 + 15 * 2.0 ** -9) + 15 * 2.0 ** -120).all()
     assert (got == want).all()
     # expanded: the values, rounded once
     ids = np.concatenate([np.unique(slots // ps)[::-1], [-1]])
