@@ -64,6 +64,8 @@ def test_append(K, d, ps, hkv, t):
         rec = o.record_bytes(*o.pack4(xs))
         want[slots // ps, kv, slots % ps] = rec
         val, scale, _ = o.unpack4(rec)
+        # Half a code, and 15 codes times the scale's rounding.  A group whose spread / 15 is below 2^-120 has scale 0 and
+        # comes back as its minimum: off by its spread at most, which is below 15 * 2^-120.
         assert (np.abs(val - xs) <= scale * (0.5 + 15 * 2.0 ** -9) + 15 * 2.0 ** -120).all()
     assert (got == want).all()
     # expanded: the values, rounded once
