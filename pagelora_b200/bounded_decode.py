@@ -172,6 +172,7 @@ class BoundedDecoder(TreeDecoder):
     def fork(self, src: list[int], dst: list[int]) -> None:
         """As TreeDecoder's; positions, weights and records go with the row."""
 
+        empty = self.num == 0
         if self.kv4 is not None:
             s, d = self._row_ids(src), self._row_ids(dst)
             if len(src) != len(dst):
@@ -183,11 +184,12 @@ class BoundedDecoder(TreeDecoder):
             self.lens.copy_(self._row_lens())
         else:
             super().fork(src, dst)
+        # The rows that the call began.  A refused one began none, whatever its dst held; a dst listed twice is refused.
         s, d = self._row_ids(src).long(), self._row_ids(dst).long()
-        same = self.lens[d] == self.lens[s]  # (a refused fork leaves the row empty)
-        self.pos[d] = torch.where(same, self.pos[s], 0)
+        began = empty[d] & (self.num[d] > 0)
+        self.pos[d] = torch.where(began, self.pos[s], self.pos[d])
         if self.budget is not None:
-            self.weight[d] = torch.where(same[:, None], self.weight[s], 0.0)
+            self.weight[d] = torch.where(began[:, None], self.weight[s], self.weight[d])
 
     def release(self, rows: list[int]) -> None:
         super().release(rows)
