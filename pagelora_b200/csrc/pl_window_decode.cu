@@ -356,8 +356,10 @@ __global__ void __launch_bounds__(kLineAccum)
     if (first >= t1) break;
     if (sp.n == 0) continue;
     __syncthreads();
-    for (int h = threadIdx.x; h < a.num_qo_heads; h += kLineAccum)
-      lse2[h] = lse[(int64_t)r * a.num_qo_heads + h] * kLog2e;
+    for (int h = threadIdx.x; h < a.num_qo_heads; h += kLineAccum) {
+      const float l = lse[(int64_t)r * a.num_qo_heads + h];
+      lse2[h] = l == -INFINITY ? INFINITY : l * kLog2e;  // a row that sees nothing gives nothing (-inf less -inf is NaN)
+    }
     __syncthreads();
     const int64_t tile = t0 + threadIdx.x / kTile;
     const int64_t pos = (tile - first) * kTile + threadIdx.x % kTile;
