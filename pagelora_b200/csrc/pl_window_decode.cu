@@ -352,9 +352,9 @@ __global__ void __launch_bounds__(kLineAccum)
   const int lo = first_row;
   for (int r = lo; r < a.batch; ++r) {
     const RowSpan sp = row_span(a, r, false);
+    if (sp.n == 0) continue;  // (a table outside the entries may begin anywhere: the rows behind it count)
     const int64_t first = (int64_t)sp.begin * per;
     if (first >= t1) break;
-    if (sp.n == 0) continue;
     __syncthreads();
     for (int h = threadIdx.x; h < a.num_qo_heads; h += kLineAccum) {
       const float l = lse[(int64_t)r * a.num_qo_heads + h];

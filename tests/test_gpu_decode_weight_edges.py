@@ -53,3 +53,22 @@ def test_decode_of_rows_whose_pages_are_not_in_the_pool(K, hq, hkv, d):
     p = o.attend(host["q"][2], k, v, see, d ** -0.5)[2]
     _weights_ok(weight[2:], before[2:].cpu(), [p.sum(0)], [48])
     assert torch.equal(weight[2, 16:32], before[2, 16:32])
+
+
+@pytest.mark.parametrize("ends", [[0, 4, 1000, 8, 12], [0, 1000, 8, 12, 16], [0, 4, -3, 8, 12]])
+def test_decode_of_rows_behind_a_table_outside_the_entries(K, ends):
+    lens = [60, 61, 62, 63]
+    host, dev = _case(lens, [1] * 4, 8, 2, 64, 16, 12)
+    weight, status = torch.zeros(4, 64, device="cuda"), _status()
+    indices = dev["indices"]  # 16 entries
+    last = _i32([12] * 4)
+    K.paged_decode_weights(dev["q"], dev["cache"], _i32(ends), indices, last, weight, status=status)
+    assert int(status.item()) == 1
+    for r in range(4):
+        a, b = ends[r], ends[r + 1]
+        if not 0 <= a <= b <= 16:
+            assert (weight[r] == 0).all()
+            continue
+        alone = torch.zeros(1, 64, device="cuda")
+        K.paged_decode_weights(dev["q"][r:r + 1], dev["cache"], _i32([0, b - a]), indices[a:b].contiguous(), last[:1], alone)
+        assert torch.allclose(weight[r], alone[0], rtol=2.0 ** -11, atol=1e-9) and (weight[r, :60] > 0).all(), r
