@@ -71,13 +71,17 @@ struct PromptWeightCfg {
 };
 
 // 2^x of a pair by range reduction to [-1/2, 1/2] and a polynomial of degree 5
-// of least relative error there, 1 at 0 (9.2e-8; 1.9e-7 with fp32's roundings,
-// where the multi-function unit has 2.4e-7).  x below -127 counts as -127,
-// whose bits come out as 0; NaN stays NaN.
+// of least relative error there, 1 at 0 (1.2e-7 with its coefficients in fp32;
+// 1.8e-7 with the roundings of its steps, where the multi-function unit has
+// 2.4e-7).  x below -127 counts as -127, whose bits come out as 0, and above
+// 128 as 128, whose bits are inf.  NaN has no bits that the exponent's addition
+// would leave a NaN, so 0 x is added at the end.
 __device__ __forceinline__ float2 pw_exp2_pair(float2 x) {
   auto clamp = [](float v) {
     float r;
-    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(r) : "f"(v));  // -127
+    asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, 0fC2FE0000;\n\tmin.NaN.f32 %0, t, 0f43000000;\n\t}"  // -127, 128
+        : "=f"(r)
+        : "f"(v));
     return r;
   };
   auto both = [](float v) { return make_float2(v, v); };
@@ -90,8 +94,9 @@ __device__ __forceinline__ float2 pw_exp2_pair(float2 x) {
   p = fma_f32x2(p, f, both(0.24022242426872253f));
   p = fma_f32x2(p, f, both(0.6931470036506653f));
   p = fma_f32x2(p, f, both(1.f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
+  p = make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
+                  __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
+  return fma_f32x2(x, both(0.f), p);
 }
 
 // Request and run of positions that block `x` of the line of runs takes; a
