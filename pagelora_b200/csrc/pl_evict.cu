@@ -130,7 +130,7 @@ __device__ __forceinline__ bool pw_find(const PromptWeightArgs& a, int x, PwSpan
   int before = 0;
   for (int base = 0; base < a.batch; base += 32) {
     const int b = base + lane;
-    const int len = b < a.batch ? pw_kv_len(a, b, x == 0) : 0;
+    const int len = b < a.batch ? pw_kv_len(a, b, false) : 0;
     const int n = (len + kPwRun - 1) / kPwRun;
     int incl = n;
 #pragma unroll
@@ -433,22 +433,27 @@ __global__ void __launch_bounds__(kPwThreads, 1)
 
 // weight[b][pos] += the sums of the kv heads and of the chunks whose queries see
 // the position's run, in this order; a thread per position of the page
-// table's line.
+// table's line.  The requests that hold the block's entries are looked for one
+// by one, since requests with bad tables (which block 0 reports) may stand
+// between them.
 __global__ void __launch_bounds__(256)
     prompt_weight_add_kernel(const PromptWeightArgs a, int32_t hkv, float* weight, int64_t weight_stride,
                              int32_t capacity) {
+  __shared__ int32_t owner[256 / 16];
   pdl_launch_dependents();
   pdl_wait();
   const int64_t all = a.total_pages * a.page_size;
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int entries = 256 / a.page_size, e0 = (int)(blockIdx.x * entries);
+  if (threadIdx.x < entries) owner[threadIdx.x] = a.batch;
+  __syncthreads();
+  for (int b = threadIdx.x; b < a.batch; b += 256)
+    if (pw_kv_len(a, b, blockIdx.x == 0) > 0)
+      for (int e = max(a.kv_indptr[b], e0); e < min(a.kv_indptr[b + 1], e0 + entries); ++e) atomicMin(&owner[e - e0], b);
+  __syncthreads();
   if (at >= all) return;
-  const int32_t entry = (int32_t)(at / a.page_size);
-  int lo = 0, hi = a.batch;  // the row that holds the entry
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (a.kv_indptr[mid + 1] > entry) hi = mid; else lo = mid + 1;
-  }
-  if (lo >= a.batch || a.kv_indptr[lo] > entry) return;
+  const int lo = owner[threadIdx.x / a.page_size];
+  if (lo >= a.batch) return;
   const int len = pw_kv_len(a, lo, false);
   const int64_t pos = at - (int64_t)a.kv_indptr[lo] * a.page_size;
   if (pos >= len) return;
@@ -731,14 +736,14 @@ extern "C" int32_t pl_paged_prefill_weights(const void* q, int64_t q_stride_t, i
       (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) || num_kv_heads > 65535 ||
       total_pages * page_size > 0x7FFFFFFFll || num_pages > 0x3FFFFFFFll)
     return PL_ERR_UNSUPPORTED;
-  if (batch == 0 || total_q == 0 || total_pages == 0) return PL_OK;
-  if (q == nullptr || qo_indptr == nullptr || kv_indptr == nullptr || kv_indices == nullptr ||
+  if (batch == 0 || total_q == 0) return PL_OK;
+  if (q == nullptr || qo_indptr == nullptr || kv_indptr == nullptr || (kv_indices == nullptr && total_pages > 0) ||
       kv_last_page_len == nullptr || lse == nullptr)
     return PL_ERR_INVALID_ARGUMENT;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv_cache)) & 15) != 0 || q_stride_t <= 0 || q_stride_h <= 0 || q_stride_t % 8 != 0 || q_stride_h % 8 != 0)
     return PL_ERR_INVALID_ARGUMENT;
-  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
-      workspace_bytes < pl_prefill_weights_workspace_bytes(num_kv_heads, page_size, total_pages))
+  if (total_pages > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
+                          workspace_bytes < pl_prefill_weights_workspace_bytes(num_kv_heads, page_size, total_pages)))
     return PL_ERR_WORKSPACE_TOO_SMALL;
 
   pl::PromptWeightArgs a = {};
@@ -763,6 +768,12 @@ extern "C" int32_t pl_paged_prefill_weights(const void* q, int64_t q_stride_t, i
   a.partial = static_cast<float*>(workspace);
   a.status = status_dev;
 
+  const int64_t add = (total_pages * page_size + 255) / 256;
+  auto launch_add = [&](int64_t blocks) {
+    return pl_host::launch_pdl(pl::prompt_weight_add_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a,
+                               num_kv_heads, weight, weight_stride, weight_capacity);
+  };
+  if (total_pages == 0) return launch_add(1);  // tokens without a cached position: reported
   CUtensorMap kv_map, q_map;
   int32_t st = pl_host::kv_tensor_map(kv_cache, num_pages, num_kv_heads, head_dim, page_size, &kv_map);
   if (st != PL_OK) return st;
@@ -783,10 +794,7 @@ extern "C" int32_t pl_paged_prefill_weights(const void* q, int64_t q_stride_t, i
   if (blocks > 0x7FFFFFFF) return PL_ERR_UNSUPPORTED;
   st = head_dim == 128 ? launch_prompt_weights<128>(kv_map, q_map, a, blocks, stream)
                        : launch_prompt_weights<64>(kv_map, q_map, a, blocks, stream);
-  if (st != PL_OK) return st;
-  const int64_t add = (total_pages * page_size + 255) / 256;
-  return pl_host::launch_pdl(pl::prompt_weight_add_kernel, dim3((unsigned)add), dim3(256), 0, stream, a,
-                             num_kv_heads, weight, weight_stride, weight_capacity);
+  return st != PL_OK ? st : launch_add(add);
 }
 
 extern "C" int32_t pl_evict_select(const float* weight, int64_t weight_stride, int32_t capacity, const int32_t* lens,

@@ -114,3 +114,51 @@ def test_one_exponential_of_a_prompt(K, at):
     s = torch.full((128,), -INF)
     s[:64] = -1e30
     assert (_exact_scores(K, s.cuda(), 1.0, at) == 0).all()
+
+
+# ------------------------------------------------------------------ tables
+def _many(seed):
+    return _case([20 + i for i in range(40)], [5] * 40, 4, 2, 64, 16, seed)
+
+
+def test_prompts_behind_the_first_requests_report_bad_tables(K):
+    host, dev = _many(3)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    good = _prompt(K, host, dev, status=status)
+    assert int(status.item()) == 0 and (good[:, :20] > 0).all()
+
+    def past(tables):
+        tables[1] = tables[1].clone()
+        tables[1][36] = 100000  # the end of request 35, the beginning of request 36
+
+    got = _prompt(K, host, dev, past, status)
+    rest = [r for r in range(40) if r not in (35, 36)]
+    assert int(status.item()) == 1
+    assert torch.equal(got[rest], good[rest]) and (got[35:37] == 0).all()
+
+
+def test_prompts_behind_the_first_requests_report_too_many_tokens(K):
+    lens = [20 + i for i in range(40)]
+    host, dev = _case(lens, [5] * 39 + [59], 4, 2, 64, 16, 3)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    good = _prompt(K, host, dev, status=status)
+    assert int(status.item()) == 0
+    tables = [dev["qo"], dev["indptr"], dev["indices"], dev["last"]]
+    lse = torch.empty(dev["q"].shape[:2], device="cuda")
+    K.paged_prefill(dev["q"], dev["cache"], *tables, out_lse=lse)
+    last = dev["last"].clone()
+    last[39] = 1  # 49 positions for 59 tokens
+    weight = torch.zeros(40, 200, device="cuda")
+    K.paged_prefill_weights(dev["q"], dev["cache"], *tables[:3], last, lse, weight, status=status)
+    assert int(status.item()) == 1
+    assert torch.equal(weight[:39], good[:39]) and (weight[39] == 0).all()
+
+
+def test_prompts_without_any_page_are_reported(K):
+    q = torch.randn(3, 4, 64, device="cuda").bfloat16()
+    cache = torch.zeros(2, 2, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+    weight, status = torch.full((2, 10), 3.0, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    K.paged_prefill_weights(q, cache, _i32([0, 3, 3]), _i32([0, 0, 0]), none, _i32([0, 0]),
+                            torch.zeros(3, 4, device="cuda"), weight, status=status)
+    assert int(status.item()) == 1 and (weight == 3).all()
