@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       }
     }
     tc_fence_after();
-    const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+    const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // (a query of NaN has a sum of NaN)
     bf16* dst = a.out + (int64_t)(qo_begin + tok) * a.out_stride_t + (int64_t)head * a.out_stride_h;
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     }
     if (a.lse != nullptr && row_ok && !flags[0])
       a.lse[(int64_t)(qo_begin + tok) * a.num_qo_heads + head] =
-          l_run > 0.f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+          l_run == 0.f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
   }
 
   // ------------------------------------------------------------ teardown
