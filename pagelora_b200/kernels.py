@@ -1206,9 +1206,11 @@ def paged_window_prefill(
     if batch == 0 or total_q == 0:
         return out
     if kv_indices.numel() == 0:  # no request has a cached position: nothing to see
+        at = torch.arange(total_q, device=q.device)
+        asked = (at >= qo_indptr[0]) & (at < qo_indptr[-1])  # (other rows stay as they are)
         if out_lse is not None:
-            out_lse.fill_(-math.inf)
-        return out.zero_()
+            out_lse.view(-1)[:total_q * hq].view(total_q, hq).masked_fill_(asked[:, None], -math.inf)
+        return out.masked_fill_(asked[:, None, None], 0)
     call("pl_paged_window_prefill", q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), num_pages,
          qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), batch,
          total_q, hq, hkv, d, page_size, d ** -0.5 if sm_scale is None else float(sm_scale), window, sinks,

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_gpu_window_attention import _case
+from tests.test_gpu_window_attention import _case, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,14 @@ def test_log_sums_of_prompt_queries_of_nan(K, window, d):
     assert out[bad].isnan().all() and lse[bad].isnan().all()
     assert torch.equal(out[~bad], clean[~bad]) and torch.equal(lse[~bad], clean_lse[~bad])
     assert (out[60:62] == 0).all() and torch.isneginf(lse[60:62]).all()
+
+
+def test_window_prompts_without_pages_leave_the_rows_behind_the_last(K):
+    q = torch.randn(6, 4, 64, device="cuda").bfloat16()
+    cache = torch.randn(2, 2, 16, 2, 64, device="cuda").bfloat16()
+    out, lse = torch.full_like(q, 5.0), torch.full((6, 4), 7.0, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    K.paged_window_prefill(q, cache, _i32([0, 1, 4]), _i32([0, 0, 0]), none, _i32([0, 0]), window=8, sinks=1, out=out,
+                           out_lse=lse)
+    assert (out[:4] == 0).all() and torch.isneginf(lse[:4]).all()
+    assert (out[4:] == 5).all() and (lse[4:] == 7).all()
