@@ -63,8 +63,9 @@ class BoundedDecoder(TreeDecoder):
             raise ValueError("a bounded decoder needs a window, an eviction budget or a 4-bit cache")
         if window is not None:
             K._need_window(window.size, window.sinks)
-        if evict is not None and (evict.sinks < 0 or evict.recent < 0 or evict.sinks + evict.recent > evict.tokens):
-            raise ValueError("a budget needs sinks >= 0, recent >= 0 and sinks + recent <= tokens")
+        if evict is not None and (evict.tokens < 1 or evict.sinks < 0 or evict.recent < 0 or
+                                  evict.sinks + evict.recent > evict.tokens):
+            raise ValueError("a budget needs tokens >= 1, sinks >= 0, recent >= 0 and sinks + recent <= tokens")
         if engine.spec.num_qo_heads > 16 * engine.spec.num_kv_heads:
             raise ValueError("at most 16 query heads per kv head")
         super().__init__(engine)
