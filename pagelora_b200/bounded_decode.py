@@ -6,7 +6,8 @@
 rows fork and end) and decodes one token per row and step with one of
 
 * a sliding window with sinks (``window``): every layer's attention is
-  paged_window_decode;
+  paged_window_decode, and :meth:`BoundedDecoder.trim` gives back what no later
+  token sees;
 * eviction by accumulated attention weight (``evict``): the steps'
   paged_decode_weights note what every cached token receives, over heads and
   layers, and :meth:`BoundedDecoder.evict` cuts the rows that outgrew their
@@ -169,6 +170,26 @@ class BoundedDecoder(TreeDecoder):
         done = (lens == self._keep_from + self._keep_count).all()
         self.weight, self._weight_next = torch.where(done, self._weight_next, self.weight), self.weight
         self.lens.copy_(lens)
+
+    @torch.no_grad()
+    def trim(self) -> None:
+        """Rows give back what no later token sees: a row longer than ``sinks`` +
+        ``size`` of the window keeps its first ``sinks`` and last ``size`` tokens.
+        What stays moves to new pages in every layer, so a call is for when rows
+        have grown by many tokens, not for every step.  One that is refused (no
+        free pages to move what stays) changes no row."""
+
+        if self.window is None:
+            raise ValueError("the decoder was built without a window (window)")
+        size, sinks = self.window.size, self.window.sinks
+        if sinks + size >= self.cap * self.e.page_size:
+            return  # no row is longer
+        cut = self.lens > sinks + size
+        keep_from, count = torch.where(cut, sinks, self.lens), cut.to(torch.int32) * size
+        keep = (self.lens - size)[:, None] + torch.arange(size, dtype=torch.int32, device=self.lens.device)
+        K.cache_compact(self.e.kv if self.kv4 is None else self.kv4, self.refcount, self.table, self.num, self.last,
+                        keep_from, keep, count, status=self.status)
+        self.lens.copy_(self._row_lens())
 
     def fork(self, src: list[int], dst: list[int]) -> None:
         """As TreeDecoder's; positions, weights and records go with the row."""

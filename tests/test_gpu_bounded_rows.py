@@ -4,7 +4,9 @@ later token sees, and the pool that a 4-bit cache leaves unused."""
 from __future__ import annotations
 
 import pytest
+import torch
 
+from test_gpu_bounded_decode import Bounded
 from test_gpu_tree_decode_refusals import Run
 
 pytestmark = pytest.mark.gpu
@@ -19,3 +21,77 @@ def test_a_budget_keeps_a_token(cuda_device):
     with pytest.raises(ValueError):
         BoundedDecoder(run.dec.e, evict=EvictBudget(0, sinks=0, recent=0))
     BoundedDecoder(run.dec.e, evict=EvictBudget(1, sinks=0, recent=0))
+
+
+def _held(dec):
+    """Every row's cached tokens [position, layer, ...] of the pool that the decoder reads."""
+
+    pool = dec.e.kv if dec.kv4 is None else dec.kv4
+    for r, n in enumerate(dec.lens.tolist()):
+        pos = torch.arange(n, device=pool.device)
+        yield pool[:, dec.table[r, pos // 16].long(), :, pos % 16].clone()
+
+
+@pytest.mark.parametrize("kv4", [False, True])
+def test_trim_keeps_sinks_and_window(cuda_device, kv4):
+    from pagelora_b200.bounded_decode import Window
+
+    run = Bounded(cuda_device, [100, 15, 33, 26, 70], window=Window(24, 2), kv4=kv4, engine=dict(max_context=192))
+    run.step()
+    run.release(1)
+    run.release(4)
+    run.dec.fork([0], [4])  # shared pages
+    run.history[4], run.cur[4] = list(run.history[0]), run.cur[0] ^ 1
+    run.step()
+    old, lens, pos = list(_held(run.dec)), run.dec.lens.tolist(), run.dec.pos.clone()
+    assert lens == [102, 0, 35, 28, 102]
+    run.dec.trim()
+    run.dec.check()
+    assert run.dec.lens.tolist() == [26, 0, 26, 26, 26] and torch.equal(run.dec.pos, pos)
+    for n, a, b in zip(lens, old, _held(run.dec)):
+        keep = list(range(min(n, 2))) + list(range(max(2, n - 24), n))
+        assert torch.equal(b, a[keep])
+    assert int((run.dec.refcount > 0).sum()) == 2 * 4  # two pages a row
+    again = list(_held(run.dec))
+    run.dec.trim()
+    run.dec.check()
+    assert all(torch.equal(a, b) for a, b in zip(again, _held(run.dec)))
+    run.step()
+    assert run.dec.lens.tolist() == [27, 0, 27, 27, 27]
+
+
+def test_a_text_longer_than_the_rows(cuda_device):
+    """With trim() now and then a window's decoder goes on in seven pages a row as one does that keeps them all."""
+
+    from pagelora_b200.bounded_decode import Window
+
+    lens = [60, 15, 33]
+    small = Bounded(cuda_device, lens, window=Window(24, 2), engine=dict(max_context=96))
+    large = Bounded(cuda_device, lens, window=Window(24, 2), engine=dict(max_context=400))
+    for i in range(300):
+        small.cur = list(large.cur)
+        a, b = small.step(), large.step()
+        assert (a.float() - b.float()).abs().max() < 0.1, i
+        if i % 40 == 39:
+            small.dec.trim()
+            small.dec.check()
+            assert small.dec.lens.tolist() == [26, 26, 26]
+    assert small.dec.pos.tolist() == [360, 315, 333] == large.dec.lens.tolist()
+
+
+def test_a_refused_trim_changes_nothing(cuda_device):
+    from pagelora_b200.bounded_decode import EvictBudget, Window
+
+    run = Bounded(cuda_device, [96, 96], window=Window(50, 2), engine=dict(max_context=96, num_pages=14))
+    run.step()  # 14 pages: all taken
+    before, pos = run.state(), run.dec.pos.clone()
+    run.dec.trim()  # no page to move the kept tokens to
+    run.unchanged(before, "PL_ERR_POOL_EXHAUSTED")
+    assert torch.equal(run.dec.pos, pos)
+    run.step()
+    with pytest.raises(ValueError):
+        Bounded(cuda_device, [20], evict=EvictBudget(64)).dec.trim()
+    run = Bounded(cuda_device, [20], window=Window(2 ** 31 - 1), engine=dict(max_context=96))
+    run.dec.trim()  # no row can be longer
+    run.dec.check()
+    assert run.dec.lens.tolist() == [20]
