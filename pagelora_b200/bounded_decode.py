@@ -54,7 +54,8 @@ class EvictBudget:
 
 class BoundedDecoder(TreeDecoder):
     """``engine.step_*`` must not be used any more; with ``kv4`` neither its bf16
-    pages, which stay as they were."""
+    pages, which stay as they were, beside the records.  The decoder does not
+    read them again: ``engine.kv = None`` gives their memory back."""
 
     def __init__(self, engine: BatchDecodeEngine, *, window: Window | None = None, evict: EvictBudget | None = None,
                  kv4: bool = False) -> None:
@@ -83,11 +84,14 @@ class BoundedDecoder(TreeDecoder):
         if kv4:
             layers, pages, _, ps, hkv, d = engine.kv.shape
             self.kv4 = torch.zeros(layers, pages, 2, ps, hkv, K.kv4_record_bytes(d), dtype=torch.uint8, device=dev)
-            slot = torch.arange(pages * ps, dtype=torch.int32, device=dev)
-            page, off = slot // ps, slot % ps
+            some = max(1, (1 << 24) // (ps * hkv * d))  # pages a call: its K and V are copied, 32 MB each
+            slot = torch.arange(min(some, pages) * ps, dtype=torch.int32, device=dev)
             for li in range(layers):
-                k, v = (engine.kv[li, :, i].reshape(pages * ps, hkv, d) for i in (0, 1))
-                K.kv4_append(k, v, self.kv4[li], page, off, self.status)
+                for p0 in range(0, pages, some):
+                    x = engine.kv[li, p0:p0 + some]
+                    n = x.shape[0] * ps
+                    k, v = (x[:, i].reshape(n, hkv, d) for i in (0, 1))
+                    K.kv4_append(k, v, self.kv4[li], slot[:n] // ps + p0, slot[:n] % ps, self.status)
             # the step's new K/V, one page a row, on their way into the records
             self._staged = torch.zeros(self.rows, 2, 1, hkv, d, dtype=torch.bfloat16, device=dev)
             self._staged_page = torch.arange(self.rows, dtype=torch.int32, device=dev)

@@ -95,3 +95,45 @@ def test_a_refused_trim_changes_nothing(cuda_device):
     run.dec.trim()  # no row can be longer
     run.dec.check()
     assert run.dec.lens.tolist() == [20]
+
+
+def test_a_4_bit_cache_without_the_bf16_pool(cuda_device):
+    from pagelora_b200.bounded_decode import Window
+
+    runs = [Bounded(cuda_device, [40, 15, 33], window=Window(24, 2), kv4=True, engine=dict(max_context=4000))
+            for _ in range(2)]
+    gone = runs[1].dec.e
+    pool = gone.kv.numel() * 2
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    gone.kv = None
+    assert before - torch.cuda.memory_allocated() >= pool
+    for step in range(3):
+        a, b = (run.step() for run in runs)
+        assert torch.equal(a, b)
+        for run in runs:
+            if step == 0:
+                run.release(1)
+                run.dec.fork([0], [1])
+                run.history[1], run.cur[1] = list(run.history[0]), run.cur[0] ^ 1
+            run.dec.trim()
+            run.dec.check()
+    for x, y in zip(_held(runs[0].dec), _held(runs[1].dec)):
+        assert torch.equal(x, y)
+
+
+def test_the_records_of_a_large_pool(cuda_device):
+    """Pages behind the first run of the quantisation as well."""
+
+    from oracle import small_cache as o
+    from pagelora_b200.bounded_decode import BoundedDecoder
+
+    run = Run(cuda_device, [20], num_pages=9000)  # 4096 pages of 16 tokens, 2 heads a call
+    kv = run.dec.e.kv
+    for p in (4095, 4096, 8191, 8192, 8999):
+        kv[:, p].normal_()
+    dec = BoundedDecoder(run.dec.e, kv4=True)
+    for li in range(kv.shape[0]):
+        for p in (0, 4095, 4096, 8191, 8192, 8999):
+            assert (dec.kv4[li, p].cpu().numpy() == o.record_bytes(*o.pack4(kv[li, p].float().cpu().numpy()))).all(), (li, p)
+    assert (dec.kv4[:, 4097:8191] == 0).all()
