@@ -448,7 +448,8 @@ int32_t pl_splitkv_exchange_merge(const float *part,
  *   total_q     >= qo_indptr[batch]; sizes the grid and bounds every q/out access
  *   out         bf16 like q; out_lse nullable fp32 [total_q, num_qo_heads], natural log
  * head_dim 64 or 128, page_size 16/32/64/128, num_qo_heads / num_kv_heads
- * <= 128.  Rows with no visible key get O = 0 (LSE -inf).  Device errors
+ * <= 128.  Rows with no visible key get O = 0 (LSE -inf), a query of NaN that
+ * sees one gets NaN in both.  Device errors
  * (PL_ERR_PAGE_OUT_OF_RANGE: the page reads as zeros; PL_ERR_INVALID_ARGUMENT:
  * qo_indptr outside [0, total_q]) go to *status_dev.
  */
@@ -1155,15 +1156,20 @@ int32_t pl_paged_window_prefill(const void *q, int64_t q_stride_t,
  *
  * pl_kv4_append: K and V bf16 [num_tokens][num_kv_heads][head_dim] (heads
  * contiguous, 16-byte aligned rows) go to (page_id[t], page_offset[t]); a
- * slot outside the pool writes PL_ERR_PAGE_OUT_OF_RANGE and is left out.
+ * slot outside the pool writes PL_ERR_PAGE_OUT_OF_RANGE and is left out.  The
+ * slots of a call are distinct: one that is listed twice may hold parts of both.
  *
  * pl_kv4_expand: out[i], bf16 [2][page_size][num_kv_heads][head_dim], receives
  * the values of page page_ids[i], rounded once; an entry of -1 is left out.
  *
  * pl_paged_kv4_decode: one query token per row over the records (their values
  * are not rounded); arguments as pl_paged_window_decode, window 0: the whole
- * context.  Elements of q and scales are below 2^56 in size.  An entry outside
- * the pool writes PL_ERR_PAGE_OUT_OF_RANGE and counts as a page of zeros.
+ * context.  Elements of q are below 2^56 in size, and V's values (minima and
+ * 15 scales) times the row's positions below 2^55: larger ones overflow to inf
+ * or NaN without a status.  Where all of V is below 2^-53 in size O is exact to
+ * steps of 2^-76.  An entry outside the pool writes PL_ERR_PAGE_OUT_OF_RANGE
+ * and counts as a page of zeros, as in the prompt forms (pl_paged_window_decode
+ * does not see it).
  */
 int32_t pl_kv4_append(const void *k, int64_t k_stride, const void *v,
                       int64_t v_stride, void *kv4_cache, int64_t num_pages,
@@ -1207,10 +1213,10 @@ int32_t pl_paged_kv4_decode(const void *q, int64_t q_stride_b,
  * query tokens i and heads h of exp(sm_scale q_ih . k_j - lse[i][h]) where i
  * sees j (causal: the request's tokens are its last cached positions).  lse
  * fp32 [total_q][num_qo_heads] as an attention of the same q and cache wrote
- * it (-inf: the query gives nothing).  q (positive strides), kv_cache and the
+ * it (-inf: the query gives nothing; NaN, or a query of NaN: NaN).  q (positive strides), kv_cache and the
  * tables as pl_paged_prefill; a request with more tokens than cached positions
  * or with tables outside kv_indices or q writes PL_ERR_INVALID_ARGUMENT and is
- * left out.
+ * left out; the other requests are not touched by it.
  *
  * pl_evict_select: what row r of lens[r] cached positions keeps.  A row of at
  * most budget positions keeps all: keep_from = lens[r], keep_count = 0.
@@ -1219,8 +1225,8 @@ int32_t pl_paged_kv4_decode(const void *q, int64_t q_stride_b,
  * first among equals (-0 equals 0, NaN is above all): keep_from = sinks,
  * keep[r] = the other positions, ascending, keep_count = budget - sinks.  Rest
  * of keep[r]: -1.  These are pl_cache_compact's arguments.  out_weight
- * [num_rows][capacity] (not overlapping weight) receives the kept positions'
- * weights in their new order, then 0.  keep_width >= budget - sinks, sinks +
+ * [num_rows][capacity] receives the kept positions' weights in their new order,
+ * then 0; no output overlaps weight or lens.  keep_width >= budget - sinks, sinks +
  * recent <= budget.  A row with lens < 0 or > capacity writes
  * PL_ERR_INVALID_ARGUMENT and keeps all.
  */

@@ -16,6 +16,14 @@ rows fork and end) and decodes one token per row and step with one of
   quantised once, new tokens as they come (kv4_append), and the attention runs
   over the records (paged_kv4_decode).
 
+The prompt is the engine's, with full attention over bf16, and notes no weights:
+:attr:`BoundedDecoder.weight` [rows, positions] starts at 0, so an eviction goes
+by the steps so far and, among positions without weight, keeps the lower ones.  A
+caller with the prompt's queries and log sums adds its weights there
+(paged_prefill_weights, layer by layer).  A step that notes weights takes a
+workspace by the rows' capacity, not their length: 4 bytes a position and query
+head of every row.
+
 Keys keep the rotation of the position where they were computed, so a new
 token's position counts all tokens that the row has had, evicted ones too.  No
 step waits for the device, except the first after rows ended or began.  No

@@ -58,11 +58,12 @@ __device__ __forceinline__ uint32_t fms_bf16x2(uint32_t a, uint32_t b, uint32_t 
 // ----------------------------------------------------------------- append
 // Eight lanes take one record (K or V of one head of one token): D / 8
 // channels a lane, a group's extremes by three exchanges.  Differences are
-// taken between halves of the values, which neither overflow nor round, so
-// every finite bf16 input has finite scales.  A group with inf or NaN
-// decodes to NaN.  A code comes from a product with 1 / scale and is put right
-// by its remainder (ties are common among bf16 values; dividing where one was
-// near cost 44 us for 16384 tokens of 8 heads).
+// taken between halves of the values, which do not overflow, so every finite
+// bf16 input has finite scales; they round (once, to fp32) where the values'
+// exponents lie more than 16 apart.  A group with inf or NaN decodes to NaN.  A
+// code comes from a product with 1 / scale and is put right by its remainder,
+// exact for that difference (ties are common among bf16 values; dividing where
+// one was near cost 44 us for 16384 tokens of 8 heads).
 // Bound by HBM: 2 D bytes in, D / 2 + 16 out.
 template <int D>
 __global__ void __launch_bounds__(256)
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(256)
 //   O_dh = sum_j (p_jh s_jG)(c_jd - 8) + sum_j p_jh m_jG + 8 sum_j p_jh s_jG.
 // sum_G m Q is one product with Q in three bf16 parts (exact to 2^-24); the
 // last two sums are the rows of one product with the tile's tails.  K is
-// exact.  p is rounded to bf16 (2^-9, as elsewhere); p s enters as a bf16 value
+// exact.  p is rounded to bf16 (2^-8, as elsewhere); p s enters as a bf16 value
 // and its exact remainder, since a group's spread can exceed a channel's: one
 // rounded p s gave a relative error of 0.0031 in place of 0.0023 (and 616 us
 // in place of 697, for 64 rows of 8192 positions and 32 kv heads; remainders
@@ -235,10 +236,17 @@ __global__ void __launch_bounds__(256)
 // P^T is turned into the operand layout before the scales go on, as packed
 // pairs.
 //
+// The powers of two bound the range: q below 2^56 in size, V's values times the
+// row's positions below 2^55 (p reaches 2^68, and their sums are fp32), and
+// steps of 2^-76 in O where all of V is smaller than 2^-53.
+//
 // The bytes (160 a position and head at head_dim 128 where bf16 has 512) are
-// within reach of HBM, 412 us there; what bounds it is issue: about 390
-// instructions a tile and head, half of them on the half-rate logic pipe, and
-// 26 products.  Two CTAs share an SM where a group fits one column block (128
+// within reach of HBM, 412 us there.  No unit is full: of the issue slots 59 %
+// are taken (about 390 instructions a tile and head), of the logic pipe's 48,
+// the tensor pipe is active for 32 %, HBM at 47.  What bounds it is the latency
+// of dependent instructions with four warps a scheduler: an instruction of a
+// warp takes 6.3 cycles, 1.3 of fixed latency, 1.0 for a pipe, 1.1 for its turn,
+// 0.9 for memory.  Two CTAs share an SM where a group fits one column block (128
 // registers a thread), and the next tile's scores stand between this one's
 // values (646 -> 616 us), so that one's latencies are the other's issue slots.
 template <int D, int NT>

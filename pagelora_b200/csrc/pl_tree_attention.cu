@@ -44,7 +44,7 @@
 // P.V -> next scores of each of two row tiles in turn: 8 requests of 64 tokens
 // at 32768 positions take 737 us in two layers, 747 TFLOP/s (660 us before the
 // power limit lowers the clock from 1.8 to 1.6 GHz).  The prefill kernel, which
-// does not wait for the maximum, does the same products at 1050 TFLOP/s.
+// does not wait for the maximum, does the same products at 998 TFLOP/s.
 #include "pl_common.cuh"
 
 namespace pl {

@@ -18,8 +18,9 @@
 // The eight warps' states are joined in shared memory at an item's end.
 //
 // Bound by HBM: 512 bytes of K and V per position and kv head at head_dim 128
-// for 16 x 8 tensor-core columns.  P enters the tensor core as bf16 (relative
-// 2^-9 a term, below the rounding of the output); maxima, sums and O are fp32.
+// for 16 x 8 tensor-core columns.  P enters the tensor core as bf16 (at most
+// 2^-8 relative a term, as the output's own rounding; over many terms it
+// averages out); maxima, sums and O are fp32.
 #include <mutex>
 
 #include "pl_line_decode.cuh"

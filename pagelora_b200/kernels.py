@@ -1287,7 +1287,7 @@ def _need_kv4(cache: torch.Tensor, head_dim: int) -> None:
 def kv4_append(k: torch.Tensor, v: torch.Tensor, kv4_cache: torch.Tensor, page_id: torch.Tensor,
                page_offset: torch.Tensor, status: torch.Tensor | None = None) -> None:
     """Quantise k, v [T, Hkv, D] bf16 into the 4-bit pool at (page_id[t],
-    page_offset[t]) (pl_kv4_append)."""
+    page_offset[t]), distinct slots (pl_kv4_append)."""
 
     _need_cuda(k, v, kv4_cache)
     _need(k, torch.bfloat16, "k")
@@ -1341,7 +1341,8 @@ def paged_kv4_decode(
 ) -> torch.Tensor:
     """Paged decode of one token per row straight over a 4-bit pool
     (pl_paged_kv4_decode): q [B, Hq, D] bf16; ``window`` and ``sinks`` as
-    :func:`paged_window_decode` (None: the whole context)."""
+    :func:`paged_window_decode` (None: the whole context).  Elements of q are
+    below 2**56 in size and V's values times a row's positions below 2**55."""
 
     _need_cuda(q, kv4_cache, out, workspace)
     _need_queries(q, "batch")

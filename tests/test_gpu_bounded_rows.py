@@ -137,3 +137,23 @@ def test_the_records_of_a_large_pool(cuda_device):
         for p in (0, 4095, 4096, 8191, 8192, 8999):
             assert (dec.kv4[li, p].cpu().numpy() == o.record_bytes(*o.pack4(kv[li, p].float().cpu().numpy()))).all(), (li, p)
     assert (dec.kv4[:, 4097:8191] == 0).all()
+
+
+@pytest.mark.parametrize("kv4", [False, True])
+def test_a_refused_step_changes_nothing(cuda_device, kv4):
+    from pagelora_b200.bounded_decode import Window
+
+    run = Bounded(cuda_device, [96, 40], window=Window(24, 2), kv4=kv4, engine=dict(max_context=96, num_pages=10))
+    run.step()  # 7 + 3 pages: all taken
+    for _ in range(7):
+        run.step()  # the second row's last page is full now
+    before, pos = run.state() + list(_held(run.dec)), run.dec.pos.clone()
+    nxt, _ = run.dec.step(torch.tensor(run.cur, dtype=torch.int64, device=cuda_device))
+    assert (nxt == -1).all()
+    run.unchanged(before[:-2], "PL_ERR_POOL_EXHAUSTED")
+    assert torch.equal(run.dec.pos, pos) and all(torch.equal(a, b) for a, b in zip(before[-2:], _held(run.dec)))
+    run.release(1)
+    run.step()
+    run.dec.trim()
+    run.dec.check()
+    run.step()

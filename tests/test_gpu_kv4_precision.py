@@ -163,3 +163,16 @@ def test_a_prompt_over_a_4_bit_cache(K, window):
     if window is None:
         dev = dict(q=q[-1:].cuda(), cache=cache, indptr=_i32([0, pages]), indices=_i32(ids), last=_i32(host["last"]))
         _tight(_run(K, dev)[0], host)
+
+
+@pytest.mark.gpu
+def test_values_below_the_range_of_the_sums(K):
+    """All of V is below 2^-53 in size: O is exact to a step of 2^-76 for each of its sums' terms."""
+
+    rng = np.random.default_rng(6)
+    x = _bf16(rng.normal(size=(9, 2, 16, 2, 64)) * 2.0 ** -58).float().numpy()
+    host, dev = _case([140], 4, 2, 64, 16, 7)
+    host["rec"] = o.record_bytes(*o.pack4(x))
+    host["indices"] = np.arange(9)
+    dev.update(cache=torch.as_tensor(host["rec"]).cuda(), indices=_i32(host["indices"]))
+    _tight(_run(K, dev)[0], host, 140 * 2.0 ** -76)
