@@ -28,7 +28,7 @@ namespace pl {
 // units (16 a cycle) beside 512 cycles of products at head_dim 128, so a
 // quarter of the pairs is computed on the FMA pipe instead (pw_exp2_pair, nine
 // cycles an element; none 393, a quarter 381, half 421 us at 8192 tokens, 32
-// heads).  Measured 374 us there, 0.73 PFLOP/s: 1250 cycles a product, of
+// heads).  Measured 377 us there, 0.73 PFLOP/s: 1250 cycles a product, of
 // which the chain product -> commit -> read -> exponentials of a buffer and
 // its successor's is what is left; tensor memory holds no third one.
 constexpr int kPwM = 128;                   // positions of a product
